@@ -289,6 +289,122 @@ SDPA_B200_API int sdpa_b200_sum_bias_grad(const void* grad, int64_t batch_stride
                                           int32_t batch, int32_t heads, int32_t seqlen_q, int32_t seqlen_k, int32_t over_batch,
                                           int32_t over_heads, void* out, int32_t dtype, void* stream);
 
+/* ---- rotary positions -------------------------------------------------------------------------------------------------
+ * q_out, k_out <- q, k with the first rotary_dim elements of every row turned by the angles of its token:
+ *   angle_j = position[axis(j)] * inv_freq[j],  (x, y) -> scaling * (x cos - y sin, x sin + y cos)
+ * over the pairs (j, j + rotary_dim / 2), or (2j, 2j + 1) with `interleaved`; the other elements are copied. axis(j) is the
+ * section that pair j falls into, so that sections of time, height and width turn by three positions of a token. The angle is
+ * formed in 64 bits, since in 32 that of a far position is lost. `inverse` turns by the negative angle: the gradient of q and k out
+ * of that of the results. q_out / k_out may be q / k themselves. No counterpart in the reference, whose models bring their own. */
+typedef struct sdpa_b200_rotary_params {
+  const void* q;
+  const void* k; /* NULL with heads_k == 0 */
+  void* q_out;
+  void* k_out;
+  const void* positions; /* int32, or int64 with positions_64; [axes][batch][length] by the strides below, in elements */
+  const float* inv_freq; /* [rotary_dim / 2] */
+  int32_t batch, length, heads_q, heads_k;
+  int32_t head_dim;    /* a multiple of 8, at most 256 */
+  int32_t rotary_dim;  /* a multiple of 16, at most head_dim */
+  int32_t axes;        /* 1 to 4 */
+  int32_t sections[4]; /* pairs per axis, together rotary_dim / 2 */
+  int32_t interleaved, inverse, positions_64;
+  int32_t dtype; /* SDPA_B200_BF16 or SDPA_B200_F16 */
+  float scaling;
+  /* elements, multiples of 8; those of inputs may be 0 (broadcast) */
+  int64_t q_batch_stride, q_head_stride, q_row_stride;
+  int64_t k_batch_stride, k_head_stride, k_row_stride;
+  int64_t qo_batch_stride, qo_head_stride, qo_row_stride;
+  int64_t ko_batch_stride, ko_head_stride, ko_row_stride;
+  int64_t pos_axis_stride, pos_batch_stride, pos_row_stride;
+} sdpa_b200_rotary_params;
+
+SDPA_B200_API int sdpa_b200_rotary(const sdpa_b200_rotary_params* p, void* stream);
+
+/* ---- the 8-bit paged cache ---------------------------------------------------------------------------------------------
+ * Keys and values live in blocks of block_size tokens: codes [num_blocks][heads_kv][block_size][head_dim], e4m3 or int8, with one
+ * fp32 scale per block and head; an element is code * scale. A request's token at position p is in the block block_table[request]
+ * [p / block_size], at p % block_size; that place in the cache, block * block_size + p % block_size, is called its slot. No
+ * counterpart in the reference, which has no paged cache. */
+enum { SDPA_B200_E4M3 = 0, SDPA_B200_INT8 = 1 };
+
+/* One serving step's bookkeeping. new_tokens[i] tokens are added to request i (negative: that many are taken back), and what it needs
+ * or no longer needs of blocks moves between block_table and a ring of free ones. The ring holds ring_state[1] free blocks from index
+ * ring_state[0] on, modulo num_blocks; blocks are taken at its front, request by request, page by page, and given back at its end.
+ * Written: seq_lens[i] = cached_lens[i] + new_tokens[i]; cu_seqlens[batch + 1], the offsets of the requests' new tokens; positions and
+ * slots of these num_tokens tokens, 0 and -1 behind the last one; the new blocks in block_table (entries behind a request's last block
+ * mean nothing and are left as they are); blocks given back, in the ring; next_state.
+ * All or nothing: where a request would get a negative length, more than max_blocks blocks or tokens behind num_tokens, next_state[2] is
+ * -1 - (the first such request), where blocks are lacking their number, else 0; a step that is refused so changes nothing, and seq_lens,
+ * cu_seqlens, positions, slots are those of a step without new tokens. seq_lens may be cached_lens and next_state may be ring_state. */
+typedef struct sdpa_b200_plan_params {
+  const int32_t* cached_lens; /* [batch] */
+  const int32_t* new_tokens;  /* [batch] */
+  int32_t* block_table;       /* [batch][table_stride], the first max_blocks of each row */
+  int32_t* ring;              /* [num_blocks] */
+  const int32_t* ring_state;  /* [3] */
+  int32_t* seq_lens;          /* [batch] */
+  int32_t* cu_seqlens;        /* [batch + 1] */
+  int32_t* positions;         /* [num_tokens] */
+  int32_t* slots;             /* [num_tokens] */
+  int32_t* next_state;        /* [3] */
+  int64_t table_stride;
+  int32_t batch, max_blocks, num_blocks, block_size, num_tokens; /* block_size: 16, 32, 64 or 128; num_blocks * block_size < 2^31 */
+} sdpa_b200_plan_params;
+
+SDPA_B200_API int sdpa_b200_plan_step(const sdpa_b200_plan_params* p, void* stream);
+
+typedef struct sdpa_b200_cache_params {
+  /* codes by (block, head, token) strides in bytes, multiples of 16, head_dim contiguous; 16-byte aligned */
+  void* k_cache;
+  void* v_cache;
+  float* k_scale; /* [num_blocks][heads_kv] */
+  float* v_scale;
+  int64_t k_block_stride, k_head_stride, k_row_stride;
+  int64_t v_block_stride, v_head_stride, v_row_stride;
+  int32_t num_blocks, block_size, heads_kv, head_dim; /* block_size: 16, 32, 64 or 128; head_dim: 64 or 128 */
+  int32_t code;  /* SDPA_B200_E4M3 or SDPA_B200_INT8 */
+  int32_t dtype; /* of key, value, q, out: SDPA_B200_BF16 or SDPA_B200_F16 */
+  /* store */
+  const void* key; /* [num_tokens][heads_kv][head_dim] by strides in elements, multiples of 8 */
+  const void* value;
+  int64_t key_row_stride, key_head_stride;
+  int64_t value_row_stride, value_head_stride;
+  const int32_t* slots;
+  int32_t num_tokens;
+  /* attention */
+  int32_t batch;
+  const void* q; /* [total_q][heads_q][head_dim] by strides in elements, multiples of 8 */
+  void* out;
+  float* lse; /* [heads_q][total_q] */
+  int64_t q_row_stride, q_head_stride;
+  int64_t o_row_stride, o_head_stride;
+  const int32_t* block_table;  /* [batch][table_stride], the first max_blocks of each row */
+  const int32_t* seq_lens;     /* [batch]: tokens of each request in the cache, those of q among them */
+  const int32_t* cu_seqlens_q; /* [batch + 1]; NULL: one row of q per request */
+  int64_t table_stride;
+  int32_t max_blocks, heads_q, total_q;
+  int32_t max_seqlen_q, max_seqlen_k; /* at least the longest request's */
+  int32_t is_causal;                  /* bottom-right aligned, as everywhere here */
+  float softmax_scale;
+  uint32_t* device_status; /* as in sdpa_b200_params */
+} sdpa_b200_cache_params;
+
+/* Puts the keys and values of a step into the cache. Every (block, head) that gets tokens has its scale raised to the smallest power of two
+ * at which the largest of them is a code (448 for e4m3, 127 for int8), unless it is that large already; earlier tokens of the block are
+ * rounded again to a scale that has grown. A block whose first place is written starts anew. Tokens with a negative slot, or one behind the
+ * cache, are left out. The tokens of one block stand next to each other, with rising slots, as sdpa_b200_plan_step gives them (the same slot
+ * twice in a row: the later token stays; fewer than 32 tokens that are left out may stand between them); a block that comes up again
+ * behind tokens of another one is not allowed, since the two parts are worked on at the same time. A NaN or infinite element becomes NaN in e4m3; int8 has none, there the scale becomes NaN until the
+ * block starts anew. */
+SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* stream);
+
+/* out, lse <- attention of each request's last rows of q over its tokens in the cache. A row without a visible key gets out = 0 and lse = +inf;
+ * rows of q outside every request are left unwritten; a block number outside the cache makes the rows that see it NaN (with lse = +inf, as NaN rows have here). Nothing at or behind
+ * seq_lens counts, whatever stands there. (A NaN among the values themselves may reach every row of its request, as 0 * NaN.) */
+SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);
+SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 /* How many of this library's kernels the calling process has launched so far. */
 SDPA_B200_API uint64_t sdpa_b200_launch_count(void);
 

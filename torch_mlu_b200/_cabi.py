@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libsdpa_b200.so")
 OK, INVALID_ARG, UNSUPPORTED, LAUNCH_FAILED, DEVICE_TIMEOUT, NO_DEVICE = range(6)
 KERNEL_AUTO, KERNEL_PREFILL, KERNEL_DECODE = 0, 1, 2
 DTYPE_BF16, DTYPE_F16 = 0, 1
+CODE_E4M3, CODE_INT8 = 0, 1
 
 # every symbol include/sdpa_b200.h declares
 EXPORTED_SYMBOLS = (
@@ -37,6 +38,11 @@ EXPORTED_SYMBOLS = (
     "sdpa_b200_mask_to_bias",
     "sdpa_b200_pad_bias",
     "sdpa_b200_sum_bias_grad",
+    "sdpa_b200_rotary",
+    "sdpa_b200_plan_step",
+    "sdpa_b200_cache_store",
+    "sdpa_b200_cache_attention_workspace_bytes",
+    "sdpa_b200_cache_attention",
     "sdpa_b200_launch_count",
 )
 STATIC_SCRATCH_BYTES = 16 << 20
@@ -67,6 +73,48 @@ class SdpaParams(ctypes.Structure):
         ("bias_t", c_void_p), ("bias_t_batch_stride", c_int64), ("bias_t_head_stride", c_int64), ("bias_t_row_stride", c_int64),
         ("deterministic", c_int32), ("sm_margin", c_int32),
         ("device_status", c_void_p),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+        ("positions", c_void_p), ("inv_freq", c_void_p),
+        ("batch", c_int32), ("length", c_int32), ("heads_q", c_int32), ("heads_k", c_int32),
+        ("head_dim", c_int32), ("rotary_dim", c_int32), ("axes", c_int32), ("sections", c_int32 * 4),
+        ("interleaved", c_int32), ("inverse", c_int32), ("positions_64", c_int32), ("dtype", c_int32), ("scaling", c_float),
+        ("q_batch_stride", c_int64), ("q_head_stride", c_int64), ("q_row_stride", c_int64),
+        ("k_batch_stride", c_int64), ("k_head_stride", c_int64), ("k_row_stride", c_int64),
+        ("qo_batch_stride", c_int64), ("qo_head_stride", c_int64), ("qo_row_stride", c_int64),
+        ("ko_batch_stride", c_int64), ("ko_head_stride", c_int64), ("ko_row_stride", c_int64),
+        ("pos_axis_stride", c_int64), ("pos_batch_stride", c_int64), ("pos_row_stride", c_int64),
+    ]
+
+
+class PlanParams(ctypes.Structure):
+    _fields_ = [
+        ("cached_lens", c_void_p), ("new_tokens", c_void_p), ("block_table", c_void_p), ("ring", c_void_p), ("ring_state", c_void_p),
+        ("seq_lens", c_void_p), ("cu_seqlens", c_void_p), ("positions", c_void_p), ("slots", c_void_p), ("next_state", c_void_p),
+        ("table_stride", c_int64),
+        ("batch", c_int32), ("max_blocks", c_int32), ("num_blocks", c_int32), ("block_size", c_int32), ("num_tokens", c_int32),
+    ]
+
+
+class CacheParams(ctypes.Structure):
+    _fields_ = [
+        ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("k_block_stride", c_int64), ("k_head_stride", c_int64), ("k_row_stride", c_int64),
+        ("v_block_stride", c_int64), ("v_head_stride", c_int64), ("v_row_stride", c_int64),
+        ("num_blocks", c_int32), ("block_size", c_int32), ("heads_kv", c_int32), ("head_dim", c_int32),
+        ("code", c_int32), ("dtype", c_int32),
+        ("key", c_void_p), ("value", c_void_p),
+        ("key_row_stride", c_int64), ("key_head_stride", c_int64), ("value_row_stride", c_int64), ("value_head_stride", c_int64),
+        ("slots", c_void_p), ("num_tokens", c_int32),
+        ("batch", c_int32), ("q", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("q_row_stride", c_int64), ("q_head_stride", c_int64), ("o_row_stride", c_int64), ("o_head_stride", c_int64),
+        ("block_table", c_void_p), ("seq_lens", c_void_p), ("cu_seqlens_q", c_void_p), ("table_stride", c_int64),
+        ("max_blocks", c_int32), ("heads_q", c_int32), ("total_q", c_int32), ("max_seqlen_q", c_int32), ("max_seqlen_k", c_int32),
+        ("is_causal", c_int32), ("softmax_scale", c_float), ("device_status", c_void_p),
     ]
 
 
@@ -134,6 +182,14 @@ def load() -> ctypes.CDLL:
     lib.sdpa_b200_sum_bias_grad.restype = c_int
     lib.sdpa_b200_sum_bias_grad.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                             c_int32, c_void_p]
+    for name, struct in (("sdpa_b200_rotary", RotaryParams), ("sdpa_b200_plan_step", PlanParams), ("sdpa_b200_cache_store", CacheParams)):
+        fn = getattr(lib, name)
+        fn.restype = c_int
+        fn.argtypes = [POINTER(struct), c_void_p]
+    lib.sdpa_b200_cache_attention_workspace_bytes.restype = c_int
+    lib.sdpa_b200_cache_attention_workspace_bytes.argtypes = [POINTER(CacheParams), POINTER(c_size_t)]
+    lib.sdpa_b200_cache_attention.restype = c_int
+    lib.sdpa_b200_cache_attention.argtypes = [POINTER(CacheParams), c_void_p, c_size_t, c_void_p]
     _lib = lib
     return lib
 

@@ -1,0 +1,188 @@
+// One serving step's bookkeeping on the GPU: which blocks of the paged cache belong to which request, where each new token goes, which blocks
+// are free. No counterpart in the reference, which has no paged cache.
+//
+// With lengths c_i and c_i + n_i and pages(x) = ceil(x / block_size), request i takes max(0, pages(c_i + n_i) - pages(c_i)) blocks off the front of
+// the ring of free ones and gives max(0, the reverse) back at its end; the running sums over the requests say at which place of the ring each finds
+// its own, and where its tokens stand. All of it is a few loads deep: a launch's latency bounds it, not bytes. So it is one cluster: every block of it
+// forms the running sums for itself (in shared memory, 12 bytes a request), then they share out the tokens and the pages, and a cluster barrier keeps the
+// state from being written before all have read it, which lets a caller hand over the same tensors for old and new state.
+#include "kernels.h"
+#include "ptx_sm100.cuh"
+
+namespace sdpa_b200 {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kMaxBatch = 16384;  // three running sums of it fit a block's shared memory
+
+struct Sums {
+  int tokens, need, freed;
+};
+
+__device__ __forceinline__ int pages_of(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
+
+__global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_params p, int shift) {
+  extern __shared__ int sums[];  // [batch] each: tokens, blocks taken, blocks given back, before request i
+  int* s_tokens = sums;
+  int* s_need = sums + p.batch;
+  int* s_freed = sums + 2 * p.batch;
+  __shared__ Sums warp_sums[kThreads / 32];
+  __shared__ int first_bad;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x, ranks = gridDim.x;
+  if (tid == 0) first_bad = p.batch;
+  const int first = p.ring_state[0], count = p.ring_state[1];
+  __syncthreads();
+
+  // ---- running sums over the requests, kThreads at a time
+  long long all_tokens = 0, all_need = 0, all_freed = 0;
+  for (int base = 0; base < p.batch; base += kThreads) {
+    const int i = base + tid;
+    Sums mine = {0, 0, 0};
+    bool bad = false;
+    if (i < p.batch) {
+      const int c = p.cached_lens[i], n = p.new_tokens[i];
+      const long long len = static_cast<long long>(c) + n;
+      const long long most = static_cast<long long>(p.max_blocks) << shift;
+      bad = c < 0 || c > most || len < 0 || len > most || n > p.num_tokens;
+      if (!bad) {
+        const int had = pages_of(c, shift), has = pages_of(static_cast<int>(len), shift);
+        mine = {n > 0 ? n : 0, has > had ? has - had : 0, had > has ? had - has : 0};
+      }
+    }
+    Sums run = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int a = __shfl_up_sync(0xffffffffu, run.tokens, d), b = __shfl_up_sync(0xffffffffu, run.need, d), c = __shfl_up_sync(0xffffffffu, run.freed, d);
+      if (lane >= d) {
+        run.tokens += a;
+        run.need += b;
+        run.freed += c;
+      }
+    }
+    if (lane == 31) warp_sums[warp] = run;
+    __syncthreads();
+    long long t0 = all_tokens, n0 = all_need, f0 = all_freed;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const Sums s = warp_sums[w];
+      if (w < warp) {
+        t0 += s.tokens;
+        n0 += s.need;
+        f0 += s.freed;
+      }
+      all_tokens += s.tokens;
+      all_need += s.need;
+      all_freed += s.freed;
+    }
+    if (i < p.batch) {
+      const long long end = t0 + run.tokens;
+      s_tokens[i] = static_cast<int>(end - mine.tokens);
+      s_need[i] = static_cast<int>(n0 + run.need - mine.need);
+      s_freed[i] = static_cast<int>(f0 + run.freed - mine.freed);
+      if (bad || end > p.num_tokens) atomicMin(&first_bad, i);
+    }
+    __syncthreads();
+  }
+  // No sum has passed 32 bits in front of the first bad request: tokens end at 2 * num_tokens at most, pages at batch * max_blocks (checked by the host).
+  const int refused = first_bad < p.batch ? -1 - first_bad : all_need > count ? static_cast<int>(all_need - count) : 0;
+  const bool fine = refused == 0;
+  const int total = fine ? static_cast<int>(all_tokens) : 0;
+  // `at` places behind the ring's front; first and count are the caller's, so the result is brought into the ring in any case
+  auto ring_at = [&](long long at) {
+    const long long x = (first + at) % p.num_blocks;
+    return static_cast<int>(x < 0 ? x + p.num_blocks : x);
+  };
+
+  // ---- tokens: the request of each by bisection in the running sums
+  for (int t = rank * kThreads + tid; t < p.num_tokens; t += ranks * kThreads) {
+    int pos = 0, slot = -1;
+    if (t < total) {
+      int lo = 0, hi = p.batch - 1;  // the last request whose tokens begin at or before t, among which empty ones come first
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (s_tokens[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int c = p.cached_lens[lo];
+      pos = c + t - s_tokens[lo];
+      const int page = pos >> shift, had = pages_of(c, shift);
+      const int block = page < had ? p.block_table[lo * p.table_stride + page] : p.ring[ring_at(s_need[lo] + page - had)];
+      slot = block < 0 || block >= p.num_blocks ? -1 : (block << shift) + (pos & ((1 << shift) - 1));
+    }
+    p.positions[t] = pos;
+    p.slots[t] = slot;
+  }
+  // ---- pages that change hands: a warp per request
+  if (fine) {
+    for (int i = rank * (kThreads / 32) + warp; i < p.batch; i += ranks * (kThreads / 32)) {
+      const int c = p.cached_lens[i], had = pages_of(c, shift), has = pages_of(c + p.new_tokens[i], shift);
+      int32_t* row = p.block_table + i * p.table_stride;
+      for (int page = had + lane; page < has; page += 32) row[page] = p.ring[ring_at(s_need[i] + page - had)];
+      for (int page = has + lane; page < had; page += 32) p.ring[ring_at(static_cast<long long>(count) + s_freed[i] + page - has)] = row[page];
+    }
+  }
+  cluster_sync();  // everybody has read the old lengths and state
+  for (int i = rank * kThreads + tid; i < p.batch; i += ranks * kThreads) {
+    p.seq_lens[i] = p.cached_lens[i] + (fine ? p.new_tokens[i] : 0);
+    p.cu_seqlens[i] = fine ? s_tokens[i] : 0;
+  }
+  if (rank == 0 && tid == 0) {
+    p.cu_seqlens[p.batch] = total;
+    p.next_state[0] = fine ? ring_at(all_need) : first;
+    p.next_state[1] = fine ? static_cast<int>(count - all_need + all_freed) : count;
+    p.next_state[2] = refused;
+  }
+}
+
+}  // namespace
+}  // namespace sdpa_b200
+
+extern "C" SDPA_B200_API int sdpa_b200_plan_step(const sdpa_b200_plan_params* p, void* stream) {
+  using namespace sdpa_b200;
+  if (p == nullptr) {
+    set_error("plan_step: params is NULL");
+    return SDPA_B200_INVALID_ARG;
+  }
+  const void* given[] = {p->cached_lens, p->new_tokens, p->block_table, p->ring, p->ring_state, p->seq_lens, p->cu_seqlens, p->positions, p->slots, p->next_state};
+  for (const void* x : given) {
+    if (x == nullptr || (reinterpret_cast<uintptr_t>(x) & 3u) != 0) {
+      set_error("plan_step: a pointer is NULL or not 4-byte aligned");
+      return SDPA_B200_INVALID_ARG;
+    }
+  }
+  if (p->batch <= 0 || p->batch > kMaxBatch || p->num_tokens <= 0 || p->max_blocks <= 0 || p->num_blocks <= 0 || p->table_stride < p->max_blocks) {
+    set_error("plan_step: batch (1 to %d), num_tokens, max_blocks and num_blocks must be positive, a table row must hold max_blocks (got %d, %d, %d, %d, "
+              "%lld)", kMaxBatch, p->batch, p->num_tokens, p->max_blocks, p->num_blocks, static_cast<long long>(p->table_stride));
+    return SDPA_B200_INVALID_ARG;
+  }
+  int shift = 4;
+  while (shift < 7 && (1 << shift) != p->block_size) ++shift;
+  if ((1 << shift) != p->block_size) {
+    set_error("plan_step: block_size must be 16, 32, 64 or 128 (got %d)", p->block_size);
+    return SDPA_B200_INVALID_ARG;
+  }
+  if ((static_cast<int64_t>(p->num_blocks) << shift) > INT32_MAX || (static_cast<int64_t>(p->max_blocks) << shift) > INT32_MAX ||
+      static_cast<int64_t>(p->batch) * p->max_blocks > INT32_MAX || p->num_tokens > (1 << 30)) {
+    set_error("plan_step: slots, positions and table entries are counted in 32 bits");
+    return SDPA_B200_INVALID_ARG;
+  }
+  int st = check_device();
+  if (st != SDPA_B200_OK) return st;
+  const size_t smem = static_cast<size_t>(p->batch) * 3 * sizeof(int);
+  if (smem > 40 * 1024) {
+    const cudaError_t err = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBatch * 3 * static_cast<int>(sizeof(int)));
+    if (err != cudaSuccess) {
+      set_error("plan_step: launch failed: %s", cudaGetErrorString(err));
+      return SDPA_B200_LAUNCH_FAILED;
+    }
+  }
+  // one block for a decode step; for more tokens up to eight, the largest cluster that every device takes
+  const int ranks = p->num_tokens <= 2 * kThreads ? 1 : p->num_tokens <= 8 * kThreads ? 4 : 8;
+  const cudaError_t err = launch_behind(plan_kernel, dim3(ranks), kThreads, smem, static_cast<cudaStream_t>(stream), false, ranks, *p, shift);
+  if (err != cudaSuccess) {
+    set_error("plan_step: launch failed: %s", cudaGetErrorString(err));
+    return SDPA_B200_LAUNCH_FAILED;
+  }
+  count_launch();
+  return SDPA_B200_OK;
+}

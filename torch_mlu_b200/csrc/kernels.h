@@ -23,6 +23,11 @@ int make_tensor_map_16(bool f16, CUtensorMap* map, const void* base, int head_di
                        int64_t heads, int64_t batch, int64_t row_stride, int64_t head_stride,
                        int64_t batch_stride, int box_rows);
 
+// A 4-D tensor map over the codes of a paged cache {head_dim, block_size, heads, blocks} with a {head_dim, box_rows, 1, 1} box, swizzled over head_dim
+// (64 or 128) bytes. Strides in bytes.
+int make_cache_tensor_map(CUtensorMap* map, const void* base, int head_dim, int block_size, int heads, int64_t blocks, int64_t row_stride,
+                          int64_t head_stride, int64_t block_stride, int box_rows);
+
 // Prefill forward (TMA + tcgen05), a persistent kernel with one CTA per SM.
 int launch_fwd_prefill(const sdpa_b200_params& p, void* workspace, cudaStream_t stream);
 

@@ -98,6 +98,32 @@ int make_ds_tensor_map(CUtensorMap* map, const void* base, uint32_t tiles, int b
   return SDPA_B200_OK;
 }
 
+int make_cache_tensor_map(CUtensorMap* map, const void* base, int head_dim, int block_size, int heads, int64_t blocks, int64_t row_stride,
+                          int64_t head_stride, int64_t block_stride, int box_rows) {
+  EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return SDPA_B200_NO_DEVICE;
+  }
+  // a size-1 dimension never advances, but its stride must still be a legal value
+  if (heads == 1) head_stride = row_stride;
+  if (blocks == 1) block_stride = row_stride;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(head_dim), static_cast<cuuint64_t>(block_size), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(blocks)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(row_stride), static_cast<cuuint64_t>(head_stride), static_cast<cuuint64_t>(block_stride)};
+  cuuint32_t box[4] = {static_cast<cuuint32_t>(head_dim), static_cast<cuuint32_t>(box_rows), 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (CUresult %d) for a cache of %lld blocks, strides (bytes) {token %lld, head %lld, block %lld}",
+              static_cast<int>(r), (long long)blocks, (long long)row_stride, (long long)head_stride, (long long)block_stride);
+    return SDPA_B200_INVALID_ARG;
+  }
+  return SDPA_B200_OK;
+}
+
 namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
