@@ -310,7 +310,13 @@ def test_rows_outside_every_request_are_left(cuda_device):
         q2, cu2 = torch.cat([pad, q, pad]), cu + 3
         out = torch.full_like(q2, 7.0)
         lse = torch.full((4, q2.shape[0]), 7.0, device=cuda_device)
-        p = kv_cache._cache_params(q2, kc, vc, ks, vs)
+        p = _cabi.CacheParams()
+        p.k_cache, p.v_cache, p.k_scale, p.v_scale = (x.data_ptr() for x in (kc, vc, ks, vs))
+        for x, c in (("k", kc), ("v", vc)):
+            for f, stride in zip(("block", "head", "row"), c.stride()):
+                setattr(p, f"{x}_{f}_stride", stride)
+        p.num_blocks, p.heads_kv, p.block_size, p.head_dim = kc.shape
+        p.code, p.dtype = _cabi.CODE_INT8, _cabi.DTYPE_BF16
         p.q, p.out, p.lse, p.block_table, p.seq_lens, p.cu_seqlens_q = (t.data_ptr() for t in (q2, out, lse, table, lens, cu2))
         p.q_row_stride = p.o_row_stride = 256
         p.q_head_stride = p.o_head_stride = 64

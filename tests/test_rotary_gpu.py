@@ -100,3 +100,106 @@ def test_refusals(cuda_device):
                            ((q, q, pos, f[:20]), {}, "multiple of 16"), ((q[:, :, :64], q, pos, f[:32]), {}, "agree")]:
         with pytest.raises(RuntimeError, match=text):
             call(*args, **kw)
+
+
+@pytest.mark.parametrize("layout", ["packed", "dense"])
+@pytest.mark.parametrize("interleaved,rot", [(False, 128), (True, 64)])
+def test_gradients(cuda_device, layout, interleaved, rot):
+    """Against the formula (the gradient is the turn backwards) and against differences of the 64-bit forward, which is linear: <dy, f(e)> for a unit
+    vector e is exact but for the rounding of the result, half a step."""
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    shapes = [(30, h, 128) if layout == "packed" else (2, h, 15, 128) for h in (6, 2)]
+    q, k, dq, dk = (torch.randn(*s, generator=g, device=cuda_device).bfloat16() for s in shapes * 2)
+    tokens = (30,) if layout == "packed" else (2, 15)
+    pos = torch.randint(0, 50000, (2,) + tokens, generator=g, device=cuda_device)
+    f, sections = _freq(rot // 2, cuda_device), (rot // 8, rot // 2 - rot // 8)
+    q.requires_grad_()
+    k.requires_grad_()
+    kw = dict(sections=sections, interleaved=interleaved, scaling=1.5)
+    a, b = rotary.rotary_embedding(q, k, pos, f, **kw)
+    assert a.requires_grad and b.requires_grad
+    gq, gk = torch.autograd.grad((a, b), (q, k), (dq, dk), retain_graph=True)
+    for got, d in ((gq, dq), (gk, dk)):
+        _check(got, d, pos, f, "gradient", inverse=True, **kw)
+    for at in [(0, 0, 0), (3, 1, 5), (29, 5, 127)] if layout == "packed" else [(0, 0, 0, 0), (1, 5, 14, 63), (1, 0, 7, 127)]:
+        e = torch.zeros(shapes[0], dtype=torch.float64, device=cuda_device)
+        e[at] = 1
+        want = float((orc.rotary(e, pos, f, **kw) * dq.double()).sum())
+        assert abs(float(gq[at]) - want) <= 2.0 ** -8 * abs(want) + 6e-7 * 1.5 * 2 * float(dq.double().abs().max())
+    # one of the two alone; a gradient that is expanded, and one whose rows the kernel cannot read
+    only, = torch.autograd.grad(b, k, dk, retain_graph=True)
+    assert torch.equal(only, gk)
+    only, = torch.autograd.grad((a, b), q, (dq, dk), retain_graph=True)
+    assert torch.equal(only, gq)
+    one = torch.ones((), device=cuda_device, dtype=torch.bfloat16).expand(shapes[0])
+    got, = torch.autograd.grad(a, q, one, retain_graph=True)
+    _check(got, one, pos, f, "expanded", inverse=True, **kw)
+    odd = torch.randn(*shapes[0][:-1], 129, generator=g, device=cuda_device).bfloat16()[..., 1:]
+    got, = torch.autograd.grad(a, q, odd, retain_graph=True)
+    _check(got, odd, pos, f, "odd rows", inverse=True, **kw)
+
+
+def test_second_derivative_and_shared_inputs(cuda_device):
+    """The backward is differentiable itself; a leaf used by both and an input expanded over heads get the sum of their gradients."""
+    pos, f = torch.arange(9, device=cuda_device), _freq(32, cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    x = torch.randn(9, 1, 64, generator=g, device=cuda_device).half().requires_grad_()
+    v = torch.randn(9, 4, 64, generator=g, device=cuda_device).half().requires_grad_()
+    y, _ = rotary.rotary_embedding(x.expand(-1, 4, -1), None, pos, f)
+    gx, = torch.autograd.grad(y, x, v, create_graph=True)
+    want = orc.rotary(v, pos, f, inverse=True).sum(1, keepdim=True)
+    assert bool(((gx.double() - want).abs() <= 2.0 ** -11 * (want.abs() + 4 * 4) + 1e-5).all())  # four rounded rows, then their sum in f16, twice
+    w = torch.randn(9, 1, 64, generator=g, device=cuda_device).half()
+    gv, = torch.autograd.grad(gx, v, w)
+    want = orc.rotary(w, pos, f)
+    assert bool(((gv.double() - want).abs() <= 2.0 ** -11 * want.abs() + 1e-5).all())
+    a, b = rotary.rotary_embedding(x, x, pos, f)
+    g1, = torch.autograd.grad((a, b), x, (w, w))
+    _check(g1 / 2, w, pos, f, "shared", inverse=True)
+
+
+def test_autograd_refuses_what_it_would_get_wrong(cuda_device):
+    pos, f = torch.arange(9, device=cuda_device), _freq(32, cuda_device)
+    x = torch.randn(9, 2, 64, device=cuda_device).half()
+    with pytest.raises(RuntimeError, match="no gradient: use rotary_embedding"):
+        rotary.rotary_embedding_(x.clone().requires_grad_(), None, pos, f)
+    with pytest.raises(RuntimeError, match="elements of their own"):
+        rotary.rotary_embedding_(x[:, :1].expand(-1, 2, -1), None, pos, f)
+    with pytest.raises(RuntimeError, match="ordinary tensor"):
+        torch.func.grad(lambda t: rotary.rotary_embedding(t, None, pos, f)[0].float().sum())(x)
+    # a tensor saved for a backward pass and then turned in place is noticed
+    y = (x.clone().requires_grad_() * 2)
+    z = y * y
+    with torch.no_grad():
+        rotary.rotary_embedding_(y, None, pos, f)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+
+def test_captured_training_step(cuda_device):
+    """Forward and backward into a graph, replayed on new data, while an eager graph of the same values lives. The captured step has a leaf of its own over
+    them: torch ties a leaf's gradient node to the stream that first used it, and a capture cannot wait for the default stream, whatever the operator."""
+    pos, f = torch.arange(40, device=cuda_device), _freq(64, cuda_device)
+    q = torch.randn(40, 4, 128, device=cuda_device).bfloat16().requires_grad_()
+    d = torch.randn(40, 4, 128, device=cuda_device).bfloat16()
+    leaf = q.detach().requires_grad_()
+    step = lambda: (lambda y: (y.detach(), *torch.autograd.grad(y, leaf, d)))(rotary.rotary_embedding(leaf, None, pos, f)[0])
+    alive = rotary.rotary_embedding(q, None, pos, f)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, gq = step()
+    for _ in range(2):
+        with torch.no_grad():
+            q.copy_(torch.randn_like(q))
+            d.copy_(torch.randn_like(d))
+            pos += 1000
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(y, q.detach(), pos, f, "replayed")
+        _check(gq, d, pos, f, "replayed gradient", inverse=True)
+    del alive

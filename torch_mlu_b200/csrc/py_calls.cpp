@@ -215,6 +215,77 @@ PyObject* py_sdpa(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// plan_step(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens, in_place)
+PyObject* py_plan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect_args(n, 8);
+  const Tensor &cached = tensor_arg(a[0], "cached_lens"), &added = tensor_arg(a[1], "new_tokens"), &table = tensor_arg(a[2], "block_table"),
+               &ring = tensor_arg(a[3], "ring"), &state = tensor_arg(a[4], "ring_state");
+  const int64_t block_size = int_arg(a[5]), num_tokens = int_arg(a[6]);
+  const bool in_place = bool_arg(a[7]);
+  const auto r = call([&] { return plan_step(cached, added, table, ring, state, block_size, num_tokens, in_place); });
+  return tuple_of({r[0], r[1], r[2], r[3], r[4]});
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_store(key, value, slots, key_cache, value_cache, key_scale, value_scale)
+PyObject* py_cache_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect_args(n, 7);
+  const Tensor &key = tensor_arg(a[0], "key"), &value = tensor_arg(a[1], "value"), &slots = tensor_arg(a[2], "slots"), &kc = tensor_arg(a[3], "key_cache"),
+               &vc = tensor_arg(a[4], "value_cache"), &ks = tensor_arg(a[5], "key_scale"), &vs = tensor_arg(a[6], "value_scale");
+  call([&] {
+    cache_store(key, value, slots, kc, vc, ks, vs);
+    return 0;
+  });
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_q, max_k, is_causal, scale)
+PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect_args(n, 12);
+  const Tensor &q = tensor_arg(a[0], "query"), &kc = tensor_arg(a[1], "key_cache"), &vc = tensor_arg(a[2], "value_cache"), &ks = tensor_arg(a[3], "key_scale"),
+               &vs = tensor_arg(a[4], "value_scale"), &table = tensor_arg(a[5], "block_table"), &lens = tensor_arg(a[6], "seq_lens");
+  const c10::optional<Tensor> cu = optional_tensor(a[7], "cu_seqlens");
+  const int64_t max_q = int_arg(a[8]);
+  c10::optional<int64_t> max_k;
+  if (a[9] != Py_None) max_k = int_arg(a[9]);
+  const bool causal = bool_arg(a[10]);
+  const c10::optional<double> scale = optional_float(a[11]);
+  auto r = call([&] { return cache_attention(q, kc, vc, ks, vs, table, lens, cu, max_q, max_k, causal, scale); });
+  return tuple_of({std::get<0>(r), std::get<1>(r)});
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary(query, key or None, positions, inv_freq, sections or None, interleaved, scaling, in_place)
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect_args(n, 8);
+  const Tensor& q = tensor_arg(a[0], "query");
+  const Tensor key = a[1] == Py_None ? Tensor() : tensor_arg(a[1], "key");
+  const Tensor &positions = tensor_arg(a[2], "positions"), &inv_freq = tensor_arg(a[3], "inv_freq");
+  std::vector<int64_t> sections;
+  if (a[4] != Py_None) {
+    THPObjectPtr seq(PySequence_Fast(a[4], "sections must be a sequence of numbers of pairs"));
+    if (!seq) throw python_error();
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(seq.get()); ++i) sections.push_back(int_arg(PySequence_Fast_GET_ITEM(seq.get(), i)));
+    if (sections.empty()) sections.push_back(-1);  // refused as every other wrong number of them
+  }
+  const bool interleaved = bool_arg(a[5]), in_place = bool_arg(a[7]);
+  const double scaling = float_arg(a[6]);
+  auto r = call([&] { return rotary(q, key, positions, inv_freq, sections, interleaved, scaling, in_place); });
+  if (std::get<1>(r).defined()) return tuple_of({std::get<0>(r), std::get<1>(r)});
+  THPObjectPtr t(PyTuple_New(2)), first(THPVariable_Wrap(std::get<0>(r)));
+  if (!t || !first) throw python_error();
+  PyTuple_SET_ITEM(t.get(), 0, first.release());
+  Py_INCREF(Py_None);
+  PyTuple_SET_ITEM(t.get(), 1, Py_None);
+  return t.release();
+  END_HANDLE_TH_ERRORS
+}
+
 // status_word(device index): the int32 tensor the kernels launched through this module report time-outs in
 PyObject* py_status_word(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -238,6 +309,10 @@ PyMethodDef g_methods[] = {
     FAST("varlen_backward", py_varlen_backward),
     FAST("flash_attention_forward", py_flash_attention_forward),
     FAST("sdpa", py_sdpa),
+    FAST("plan_step", py_plan_step),
+    FAST("cache_store", py_cache_store),
+    FAST("cache_attention", py_cache_attention),
+    FAST("rotary", py_rotary),
     FAST("status_word", py_status_word),
     {"set_status_error", py_set_status_error, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -33,8 +33,6 @@ namespace b200_glue {
 
 using at::Tensor;
 
-namespace {
-
 // Uninitialised device tensors without the dispatcher round trip of at::empty (a few hundred nanoseconds each, of calls
 // whose kernels run for a few microseconds). Where torch promises a value for uninitialised memory (deterministic algorithms),
 // the dispatcher's functions are used, which write it.
@@ -46,6 +44,8 @@ Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& lik
   if (fills_uninitialised()) return at::empty(sizes, like.options().dtype(dtype));
   return at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt);
 }
+
+namespace {
 
 // [B, H, L, D] tensor in the memory order of a [B, L, H, D] buffer, which the reference returns (attention.cpp:146-148)
 Tensor new_heads_second(int64_t B, int64_t H, int64_t L, int64_t D, const Tensor& like) {

@@ -7,6 +7,7 @@
 
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/sdpa_b200.h"
 
@@ -53,6 +54,10 @@ struct BackwardOptions {
 
 double scale_or_default(const at::Tensor& q, c10::optional<double> scale);
 
+// An uninitialised tensor, without the dispatcher where torch promises no value for its memory.
+bool fills_uninitialised();
+at::Tensor new_tensor(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& like);
+
 // One int32 per device that every call made through this glue hands to the kernels.
 at::Tensor& status_word(int device);
 
@@ -92,5 +97,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_backward_with_dropout(
 // is not one of the plain cases served here (the caller then goes through the full choice procedure of sdp_choice.py).
 at::Tensor sdpa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& attn_mask,
                 double dropout_p, bool is_causal, c10::optional<double> scale);
+
+// serving_calls.cpp: rotary positions, the 8-bit paged cache (kv_cache.py, rotary.py)
+std::vector<at::Tensor> plan_step(const at::Tensor& cached_lens, const at::Tensor& new_tokens, const at::Tensor& block_table, const at::Tensor& ring,
+                                  const at::Tensor& ring_state, int64_t block_size, int64_t num_tokens, bool in_place);
+void cache_store(const at::Tensor& key, const at::Tensor& value, const at::Tensor& slots, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                 const at::Tensor& key_scale, const at::Tensor& value_scale);
+std::tuple<at::Tensor, at::Tensor> cache_attention(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                                                   const at::Tensor& key_scale, const at::Tensor& value_scale, const at::Tensor& block_table,
+                                                   const at::Tensor& seq_lens, const c10::optional<at::Tensor>& cu_seqlens, int64_t max_seqlen_q,
+                                                   c10::optional<int64_t> max_seqlen_k, bool causal, c10::optional<double> scale);
+// (query, key) turned; the second is undefined without a key
+std::tuple<at::Tensor, at::Tensor> rotary(const at::Tensor& query, const at::Tensor& key, const at::Tensor& positions, const at::Tensor& inv_freq,
+                                          const std::vector<int64_t>& sections, bool interleaved, double scaling, bool in_place);
 
 }  // namespace b200_glue

@@ -1,4 +1,4 @@
-"""Builds and loads the torch glue (csrc/torch_glue.cpp, sdpa_autograd.cpp, py_calls.cpp -> lib/libsdpa_b200_torch.so).
+"""Builds and loads the torch glue (csrc/torch_glue.cpp, sdpa_autograd.cpp, serving_calls.cpp, py_calls.cpp -> lib/libsdpa_b200_torch.so).
 
 After ``load()``:
 * ``torch.ops.b200_sdpa._scaled_dot_product_flash_attention`` (+ ``_backward``) and
@@ -20,7 +20,7 @@ from . import _cabi, build as native_build
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
-SOURCES = ["torch_glue.cpp", "sdpa_autograd.cpp", "py_calls.cpp"]
+SOURCES = ["torch_glue.cpp", "sdpa_autograd.cpp", "serving_calls.cpp", "py_calls.cpp"]
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(_cabi.LIB_DIR, "libsdpa_b200_torch.so")
 calls = None  # the module of csrc/py_calls.cpp, once load() has run
