@@ -58,6 +58,23 @@ __device__ __forceinline__ uint32_t values_to_codes(float a, float b, float c, f
   }
 }
 
+// The same for finite values times `inv`, a power of two, that are known to be within the largest code.
+template <bool kInt8>
+__device__ __forceinline__ uint32_t values_to_codes_within(float a, float b, float c, float d, float inv) {
+  if constexpr (kInt8) {
+    // 1.5 * 2^23 + x has x, rounded, in its low bits
+    auto one = [inv](float x) { return __float_as_uint(fmaf(x, inv, 12582912.f)); };
+    return __byte_perm(__byte_perm(one(a), one(b), 0x0040), __byte_perm(one(c), one(d), 0x0040), 0x5410);
+  } else {
+    const float2 ab = mul2(make_float2(a, b), make_float2(inv, inv)), cd = mul2(make_float2(c, d), make_float2(inv, inv));
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}\n"
+        : "=r"(r)
+        : "f"(ab.x), "f"(ab.y), "f"(cd.x), "f"(cd.y));
+    return r;
+  }
+}
+
 // log2 of a block size, or -1
 inline int block_shift(int block_size) {
   for (int shift = 4; shift <= 7; ++shift)

@@ -6,14 +6,20 @@
 // dequantised element is exact in 16 bits.
 //
 // Bound by HBM for prompts (two bytes read and one written per element), by latency for decode steps. The tokens of one block stand next to each other,
-// so a run of them is found from the slots alone: it begins where a token's block is not that of the token with a place in front. A warp takes (a run, a head,
-// keys or values): the first pass over its rows gives the largest element, the second the codes.
+// so a run of them is found from the slots alone: it begins where a token's block is not that of the token with a place in front. A CTA takes a window of
+// tokens for one head of the keys or values; its first warp finds the runs that begin there. Runs of a few tokens (decode steps) are a warp's each; on a
+// longer one all warps work, each thread with its elements in registers between the largest element and the codes, so that they are read once.
+// Measured (8192 tokens of 4 prompts, 8 heads of 128, bf16 beside their queries to e4m3): 57 us with a warp for each run, which found it by itself, and
+// elements looked at one by one; 21 with a warp that finds runs for the CTA and the largest element two at a time as integers; 16.5 with a path of its own for
+// runs without gaps (3 TB/s). Asking L2 for the window's rows while the runs are found gave nothing.
 #include "cache_common.cuh"
 
 namespace sdpa_b200 {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kHeld = 8;         // rows that a thread keeps in registers
+constexpr int kMostWindow = 64;  // tokens of a window
 
 struct StoreSide {
   const uint16_t* in;
@@ -26,6 +32,7 @@ struct StoreParams {
   StoreSide side[2];  // keys, values
   const int32_t* slots;
   int tokens, heads, num_slots, shift;
+  int window;  // tokens of a CTA: 4, or a multiple of 32 up to kMostWindow
 };
 
 template <bool kF16>
@@ -34,93 +41,220 @@ __device__ __forceinline__ void to_floats(const uint4& w, float (&x)[8]) {
   x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
 }
 
+// What a thread has of a run's rows: row0, row0 + step, ... of n, eight elements of each
+struct Rows {
+  const uint16_t* in;
+  uint8_t* cache;
+  float* scale;
+  int64_t in_row, row;
+  int row0, step, n, place;
+};
+
+// Earlier tokens of the block rounded again to a scale that has grown. `down` = 1 / new scale, a power of two.
+template <bool kInt8>
+__device__ __noinline__ void round_again(const Rows& w, float old, float down) {
+  for (int r = w.row0; r < w.place; r += w.step) {
+    const uint2 codes = *reinterpret_cast<const uint2*>(w.cache + r * w.row);
+    uint32_t h[4];
+    codes_to_f16<kInt8>(codes.x, h[0], h[1]);
+    codes_to_f16<kInt8>(codes.y, h[2], h[3]);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = unpack_16x2<true>(h[e]);
+      v[2 * e] = f.x * old * down;
+      v[2 * e + 1] = f.y * old * down;
+    }
+    *reinterpret_cast<uint2*>(w.cache + r * w.row) = make_uint2(values_to_codes<kInt8>(v[0], v[1], v[2], v[3]), values_to_codes<kInt8>(v[4], v[5], v[6], v[7]));
+  }
+}
+
+__device__ __forceinline__ uint32_t larger(uint32_t top, const uint4& w) {
+  return __vmaxu2(__vmaxu2(top, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+}
+template <uint32_t kInf>
+__device__ __forceinline__ uint32_t larger_finite(uint32_t top, const uint4& w) {
+  const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = words[i] & 0x7fffu, hi = words[i] >> 16 & 0x7fffu;
+    top = max(top, max(lo < kInf ? lo : 0u, hi < kInf ? hi : 0u));
+  }
+  return top;
+}
+
+// Tokens [first, first + count) of the call, one block's; `rows`: their places are place, place + 1, ..., none left out
+struct Run {
+  int first, count, block, place;
+  bool rows;
+};
+
 template <int kD, bool kInt8, bool kF16>
-__global__ void __launch_bounds__(kWarps * 32) store_kernel(const StoreParams p) {
-  constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // lanes per row, rows per step of the warp
-  const int lane = threadIdx.x & 31, sub = lane / kLanes, at = lane % kLanes * 8;
-  const int t0 = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int head = blockIdx.y >> 1;
-  if (t0 >= p.tokens) return;
+__global__ void __launch_bounds__(kWarps * 32, 6) store_kernel(const StoreParams p) {
+  constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // lanes per row, rows per step of a warp
+  __shared__ Run runs[kMostWindow];
+  __shared__ int num_runs;
+  __shared__ uint32_t warp_top[2][kWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / kLanes, at = lane % kLanes * 8;
+  const int mask = (1 << p.shift) - 1;
+  // the heads of a window stand next to each other: together they read whole tokens
+  const int unit = blockIdx.x % (2 * p.heads), head = unit >> 1, own0 = static_cast<int>(blockIdx.x / (2 * p.heads)) * p.window;
+  const StoreSide& x = p.side[unit & 1];
   auto block_of = [&](int t) {
-    const int slot = p.slots[t];
+    const int slot = t < p.tokens ? p.slots[t] : -1;
     return slot < 0 || slot >= p.num_slots ? -1 : slot >> p.shift;
   };
-  const int block = block_of(t0);
-  if (block < 0) return;
-  // first of its run? The nearest token in front that has a place, within 32
-  const int front = lane < t0 ? block_of(t0 - 1 - lane) : -1;
-  const unsigned placed = __ballot_sync(0xffffffffu, front >= 0), mine = __ballot_sync(0xffffffffu, front == block);
-  if ((placed & -placed & mine) != 0) return;
-  int n = 1;  // tokens of the run, and of those left out in between
-  for (;;) {
-    const int b = t0 + n + lane < p.tokens ? block_of(t0 + n + lane) : -1;
-    const unsigned same = __ballot_sync(0xffffffffu, b == block), other = __ballot_sync(0xffffffffu, b >= 0 && b != block);
-    const unsigned run = same & (other == 0 ? ~0u : (other & -other) - 1);  // in front of the first token of another block
-    if (run != 0) n += 32 - __clz(run);
-    if (run == 0 || other != 0) break;
-  }
-  const StoreSide& x = p.side[blockIdx.y & 1];
-  const uint16_t* in = x.in + t0 * x.in_row + head * x.in_head + at;
-  uint8_t* cache = x.cache + block * x.block + head * x.head + at;
-  const int mask = (1 << p.shift) - 1, place = p.slots[t0] & mask;
 
-  // ---- the largest finite element
-  float largest = 0.f;
-  bool broken = false;
-  for (int r = sub; r < n; r += kRows) {
-    if (block_of(t0 + r) < 0) continue;
-    float v[8];
-    to_floats<kF16>(*reinterpret_cast<const uint4*>(in + r * x.in_row), v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(v[e]);
-      if (a < INFINITY) largest = fmaxf(largest, a);
-      else broken = true;
-    }
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, d));
-  broken = __any_sync(0xffffffffu, broken);
-  float* scale = x.scale + static_cast<int64_t>(block) * p.heads + head;
-  const float need = scale_for<kInt8>(largest);
-  float now = need;
-  if (place > 0) {
-    const float old = *scale;
-    now = old >= need || isnan(old) ? old : need;
-    if (now != old && !isnan(old)) {
-      // ---- the scale has grown: earlier tokens are rounded again
-      const float down = 1.f / now;  // a power of two: exact
-      for (int r = sub; r < place; r += kRows) {
-        const uint2 codes = *reinterpret_cast<const uint2*>(cache + r * x.row);
-        uint32_t h[4];
-        codes_to_f16<kInt8>(codes.x, h[0], h[1]);
-        codes_to_f16<kInt8>(codes.y, h[2], h[3]);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack_16x2<true>(h[e]);
-          v[2 * e] = f.x * old * down;
-          v[2 * e + 1] = f.y * old * down;
+  if (warp == 0) {
+    // whether a token stands right behind the one in front of it
+    auto follows = [&](int t) { return t < p.tokens && t > 0 && p.slots[t] == p.slots[t - 1] + 1; };
+    // ---- the runs that begin in the window: where the nearest token with a place in front, within 32, is in another block
+    int found = 0;
+    int front = lane < own0 ? block_of(own0 - 1 - lane) : -1;
+    unsigned front_placed = __ballot_sync(0xffffffffu, front >= 0);
+    int last = front_placed ? own0 - __ffs(front_placed) : -64;  // the nearest token with a place, and its block
+    int last_block = __shfl_sync(0xffffffffu, front, front_placed ? __ffs(front_placed) - 1 : 0);
+    const int end = own0 + p.window;
+    int tail = block_of(end + lane), tail2 = block_of(end + 32 + lane);  // asked for early: the last run often goes on there
+    int next = own0 + lane < own0 + p.window || p.window >= 32 ? block_of(own0 + lane) : -1;
+    for (int base = own0; base < own0 + p.window; base += 32) {
+      const int b = lane < p.window ? next : -1;
+      next = base + 32 < own0 + p.window ? block_of(base + 32 + lane) : -1;
+      const unsigned placed = __ballot_sync(0xffffffffu, b >= 0), below = placed & ((1u << lane) - 1);
+      const int from_lane = __shfl_sync(0xffffffffu, b, below ? 31 - __clz(below) : 0);
+      const int before = below ? from_lane : base + lane - last <= 32 ? last_block : -1;
+      const bool begins = b >= 0 && b != before;
+      const unsigned firsts = __ballot_sync(0xffffffffu, begins), parted = ~__ballot_sync(0xffffffffu, follows(base + lane));
+      // a run that has begun ends with the last token in front of the next one
+      if (placed != 0) {
+        const unsigned of_last = firsts ? placed & ((firsts & -firsts) - 1) : placed;
+        if (found > 0 && of_last != 0 && lane == 0) {
+          runs[found - 1].count = base + 32 - __clz(of_last) - runs[found - 1].first;
+          runs[found - 1].rows = runs[found - 1].rows && (parted << __clz(of_last)) == 0;
         }
-        *reinterpret_cast<uint2*>(cache + r * x.row) = make_uint2(values_to_codes<kInt8>(v[0], v[1], v[2], v[3]), values_to_codes<kInt8>(v[4], v[5], v[6], v[7]));
+      }
+      if (begins) {
+        const unsigned behind = firsts & ~((2u << lane) - 1);
+        const unsigned mine = placed & ~((1u << lane) - 1) & (behind ? (behind & -behind) - 1 : ~0u);
+        const int n = 32 - __clz(mine) - lane;
+        // bits lane + 1 to lane + n - 1
+        const unsigned inside = (n >= 32 ? ~0u : (1u << n) - 1) << lane & ~(1u << lane);
+        runs[found + __popc(firsts & ((1u << lane) - 1))] = {base + lane, n, b, p.slots[base + lane] & mask, (parted & inside) == 0};
+      }
+      __syncwarp();
+      found += __popc(firsts);
+      if (placed != 0) {
+        last = base + 31 - __clz(placed);
+        last_block = __shfl_sync(0xffffffffu, b, 31 - __clz(placed));
       }
     }
+    // the last one may go on behind the window
+    if (found > 0) {
+      Run run = runs[found - 1];
+      for (int base = end;; base += 32) {
+        const int b = tail;
+        tail = tail2;
+        const unsigned same = __ballot_sync(0xffffffffu, b == run.block), other = __ballot_sync(0xffffffffu, b >= 0 && b != run.block);
+        const unsigned more = same & (other == 0 ? ~0u : (other & -other) - 1);  // in front of the first token of another block
+        if (more == 0 || base + __ffs(more) - (run.first + run.count) > 32) break;
+        run.rows = run.rows && (~__ballot_sync(0xffffffffu, follows(base + lane)) << __clz(more)) == 0;
+        run.count = base + 32 - __clz(more) - run.first;
+        if (other != 0) break;
+        tail2 = block_of(base + 64 + lane);
+      }
+      __syncwarp();
+      if (lane == 0) runs[found - 1] = run;
+    }
+    if (lane == 0) num_runs = found;
   }
-  if (kInt8 && broken) now = __int_as_float(0x7fffffff);
-  __syncwarp();  // every lane has read the old scale
-  if (lane == 0) *scale = now;
+  __syncthreads();
 
-  // ---- codes
-  const bool exact = (__float_as_uint(now) & 0x7fffffu) == 0;  // a power of two: multiplying by the reciprocal is dividing
-  const float inv = 1.f / now;
-  for (int r = sub; r < n; r += kRows) {
-    const int slot = p.slots[t0 + r];
-    if (slot < 0 || slot >= p.num_slots || (r + 1 < n && p.slots[t0 + r + 1] == slot)) continue;  // the next token has the same place: that one stays
-    float v[8];
-    to_floats<kF16>(*reinterpret_cast<const uint4*>(in + r * x.in_row), v);
+  const int count = num_runs;
+  int shared_runs = 0;
+  for (int turn = 0; turn < count; ++turn) {
+    const int t0 = runs[turn].first, n = runs[turn].count, block = runs[turn].block, place = runs[turn].place;
+    const bool alone = n <= kRows * kHeld;
+    if (alone && turn % kWarps != warp) continue;
+    const Rows w = {x.in + t0 * x.in_row + head * x.in_head + at, x.cache + block * x.block + head * x.head + at,
+                    x.scale + static_cast<int64_t>(block) * p.heads + head, x.in_row, x.row, alone ? sub : warp * kRows + sub, alone ? kRows : kWarps * kRows, n, place};
+    const float old = place > 0 ? *w.scale : 0.f;
+    // The largest of `top` over the run's warps. One barrier for each is enough, with words that change with every call; also: every warp has read the old scale
+    auto over_warps = [&](uint32_t top) {
+      top = __reduce_max_sync(0xffffffffu, __vmaxu2(top, top >> 16) & 0xffffu);
+      if (alone) {
+        __syncwarp();
+        return top;
+      }
+      const int buf = shared_runs++ & 1;
+      if (lane == 0) warp_top[buf][warp] = top;
+      __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = exact ? v[e] * inv : __fdiv_rn(v[e], now);
-    *reinterpret_cast<uint2*>(cache + (slot & mask) * x.row) = make_uint2(values_to_codes<kInt8>(v[0], v[1], v[2], v[3]), values_to_codes<kInt8>(v[4], v[5], v[6], v[7]));
+      for (int i = 0; i < kWarps; ++i) top = max(top, warp_top[buf][i]);
+      return top;
+    };
+    auto new_scale = [&](uint32_t top, bool broken) {
+      const float need = scale_for<kInt8>(unpack_16x2<kF16>(top).x);
+      float now = place > 0 && (old >= need || isnan(old)) ? old : need;
+      if (place > 0 && now != old && !isnan(old)) round_again<kInt8>(w, old, 1.f / now);
+      if (kInt8 && broken) now = __int_as_float(0x7fffffff);
+      if (lane == 0 && (alone || warp == 0)) *w.scale = now;
+      return now;
+    };
+
+    // ---- 16-bit floats without their signs are ordered as integers, infinity and NaN behind all numbers: two at a time
+    constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
+    uint4 held[kHeld];
+    uint32_t top = 0u;
+    const bool fits = runs[turn].rows && n <= kHeld * w.step;
+    if (fits) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int r = w.row0 + i * w.step;
+        held[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < n) held[i] = *reinterpret_cast<const uint4*>(w.in + r * w.in_row);
+      }
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) top = larger(top, held[i]);
+    } else {
+      for (int r = w.row0; r < n; r += w.step)
+        if (block_of(t0 + r) >= 0) top = larger(top, *reinterpret_cast<const uint4*>(w.in + r * w.in_row));
+    }
+    top = over_warps(top);
+    const bool broken = top >= kInf;  // the same in all warps of the run
+    if (broken) {  // the largest finite one
+      top = 0u;
+      for (int r = w.row0; r < n; r += w.step)
+        if (block_of(t0 + r) >= 0) top = larger_finite<kInf>(top, *reinterpret_cast<const uint4*>(w.in + r * w.in_row));
+      top = over_warps(top);
+    }
+    const float now = new_scale(top, broken);
+
+    // ---- codes. All elements are within the largest code where none is infinite or NaN; with a scale that is a power of two, multiplying by the
+    // reciprocal is dividing. Elsewhere each element is looked at.
+    if (fits && !broken && (__float_as_uint(now) & 0x7fffffu) == 0) {
+      const float inv = 1.f / now;
+      uint8_t* to = w.cache + place * w.row;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int r = w.row0 + i * w.step;
+        if (r >= n) continue;
+        float v[8];
+        to_floats<kF16>(held[i], v);
+        *reinterpret_cast<uint2*>(to + r * w.row) =
+            make_uint2(values_to_codes_within<kInt8>(v[0], v[1], v[2], v[3], inv), values_to_codes_within<kInt8>(v[4], v[5], v[6], v[7], inv));
+      }
+    } else {
+      for (int r = w.row0; r < n; r += w.step) {
+        const int slot = p.slots[t0 + r];
+        // the same slot again with the next token: the later stays
+        if (block_of(t0 + r) < 0 || (r + 1 < n && p.slots[t0 + r + 1] == slot)) continue;
+        float v[8];
+        to_floats<kF16>(*reinterpret_cast<const uint4*>(w.in + r * w.in_row), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __fdiv_rn(v[e], now);
+        *reinterpret_cast<uint2*>(w.cache + (slot & mask) * w.row) = make_uint2(values_to_codes<kInt8>(v[0], v[1], v[2], v[3]), values_to_codes<kInt8>(v[4], v[5], v[6], v[7]));
+      }
+    }
   }
 }
 
@@ -171,7 +305,15 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params*
   s.heads = p->heads_kv;
   s.shift = block_shift(p->block_size);
   s.num_slots = p->num_blocks << s.shift;
-  const dim3 grid((p->num_tokens + kWarps - 1) / kWarps, 2 * p->heads_kv);
+  // few tokens: a warp for each, whatever the runs are; many: windows that begin one or two runs of a block
+  const int64_t units = 2 * static_cast<int64_t>(p->heads_kv);
+  s.window = p->num_tokens * units <= 148 * 64 ? kWarps : p->block_size >= 64 ? 64 : 32;
+  const int64_t ctas = (p->num_tokens + s.window - 1) / s.window * units;
+  if (ctas > INT32_MAX) {
+    set_error("cache_store: too many tokens (%d) for %d heads", p->num_tokens, p->heads_kv);
+    return SDPA_B200_INVALID_ARG;
+  }
+  const unsigned grid = static_cast<unsigned>(ctas);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const bool f16 = p->dtype == SDPA_B200_F16;
   auto launch = [&](auto dim, auto int8) {
