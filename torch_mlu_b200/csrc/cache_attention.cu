@@ -5,15 +5,20 @@
 // over the cached tokens j of the request, j <= i + len - rows of q where causal. Two paths:
 //
 // 1. Few rows per request (decode steps, drafted tokens): cache_stream_kernel, bound by the codes that come out of HBM. A unit is (request,
-//    kv head, chunk of up to 16 rows (query token, query head of the group)): the rows ride in the M dimension of mma.sync.m16n8k16, so that codes are
-//    read once for all of them. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 tokens,
+//    kv head, chunk of up to 64 rows (query token, query head of the group)), whose codes are read once for all its rows: S^T = K Q^T and O^T = V^T W^T in
+//    mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 tokens,
 //    so that all SMs stream the same number of bytes however long each request is. A unit that several CTAs worked on leaves fp32 parts in the workspace,
 //    at most two per CTA, and a second kernel merges them.
+//    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a copy takes its warp about
+//    100 cycles, which one warp with 16 of them per tile of 16 KB - blocks of 16 tokens, head_dim 64 - could not keep up with); four do the arithmetic, as 1, 2 or 4 groups of 8 or 16
+//    rows by 4, 2 or 1 parts of a tile's tokens.
 //    Codes become f16, exactly. Q rows are brought to f16 by a power of two each (their largest element to 2^14..2^15: a bf16 element loses
-//    only what is 2^-39 of the row's largest), P is f16 in [0, 2^15], whose smaller weights keep all 11 bits down to 2^-29 of the largest; the scales of blocks
-//    go onto the fp32 scores and products. Sums are fp32.
+//    only what is 2^-39 of the row's largest). The scale of K goes onto the fp32 scores; that of V into the exponent, so that the weights w_j = 2^(s_j + log2 vs_j - m) with
+//    m their running maximum are f16 numbers of up to 2^15 which keep all 11 bits down to 2^-29 of the largest, whatever scales blocks have, and the products add up in the
+//    tensor core's fp32 accumulators without a pass over them. The sum of the softmax takes w_j / vs_j in fp32.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors in the
 //    workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest.
+#include <algorithm>
 #include <type_traits>
 
 #include "cache_common.cuh"
@@ -21,13 +26,15 @@
 namespace sdpa_b200 {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kStepTokens = 32;                   // tokens a warp handles per step
-constexpr int kTileTokens = kWarps * kStepTokens;  // 128
+constexpr int kWarps = 4;                  // those that do the arithmetic
+constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are dealt out as for six warps anyway
+constexpr int kStepTokens = 32;            // tokens a warp handles at a time
+constexpr int kTileTokens = 128;
+constexpr int kSlots = kTileTokens / 16;   // the fewest tokens with scales of their own are 16
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
-constexpr int kRows = 16;     // most rows of a unit
+constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
+constexpr float kSumUnit = 0x1p-40f;       // sums are kept in this unit, so that those over blocks of the least scale stay in range
 
 struct StreamParams {
   const uint16_t* q;
@@ -43,13 +50,14 @@ struct StreamParams {
   struct SharedUnit* shared_units;  // one per CTA
   uint32_t* status;
   int64_t q_row, q_head, o_row, o_head, table_stride;
-  int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, grid, causal, f16;
+  int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
+  int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
   float scale_log2;
 };
 
 // The unit that begins in a CTA's share and ends in a later one's: what the merge kernel needs to know. `last` < 0: there is none.
 struct SharedUnit {
-  int request, unit, last, slot;
+  int last, slot, head, row0, rows, q0;  // the CTA that ends it; where the first CTA's part is; kv head, rows [row0, row0 + rows) of the request whose tokens begin at q0
 };
 
 // A request as units see it
@@ -61,437 +69,541 @@ struct Request {
 __device__ __forceinline__ Request request_at(const StreamParams& p, int b) {
   Request r;
   r.index = b;
-  r.len = max(p.seq_lens[b], 0);
+  r.len = min(max(p.seq_lens[b], 0), p.max_len);
   r.q0 = p.cu_q ? p.cu_q[b] : b;
   r.rows_q = p.cu_q ? max(p.cu_q[b + 1] - r.q0, 0) : 1;
   if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
   r.tiles = max((r.len + kTileTokens - 1) / kTileTokens, 1);  // an empty request has rows to write too
-  r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) / p.rows);
+  r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
   return r;
 }
 
-// Stages of each warp's ring: what lets two CTAs share an SM's 228 KB.
-template <bool kHi, int kD>
-__host__ __device__ constexpr int ring_stages() { return (kHi ? 2 : 3) * (128 / kD); }
+// Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB.
 template <int kD>
-__host__ __device__ constexpr uint32_t stage_bytes() { return 2u * kStepTokens * kD; }
-template <bool kHi, int kD>
-__host__ __device__ constexpr int merge_floats() { return ((kHi ? 4 : 2) * (kD / 8) + (kHi ? 4 : 2)) * 32; }
-template <bool kHi, int kD>
+__host__ __device__ constexpr int ring_stages() { return 3 * (128 / kD); }
+template <int kD>
+__host__ __device__ constexpr uint32_t stage_bytes() { return 2u * kTileTokens * kD; }
+template <int kD>
 __host__ __device__ constexpr uint32_t stream_smem_bytes() {
-  constexpr int kSt = ring_stages<kHi, kD>();
-  return 1024 + kWarps * kSt * stage_bytes<kD>() + (kWarps - 1) * merge_floats<kHi, kD>() * 4 + kWarps * kSt * (8 + 16) + 16;
+  return 1024 + ring_stages<kD>() * (stage_bytes<kD>() + kSlots * 16 + 16) + 16 + kWarps * 16 * 8;
 }
 
-// kHi: a unit has more than 8 rows, so fragment rows 8-15 are in use too.
-template <bool kHi, int kD, bool kInt8>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
-cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
-  constexpr int kKSteps = kD / 16;
-  constexpr int kNBlocks = kD / 8;
-  constexpr int kSt = ring_stages<kHi, kD>();
-  constexpr uint32_t kStageBytes = stage_bytes<kD>();
-  constexpr int kMergeFloats = merge_floats<kHi, kD>();
-  constexpr float kBias = 15.f;  // P is kept as 2^15 * weight: the largest is 2^15, the smallest normal one 2^-29 of it
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ int64_t warp_tiles[kWarps];
-  __shared__ int64_t start_before;
-  __shared__ int start_request;
-  const uint32_t raw_addr = smem_u32(smem_raw);
-  const uint32_t base = (raw_addr + 1023u) & ~1023u;
-  float* merge = reinterpret_cast<float*>(smem_raw + (base - raw_addr) + kWarps * kSt * kStageBytes);
-  float4* stage_scales = reinterpret_cast<float4*>(merge + (kWarps - 1) * kMergeFloats);  // (ks, vs) of the two halves of a step
-  const uint32_t bars = smem_u32(stage_scales + kWarps * kSt);
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(stage_scales + kWarps * kSt) + kWarps * kSt);
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// barrier over the warps that do the arithmetic
+__device__ __forceinline__ void arithmetic_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  const int g = lane >> 2;  // fragment row / token within a block of 8
-  const int t = lane & 3;
-  const uint32_t ring = base + warp * (kSt * kStageBytes);
-  const uint32_t bar = bars + warp * (kSt * 8);
-  float4* scales = stage_scales + warp * kSt;
+// One 8 x 8 matrix of 16-bit elements: row g, columns 2t and 2t + 1 in, row 2t and 2t + 1, column g out
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// over the eight lanes that share t = lane % 4
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+  for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+  return x;
+}
+__device__ __forceinline__ float column_sum(float x) {
+#pragma unroll
+  for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kWarps * kSt; ++i) mbar_init(bars + 8 * i, 1);
-    *abort_flag = 0;
-    start_request = -1;
-    fence_mbar_init();
+// A CTA's share of the list of all tiles, [first, last), and the request that it begins in. Equal shares, the first of them one tile longer where they do not come out even.
+struct Share {
+  int first, last, request, before;  // before: tiles in front of the request's
+  int each, longer, ctas;            // tiles of a share, how many shares have one more, how many there are
+  __device__ __forceinline__ int cta_of(int tile) const {
+    const int in_longer = longer * (each + 1);
+    return tile < in_longer ? tile / (each + 1) : longer + (tile - in_longer) / each;
   }
-  if (elect_one()) {
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-  }
-  wait_for_previous_grid();
-  if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
-  __syncthreads();
+};
 
-  // ---- this CTA's share of the list of all tiles: sum over the requests, then the request that the share begins in
+// Every warp finds it for itself, so that none waits for another.
+__device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int lane) {
   auto tiles_of = [&](int b) -> int64_t {
     if (b >= p.batch) return 0;
     const Request r = request_at(p, b);
     return static_cast<int64_t>(r.tiles) * r.units;
   };
   int64_t total = 0;
-  for (int b = threadIdx.x; b < p.batch; b += kThreads) total += tiles_of(b);
+#pragma unroll 4
+  for (int b = lane; b < p.batch; b += 32) total += tiles_of(b);
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
-  if (lane == 0) warp_tiles[warp] = total;
-  __syncthreads();
-  total = warp_tiles[0] + warp_tiles[1] + warp_tiles[2] + warp_tiles[3];
-  const int64_t ctas = min(total, static_cast<int64_t>(p.grid));  // those that get a tile: the others would leave no part where the merge looks for one
-  const int64_t index = min(static_cast<int64_t>(blockIdx.x), ctas), end_index = min(index + 1, ctas);
-  const int64_t first = ctas ? index * total / ctas : 0, last = ctas ? end_index * total / ctas : 0;
-  if (first < last) {
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-      const int64_t mine = tiles_of(b0 + threadIdx.x);
-      int64_t run = mine;
+  Share s = {0, 0, 0, 0, 0, 0, 0};
+  if (total <= 0 || total > INT32_MAX) return s;  // (2^31 tiles: offsets that are none)
+  const int tiles = static_cast<int>(total);
+  s.ctas = min(tiles, p.grid);  // those that get a tile: the others would leave no part where the merge looks for one
+  s.each = tiles / s.ctas;
+  s.longer = tiles - s.each * s.ctas;
+  if (cta >= s.ctas) return s;
+  s.first = cta * s.each + min(cta, s.longer);
+  s.last = s.first + s.each + (cta < s.longer ? 1 : 0);
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int mine = static_cast<int>(tiles_of(b0 + lane));
+    int run = mine;
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += x;
-      }
-      __syncthreads();
-      if (lane == 31) warp_tiles[warp] = run;
-      __syncthreads();
-      int64_t at = before;
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) at += warp_tiles[w];
-        before += warp_tiles[w];
-      }
-      at += run - mine;
-      if (first >= at && first < at + mine) {
-        start_request = b0 + threadIdx.x;
-        start_before = at;
-      }
-      if (first < before) break;
+    for (int d = 1; d < 32; d *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, run, d);
+      if (lane >= d) run += x;
     }
-    __syncthreads();
+    const unsigned behind = __ballot_sync(0xffffffffu, s.first < s.before + run);
+    if (behind != 0) {
+      const int at = __ffs(behind) - 1;
+      s.request = b0 + at;
+      s.before += __shfl_sync(0xffffffffu, run - mine, at);
+      break;
+    }
+    s.before += __shfl_sync(0xffffffffu, run, 31);
   }
-  const int64_t n_tiles = last - first;
-  SharedUnit left = {0, 0, -1, 0};
-  if (n_tiles > 0 && start_request >= 0) {
-    // ---- the load side of the warp's ring: its own request, unit and tile, kSt steps ahead of the arithmetic
-    Request ld = request_at(p, start_request);
-    int ld_unit = static_cast<int>((first - start_before) / ld.tiles);
-    int ld_tile = static_cast<int>((first - start_before) % ld.tiles);
-    int64_t ld_left = n_tiles;  // tiles of the share that have not been looked at
-    int ld_step = 0;            // stages filled
-    int group_of = -1, group_unit = -1, group_request = -1;
-    int g_id = -1;  // lane i: page 32 * group_of + i of ld, its block and scales
-    float g_ks = 0.f, g_vs = 0.f;
-    auto next_unit = [&](Request& r, int& unit) {
-      if (++unit < r.units) return;
-      unit = 0;
-      int b = r.index + 1;
-      do r = request_at(p, b++);
-      while (r.units == 0);  // more tiles are left, so there is one
+  return s;
+}
+
+// kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
+template <int kRowBlocks, int kRowWarps, int kD, bool kInt8>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
+  constexpr int kChunks = kD / 16;                           // 16 dimensions each
+  constexpr int kSt = ring_stages<kD>();
+  constexpr uint32_t kStageBytes = stage_bytes<kD>();
+  constexpr int kParts = kWarps / kRowWarps;                 // of a tile's tokens
+  constexpr int kPartTokens = kTileTokens / kParts;
+  constexpr int kRowsOfWarp = 8 * kRowBlocks;
+  constexpr float kBias = 15.f;  // weights are kept times 2^15: the largest is 2^15, the smallest normal f16 number 2^-29 of it
+  constexpr int kState = kChunks * kRowBlocks * 4 * 32;      // floats of a warp's accumulators
+  static_assert(kWarps * kState * 4 <= kStageBytes || kParts == 1, "the warps' states do not fit a tile's place");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t ring = (raw_addr + 1023u) & ~1023u;
+  uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
+  float4* slot_scales = reinterpret_cast<float4*>(ring_ptr + kSt * kStageBytes);  // [stage][16 tokens]: of K, log2 of that of V, kSumUnit over that of V
+  float2* row_state = reinterpret_cast<float2*>(slot_scales + kSt * kSlots);      // [warp][row]: maximum and sum
+  const uint32_t full = smem_u32(row_state + kWarps * 16), empty = full + 8 * kSt;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(row_state + kWarps * 16) + 2 * kSt);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(full + 8 * i, 2);
+      mbar_init(empty + 8 * i, kWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp >= kWarps && elect_one()) tma_prefetch_desc(warp == kWarps ? &tm_k : &tm_v);
+  __syncthreads();
+  wait_for_previous_grid();
+  if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
+  const Share share = share_of(p, blockIdx.x, lane);
+  const int n_tiles = share.last - share.first;
+  // the next unit's request, or one without units behind the last
+  auto next_unit = [&](Request& r, int& unit) {
+    if (++unit < r.units) return;
+    unit = 0;
+    int b = r.index + 1;
+    do {
+      if (b >= p.batch) {
+        r = {b, 0, 0, 0, 1, 0};
+        return;
+      }
+      r = request_at(p, b++);
+    } while (r.units == 0);
+  };
+
+  if (n_tiles > 0 && warp >= kWarps) {
+    // ================================================================ the loading warps, one for K and one for V
+    // Lane i has page 32 * group + i of a unit: block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page) and scale. Three
+    // groups are under way: the one that tiles are copied from, the next with its scales, and the block numbers of the one behind.
+    const bool keys = warp == kWarps;
+    const CUtensorMap* map = keys ? &tm_k : &tm_v;
+    const float* scales = keys ? p.k_scale : p.v_scale;
+    struct Place {
+      Request r;
+      int unit, group, head;
     };
-    // fills the next stage, if the share has a step of this warp left
-    auto load_next = [&]() {
-      while (ld_left > 0) {
-        const int tok = ld_tile * kTileTokens + warp * kStepTokens;
-        const bool have = tok < ld.len;
-        if (have) {
-          const int page = tok >> p.shift, grp = page >> 5;
-          if (grp != group_of || ld_unit != group_unit || ld.index != group_request) {
-            group_of = grp;
-            group_unit = ld_unit;
-            group_request = ld.index;
-            const int mine = grp * 32 + lane;
-            g_id = -1;
-            g_ks = g_vs = 0.f;
-            if ((static_cast<int64_t>(mine) << p.shift) < ld.len) {
-              if (mine < p.max_blocks) g_id = p.block_table[ld.index * p.table_stride + mine];
-              if (g_id >= 0 && g_id < p.num_blocks) {
-                const int64_t at = static_cast<int64_t>(g_id) * p.heads_kv + ld_unit % p.heads_kv;
-                g_ks = p.k_scale[at];
-                g_vs = p.v_scale[at];
-              } else {
-                g_id = p.num_blocks;  // behind the cache: the copy brings zeros, the scale makes the scores of those who see them NaN
-                g_ks = __int_as_float(0x7fffffff);
-              }
-            }
-          }
-          const bool halves = p.shift == 4;  // two blocks per step
-          const int src = page & 31, src2 = halves ? (src + 1) & 31 : src;  // a step begins at an even page
-          const int id0 = __shfl_sync(0xffffffffu, g_id, src), id1 = __shfl_sync(0xffffffffu, g_id, src2);
-          const float4 sc = make_float4(__shfl_sync(0xffffffffu, g_ks, src), __shfl_sync(0xffffffffu, g_vs, src),
-                                        __shfl_sync(0xffffffffu, g_ks, src2), __shfl_sync(0xffffffffu, g_vs, src2));
-          const uint32_t st = ld_step % kSt;
-          const uint32_t k_dst = ring + st * kStageBytes, v_dst = k_dst + kStepTokens * kD, full = bar + 8 * st;
-          if (elect_one()) {
-            scales[st] = sc;
-            mbar_arrive_expect_tx(full, kStageBytes);
-            const int head = ld_unit % p.heads_kv;
-            if (halves) {
-              const int other = id1 < 0 ? p.num_blocks : id1;  // no such page: zeros
-              tma_load_4d(k_dst, &tm_k, full, 0, 0, head, id0);
-              tma_load_4d(k_dst + 16 * kD, &tm_k, full, 0, 0, head, other);
-              tma_load_4d(v_dst, &tm_v, full, 0, 0, head, id0);
-              tma_load_4d(v_dst + 16 * kD, &tm_v, full, 0, 0, head, other);
-            } else {
-              const int row = tok & ((1 << p.shift) - 1);
-              tma_load_4d(k_dst, &tm_k, full, 0, row, head, id0);
-              tma_load_4d(v_dst, &tm_v, full, 0, row, head, id0);
-            }
-          }
-          ++ld_step;
-        }
-        --ld_left;
-        if (++ld_tile == ld.tiles) {
-          ld_tile = 0;
-          if (ld_left > 0) next_unit(ld, ld_unit);
-        }
-        if (have) return;
+    auto advance = [&](Place& x) {
+      if (static_cast<int64_t>((x.group + 1) * 32) << p.shift < x.r.len) {
+        ++x.group;
+      } else {
+        x.group = 0;
+        if (x.r.units > 0) next_unit(x.r, x.unit);
+        x.head = x.unit % p.heads_kv;
       }
     };
-    for (int i = 0; i < kSt; ++i) load_next();
+    auto block_at = [&](const Place& x) {
+      const int page = x.group * 32 + lane;
+      if ((static_cast<int64_t>(page) << p.shift) >= x.r.len) return -1;
+      const int id = page < p.max_blocks ? p.block_table[x.r.index * p.table_stride + page] : -1;
+      return id >= 0 && id < p.num_blocks ? id : p.num_blocks;
+    };
+    auto scale_at = [&](const Place& x, int id) {
+      if (id >= 0 && id < p.num_blocks) return scales[static_cast<int64_t>(id) * p.heads_kv + x.head];
+      return keys && id == p.num_blocks ? __int_as_float(0x7fffffff) : 0.f;  // none in the cache: the scores of those who see it are NaN
+    };
+    Place cur, nxt, far;
+    cur.r = request_at(p, share.request);
+    cur.unit = (share.first - share.before) / cur.r.tiles;
+    cur.head = cur.unit % p.heads_kv;
+    int tile = (share.first - share.before) - cur.unit * cur.r.tiles;
+    cur.group = ((tile * kTileTokens) >> p.shift) >> 5;
+    nxt = far = cur;
+    int id = block_at(cur), next_id = -1, far_id = -1;
+    float scale = scale_at(cur, id), next_scale = 0.f;
+    auto next_group = [&]() {
+      cur = nxt, id = next_id, scale = next_scale;
+      nxt = far, next_id = far_id;
+      next_scale = scale_at(nxt, next_id);
+      advance(far);
+      far_id = block_at(far);
+    };
+    const int pages = kTileTokens >> p.shift;  // of a tile
+    bool ok = true;
+    int step = 0;
+    for (int done = 0; done < n_tiles; ++done) {
+      const int page0 = (tile * kTileTokens) >> p.shift;
+      if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
+      const bool tokens = tile * kTileTokens < cur.r.len;
+      const uint32_t st = step % kSt, bar = full + 8 * st;
+      if (tokens) {
+        const uint32_t dst = ring + st * kStageBytes + (keys ? 0u : kTileTokens * kD);
+        if (ok && step >= kSt) ok = mbar_wait(empty + 8 * st, (step / kSt + 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int mine = __shfl_sync(0xffffffffu, id, ((page0 & 31) + lane) & 31);
+        const int n = __popc(__ballot_sync(0xffffffffu, lane < pages && mine >= 0));
+        if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(n << p.shift) * kD);
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+          const int block = __shfl_sync(0xffffffffu, mine, i);
+          if (elect_one()) tma_load_4d(dst + (i << p.shift) * kD, map, bar, 0, 0, cur.head, block);
+        }
+      }
+      if (done == 0) {  // the first copies are under way
+        advance(nxt);
+        next_id = block_at(nxt);
+        far = nxt;
+        advance(far);
+        far_id = block_at(far);
+      }
+      if (tokens) {
+        const int src = (page0 & 31) + ((lane % kSlots) * 16 >> p.shift);
+        const float own = __shfl_sync(0xffffffffu, scale, src);
+        float* slot = reinterpret_cast<float*>(slot_scales + st * kSlots + lane);
+        if (lane < kSlots) {
+          if (keys) {
+            slot[0] = own;
+          } else {
+            const float used = isnan(own) ? own : fmaxf(own, kLeastScale);
+            slot[1] = log2f(used);
+            slot[2] = kSumUnit / used;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        ++step;
+      }
+      if (done == 0) next_scale = scale_at(nxt, next_id);
+      if (++tile == cur.r.tiles) {
+        tile = 0;
+        next_group();
+      }
+    }
+  }
 
+  SharedUnit left = {-1, 0, 0, 0, 0, 0};
+  if (n_tiles > 0 && warp < kWarps) {
+    // ================================================================ the arithmetic. Fragments: a thread has rows 2t and 2t + 1 of every 8
+    const int g = lane >> 2;
+    const int t = lane & 3;
+    const int row_group = warp / kParts, part = warp % kParts;
     const int mrow = lane & 7, mat = lane >> 3;
-    auto chunk_at = [&](int row, int chunk) -> uint32_t {  // byte offset of a 16-byte chunk of a row in a swizzled stage
+    auto chunk_at = [&](int row, int chunk) -> uint32_t {  // byte offset of a 16-byte chunk of a row in a swizzled tile
       if constexpr (kD == 128) return row * 128 + ((chunk ^ (row & 7)) << 4);
       return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
     };
     bool ok = true;
-    int step = 0;  // stages read
-    Request r = request_at(p, start_request);
-    int unit = static_cast<int>((first - start_before) / r.tiles);
-    int tile = static_cast<int>((first - start_before) % r.tiles);
+    int step = 0;  // tiles read
+    Request r = request_at(p, share.request);
+    int unit = (share.first - share.before) / r.tiles;
+    int tile = (share.first - share.before) - unit * r.tiles;
     bool first_unit = true;
-    for (int64_t done = 0; done < n_tiles;) {
-      const int seg_tiles = static_cast<int>(min(n_tiles - done, static_cast<int64_t>(r.tiles - tile)));
-      const int head = unit % p.heads_kv, row0 = unit / p.heads_kv * p.rows;
+    for (int done = 0; done < n_tiles;) {
+      const int seg_tiles = min(n_tiles - done, r.tiles - tile);
+      const int row0 = unit / p.heads_kv * p.rows, head = unit - unit / p.heads_kv * p.heads_kv;
       const int n_rows = min(p.rows, r.rows_q * p.group - row0);
-      // ---- rows g and g + 8: where they are, the tokens they see, their elements as f16
-      uint32_t qa[kKSteps][4];
-      float factor[2];
-      int limit[2];
+      const int my_row0 = row0 + kRowsOfWarp * row_group;
+      // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 4t..4t+3 of every 16
+      uint32_t qb[kRowBlocks][kChunks][2];
+      float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale
+      int2 limit[kRowBlocks];     // how many tokens they see
 #pragma unroll
-      for (int hi = 0; hi < 2; ++hi) {
-        const int row = row0 + g + 8 * hi;
-        const int i = row / p.group;
-        limit[hi] = p.causal ? min(r.len, i + 1 + r.len - r.rows_q) : r.len;
-        uint2 w[kKSteps];
-        const bool have = (kHi || hi == 0) && g + 8 * hi < n_rows;
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        const int row = my_row0 + 8 * nb + g, i = row / p.group;
+        const bool have = row < row0 + n_rows;
         const uint16_t* src = p.q + (r.q0 + i) * p.q_row + (head * p.group + row - i * p.group) * p.q_head + 4 * t;
+        uint2 w[kChunks];
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) w[k] = have ? *reinterpret_cast<const uint2*>(src + 16 * k) : make_uint2(0u, 0u);
         float largest = 0.f;
 #pragma unroll
-        for (int k = 0; k < kKSteps; ++k) {
-          w[k] = have ? *reinterpret_cast<const uint2*>(src + 16 * k) : make_uint2(0u, 0u);
+        for (int k = 0; k < kChunks; ++k) {
           const float2 a = p.f16 ? unpack_16x2<true>(w[k].x) : unpack_16x2<false>(w[k].x), b = p.f16 ? unpack_16x2<true>(w[k].y) : unpack_16x2<false>(w[k].y);
           largest = fmaxf(largest, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
         }
         largest = quad_max(largest);
         const int e = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -100), 127);
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e) << 23);
-        factor[hi] = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
+        const float down = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e) << 23);
 #pragma unroll
-        for (int k = 0; k < kKSteps; ++k) {
+        for (int k = 0; k < kChunks; ++k) {
           const float2 a = p.f16 ? unpack_16x2<true>(w[k].x) : unpack_16x2<false>(w[k].x), b = p.f16 ? unpack_16x2<true>(w[k].y) : unpack_16x2<false>(w[k].y);
-          qa[k][hi] = pack_f16x2(a.x * up, a.y * up);
-          qa[k][2 + hi] = pack_f16x2(b.x * up, b.y * up);
+          qb[nb][k][0] = pack_f16x2(a.x * up, a.y * up);
+          qb[nb][k][1] = pack_f16x2(b.x * up, b.y * up);
         }
+        const int sees = p.causal ? min(r.len, i + 1 + r.len - r.rows_q) : r.len;
+        factor[nb] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
+        limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
-      const int seen_by_all = p.causal ? min(r.len, row0 / p.group + 1 + r.len - r.rows_q) : r.len;
+      // tokens that all of the warp's rows see, and those that any of them does
+      const int last_row = min(my_row0 + kRowsOfWarp - 1, row0 + n_rows - 1);
+      const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.len - r.rows_q) : r.len;
+      const int seen_by_any = my_row0 >= row0 + n_rows ? 0 : p.causal ? min(r.len, last_row / p.group + 1 + r.len - r.rows_q) : r.len;
 
-      float o[kNBlocks][4];
+      float o[kRowBlocks][kChunks][4];  // dimensions 2g, 2g, 2g + 1, 2g + 1 of every 16, rows 2t, 2t + 1, 2t, 2t + 1
+      float2 m[kRowBlocks], l[kRowBlocks];  // running maximum of score + log2 of V's scale; this thread's share of the sums, in units of kSumUnit
 #pragma unroll
-      for (int nb = 0; nb < kNBlocks; ++nb) o[nb][0] = o[nb][1] = o[nb][2] = o[nb][3] = 0.f;
-      float m[2] = {-INFINITY, -INFINITY};  // running max, log2 domain
-      float l[2] = {0.f, 0.f};              // this thread's share of the running sums, times 2^kBias
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        m[nb] = make_float2(-INFINITY, -INFINITY);
+        l[nb] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) o[nb][ch][0] = o[nb][ch][1] = o[nb][ch][2] = o[nb][ch][3] = 0.f;
+      }
 
       for (int i = 0; i < seg_tiles; ++i) {
-        const int tok = (tile + i) * kTileTokens + warp * kStepTokens;
-        if (tok >= r.len) continue;
+        const int tile_tok = (tile + i) * kTileTokens;
+        if (tile_tok >= r.len) break;  // a request without tokens
         const uint32_t st = step % kSt;
-        const uint32_t k_smem = ring + st * kStageBytes, v_smem = k_smem + kStepTokens * kD;
-        if (ok) ok = mbar_wait(bar + 8 * st, (step / kSt) & 1, abort_flag);
+        if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        ++step;
         __syncwarp();
-        const float4 sc = scales[st];  // written by a lane of this warp
+#pragma unroll 1
+        for (int c = 0; c < kPartTokens; c += kStepTokens) {
+          const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
+          if (tok >= seen_by_any) break;
+          const uint32_t k_smem = ring + st * kStageBytes + in_tile * kD, v_smem = k_smem + kTileTokens * kD;
 
-        // ---- S = Q K^T. The contraction runs over head_dim in the order in which ldmatrix hands out bytes: thread t has dimensions
-        // 4t..4t+3 of every 16, of K and of Q
-        float s[4][4];
+          // ---- S^T = K Q^T, 16 tokens at a time. The contraction runs over head_dim in the order in which ldmatrix hands out bytes
+          float s[kRowBlocks][2][4];  // tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
 #pragma unroll
-        for (int blk = 0; blk < 4; ++blk) {
-          s[blk][0] = s[blk][1] = s[blk][2] = s[blk][3] = 0.f;
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int ch = 0; ch < kKSteps; ch += 4) {
-            uint32_t kf[4];
-            ldmatrix_x4(k_smem + chunk_at(blk * 8 + mrow, ch + mat), kf);
+            for (int nb = 0; nb < kRowBlocks; ++nb) s[nb][half][0] = s[nb][half][1] = s[nb][half][2] = s[nb][half][3] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t b0, b1;
-              codes_to_f16<kInt8>(kf[j], b0, b1);
-              mma_rows<kHi, true>(s[blk], qa[ch + j], b0, b1);
+            for (int ch = 0; ch < kChunks; ch += 2) {
+              uint32_t kf[4];  // tokens 0-7 and 8-15 of a chunk, the same of the next
+              ldmatrix_x4(k_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), kf);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t a0, a1, a2, a3;
+                codes_to_f16<kInt8>(kf[2 * e], a0, a2);
+                codes_to_f16<kInt8>(kf[2 * e + 1], a1, a3);
+#pragma unroll
+                for (int nb = 0; nb < kRowBlocks; ++nb) mma_16816<true>(s[nb][half], a0, a1, a2, a3, qb[nb][ch + e][0], qb[nb][ch + e][1]);
+              }
+            }
+          }
+          const float4 sc0 = slot_scales[st * kSlots + in_tile / 16], sc1 = slot_scales[st * kSlots + in_tile / 16 + 1];
+          uint32_t pb[kRowBlocks][2][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
+          bool moved = false;
+          float2 a[kRowBlocks];
+#pragma unroll
+          for (int nb = 0; nb < kRowBlocks; ++nb) {
+            // scores and log2 of V's scale, masked where a row ends inside the step
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float ks = half ? sc1.x : sc0.x, lv = half ? sc1.y : sc0.y;
+              const float fx = factor[nb].x * ks, fy = factor[nb].y * ks;
+              s[nb][half][0] = fmaf(s[nb][half][0], fx, lv);
+              s[nb][half][1] = fmaf(s[nb][half][1], fy, lv);
+              s[nb][half][2] = fmaf(s[nb][half][2], fx, lv);
+              s[nb][half][3] = fmaf(s[nb][half][3], fy, lv);
+            }
+            if (tok + kStepTokens > seen_by_all) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                const int j = tok + half * 16 + g;
+                if (j >= limit[nb].x) s[nb][half][0] = -INFINITY;
+                if (j >= limit[nb].y) s[nb][half][1] = -INFINITY;
+                if (j + 8 >= limit[nb].x) s[nb][half][2] = -INFINITY;
+                if (j + 8 >= limit[nb].y) s[nb][half][3] = -INFINITY;
+              }
+            }
+            const float mx = fmaxf(m[nb].x, column_max(fmaxf(fmaxf(s[nb][0][0], s[nb][0][2]), fmaxf(s[nb][1][0], s[nb][1][2]))));
+            const float my = fmaxf(m[nb].y, column_max(fmaxf(fmaxf(s[nb][0][1], s[nb][0][3]), fmaxf(s[nb][1][1], s[nb][1][3]))));
+            // a row that has seen no key has o = l = 0: any finite factor will do
+            a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
+            moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
+            m[nb] = make_float2(mx, my);
+            const float ux = mx == -INFINITY ? 0.f : mx - kBias, uy = my == -INFINITY ? 0.f : my - kBias;
+            l[nb].x *= a[nb].x;
+            l[nb].y *= a[nb].y;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const float rv = half ? sc1.z : sc0.z;
+              const float x0 = ex2_approx(s[nb][half][0] - ux), y0 = ex2_approx(s[nb][half][1] - uy);
+              const float x1 = ex2_approx(s[nb][half][2] - ux), y1 = ex2_approx(s[nb][half][3] - uy);
+              l[nb].x = fmaf(x0 + x1, rv, l[nb].x);
+              l[nb].y = fmaf(y0 + y1, rv, l[nb].y);
+              pb[nb][half][0] = transpose_8x8(pack_f16x2(x0, y0));
+              pb[nb][half][1] = transpose_8x8(pack_f16x2(x1, y1));
+            }
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nb = 0; nb < kRowBlocks; ++nb)
+#pragma unroll
+              for (int ch = 0; ch < kChunks; ++ch) {
+                o[nb][ch][0] *= a[nb].x;
+                o[nb][ch][1] *= a[nb].y;
+                o[nb][ch][2] *= a[nb].x;
+                o[nb][ch][3] *= a[nb].y;
+              }
+          }
+          // ---- O^T += V^T W^T, 16 tokens at a time. What stands behind the request's last token may be anything: it must not meet a weight of 0
+          auto add_half = [&](int half, uint32_t keep0, uint32_t keep1) {
+#pragma unroll
+            for (int ch = 0; ch < kChunks; ch += 2) {
+              uint32_t vf[4];
+              ldmatrix_x4_trans(v_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), vf);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t even0, odd0, even1, odd1;  // f16 pairs of two tokens: dimension 2g, dimension 2g + 1
+                codes_to_f16_by_two<kInt8>(vf[2 * e] & keep0, even0, odd0);
+                codes_to_f16_by_two<kInt8>(vf[2 * e + 1] & keep1, even1, odd1);
+#pragma unroll
+                for (int nb = 0; nb < kRowBlocks; ++nb)
+                  mma_16816<true>(o[nb][ch + e], even0, odd0, even1, odd1, half ? pb[nb][1][0] : pb[nb][0][0], half ? pb[nb][1][1] : pb[nb][0][1]);
+              }
+            }
+          };
+          if (tok + kStepTokens <= r.len) {
+            add_half(0, ~0u, ~0u);
+            add_half(1, ~0u, ~0u);
+          } else {
+            auto keep = [&](int j) { return (j < r.len ? 0xffffu : 0u) | (j + 1 < r.len ? 0xffff0000u : 0u); };
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+              const int j = tok + half * 16 + 2 * t;
+              if (tok + half * 16 < r.len) add_half(half, keep(j), keep(j + 8));
             }
           }
         }
-        // ---- scores in the log2 domain (thread holds tokens tok + blk * 8 + 2t + {0, 1}), masked where a row ends inside the step
-#pragma unroll
-        for (int blk = 0; blk < 4; ++blk) {
-          const float ks = blk < 2 ? sc.x : sc.z;
-          s[blk][0] *= factor[0] * ks;
-          s[blk][1] *= factor[0] * ks;
-          s[blk][2] *= factor[1] * ks;
-          s[blk][3] *= factor[1] * ks;
-        }
-        if (tok + kStepTokens > seen_by_all) {
-#pragma unroll
-          for (int blk = 0; blk < 4; ++blk) {
-            const int j = tok + blk * 8 + 2 * t;
-            if (j >= limit[0]) s[blk][0] = -INFINITY;
-            if (j + 1 >= limit[0]) s[blk][1] = -INFINITY;
-            if (j >= limit[1]) s[blk][2] = -INFINITY;
-            if (j + 1 >= limit[1]) s[blk][3] = -INFINITY;
-          }
-        }
-        uint32_t pa[2][4];
-        float a[2] = {1.f, 1.f};
-#pragma unroll
-        for (int hi = 0; hi < (kHi ? 2 : 1); ++hi) {
-          float top = fmaxf(s[0][2 * hi], s[0][2 * hi + 1]);
-#pragma unroll
-          for (int blk = 1; blk < 4; ++blk) top = max3(top, s[blk][2 * hi], s[blk][2 * hi + 1]);
-          const float mn = fmaxf(m[hi], quad_max(top));
-          // a row that has seen no key has o = l = 0: any finite factor will do
-          a[hi] = mn == -INFINITY ? 1.f : ex2_approx(m[hi] - mn);
-          m[hi] = mn;
-          const float u = mn == -INFINITY ? 0.f : mn - kBias;
-          float sum = 0.f;
-#pragma unroll
-          for (int blk = 0; blk < 4; ++blk) {
-            const float x = ex2_approx(s[blk][2 * hi] - u), y = ex2_approx(s[blk][2 * hi + 1] - u);
-            sum += x + y;
-            pa[blk >> 1][(blk & 1) * 2 + hi] = pack_f16x2(x, y);
-          }
-          l[hi] = fmaf(l[hi], a[hi], sum);
-        }
-        if constexpr (!kHi) pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
-        if (__any_sync(0xffffffffu, a[0] != 1.f || a[1] != 1.f)) {
-#pragma unroll
-          for (int nb = 0; nb < kNBlocks; ++nb) {
-            o[nb][0] *= a[0];
-            o[nb][1] *= a[0];
-            o[nb][2] *= a[1];
-            o[nb][3] *= a[1];
-          }
-        }
-        // what stands behind the request's last token may be anything: it must not meet a weight of 0
-        uint32_t keep[2][2] = {{~0u, ~0u}, {~0u, ~0u}};
-        if (tok + kStepTokens > r.len) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int j = tok + half * 16 + e * 8 + 2 * t;
-              keep[half][e] = (j < r.len ? 0xffffu : 0u) | (j + 1 < r.len ? 0xffff0000u : 0u);
-            }
-        }
-        // ---- O += vs * (P V), 16 tokens at a time
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (half == 1 && tok + 16 >= r.len) break;
-          const float vs = half ? sc.w : sc.y;
-#pragma unroll
-          for (int ch = 0; ch < kKSteps; ch += 2) {
-            uint32_t vf[4];
-            ldmatrix_x4_trans(v_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), vf);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t even0, odd0, even1, odd1;  // f16 pairs of two tokens: dimension 2g, dimension 2g + 1
-              codes_to_f16_by_two<kInt8>(vf[2 * e] & keep[half][0], even0, odd0);
-              codes_to_f16_by_two<kInt8>(vf[2 * e + 1] & keep[half][1], even1, odd1);
-              float d[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-              mma_rows<kHi, true>(d[0], pa[half], even0, even1);
-              mma_rows<kHi, true>(d[1], pa[half], odd0, odd1);
-#pragma unroll
-              for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int y = 0; y < (kHi ? 4 : 2); ++y) o[2 * (ch + e) + x][y] = fmaf(d[x][y], vs, o[2 * (ch + e) + x][y]);
-            }
-          }
-        }
-        __syncwarp();  // the stage has been read by every lane: refill it
-        if (ok) load_next();
-      }
-
-      // ---- merge the four warps: 1-3 hand their state over in fragment order, warp 0 folds it into its own
-#pragma unroll
-      for (int hi = 0; hi < 2; ++hi) l[hi] = quad_sum(l[hi]);
-      __syncthreads();  // warp 0 has read what the previous unit left here
-      constexpr int kPer = kHi ? 4 : 2, kTail = kNBlocks * kPer * 32;
-      if (warp > 0) {
-        float* dst = merge + (warp - 1) * kMergeFloats + lane;
-#pragma unroll
-        for (int nb = 0; nb < kNBlocks; ++nb)
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) dst[(nb * kPer + e) * 32] = o[nb][e];
-#pragma unroll
-        for (int hi = 0; hi < (kHi ? 2 : 1); ++hi) {
-          dst[kTail + 64 * hi] = m[hi];
-          dst[kTail + 64 * hi + 32] = l[hi];
+        // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
+        if (i + 1 < seg_tiles) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * st);
+          ++step;
         }
       }
-      __syncthreads();
+      const bool tokens = r.len > 0;
+      const uint32_t st = step % kSt;
+#pragma unroll
+      for (int nb = 0; nb < kRowBlocks; ++nb) l[nb] = make_float2(column_sum(l[nb].x), column_sum(l[nb].y));
+      // ---- the parts of a tile's tokens come together: every warp takes some of the dimensions, of all parts
+      constexpr int kMine = kChunks / kParts;
+      float* states = reinterpret_cast<float*>(ring_ptr + st * kStageBytes) + row_group * kParts * kState + lane;
+      if (kParts > 1 && tokens) {
+        arithmetic_sync();
+#pragma unroll
+        for (int nb = 0; nb < kRowBlocks; ++nb) {
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) states[part * kState + ((nb * kChunks + ch) * 4 + e) * 32] = o[nb][ch][e];
+          if (g == 0) {
+            row_state[warp * 16 + 8 * nb + 2 * t] = make_float2(m[nb].x, l[nb].x);
+            row_state[warp * 16 + 8 * nb + 2 * t + 1] = make_float2(m[nb].y, l[nb].y);
+          }
+        }
+        arithmetic_sync();
+      }
       const bool whole = seg_tiles == r.tiles;
       const int slot = first_unit ? 0 : 1;
-      if (warp == 0) {
 #pragma unroll
-        for (int hi = 0; hi < (kHi ? 2 : 1); ++hi) {
-          float mm = m[hi];
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        float acc[kMine][4];
+        float mm[2] = {m[nb].x, m[nb].y}, sum[2] = {l[nb].x, l[nb].y};
+        if (kParts > 1 && tokens) {
+          float2 others[2][kParts];
 #pragma unroll
-          for (int w = 0; w < kWarps - 1; ++w) mm = fmaxf(mm, merge[w * kMergeFloats + kTail + 64 * hi + lane]);
-          auto weight = [&](float x) { return x == -INFINITY ? 0.f : ex2_approx(x - mm); };
-          float f = weight(m[hi]), sum = l[hi] * f;
+          for (int x = 0; x < 2; ++x) {
+            mm[x] = -INFINITY;
+            sum[x] = 0.f;
 #pragma unroll
-          for (int nb = 0; nb < kNBlocks; ++nb) {
-            o[nb][2 * hi] *= f;
-            o[nb][2 * hi + 1] *= f;
-          }
-#pragma unroll
-          for (int w = 0; w < kWarps - 1; ++w) {
-            const float* src = merge + w * kMergeFloats + lane;
-            f = weight(src[kTail + 64 * hi]);
-            sum += src[kTail + 64 * hi + 32] * f;
-#pragma unroll
-            for (int nb = 0; nb < kNBlocks; ++nb) {
-              o[nb][2 * hi] += src[(nb * kPer + 2 * hi) * 32] * f;
-              o[nb][2 * hi + 1] += src[(nb * kPer + 2 * hi + 1) * 32] * f;
+            for (int w = 0; w < kParts; ++w) {
+              others[x][w] = row_state[(row_group * kParts + w) * 16 + 8 * nb + 2 * t + x];
+              mm[x] = fmaxf(mm[x], others[x][w].x);
             }
           }
-          const int rr = g + 8 * hi;
-          if (rr < n_rows) {
-            const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays NaN
-            const float lse2 = sum == 0.f ? -INFINITY : mm - kBias + log2f(sum);
-            if (whole) {
-              const int row = row0 + rr, i = row / p.group, hq = head * p.group + row - i * p.group;
-              uint16_t* dst = p.out + (r.q0 + i) * p.o_row + hq * p.o_head + 4 * t;
 #pragma unroll
-              for (int ch = 0; ch < kKSteps; ++ch) {  // dimensions 4t..4t+3 of every 16: even, odd, even, odd
-                const float x0 = o[2 * ch][2 * hi] * inv, x1 = o[2 * ch + 1][2 * hi] * inv, x2 = o[2 * ch][2 * hi + 1] * inv, x3 = o[2 * ch + 1][2 * hi + 1] * inv;
-                *reinterpret_cast<uint2*>(dst + 16 * ch) = p.f16 ? make_uint2(pack_f16x2(x0, x1), pack_f16x2(x2, x3)) : make_uint2(pack_bf16x2(x0, x1), pack_bf16x2(x2, x3));
-              }
-              if (t == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
-            } else {
-              const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + rr;
-              float* dst = p.part_o + at * kD + 4 * t;
+          for (int ch = 0; ch < kMine; ++ch) acc[ch][0] = acc[ch][1] = acc[ch][2] = acc[ch][3] = 0.f;
 #pragma unroll
-              for (int ch = 0; ch < kKSteps; ++ch)
-                *reinterpret_cast<float4*>(dst + 16 * ch) = make_float4(o[2 * ch][2 * hi] * inv, o[2 * ch + 1][2 * hi] * inv, o[2 * ch][2 * hi + 1] * inv, o[2 * ch + 1][2 * hi + 1] * inv);
-              if (t == 0) p.part_lse[at] = lse2;
+          for (int w = 0; w < kParts; ++w) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              f[x] = others[x][w].x == -INFINITY ? 0.f : ex2_approx(others[x][w].x - mm[x]);
+              sum[x] = fmaf(others[x][w].y, f[x], sum[x]);
             }
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[ch][e] = fmaf(states[w * kState + ((nb * kChunks + part * kMine + ch) * 4 + e) * 32], f[e & 1], acc[ch][e]);
+          }
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < kMine; ++ch)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[ch][e] = o[nb][ch][e];  // all of them, or zeros
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int row = my_row0 + 8 * nb + 2 * t + x;
+          if (row >= row0 + n_rows) continue;
+          const float inv = sum[x] > 0.f ? kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN
+          const float lse2 = sum[x] == 0.f ? -INFINITY : mm[x] - kBias - log2f(kSumUnit) + log2f(sum[x]);
+          const int dim0 = part * kMine * 16 + 2 * g;
+          if (whole) {
+            const int i = row / p.group, hq = head * p.group + row - i * p.group;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (r.q0 + i) * p.o_row + hq * p.o_head + dim0);
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch) {
+              const float even = acc[ch][x] * inv, odd = acc[ch][2 + x] * inv;
+              dst[8 * ch] = p.f16 ? pack_f16x2(even, odd) : pack_bf16x2(even, odd);
+            }
+            if (g == 0 && part == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum[x] > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
+          } else {
+            const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
+            float* dst = p.part_o + at * kD + dim0;
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + 16 * ch) = make_float2(acc[ch][x] * inv, acc[ch][2 + x] * inv);
+            if (g == 0 && part == 0) p.part_lse[at] = lse2;
           }
         }
       }
-      if (tile == 0 && !whole) {  // begun here, ended by the CTA whose share holds its last tile
-        const int64_t end = first + done + r.tiles - 1;
-        left = {r.index, unit, static_cast<int>(((end + 1) * ctas - 1) / total), slot};
+      if (tokens) {
+        fence_proxy_async_smem();  // what was handed over goes before the copy into the same place
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * st);
+        ++step;
       }
+      // begun here, ended by the CTA whose share holds its last tile
+      if (tile == 0 && !whole) left = {share.cta_of(share.first + done + r.tiles - 1), slot, head, row0, n_rows, r.q0};
       done += seg_tiles;
       tile = 0;
       first_unit = false;
@@ -507,44 +619,54 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 template <int kD>
 __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) {
   constexpr int kPer = kD / 32;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rr = blockIdx.y * 4 + warp;
+  const int lane = threadIdx.x & 31, rr = blockIdx.y * 4 + (threadIdx.x >> 5), first = blockIdx.x;
   wait_for_previous_grid();
   launch_dependents();
-  const SharedUnit u = p.shared_units[blockIdx.x];
-  if (u.last < 0) return;
-  const Request r = request_at(p, u.request);
-  const int row = u.unit / p.heads_kv * p.rows + rr;
-  if (rr >= p.rows || row >= r.rows_q * p.group) return;
-  auto part = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == static_cast<int>(blockIdx.x) ? u.slot : 0)) * p.rows + rr; };
-  float top = -INFINITY;
+  const SharedUnit u = p.shared_units[first];
+  if (u.last < 0 || rr >= u.rows) return;
+  auto part = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == first ? u.slot : 0)) * p.rows + rr; };
+  float top = -INFINITY, sum = 0.f, acc[kPer];
   bool nan = false;
-  for (int c = blockIdx.x + lane; c <= u.last; c += 32) {
-    const float x = p.part_lse[part(c)];
-    nan = nan || isnan(x);
-    top = fmaxf(top, x);
-  }
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  nan = __any_sync(0xffffffffu, nan);
-  float sum = 0.f, acc[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-  if (top != -INFINITY) {
-#pragma unroll 4
-    for (int c = blockIdx.x; c <= u.last; ++c) {
-      const int64_t at = part(c);
-      const float x = p.part_lse[at], w = x == -INFINITY ? 0.f : exp2f(x - top);
-      sum += w;
+  for (int base = first; base <= u.last; base += 32) {
+    const int n = min(32, u.last - base + 1);
+    const float x = lane < n ? p.part_lse[part(base + lane)] : -INFINITY;
+    nan = nan || __any_sync(0xffffffffu, isnan(x));
+    float mn = x;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(w, p.part_o[at * kD + e * 32 + lane], acc[e]);
+    for (int d = 1; d < 32; d *= 2) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+    mn = fmaxf(mn, top);
+    const float a = top == -INFINITY ? 0.f : exp2f(top - mn), w = x == -INFINITY ? 0.f : exp2f(x - mn);
+    top = mn;
+    float s = w;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+    sum = sum * a + s;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) acc[e] *= a;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float* src = p.part_o + part(base + j) * kD + kPer * lane;
+      float v[kPer];
+      if constexpr (kPer == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(src);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+      } else {
+        const float2 q = *reinterpret_cast<const float2*>(src);
+        v[0] = q.x, v[1] = q.y;
+      }
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wj, v[e], acc[e]);
     }
   }
-  const int i = row / p.group, hq = u.unit % p.heads_kv * p.group + row - i * p.group;
+  const int row = u.row0 + rr, i = row / p.group, hq = u.head * p.group + row - i * p.group;
   const float inv = nan ? __int_as_float(0x7fffffff) : sum > 0.f ? 1.f / sum : 0.f;
-  uint16_t* dst = p.out + (r.q0 + i) * p.o_row + hq * p.o_head;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (u.q0 + i) * p.o_row + hq * p.o_head + kPer * lane);
 #pragma unroll
-  for (int e = 0; e < kPer; ++e) dst[e * 32 + lane] = p.f16 ? to_16<true>(acc[e] * inv) : to_16<false>(acc[e] * inv);
-  if (lane == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = !nan && sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : INFINITY;
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = p.f16 ? pack_f16x2(acc[e] * inv, acc[e + 1] * inv) : pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+  if (lane == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + u.q0 + i] = !nan && sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : INFINITY;
 }
 
 // ---- many rows: the codes of all requests as packed 16-bit K and V
@@ -690,7 +812,8 @@ int check_attention(const sdpa_b200_cache_params* p) {
 }
 
 int unit_rows(const sdpa_b200_cache_params& p) {
-  return static_cast<int64_t>(p.max_seqlen_q) * (p.heads_q / p.heads_kv) <= 8 ? 8 : kRows;
+  const int64_t rows = static_cast<int64_t>(p.max_seqlen_q) * (p.heads_q / p.heads_kv);
+  return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 size_t round_256(size_t n) { return (n + 255) / 256 * 256; }
@@ -729,6 +852,8 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   p.num_blocks = c.num_blocks;
   p.shift = block_shift(c.block_size);
   p.rows = unit_rows(c);
+  p.rows_shift = p.rows == 8 ? 3 : p.rows == 16 ? 4 : p.rows == 32 ? 5 : 6;
+  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - kTileTokens) + 1);
   p.causal = c.is_causal;
   p.f16 = c.dtype == SDPA_B200_F16;
   p.scale_log2 = c.softmax_scale * 1.4426950408889634f;
@@ -741,37 +866,48 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   p.part_lse = p.part_o + rows * c.head_dim;
   p.shared_units = reinterpret_cast<SharedUnit*>(p.part_lse + rows);
   CUtensorMap tm_k, tm_v;
-  const int box = c.block_size < kStepTokens ? c.block_size : kStepTokens;
-  int st = make_cache_tensor_map(&tm_k, c.k_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.k_row_stride, c.k_head_stride, c.k_block_stride, box);
+  int st = make_cache_tensor_map(&tm_k, c.k_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.k_row_stride, c.k_head_stride, c.k_block_stride, c.block_size);
   if (st != SDPA_B200_OK) return st;
-  st = make_cache_tensor_map(&tm_v, c.v_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.v_row_stride, c.v_head_stride, c.v_block_stride, box);
+  st = make_cache_tensor_map(&tm_v, c.v_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.v_row_stride, c.v_head_stride, c.v_block_stride, c.block_size);
   if (st != SDPA_B200_OK) return st;
   cudaError_t err = cudaSuccess;
-  auto launch = [&](auto hi_tag, auto dim_tag, auto int8_tag) {
-    constexpr bool kHi = decltype(hi_tag)::value, kInt8 = decltype(int8_tag)::value;
-    constexpr int kD = decltype(dim_tag)::value;
-    constexpr uint32_t kSmem = stream_smem_bytes<kHi, kD>();
-    static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "two CTAs do not fit an SM");
-    auto kernel = cache_stream_kernel<kHi, kD, kInt8>;
+  auto launch = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag) {
+    constexpr bool kInt8 = decltype(int8_tag)::value;
+    constexpr int kRowBlocks = decltype(blocks_tag)::value, kRowWarps = decltype(rows_tag)::value, kD = decltype(dim_tag)::value;
+    constexpr uint32_t kSmem = stream_smem_bytes<kD>();
+    static_assert(kCtasPerSm * (kSmem + 1024 + 64) <= 228 * 1024, "two CTAs do not fit an SM");
+    auto kernel = cache_stream_kernel<kRowBlocks, kRowWarps, kD, kInt8>;
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (err == cudaSuccess) err = launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, false, 1, tm_k, tm_v, p);
+    if (err == cudaSuccess) err = launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, c.device_status != nullptr, 1, tm_k, tm_v, p);
   };
-  auto launch_code = [&](auto hi_tag, auto dim_tag) {
-    c.code == SDPA_B200_INT8 ? launch(hi_tag, dim_tag, std::true_type{}) : launch(hi_tag, dim_tag, std::false_type{});
+  auto launch_code = [&](auto blocks_tag, auto rows_tag, auto dim_tag) {
+    c.code == SDPA_B200_INT8 ? launch(blocks_tag, rows_tag, dim_tag, std::true_type{}) : launch(blocks_tag, rows_tag, dim_tag, std::false_type{});
   };
-  auto launch_dim = [&](auto hi_tag) {
-    c.head_dim == 64 ? launch_code(hi_tag, std::integral_constant<int, 64>{}) : launch_code(hi_tag, std::integral_constant<int, 128>{});
+  auto launch_dim = [&](auto blocks_tag, auto rows_tag) {
+    c.head_dim == 64 ? launch_code(blocks_tag, rows_tag, std::integral_constant<int, 64>{}) : launch_code(blocks_tag, rows_tag, std::integral_constant<int, 128>{});
   };
-  p.rows > 8 ? launch_dim(std::true_type{}) : launch_dim(std::false_type{});
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (p.rows == 8) launch_dim(One{}, One{});
+  else if (p.rows == 16) launch_dim(Two{}, One{});
+  else if (p.rows == 32) launch_dim(Two{}, Two{});
+  else launch_dim(Two{}, std::integral_constant<int, 4>{});
   if (err != cudaSuccess) {
     set_error("cache_attention: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;
   }
   count_launch();
   if (p.grid == 1) return SDPA_B200_OK;  // nobody to share a unit with
-  const dim3 merge_grid(p.grid - 1, (p.rows + 3) / 4);
-  err = c.head_dim == 64 ? launch_behind(cache_merge_kernel<64>, merge_grid, 128, 0, stream, true, 1, p)
-                         : launch_behind(cache_merge_kernel<128>, merge_grid, 128, 0, stream, true, 1, p);
+  cudaLaunchConfig_t cfg = {};  // under this grid's tail, under stream capture too: what stands in front is a kernel of this call
+  cfg.gridDim = dim3(p.grid - 1, p.rows / 4);
+  cfg.blockDim = dim3(128);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  err = c.head_dim == 64 ? cudaLaunchKernelEx(&cfg, cache_merge_kernel<64>, p) : cudaLaunchKernelEx(&cfg, cache_merge_kernel<128>, p);
   if (err != cudaSuccess) {
     set_error("cache_attention merge: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;
