@@ -1,9 +1,9 @@
 // Rotary positions with up to four axes (time, height, width): every row of q and k has its first rotary_dim elements turned, pair by pair, by
 // angle_j = position[axis(j)] * inv_freq[j]. The gradient is the same turn backwards. No counterpart in the reference.
 //
-// The angles are the same for all heads of a token. A block takes a few tokens: its threads form the cosines and sines of those once into
-// shared memory, then go over the (token, head, chunk) list, eight pairs a thread, with 16-byte loads and stores. The product of a position
-// and a frequency is taken in 64 bits, where it is exact, and brought into [-1, 1] half turns there: at position 10^6 the 32-bit product is off by up to
+// A warp takes a token and some of its heads: its lanes form the cosines and sines together, once, in its own part of shared memory, then each keeps those of
+// its eight pairs in registers and goes over the heads, four at a time, with 16-byte loads and stores. Bound by HBM: every element is read and written once.
+// The product of a position and a frequency is taken in 64 bits, where it is exact, and brought into [-1, 1] half turns there: at position 10^6 the 32-bit product is off by up to
 // 0.03 radians. The rest, in 32 bits, is off by 2e-7.
 #include "kernels.h"
 #include "ptx_sm100.cuh"
@@ -11,8 +11,10 @@
 namespace sdpa_b200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 4;
 constexpr int kMaxPairs = 128;
+constexpr int kBatch = 4;  // heads whose loads a lane has under way
+constexpr int kEnoughWarps = 148 * 32;
 
 struct RotaryTensor {
   const uint16_t* in;
@@ -28,80 +30,100 @@ struct RotaryParams {
   int64_t tokens;  // batch * length
   int length, heads_q, heads, head_dim, half;
   int axis_end[3];  // the first pair behind each axis but the last
-  int tokens_per_block;
-  int positions_64, interleaved;
+  int chunks, lanes_of_heads;  // chunks of a row: eight pairs each, then eight copied elements each; heads that a warp works on at a time
+  int splits, heads_per_split;  // warps per token
+  int positions_64;
   float scaling, sign;
 };
 
-// One 16-byte chunk of pairs: `a` and `b` hold the pairs' first and second elements of 8 pairs (halves apart), or eight elements = four pairs each
-// (interleaved); `cs`: their cosines and sines.
+// Two pairs (x, y), halves apart: `first` holds both x, `second` both y
 template <bool kF16>
-__device__ __forceinline__ uint32_t turn_word(uint32_t first, uint32_t second, const float2& cs0, const float2& cs1, uint32_t& second_out) {
+__device__ __forceinline__ void turn_apart(uint32_t& first, uint32_t& second, const float4& cs) {
   const float2 x = unpack_16x2<kF16>(first), y = unpack_16x2<kF16>(second);
-  second_out = pack_16x2<kF16>(fmaf(x.x, cs0.y, y.x * cs0.x), fmaf(x.y, cs1.y, y.y * cs1.x));
-  return pack_16x2<kF16>(fmaf(x.x, cs0.x, -y.x * cs0.y), fmaf(x.y, cs1.x, -y.y * cs1.y));
+  first = pack_16x2<kF16>(fmaf(x.x, cs.x, -y.x * cs.y), fmaf(x.y, cs.z, -y.y * cs.w));
+  second = pack_16x2<kF16>(fmaf(x.x, cs.y, y.x * cs.x), fmaf(x.y, cs.w, y.y * cs.z));
 }
+// One pair next to each other
 template <bool kF16>
-__device__ __forceinline__ uint32_t turn_pair(uint32_t w, const float2& cs) {
+__device__ __forceinline__ void turn_pair(uint32_t& w, float c, float s) {
   const float2 x = unpack_16x2<kF16>(w);
-  return pack_16x2<kF16>(fmaf(x.x, cs.x, -x.y * cs.y), fmaf(x.x, cs.y, x.y * cs.x));
+  w = pack_16x2<kF16>(fmaf(x.x, c, -x.y * s), fmaf(x.x, s, x.y * c));
 }
 
-template <bool kF16>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryParams p) {
-  extern __shared__ float2 turns[];  // [tokens_per_block][half]: cosine, sine
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.tokens_per_block;
-  const int tokens = static_cast<int>(min(static_cast<int64_t>(p.tokens_per_block), p.tokens - token0));
-  for (int i = threadIdx.x; i < tokens * p.half; i += kThreads) {
-    const int t = i / p.half, j = i - t * p.half;
-    const int64_t token = token0 + t, b = token / p.length;
+template <bool kF16, bool kInterleaved>
+__global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const RotaryParams p) {
+  __shared__ __align__(16) float2 turns[kWarps][kMaxPairs];  // cosine, sine
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int64_t token = item / p.splits;
+  if (token >= p.tokens) return;
+  const int split = static_cast<int>(item - token * p.splits);
+  const int b = static_cast<int>(token / p.length), row = static_cast<int>(token - static_cast<int64_t>(b) * p.length);
+  const int chunk = lane % p.chunks, head_lane = lane / p.chunks;
+  const int end = head_lane < p.lanes_of_heads ? min(p.heads, (split + 1) * p.heads_per_split) : 0;
+  const bool turned = chunk * 8 < p.half;
+  // where this lane's elements are in a row: two runs of eight that make eight pairs, or one that is copied
+  const int at = !turned ? p.half + chunk * 8 : kInterleaved ? chunk * 16 : chunk * 8;  // (the copied part begins at 2 half: chunk half / 8)
+  const int apart = kInterleaved ? 8 : p.half;
+  auto row_of = [&](int h, bool out) {
+    const bool is_q = h < p.heads_q;
+    const RotaryTensor& x = is_q ? p.q : p.k;
+    const int head = is_q ? h : h - p.heads_q;
+    return (out ? x.out + b * x.out_batch + head * x.out_head + row * x.out_row : const_cast<uint16_t*>(x.in) + b * x.in_batch + head * x.in_head + row * x.in_row) + at;
+  };
+  int h = split * p.heads_per_split + head_lane;
+  uint4 u[kBatch], v[kBatch];
+  auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (h + i * p.lanes_of_heads >= end) continue;
+      const uint16_t* in = row_of(h + i * p.lanes_of_heads, false);
+      u[i] = *reinterpret_cast<const uint4*>(in);
+      if (turned) v[i] = *reinterpret_cast<const uint4*>(in + apart);
+    }
+  };
+  load();  // under way while the angles are formed
+  for (int j = lane; j < p.half; j += 32) {
     const int axis = (j >= p.axis_end[0]) + (j >= p.axis_end[1]) + (j >= p.axis_end[2]);
-    const int64_t at = axis * p.pos_axis + b * p.pos_batch + (token - b * p.length) * p.pos_row;
-    const int64_t pos = p.positions_64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+    const int64_t where = axis * p.pos_axis + b * p.pos_batch + row * p.pos_row;
+    const int64_t pos = p.positions_64 ? static_cast<const int64_t*>(p.positions)[where] : static_cast<const int32_t*>(p.positions)[where];
     double x = static_cast<double>(pos) * static_cast<double>(p.inv_freq[j]) * 0.31830988618379067154;  // half turns
     x -= 2.0 * rint(0.5 * x);
     float s, c;
     sincospif(static_cast<float>(x), &s, &c);
-    turns[i] = make_float2(c * p.scaling, s * p.scaling * p.sign);
+    turns[warp][j] = make_float2(c * p.scaling, s * p.scaling * p.sign);
   }
-  __syncthreads();
-  // chunks of a row: those of the pairs (16 elements each), then those that are copied (8 elements each)
-  const int turned = p.half / 8, rest = (p.head_dim - 2 * p.half) / 8, chunks = turned + rest;
-  const int per_token = p.heads * chunks;
-  for (int i = threadIdx.x; i < tokens * per_token; i += kThreads) {
-    const int t = i / per_token, r = i - t * per_token;
-    const int h = r / chunks, c = r - h * chunks;
-    const int64_t token = token0 + t, b = token / p.length, row = token - b * p.length;
-    const bool is_q = h < p.heads_q;
-    const RotaryTensor& x = is_q ? p.q : p.k;
-    const int head = is_q ? h : h - p.heads_q;
-    const uint16_t* in = x.in + b * x.in_batch + head * x.in_head + row * x.in_row;
-    uint16_t* out = x.out + b * x.out_batch + head * x.out_head + row * x.out_row;
-    if (c >= turned) {
-      const int at = 2 * p.half + (c - turned) * 8;
-      *reinterpret_cast<uint4*>(out + at) = *reinterpret_cast<const uint4*>(in + at);
-      continue;
+  __syncwarp();
+  float4 cs[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) cs[i] = turned ? *reinterpret_cast<const float4*>(&turns[warp][chunk * 8 + 2 * i]) : make_float4(1.f, 0.f, 1.f, 0.f);
+  while (h < end) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (h + i * p.lanes_of_heads >= end) continue;
+      uint16_t* out = row_of(h + i * p.lanes_of_heads, true);
+      if (turned) {
+        if constexpr (kInterleaved) {
+          turn_pair<kF16>(u[i].x, cs[0].x, cs[0].y);
+          turn_pair<kF16>(u[i].y, cs[0].z, cs[0].w);
+          turn_pair<kF16>(u[i].z, cs[1].x, cs[1].y);
+          turn_pair<kF16>(u[i].w, cs[1].z, cs[1].w);
+          turn_pair<kF16>(v[i].x, cs[2].x, cs[2].y);
+          turn_pair<kF16>(v[i].y, cs[2].z, cs[2].w);
+          turn_pair<kF16>(v[i].z, cs[3].x, cs[3].y);
+          turn_pair<kF16>(v[i].w, cs[3].z, cs[3].w);
+        } else {
+          turn_apart<kF16>(u[i].x, v[i].x, cs[0]);
+          turn_apart<kF16>(u[i].y, v[i].y, cs[1]);
+          turn_apart<kF16>(u[i].z, v[i].z, cs[2]);
+          turn_apart<kF16>(u[i].w, v[i].w, cs[3]);
+        }
+        *reinterpret_cast<uint4*>(out + apart) = v[i];
+      }
+      *reinterpret_cast<uint4*>(out) = u[i];
     }
-    const float2* cs = turns + t * p.half + c * 8;
-    const int at = p.interleaved ? c * 16 : c * 8, apart = p.interleaved ? 8 : p.half;
-    uint4 u = *reinterpret_cast<const uint4*>(in + at), v = *reinterpret_cast<const uint4*>(in + at + apart);
-    if (p.interleaved) {
-      u.x = turn_pair<kF16>(u.x, cs[0]);
-      u.y = turn_pair<kF16>(u.y, cs[1]);
-      u.z = turn_pair<kF16>(u.z, cs[2]);
-      u.w = turn_pair<kF16>(u.w, cs[3]);
-      v.x = turn_pair<kF16>(v.x, cs[4]);
-      v.y = turn_pair<kF16>(v.y, cs[5]);
-      v.z = turn_pair<kF16>(v.z, cs[6]);
-      v.w = turn_pair<kF16>(v.w, cs[7]);
-    } else {
-      u.x = turn_word<kF16>(u.x, v.x, cs[0], cs[1], v.x);
-      u.y = turn_word<kF16>(u.y, v.y, cs[2], cs[3], v.y);
-      u.z = turn_word<kF16>(u.z, v.z, cs[4], cs[5], v.z);
-      u.w = turn_word<kF16>(u.w, v.w, cs[6], cs[7], v.w);
-    }
-    *reinterpret_cast<uint4*>(out + at) = u;
-    *reinterpret_cast<uint4*>(out + at + apart) = v;
+    h += kBatch * p.lanes_of_heads;
+    load();
   }
 }
 
@@ -191,19 +213,26 @@ extern "C" SDPA_B200_API int sdpa_b200_rotary(const sdpa_b200_rotary_params* p, 
     r.axis_end[a] = a < p->axes - 1 ? end : kMaxPairs;
   }
   r.positions_64 = p->positions_64;
-  r.interleaved = p->interleaved;
   r.scaling = p->scaling;
   r.sign = p->inverse ? -1.f : 1.f;
-  r.tokens_per_block = r.tokens >= 2048 ? 4 : 1;
-  const int64_t blocks = (r.tokens + r.tokens_per_block - 1) / r.tokens_per_block;
+  r.chunks = r.half / 8 + (r.head_dim - 2 * r.half) / 8;
+  r.lanes_of_heads = 32 / r.chunks;
+  // a warp per token, or where that leaves SMs idle several with a share of its heads each
+  r.splits = 1;
+  r.heads_per_split = r.heads;
+  while (r.tokens * r.splits < kEnoughWarps && r.heads_per_split > r.lanes_of_heads) {
+    r.heads_per_split = (r.heads_per_split + 2 * r.lanes_of_heads - 1) / (2 * r.lanes_of_heads) * r.lanes_of_heads;
+    r.splits = (r.heads + r.heads_per_split - 1) / r.heads_per_split;
+  }
+  const int64_t blocks = (r.tokens * r.splits + kWarps - 1) / kWarps;
   if (blocks > 0x7fffffff) {
     set_error("rotary: too many tokens");
     return SDPA_B200_INVALID_ARG;
   }
-  const size_t smem = static_cast<size_t>(r.tokens_per_block) * r.half * sizeof(float2);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p->dtype == SDPA_B200_F16) rotary_kernel<true><<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(r);
-  else rotary_kernel<false><<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(r);
+  const bool f16 = p->dtype == SDPA_B200_F16;
+  auto kernel = p->interleaved ? (f16 ? rotary_kernel<true, true> : rotary_kernel<false, true>) : (f16 ? rotary_kernel<true, false> : rotary_kernel<false, false>);
+  kernel<<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(r);
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) {
     set_error("rotary: launch failed: %s", cudaGetErrorString(err));
