@@ -3,16 +3,17 @@
 //
 // With lengths c_i and c_i + n_i and pages(x) = ceil(x / block_size), request i takes max(0, pages(c_i + n_i) - pages(c_i)) blocks off the front of
 // the ring of free ones and gives max(0, the reverse) back at its end; the running sums over the requests say at which place of the ring each finds
-// its own, and where its tokens stand. All of it is a few loads deep: a launch's latency bounds it, not bytes. So it is one cluster: every block of it
+// its own, and where its tokens stand; a token or a page finds its request by bisection in them. All of it is a few loads deep: a launch's latency bounds it, not bytes. So it is one cluster: every block of it
 // forms the running sums for itself (in shared memory, 12 bytes a request), then they share out the tokens and the pages, and a cluster barrier keeps the
-// state from being written before all have read it, which lets a caller hand over the same tensors for old and new state.
+// state from being written before all have read it, which lets a caller hand over the same tensors for old and new state. Measured on the device: 64 decoding
+// requests 4.2 us, 256 requests with 16384 tokens 7.9 us (9.3 with a warp for each request's pages and 512 threads a block).
 #include "kernels.h"
 #include "ptx_sm100.cuh"
 
 namespace sdpa_b200 {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kMaxBatch = 16384;  // three running sums of it fit a block's shared memory
 
 struct Sums {
@@ -63,7 +64,8 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_par
     if (lane == 31) warp_sums[warp] = run;
     __syncthreads();
     long long t0 = all_tokens, n0 = all_need, f0 = all_freed;
-    for (int w = 0; w < kThreads / 32; ++w) {
+    const int warps = min(kThreads, p.batch - base + 31) / 32;  // those that have requests
+    for (int w = 0; w < warps; ++w) {
       const Sums s = warp_sums[w];
       if (w < warp) {
         t0 += s.tokens;
@@ -93,32 +95,38 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_par
     return static_cast<int>(x < 0 ? x + p.num_blocks : x);
   };
 
-  // ---- tokens: the request of each by bisection in the running sums
-  for (int t = rank * kThreads + tid; t < p.num_tokens; t += ranks * kThreads) {
+  // The last of `sums` at or below x: the request that x falls to (of those that begin at one place all but the last have nothing)
+  int top = 1;
+  while (2 * top < p.batch) top *= 2;
+  auto find = [&](const int* sums, int x) {
+    int i = 0;
+    for (int s = top; s > 0; s /= 2)
+      if (i + s < p.batch && sums[i + s] <= x) i += s;
+    return i;
+  };
+  const int threads = ranks * kThreads, thread = rank * kThreads + tid;
+  // ---- tokens
+  for (int t = thread; t < p.num_tokens; t += threads) {
     int pos = 0, slot = -1;
     if (t < total) {
-      int lo = 0, hi = p.batch - 1;  // the last request whose tokens begin at or before t, among which empty ones come first
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (s_tokens[mid] <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      const int c = p.cached_lens[lo];
-      pos = c + t - s_tokens[lo];
+      const int i = find(s_tokens, t), c = p.cached_lens[i];
+      pos = c + t - s_tokens[i];
       const int page = pos >> shift, had = pages_of(c, shift);
-      const int block = page < had ? p.block_table[lo * p.table_stride + page] : p.ring[ring_at(s_need[lo] + page - had)];
-      slot = block < 0 || block >= p.num_blocks ? -1 : (block << shift) + (pos & ((1 << shift) - 1));
+      const int block = page < had ? p.block_table[i * p.table_stride + page] : p.ring[ring_at(s_need[i] + page - had)];
+      if (block >= 0 && block < p.num_blocks) slot = (block << shift) + (pos & ((1 << shift) - 1));
     }
     p.positions[t] = pos;
     p.slots[t] = slot;
   }
-  // ---- pages that change hands: a warp per request
+  // ---- pages that change hands
   if (fine) {
-    for (int i = rank * (kThreads / 32) + warp; i < p.batch; i += ranks * (kThreads / 32)) {
-      const int c = p.cached_lens[i], had = pages_of(c, shift), has = pages_of(c + p.new_tokens[i], shift);
-      int32_t* row = p.block_table + i * p.table_stride;
-      for (int page = had + lane; page < has; page += 32) row[page] = p.ring[ring_at(s_need[i] + page - had)];
-      for (int page = has + lane; page < had; page += 32) p.ring[ring_at(static_cast<long long>(count) + s_freed[i] + page - has)] = row[page];
+    for (int x = thread; x < static_cast<int>(all_need); x += threads) {
+      const int i = find(s_need, x);
+      p.block_table[i * p.table_stride + pages_of(p.cached_lens[i], shift) + x - s_need[i]] = p.ring[ring_at(x)];
+    }
+    for (int x = thread; x < static_cast<int>(all_freed); x += threads) {
+      const int i = find(s_freed, x);
+      p.ring[ring_at(static_cast<long long>(count) + x)] = p.block_table[i * p.table_stride + pages_of(p.cached_lens[i] + p.new_tokens[i], shift) + x - s_freed[i]];
     }
   }
   cluster_sync();  // everybody has read the old lengths and state
@@ -177,7 +185,7 @@ extern "C" SDPA_B200_API int sdpa_b200_plan_step(const sdpa_b200_plan_params* p,
     }
   }
   // one block for a decode step; for more tokens up to eight, the largest cluster that every device takes
-  const int ranks = p->num_tokens <= 2 * kThreads ? 1 : p->num_tokens <= 8 * kThreads ? 4 : 8;
+  const int ranks = p->num_tokens <= kThreads && p->batch <= kThreads ? 1 : p->num_tokens <= 2 * kThreads ? 4 : 8;
   const cudaError_t err = launch_behind(plan_kernel, dim3(ranks), kThreads, smem, static_cast<cudaStream_t>(stream), false, ranks, *p, shift);
   if (err != cudaSuccess) {
     set_error("plan_step: launch failed: %s", cudaGetErrorString(err));

@@ -64,9 +64,23 @@ std::vector<Tensor> plan_step(const Tensor& cached_lens, const Tensor& new_token
               "cached_lens and new_tokens must be [requests], ring [num_blocks], ring_state [3]");
   TORCH_CHECK(num_tokens > 0, "num_tokens must be positive (got ", num_tokens, ")");
   c10::cuda::CUDAGuard guard(cached_lens.device());
-  std::vector<Tensor> step = {in_place ? cached_lens : new_tensor({B}, at::kInt, cached_lens), new_tensor({B + 1}, at::kInt, cached_lens),
-                              new_tensor({num_tokens}, at::kInt, cached_lens), new_tensor({num_tokens}, at::kInt, cached_lens),
-                              in_place ? ring_state : new_tensor({3}, at::kInt, cached_lens)};
+  // the results are cut out of one allocation: five took the host longer than the step takes the GPU
+  const int64_t sizes[5] = {in_place ? 0 : B, B + 1, num_tokens, num_tokens, in_place ? 0 : 3};
+  const Tensor all = new_tensor({sizes[0] + sizes[1] + sizes[2] + sizes[3] + sizes[4]}, at::kInt, cached_lens);
+  std::vector<Tensor> step;
+  step.reserve(5);
+  int64_t at = 0;
+  for (const int64_t n : sizes) {
+    Tensor x = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    x.unsafeGetTensorImpl()->set_storage_offset(at);
+    x.unsafeGetTensorImpl()->set_sizes_contiguous(n);
+    step.push_back(std::move(x));
+    at += n;
+  }
+  if (in_place) {
+    step[0] = cached_lens;
+    step[4] = ring_state;
+  }
   sdpa_b200_plan_params p = {};
   p.cached_lens = cached_lens.data_ptr<int32_t>();
   p.new_tokens = new_tokens.data_ptr<int32_t>();
