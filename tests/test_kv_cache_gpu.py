@@ -269,6 +269,7 @@ def test_some_rows_each(cuda_device, lens, rows, hq, hkv, dim, block, code, dtyp
 
 MANY_ROWS = [
     ([700, 600], [513, 520], 8, 2, 128, 64), ([1300, 130, 64], [600, 1, 0], 4, 4, 64, 16), ([300, 1000], [299, 300], 16, 2, 128, 128), ([520], [530], 1, 1, 64, 32),
+    ([500, 0, 300], [490, 3, 300], 32, 2, 64, 16), ([257, 129, 128], [300, 129, 256], 32, 4, 64, 64), ([1000], [1000], 64, 8, 128, 32),
 ]
 
 
@@ -281,7 +282,22 @@ def test_many_rows_each(cuda_device, lens, rows, hq, hkv, dim, block, code, dtyp
     assert ops.device_status() == 0
 
 
-@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 600, 1]])
+def test_both_paths_are_taken(cuda_device):
+    """Many rows of many heads go through 16-bit copies in the workspace, which is then large; few do not, however long the table is."""
+    torch.cuda.synchronize()
+    used = []
+    for rows, hq in (([1000], 64), ([2], 64)):
+        b = _batch(cuda_device, [20000], rows, hq, 8, 128, 64, E4M3, torch.bfloat16)
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        _run(b)
+        used.append(torch.cuda.max_memory_allocated() - before)
+    copies = 2 * 20096 * 8 * 128 * 2
+    assert used[0] > copies > 3 * used[1]
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 600, 1], [3, 1100, 1]])
 def test_a_bad_block_spoils_its_own_request_only(cuda_device, rows):
     b = list(_batch(cuda_device, [700, 650, 70], rows, 8, 2, 128, 16, E4M3, torch.bfloat16))
     b[5][1, 20] = (-1, 10 ** 6)[rows[0] == 1]
@@ -304,7 +320,7 @@ def test_rows_outside_every_request_are_left(cuda_device):
     """Offsets that begin behind the first row and end in front of the last; the outputs are read through the C ABI into buffers of a known filling."""
     import ctypes
     from torch_mlu_b200 import _cabi
-    for rows, many in (([1, 2], False), ([530, 2], True)):
+    for rows, many in (([1, 2], False), ([530, 2], True), ([1600, 2], True)):
         q, kc, vc, ks, vs, table, lens, cu = _batch(cuda_device, [600, 64], rows, 4, 2, 64, 32, INT8, torch.bfloat16)
         pad = torch.full((3, 4, 64), math.nan, dtype=q.dtype, device=cuda_device)
         q2, cu2 = torch.cat([pad, q, pad]), cu + 3
@@ -333,7 +349,7 @@ def test_rows_outside_every_request_are_left(cuda_device):
         _compare(out[3:-3], lse[:, 3:-3], (q, kc, vc, ks, vs, table, lens, cu), many=many)
 
 
-@pytest.mark.parametrize("rows", [1, 560])
+@pytest.mark.parametrize("rows", [1, 560, 1100])
 def test_layouts(cuda_device, rows):
     """A cache whose blocks hold all heads of a token side by side, table rows and queries that are slices, against the plain ones: the same bits."""
     lens, each = [600, 700], [rows, 2]
@@ -392,7 +408,7 @@ def test_offsets_past_32_bits(cuda_device):
     _same_cache(kc[mine], ks[mine], *want)
 
 
-@pytest.mark.parametrize("rows", [1, 3, 530])
+@pytest.mark.parametrize("rows", [1, 3, 530, 1100])
 def test_captured_and_replayed(cuda_device, rows):
     """One captured call, replayed with other lengths, tables and queries; and two graphs that run side by side."""
     lens = [600, 900]

@@ -79,13 +79,17 @@ __device__ __forceinline__ Request request_at(const StreamParams& p, int b) {
 }
 
 // Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB.
-template <int kD>
-__host__ __device__ constexpr int ring_stages() { return 3 * (128 / kD); }
+template <int kRowWarps, int kD>
+__host__ __device__ constexpr int ring_stages() { return kD == 64 ? 6 : kRowWarps == 4 ? 2 : 3; }
 template <int kD>
 __host__ __device__ constexpr uint32_t stage_bytes() { return 2u * kTileTokens * kD; }
-template <int kD>
+// B fragments of Q: in registers where there is room; else in shared memory, for each group of 16 rows
+template <int kRowBlocks, int kD>
+__host__ __device__ constexpr bool q_in_registers() { return kRowBlocks == 1 || kD == 64; }
+template <int kRowBlocks, int kRowWarps, int kD>
 __host__ __device__ constexpr uint32_t stream_smem_bytes() {
-  return 1024 + ring_stages<kD>() * (stage_bytes<kD>() + kSlots * 16 + 16) + 16 + kWarps * 16 * 8;
+  return 1024 + ring_stages<kRowWarps, kD>() * (stage_bytes<kD>() + kSlots * 16 + 16) + 16 + kWarps * 16 * 8 +
+         (q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 16) * 2 * 128);
 }
 
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
@@ -168,7 +172,8 @@ template <int kRowBlocks, int kRowWarps, int kD, bool kInt8>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
   constexpr int kChunks = kD / 16;                           // 16 dimensions each
-  constexpr int kSt = ring_stages<kD>();
+  constexpr int kSt = ring_stages<kRowWarps, kD>();
+  constexpr bool kQInRegisters = q_in_registers<kRowBlocks, kD>();
   constexpr uint32_t kStageBytes = stage_bytes<kD>();
   constexpr int kParts = kWarps / kRowWarps;                 // of a tile's tokens
   constexpr int kPartTokens = kTileTokens / kParts;
@@ -182,8 +187,10 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
   float4* slot_scales = reinterpret_cast<float4*>(ring_ptr + kSt * kStageBytes);  // [stage][16 tokens]: of K, log2 of that of V, kSumUnit over that of V
   float2* row_state = reinterpret_cast<float2*>(slot_scales + kSt * kSlots);      // [warp][row]: maximum and sum
-  const uint32_t full = smem_u32(row_state + kWarps * 16), empty = full + 8 * kSt;
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(row_state + kWarps * 16) + 2 * kSt);
+  uint2* q_state = reinterpret_cast<uint2*>(row_state + kWarps * 16);             // [row group][block of 8 rows][chunk][lane]: B fragments
+  constexpr int kQWords = kQInRegisters ? 0 : kRowWarps * kRowBlocks * kChunks * 32;
+  const uint32_t full = smem_u32(q_state + kQWords), empty = full + 8 * kSt;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(q_state + kQWords) + 2 * kSt);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -338,7 +345,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const int n_rows = min(p.rows, r.rows_q * p.group - row0);
       const int my_row0 = row0 + kRowsOfWarp * row_group;
       // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 4t..4t+3 of every 16
-      uint32_t qb[kRowBlocks][kChunks][2];
+      uint32_t qb[kRowBlocks][kQInRegisters ? kChunks : 1][2];
+      uint2* my_q = q_state + row_group * kRowBlocks * kChunks * 32 + lane;
       float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale
       int2 limit[kRowBlocks];     // how many tokens they see
 #pragma unroll
@@ -362,13 +370,19 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) {
           const float2 a = p.f16 ? unpack_16x2<true>(w[k].x) : unpack_16x2<false>(w[k].x), b = p.f16 ? unpack_16x2<true>(w[k].y) : unpack_16x2<false>(w[k].y);
-          qb[nb][k][0] = pack_f16x2(a.x * up, a.y * up);
-          qb[nb][k][1] = pack_f16x2(b.x * up, b.y * up);
+          const uint2 packed = make_uint2(pack_f16x2(a.x * up, a.y * up), pack_f16x2(b.x * up, b.y * up));
+          if constexpr (kQInRegisters) {
+            qb[nb][k][0] = packed.x;
+            qb[nb][k][1] = packed.y;
+          } else if (part == 0) {
+            my_q[(nb * kChunks + k) * 32] = packed;
+          }
         }
         const int sees = p.causal ? min(r.len, i + 1 + r.len - r.rows_q) : r.len;
         factor[nb] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
         limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
+      if constexpr (!kQInRegisters) arithmetic_sync();
       // tokens that all of the warp's rows see, and those that any of them does
       const int last_row = min(my_row0 + kRowsOfWarp - 1, row0 + n_rows - 1);
       const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.len - r.rows_q) : r.len;
@@ -391,20 +405,32 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         __syncwarp();
-#pragma unroll 1
-        for (int c = 0; c < kPartTokens; c += kStepTokens) {
-          const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
-          if (tok >= seen_by_any) break;
-          const uint32_t k_smem = ring + st * kStageBytes + in_tile * kD, v_smem = k_smem + kTileTokens * kD;
-
-          // ---- S^T = K Q^T, 16 tokens at a time. The contraction runs over head_dim in the order in which ldmatrix hands out bytes
-          float s[kRowBlocks][2][4];  // tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
+        // ---- S^T = K Q^T, 16 tokens at a time. The contraction runs over head_dim in the order in which ldmatrix hands out bytes
+        // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
+        auto scores = [&](int c, float (&s)[kRowBlocks][2][4]) {
+          const uint32_t k_smem = ring + st * kStageBytes + (part * kPartTokens + c) * kD;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
             for (int nb = 0; nb < kRowBlocks; ++nb) s[nb][half][0] = s[nb][half][1] = s[nb][half][2] = s[nb][half][3] = 0.f;
 #pragma unroll
-            for (int ch = 0; ch < kChunks; ch += 2) {
+          for (int ch = 0; ch < kChunks; ch += 2) {
+            uint32_t q[2][kRowBlocks][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int nb = 0; nb < kRowBlocks; ++nb) {
+                if constexpr (kQInRegisters) {
+                  q[e][nb][0] = qb[nb][ch + e][0];
+                  q[e][nb][1] = qb[nb][ch + e][1];
+                } else {
+                  const uint2 w = my_q[(nb * kChunks + ch + e) * 32];
+                  q[e][nb][0] = w.x;
+                  q[e][nb][1] = w.y;
+                }
+              }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
               uint32_t kf[4];  // tokens 0-7 and 8-15 of a chunk, the same of the next
               ldmatrix_x4(k_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), kf);
 #pragma unroll
@@ -413,10 +439,18 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 codes_to_f16<kInt8>(kf[2 * e], a0, a2);
                 codes_to_f16<kInt8>(kf[2 * e + 1], a1, a3);
 #pragma unroll
-                for (int nb = 0; nb < kRowBlocks; ++nb) mma_16816<true>(s[nb][half], a0, a1, a2, a3, qb[nb][ch + e][0], qb[nb][ch + e][1]);
+                for (int nb = 0; nb < kRowBlocks; ++nb) mma_16816<true>(s[nb][half], a0, a1, a2, a3, q[e][nb][0], q[e][nb][1]);
               }
             }
           }
+        };
+#pragma unroll 1
+        for (int c = 0; c < kPartTokens; c += kStepTokens) {
+          const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
+          if (tok >= seen_by_any) break;
+          const uint32_t v_smem = ring + st * kStageBytes + in_tile * kD + kTileTokens * kD;
+          float s[kRowBlocks][2][4];
+          scores(c, s);
           const float4 sc0 = slot_scales[st * kSlots + in_tile / 16], sc1 = slot_scales[st * kSlots + in_tile / 16 + 1];
           uint32_t pb[kRowBlocks][2][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
           bool moved = false;
@@ -716,29 +750,44 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       cu_k[2 * p.batch] = before + padded;
     }
   }
-  constexpr int kLanes = kD / 16;  // 16 codes a thread
-  for (int i = tid; i < kGatherTokens * kLanes; i += 256) {
-    const int tok = blockIdx.x * kGatherTokens + i / kLanes, at = i % kLanes * 16;
-    if (tok >= padded) break;
-    const int page = tok >> p.shift, place = tok & ((1 << p.shift) - 1);
-    const int id = tok < len && page < p.max_blocks ? p.block_table[b * p.table_stride + page] : -1;
-    const bool bad = id < 0 || id >= p.num_blocks;
+  constexpr int kLanes = kD / 16, kTimes = kGatherTokens * kLanes / 256;  // 16 codes of K and of V a thread and time
+  static_assert(kTimes >= 1, "a block has threads to spare");
+  const int tok0 = blockIdx.x * kGatherTokens + tid / kLanes, at = tid % kLanes * 16;
+  int id[kTimes];
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int tok = tok0 + i * (256 / kLanes), page = tok >> p.shift;
+    id[i] = tok < len && page < p.max_blocks ? p.block_table[b * p.table_stride + page] : -1;
+  }
+  uint4 w[kTimes][2];
+  float scale[kTimes][2];
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int tok = tok0 + i * (256 / kLanes), place = tok & ((1 << p.shift) - 1);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      float scale = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;  // a block outside the cache: its scores are NaN, for those who see them
-      if (!bad) {
-        w = *reinterpret_cast<const uint4*>(p.cache[x] + id * p.block[x] + h * p.head[x] + place * p.row[x] + at);
-        scale = p.scale[x][static_cast<int64_t>(id) * p.heads + h];
-      }
-      uint32_t f[8], c[4] = {w.x, w.y, w.z, w.w};
+      w[i][x] = make_uint4(0u, 0u, 0u, 0u);
+      // a block outside the cache: its scores are NaN, for those who see them
+      scale[i][x] = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
+      if (id[i] < 0 || id[i] >= p.num_blocks) continue;
+      w[i][x] = *reinterpret_cast<const uint4*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
+      scale[i][x] = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+    const int tok = tok0 + i * (256 / kLanes);
+    if (tok >= padded) break;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      uint32_t f[8], c[4] = {w[i][x].x, w[i][x].y, w[i][x].z, w[i][x].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t lo, hi;
         codes_to_f16<kInt8>(c[e], lo, hi);
         const float2 u = unpack_16x2<true>(lo), v = unpack_16x2<true>(hi);
-        f[2 * e] = pack_16x2<kF16>(u.x * scale, u.y * scale);
-        f[2 * e + 1] = pack_16x2<kF16>(v.x * scale, v.y * scale);
+        f[2 * e] = pack_16x2<kF16>(u.x * scale[i][x], u.y * scale[i][x]);
+        f[2 * e + 1] = pack_16x2<kF16>(v.x * scale[i][x], v.y * scale[i][x]);
       }
       uint4* dst = reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at);
       dst[0] = make_uint4(f[0], f[1], f[2], f[3]);
@@ -747,12 +796,17 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
   }
 }
 
-// Rows that the longest request may have for path 1: above, path 2. At 32/8 heads a unit of 16 rows streams the cache in HBM's time, and each further one
-// adds that of its products; the prefill kernel works on tiles of 256 rows of one query head.
-constexpr int kMostStreamRows = 512;
-
+// Path 1 costs its units of 64 rows, path 2 the gathering of every kv head's tokens and the prefill kernel's waves of units of up to 256 rows of a query head, all per token in
+// the cache. So the length does not decide, and in units of 64 rows a token's gathering is 0.9 and a wave 95 (head_dim 64: 135). Measured, 4 requests of 5000 tokens,
+// us, path 1 | 2: 32/8 heads of 128, 24 rows 59 | 91, 40 80 | 93, 64 101 | 93, 96 144 | 94; 16/16, 64 61 | 112, 96 101 | 113, 160 143 | 122; 64/8, 40 123 | 153,
+// 64 186 | 154; 16/4 of 64, 64 41 | 64, 96 54 | 65, 160 82.6 | 81.7.
 bool streams(const sdpa_b200_cache_params& p) {
-  return static_cast<int64_t>(p.max_seqlen_q) * (p.heads_q / p.heads_kv) <= kMostStreamRows || p.cu_seqlens_q == nullptr;
+  const int64_t group = p.heads_q / p.heads_kv, batch = p.batch;
+  if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64) return true;
+  // requests of equal rows, or of any: half a unit each is empty then
+  const double units = p.total_q == batch * p.max_seqlen_q ? static_cast<double>(batch * ((p.max_seqlen_q * group + 63) / 64)) : p.total_q * group / 64.0 + 0.5 * batch;
+  const int64_t blocks = p.heads_q * std::max<int64_t>(batch, (p.total_q + 255) / 256);
+  return (units - 0.9 * batch) * p.heads_kv <= (p.head_dim == 64 ? 135.0 : 95.0) * static_cast<double>((blocks + 147) / 148);
 }
 
 int check_attention(const sdpa_b200_cache_params* p) {
@@ -874,8 +928,8 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   auto launch = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag) {
     constexpr bool kInt8 = decltype(int8_tag)::value;
     constexpr int kRowBlocks = decltype(blocks_tag)::value, kRowWarps = decltype(rows_tag)::value, kD = decltype(dim_tag)::value;
-    constexpr uint32_t kSmem = stream_smem_bytes<kD>();
-    static_assert(kCtasPerSm * (kSmem + 1024 + 64) <= 228 * 1024, "two CTAs do not fit an SM");
+    constexpr uint32_t kSmem = stream_smem_bytes<kRowBlocks, kRowWarps, kD>();
+    static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "two CTAs do not fit an SM");
     auto kernel = cache_stream_kernel<kRowBlocks, kRowWarps, kD, kInt8>;
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (err == cudaSuccess) err = launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, c.device_status != nullptr, 1, tm_k, tm_v, p);
