@@ -471,3 +471,82 @@ def test_refusals(cuda_device):
         kv_cache.plan_step(lens, lens, table, slots, _ints(cuda_device, [0, 2, 0]), block_size=24, num_tokens=4)
     with pytest.raises(RuntimeError, match="ring_state"):
         kv_cache.plan_step(lens, lens, table, slots, slots, block_size=16, num_tokens=4)
+
+
+# ---------------------------------------------------------------------------------------------- all of it together
+@pytest.mark.parametrize("code,dtype,block,captured", [(E4M3, torch.bfloat16, 16, False), (INT8, torch.float16, 32, False), (E4M3, torch.bfloat16, 64, True)])
+def test_serving_loop(cuda_device, code, dtype, block, captured):
+    """Requests come, grow and end over some thirty steps of two layers: prompts, decode steps, padded token counts, dropped tokens, blocks that change hands. Every
+    step's codes, scales and results are held to the restatements, on a cache that the restatements keep for themselves."""
+    layers, hq, hkv, dim, requests, most = 2, 8, 2, 64, 5, 12
+    cache = kv_cache.PagedCache(layers, 40 * 64 // block, hkv, dim, requests, most * 64 // block, block_size=block, dtype=code, device=cuda_device)
+    g = torch.Generator().manual_seed(block)
+    inv_freq = (1e4 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))).float().to(cuda_device)
+    state = [[0] * requests, [list(r) for r in cache.block_table.tolist()], cache.ring.tolist(), cache.ring_state.tolist()]
+    mirror = [[(c[i].cpu().float().nan_to_num(0).double(), s[i].cpu().double()) for c, s in ((cache.key_cache, cache.key_scale), (cache.value_cache, cache.value_scale))]
+              for i in range(layers)]
+    tokens = 150
+    q, k, v = (torch.zeros(tokens, h, dim, dtype=dtype, device=cuda_device) for h in (hq, hkv, hkv))
+    news = torch.zeros(requests, dtype=torch.int32, device=cuda_device)
+
+    def step():
+        plan = cache.step(news, tokens)
+        got = []
+        for i in range(layers):
+            qi, ki, vi = q * (i + 1), k * (i + 1), v * (1 + 0.5 * i)
+            out, lse = cache.attend(i, qi, ki, vi, 64, most * 64, inv_freq=inv_freq)
+            got.append((qi, ki, vi, out, lse))
+        return plan, got
+
+    graph = None
+    for it in range(30):
+        new = []
+        for c in state[0]:
+            r = float(torch.rand((), generator=g))
+            new.append(int(40 * r * 2) if c == 0 and r < 0.6 else 0 if c == 0 else -c if r < 0.08 or c > 600 else -min(c - 1, 3) if r < 0.2 else 1 if r < 0.9 else 60)
+        while sum(max(n, 0) for n in new) > tokens:
+            new[max(range(requests), key=lambda i: new[i])] //= 2
+        want = orc.plan_step(state[0], new, state[1], state[2], state[3], block, tokens)
+        news.copy_(torch.tensor(new, dtype=torch.int32))
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g))
+        k[want[1][-1]:] = math.nan  # behind the last token there may be anything
+        v[want[1][-1]:] = math.inf
+        if not captured:
+            plan, got = step()
+        else:
+            if graph is None:
+                keep = [t.clone() for t in (cache.lens, cache.block_table, cache.ring, cache.ring_state, cache.key_cache, cache.value_cache, cache.key_scale, cache.value_scale)]
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    step()
+                side.synchronize()
+                for t, old in zip((cache.lens, cache.block_table, cache.ring, cache.ring_state, cache.key_cache, cache.value_cache, cache.key_scale, cache.value_scale), keep):
+                    t.copy_(old)
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    plan, got = step()
+            graph.replay()
+        torch.cuda.synchronize()
+        assert [x.tolist() for x in (plan.seq_lens, plan.cu_seqlens, plan.positions, plan.slots, plan.ring_state, cache.block_table, cache.ring)] == list(want), it
+        assert cache.refused() == want[4][2]
+        state = [want[0], want[5], want[6], want[4]]
+        for i, (qi, ki, vi, out, lse) in enumerate(got):
+            for which, (x, c, s) in enumerate(((ki, cache.key_cache[i], cache.key_scale[i]), (vi, cache.value_cache[i], cache.value_scale[i]))):
+                values, scales = mirror[i][which]
+                mirror[i][which] = orc.store(x, plan.slots, values.to(code), scales)
+                used = torch.zeros(values.shape[0], values.shape[2], dtype=torch.bool)
+                for row, n in zip(state[1], state[0]):
+                    for p in range(n):
+                        used[row[p // block], p % block] = True
+                got_codes = c.cpu().float().double()
+                same = (got_codes == mirror[i][which][0]) | (got_codes.isnan() & mirror[i][which][0].isnan())
+                assert bool((same | ~used[:, None, :, None]).all()), (it, i, which)
+                touched = used.any(1)
+                assert torch.equal(s.cpu().double()[touched], mirror[i][which][1][touched])
+            live = want[1][-1]
+            if live:
+                b = (qi[:live], cache.key_cache[i], cache.value_cache[i], cache.key_scale[i], cache.value_scale[i], cache.block_table, plan.seq_lens, plan.cu_seqlens)
+                _compare(out[:live], lse[:, :live], b)
+    assert ops.device_status() == 0

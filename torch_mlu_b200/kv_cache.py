@@ -9,7 +9,7 @@ Keys and values of all requests live in blocks of ``block_size`` tokens: codes [
     store(k, v, step.slots, key_cache, value_cache, key_scale, value_scale)
     out, lse = attention(q, key_cache, value_cache, key_scale, value_scale, block_table, step.seq_lens, step.cu_seqlens, max_q, max_k)
 
-None of it reads anything back to the host. The reference has no paged cache.
+None of it reads anything back to the host. ``PagedCache`` keeps the tensors and makes these calls. The reference has no paged cache.
 """
 from __future__ import annotations
 
@@ -17,9 +17,9 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import torch_glue
+from . import rotary, torch_glue
 
-__all__ = ["plan_step", "store", "attention", "StepPlan", "BLOCK_SIZES"]
+__all__ = ["plan_step", "store", "attention", "StepPlan", "PagedCache", "BLOCK_SIZES"]
 
 BLOCK_SIZES = (16, 32, 64, 128)
 
@@ -82,3 +82,56 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     """
     return _calls().cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k,
                                     is_causal, scale)
+
+
+class PagedCache:
+    """The cache of a model's layers and its bookkeeping, for up to ``max_requests`` requests of up to ``max_blocks`` blocks each.
+
+        cache = PagedCache(layers, num_blocks, heads_kv, head_dim, max_requests, max_blocks)
+        cache.step(new_tokens, num_tokens)                          # int32 [max_requests] on the device
+        for layer in range(layers):
+            out, lse = cache.attend(layer, q, k, v, max_seqlen_q, max_seqlen_k, inv_freq=inv_freq)
+
+    A row of the table is a request; one that gets no new tokens takes no part in the step, and one that gives all of its tokens back (minus its length) is
+    free for another. Lengths and free blocks are kept on the device and written in place, so that a captured step can be replayed.
+    """
+
+    def __init__(self, layers: int, num_blocks: int, heads_kv: int, head_dim: int, max_requests: int, max_blocks: int, *, block_size: int = 64,
+                 dtype: torch.dtype = torch.float8_e4m3fn, device="cuda"):
+        if dtype not in (torch.float8_e4m3fn, torch.int8):
+            raise RuntimeError(f"the caches must both be float8_e4m3fn or int8 (got {dtype})")
+        if block_size not in BLOCK_SIZES:
+            raise RuntimeError(f"block_size must be 16, 32, 64 or 128 (got {block_size})")
+        shape = (layers, num_blocks, heads_kv, block_size, head_dim)
+        ints = dict(dtype=torch.int32, device=device)
+        self.block_size = block_size
+        self.key_cache, self.value_cache = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self.key_scale, self.value_scale = (torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+        self.block_table = torch.full((max_requests, max_blocks), -1, **ints)
+        self.lens = torch.zeros(max_requests, **ints)
+        self.ring = torch.arange(num_blocks, **ints)
+        self.ring_state = torch.tensor([0, num_blocks, 0], **ints)
+        self.plan: Optional[StepPlan] = None
+
+    def step(self, new_tokens, num_tokens: int) -> StepPlan:
+        """plan_step in place: lengths, blocks and free blocks move on by ``new_tokens``."""
+        self.plan = plan_step(self.lens, new_tokens, self.block_table, self.ring, self.ring_state, block_size=self.block_size, num_tokens=num_tokens,
+                              in_place=True)
+        return self.plan
+
+    def refused(self) -> int:
+        """Why the last step changed nothing, or 0: see plan_step. Waits for the device."""
+        return int(self.ring_state[2])
+
+    def attend(self, layer: int, query, key, value, max_seqlen_q: int = 1, max_seqlen_k: Optional[int] = None, *, inv_freq=None, positions=None,
+               sections=None, interleaved: bool = False, is_causal: bool = True, scale: Optional[float] = None):
+        """(output, logsumexp) of one layer for the tokens of the last step: keys and values ([tokens, heads_kv, head_dim]) go into the cache, then the queries
+        ([tokens, heads_q, head_dim]) see it. With ``inv_freq`` queries and keys are turned first, in place, by the step's positions or by those given
+        (see rotary.rotary_embedding)."""
+        if self.plan is None:
+            raise RuntimeError("PagedCache.attend: call step() first")
+        if inv_freq is not None:
+            rotary.rotary_embedding_(query, key, self.plan.positions if positions is None else positions, inv_freq, sections=sections, interleaved=interleaved)
+        caches = (self.key_cache[layer], self.value_cache[layer], self.key_scale[layer], self.value_scale[layer])
+        store(key, value, self.plan.slots, *caches)
+        return attention(query, *caches, self.block_table, self.plan.seq_lens, self.plan.cu_seqlens, max_seqlen_q, max_seqlen_k, is_causal=is_causal, scale=scale)
