@@ -314,6 +314,34 @@ def test_a_request_longer_than_its_table_is_nan(cuda_device):
     b[6][0] = 100000
     out, lse = _run(b, max_k=128)
     assert bool(out[0].isnan().all()) and not bool(out[1].isnan().any())
+    # all of its rows, also those that stand in front of the last
+    b = list(_batch(cuda_device, [100, 90], [5, 2], 4, 2, 64, 16, E4M3, torch.bfloat16))
+    b[6][0] = b[5].size(1) * 16 + 1
+    out, lse = _run(b, max_k=400)
+    assert bool(out[:5].isnan().all()) and not bool(out[5:].isnan().any())
+
+
+def test_inference_mode(cuda_device):
+    """Tensors made under torch.inference_mode, as a server makes them."""
+    b = _batch(cuda_device, [100, 90], [5, 2], 4, 2, 64, 16, INT8, torch.bfloat16)
+    want = _run(b)
+    with torch.inference_mode():
+        c = tuple(t.clone() for t in b)
+        out, lse = _run(c)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        k = torch.randn(3, 2, 64, device=cuda_device).bfloat16()
+        kv_cache.store(k, k, _ints(cuda_device, [0, 1, 2]), c[1], c[2], c[3], c[4])
+        step = kv_cache.plan_step(c[6], torch.ones_like(c[6]), c[5], torch.arange(8, device=cuda_device).int(), _ints(cuda_device, [0, 8, 0]), block_size=16, num_tokens=4)
+        assert step.seq_lens.tolist() == [101, 91] and step.positions.tolist() == [100, 90, 0, 0]
+
+
+def test_gradients_are_refused(cuda_device):
+    b = list(_batch(cuda_device, [100, 90], [1, 1], 4, 2, 64, 16, INT8, torch.float16))
+    b[0].requires_grad_()
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        _run(b)
+    with torch.no_grad():
+        assert not _run(b)[0].requires_grad
 
 
 def test_rows_outside_every_request_are_left(cuda_device):

@@ -165,6 +165,12 @@ def test_autograd_refuses_what_it_would_get_wrong(cuda_device):
         rotary.rotary_embedding_(x.clone().requires_grad_(), None, pos, f)
     with pytest.raises(RuntimeError, match="elements of their own"):
         rotary.rotary_embedding_(x[:, :1].expand(-1, 2, -1), None, pos, f)
+    with pytest.raises(RuntimeError, match="the same memory"):
+        rotary.rotary_embedding_(x, x, pos, f)
+    with torch.inference_mode():
+        y = x.clone()
+        want = rotary.rotary_embedding(x, None, pos, f)[0]
+        assert torch.equal(rotary.rotary_embedding_(y, None, pos, f)[0], want)
     with pytest.raises(RuntimeError, match="ordinary tensor"):
         torch.func.grad(lambda t: rotary.rotary_embedding(t, None, pos, f)[0].float().sum())(x)
     # a tensor saved for a backward pass and then turned in place is noticed

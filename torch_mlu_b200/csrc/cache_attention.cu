@@ -63,16 +63,19 @@ struct SharedUnit {
 // A request as units see it
 struct Request {
   int index, len, rows_q, q0;  // tokens in the cache, rows of q, the first of them
+  int in_front;                // row i sees i + 1 + in_front tokens where causal
   int tiles, units;            // per unit; 0 units: no rows
 };
 
 __device__ __forceinline__ Request request_at(const StreamParams& p, int b) {
   Request r;
   r.index = b;
-  r.len = min(max(p.seq_lens[b], 0), p.max_len);
+  const int len = p.seq_lens[b];
+  r.len = min(max(len, 0), p.max_len);
   r.q0 = p.cu_q ? p.cu_q[b] : b;
   r.rows_q = p.cu_q ? max(p.cu_q[b + 1] - r.q0, 0) : 1;
   if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
+  r.in_front = len > p.max_len - 1 ? r.len : r.len - r.rows_q;  // longer than the table: all its rows see the block that there is none of
   r.tiles = max((r.len + kTileTokens - 1) / kTileTokens, 1);  // an empty request has rows to write too
   r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
   return r;
@@ -215,7 +218,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     int b = r.index + 1;
     do {
       if (b >= p.batch) {
-        r = {b, 0, 0, 0, 1, 0};
+        r = {b, 0, 0, 0, 0, 1, 0};
         return;
       }
       r = request_at(p, b++);
@@ -378,15 +381,15 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             my_q[(nb * kChunks + k) * 32] = packed;
           }
         }
-        const int sees = p.causal ? min(r.len, i + 1 + r.len - r.rows_q) : r.len;
+        const int sees = p.causal ? min(r.len, i + 1 + r.in_front) : r.len;
         factor[nb] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
         limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
       if constexpr (!kQInRegisters) arithmetic_sync();
       // tokens that all of the warp's rows see, and those that any of them does
       const int last_row = min(my_row0 + kRowsOfWarp - 1, row0 + n_rows - 1);
-      const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.len - r.rows_q) : r.len;
-      const int seen_by_any = my_row0 >= row0 + n_rows ? 0 : p.causal ? min(r.len, last_row / p.group + 1 + r.len - r.rows_q) : r.len;
+      const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.in_front) : r.len;
+      const int seen_by_any = my_row0 >= row0 + n_rows ? 0 : p.causal ? min(r.len, last_row / p.group + 1 + r.in_front) : r.len;
 
       float o[kRowBlocks][kChunks][4];  // dimensions 2g, 2g, 2g + 1, 2g + 1 of every 16, rows 2t, 2t + 1, 2t, 2t + 1
       float2 m[kRowBlocks], l[kRowBlocks];  // running maximum of score + log2 of V's scale; this thread's share of the sums, in units of kSumUnit

@@ -14,12 +14,13 @@ using at::Tensor;
 
 namespace {
 
-// An ordinary CUDA tensor: a wrapper (of torch.func, of a dispatch mode, without data) has nothing that a kernel could read.
+// A CUDA tensor with memory of its own: a wrapper (of torch.func, of a dispatch mode, without data) has nothing that a kernel could read.
 void check_plain(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be on a CUDA device (this path has no CPU fallback)");
-  constexpr c10::DispatchKeySet ordinary(
-      {c10::DispatchKey::CUDA, c10::DispatchKey::ADInplaceOrView, c10::DispatchKey::AutogradCUDA, c10::DispatchKey::AutocastCUDA});
-  TORCH_CHECK(ordinary.has_all(t.key_set()) && t.layout() == at::kStrided, name, " must be an ordinary tensor");
+  constexpr c10::DispatchKeySet wrapped =
+      c10::python_ks | c10::functorch_transforms_ks |
+      c10::DispatchKeySet({c10::DispatchKey::Functionalize, c10::DispatchKey::Negative, c10::DispatchKey::Conjugate, c10::DispatchKey::ZeroTensor});
+  TORCH_CHECK(!t.key_set().has_any(wrapped) && t.layout() == at::kStrided, name, " must be an ordinary tensor");
 }
 
 void check_ints(const Tensor& t, const char* name, const Tensor& like) {
@@ -185,6 +186,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& ke
     check_ints(*cu_seqlens, "cu_seqlens", query);
     TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->size(0) == B + 1, "cu_seqlens must have requests + 1 entries");
   }
+  TORCH_CHECK(!(query.requires_grad() && at::GradMode::is_enabled()), "attention over the cache has no gradient: call it under torch.no_grad()");
   c10::cuda::CUDAGuard guard(query.device());
   Tensor out = new_tensor({T, H, query.size(2)}, query.scalar_type(), query), lse = new_tensor({H, T}, at::kFloat, query);
   if (query.numel() == 0) return {out, lse};
@@ -374,6 +376,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& query, const Tensor& key, const 
   const RotaryCall c = {sections, interleaved, false, scaling};
   if (in_place) {
     TORCH_CHECK(!needs_grad(query) && !needs_grad(key), "rotary positions in place have no gradient: use rotary_embedding");
+    TORCH_CHECK(!key.defined() || query.numel() == 0 || key.data_ptr() != query.data_ptr(), "rotary positions in place: query and key are the same memory");
     for (const Tensor* t : {&query, &key}) {
       for (int64_t i = 0; t->defined() && i < t->dim(); ++i)
         TORCH_CHECK(t->size(i) <= 1 || t->stride(i) != 0, "rotary positions in place need elements of their own (a stride is 0)");

@@ -77,7 +77,7 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace, which takes
     4 * requests * max_seqlen_k * heads_kv * head_dim bytes, and the prefill kernel runs.
 
-    A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
+    There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package).
     """
     return _calls().cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k,
