@@ -6,7 +6,7 @@
 //
 // 1. Few rows per request (decode steps, drafted tokens): cache_stream_kernel, bound by the codes that come out of HBM. A unit is (request,
 //    kv head, chunk of up to 64 rows (query token, query head of the group)), whose codes are read once for all its rows: S^T = K Q^T and O^T = V^T W^T in
-//    mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 tokens,
+//    mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 or 256 tokens,
 //    so that all SMs stream the same number of bytes however long each request is. A unit that several CTAs worked on leaves fp32 parts in the workspace,
 //    at most two per CTA, and a second kernel merges them.
 //    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a copy takes its warp about
@@ -28,9 +28,6 @@ namespace {
 
 constexpr int kWarps = 4;                  // those that do the arithmetic
 constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are dealt out as for six warps anyway
-constexpr int kStepTokens = 32;            // tokens a warp handles at a time
-constexpr int kTileTokens = 128;
-constexpr int kSlots = kTileTokens / 16;   // the fewest tokens with scales of their own are 16
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
@@ -51,6 +48,8 @@ struct StreamParams {
   uint32_t* status;
   int64_t q_row, q_head, o_row, o_head, table_stride;
   int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
+  int tile_shift;  // log2 of a tile's tokens
+  int most_tiles;  // that a request may have, so that the sum of all stays in 32 bits
   int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
   float scale_log2;
 };
@@ -76,22 +75,28 @@ __device__ __forceinline__ Request request_at(const StreamParams& p, int b) {
   r.rows_q = p.cu_q ? max(p.cu_q[b + 1] - r.q0, 0) : 1;
   if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
   r.in_front = len > p.max_len - 1 ? r.len : r.len - r.rows_q;  // longer than the table: all its rows see the block that there is none of
-  r.tiles = max((r.len + kTileTokens - 1) / kTileTokens, 1);  // an empty request has rows to write too
+  r.tiles = max((r.len + (1 << p.tile_shift) - 1) >> p.tile_shift, 1);  // an empty request has rows to write too
   r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
   return r;
 }
 
-// Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB.
-template <int kRowWarps, int kD>
-__host__ __device__ constexpr int ring_stages() { return kD == 64 ? 6 : kRowWarps == 4 ? 2 : 3; }
+// Tokens of a tile, 32 KB of K and V, and those that a warp handles at a time: its products, maxima over lanes, exponentials and products again are one long chain, in which the
+// blocks of 16 tokens run beside each other; as many as registers hold.
 template <int kD>
-__host__ __device__ constexpr uint32_t stage_bytes() { return 2u * kTileTokens * kD; }
+__host__ __device__ constexpr int tile_tokens() { return kD == 64 ? 256 : 128; }
+template <int kD>
+__host__ __device__ constexpr int step_tokens() { return kD == 64 ? 64 : 32; }
+// Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB (64 rows: Q is there too).
+template <int kRowWarps, int kD>
+__host__ __device__ constexpr int ring_stages() { return kD == 128 && kRowWarps == 4 ? 2 : 3; }
+template <int kD>
+__host__ __device__ constexpr uint32_t stage_bytes() { return 2u * tile_tokens<kD>() * kD; }
 // B fragments of Q: in registers where there is room; else in shared memory, for each group of 16 rows
 template <int kRowBlocks, int kD>
 __host__ __device__ constexpr bool q_in_registers() { return kRowBlocks == 1 || kD == 64; }
 template <int kRowBlocks, int kRowWarps, int kD>
 __host__ __device__ constexpr uint32_t stream_smem_bytes() {
-  return 1024 + ring_stages<kRowWarps, kD>() * (stage_bytes<kD>() + kSlots * 16 + 16) + 16 + kWarps * 16 * 8 +
+  return 1024 + ring_stages<kRowWarps, kD>() * (stage_bytes<kD>() + tile_tokens<kD>() + 16) + 16 + kWarps * 16 * 8 +
          (q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 16) * 2 * 128);
 }
 
@@ -131,19 +136,18 @@ struct Share {
 
 // Every warp finds it for itself, so that none waits for another.
 __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int lane) {
-  auto tiles_of = [&](int b) -> int64_t {
+  auto tiles_of = [&](int b) {
     if (b >= p.batch) return 0;
     const Request r = request_at(p, b);
-    return static_cast<int64_t>(r.tiles) * r.units;
+    return static_cast<int>(min(static_cast<int64_t>(r.tiles) * r.units, static_cast<int64_t>(p.most_tiles)));
   };
-  int64_t total = 0;
+  const int of_first = tiles_of(lane);  // of the first 32 requests
+  int tiles = of_first;
 #pragma unroll 4
-  for (int b = lane; b < p.batch; b += 32) total += tiles_of(b);
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+  for (int b = lane + 32; b < p.batch; b += 32) tiles += tiles_of(b);
+  tiles = __reduce_add_sync(0xffffffffu, tiles);
   Share s = {0, 0, 0, 0, 0, 0, 0};
-  if (total <= 0 || total > INT32_MAX) return s;  // (2^31 tiles: offsets that are none)
-  const int tiles = static_cast<int>(total);
+  if (tiles == 0) return s;
   s.ctas = min(tiles, p.grid);  // those that get a tile: the others would leave no part where the merge looks for one
   s.each = tiles / s.ctas;
   s.longer = tiles - s.each * s.ctas;
@@ -151,7 +155,7 @@ __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int la
   s.first = cta * s.each + min(cta, s.longer);
   s.last = s.first + s.each + (cta < s.longer ? 1 : 0);
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int mine = static_cast<int>(tiles_of(b0 + lane));
+    const int mine = b0 == 0 ? of_first : tiles_of(b0 + lane);
     int run = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -179,6 +183,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   constexpr bool kQInRegisters = q_in_registers<kRowBlocks, kD>();
   constexpr uint32_t kStageBytes = stage_bytes<kD>();
   constexpr int kParts = kWarps / kRowWarps;                 // of a tile's tokens
+  constexpr int kTileTokens = tile_tokens<kD>(), kStepTokens = step_tokens<kD>(), kHalves = kStepTokens / 16;
+  constexpr int kSlots = kTileTokens / 16;                   // the fewest tokens with scales of their own are 16
   constexpr int kPartTokens = kTileTokens / kParts;
   constexpr int kRowsOfWarp = 8 * kRowBlocks;
   constexpr float kBias = 15.f;  // weights are kept times 2^15: the largest is 2^15, the smallest normal f16 number 2^-29 of it
@@ -410,10 +416,10 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         __syncwarp();
         // ---- S^T = K Q^T, 16 tokens at a time. The contraction runs over head_dim in the order in which ldmatrix hands out bytes
         // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
-        auto scores = [&](int c, float (&s)[kRowBlocks][2][4]) {
+        auto scores = [&](int c, float (&s)[kRowBlocks][kHalves][4]) {
           const uint32_t k_smem = ring + st * kStageBytes + (part * kPartTokens + c) * kD;
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < kHalves; ++half)
 #pragma unroll
             for (int nb = 0; nb < kRowBlocks; ++nb) s[nb][half][0] = s[nb][half][1] = s[nb][half][2] = s[nb][half][3] = 0.f;
 #pragma unroll
@@ -433,7 +439,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 }
               }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < kHalves; ++half) {
               uint32_t kf[4];  // tokens 0-7 and 8-15 of a chunk, the same of the next
               ldmatrix_x4(k_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), kf);
 #pragma unroll
@@ -452,18 +458,20 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
           if (tok >= seen_by_any) break;
           const uint32_t v_smem = ring + st * kStageBytes + in_tile * kD + kTileTokens * kD;
-          float s[kRowBlocks][2][4];
+          float s[kRowBlocks][kHalves][4];
           scores(c, s);
-          const float4 sc0 = slot_scales[st * kSlots + in_tile / 16], sc1 = slot_scales[st * kSlots + in_tile / 16 + 1];
-          uint32_t pb[kRowBlocks][2][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
+          float4 sc[kHalves];
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) sc[half] = slot_scales[st * kSlots + in_tile / 16 + half];
+          uint32_t pb[kRowBlocks][kHalves][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
           bool moved = false;
           float2 a[kRowBlocks];
 #pragma unroll
           for (int nb = 0; nb < kRowBlocks; ++nb) {
             // scores and log2 of V's scale, masked where a row ends inside the step
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float ks = half ? sc1.x : sc0.x, lv = half ? sc1.y : sc0.y;
+            for (int half = 0; half < kHalves; ++half) {
+              const float ks = sc[half].x, lv = sc[half].y;
               const float fx = factor[nb].x * ks, fy = factor[nb].y * ks;
               s[nb][half][0] = fmaf(s[nb][half][0], fx, lv);
               s[nb][half][1] = fmaf(s[nb][half][1], fy, lv);
@@ -472,7 +480,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
             if (tok + kStepTokens > seen_by_all) {
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
+              for (int half = 0; half < kHalves; ++half) {
                 const int j = tok + half * 16 + g;
                 if (j >= limit[nb].x) s[nb][half][0] = -INFINITY;
                 if (j >= limit[nb].y) s[nb][half][1] = -INFINITY;
@@ -480,8 +488,14 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if (j + 8 >= limit[nb].y) s[nb][half][3] = -INFINITY;
               }
             }
-            const float mx = fmaxf(m[nb].x, column_max(fmaxf(fmaxf(s[nb][0][0], s[nb][0][2]), fmaxf(s[nb][1][0], s[nb][1][2]))));
-            const float my = fmaxf(m[nb].y, column_max(fmaxf(fmaxf(s[nb][0][1], s[nb][0][3]), fmaxf(s[nb][1][1], s[nb][1][3]))));
+            float mx = s[nb][0][0], my = s[nb][0][1];
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              mx = max3(mx, s[nb][half][0], s[nb][half][2]);
+              my = max3(my, s[nb][half][1], s[nb][half][3]);
+            }
+            mx = fmaxf(m[nb].x, column_max(mx));
+            my = fmaxf(m[nb].y, column_max(my));
             // a row that has seen no key has o = l = 0: any finite factor will do
             a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
             moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
@@ -490,8 +504,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             l[nb].x *= a[nb].x;
             l[nb].y *= a[nb].y;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float rv = half ? sc1.z : sc0.z;
+            for (int half = 0; half < kHalves; ++half) {
+              const float rv = sc[half].z;
               const float x0 = ex2_approx(s[nb][half][0] - ux), y0 = ex2_approx(s[nb][half][1] - uy);
               const float x1 = ex2_approx(s[nb][half][2] - ux), y1 = ex2_approx(s[nb][half][3] - uy);
               l[nb].x = fmaf(x0 + x1, rv, l[nb].x);
@@ -513,6 +527,15 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           }
           // ---- O^T += V^T W^T, 16 tokens at a time. What stands behind the request's last token may be anything: it must not meet a weight of 0
           auto add_half = [&](int half, uint32_t keep0, uint32_t keep1) {
+            uint32_t weights[kRowBlocks][2];
+#pragma unroll
+            for (int nb = 0; nb < kRowBlocks; ++nb)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                weights[nb][e] = pb[nb][0][e];
+#pragma unroll
+                for (int x = 1; x < kHalves; ++x) weights[nb][e] = half == x ? pb[nb][x][e] : weights[nb][e];
+              }
 #pragma unroll
             for (int ch = 0; ch < kChunks; ch += 2) {
               uint32_t vf[4];
@@ -523,18 +546,17 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 codes_to_f16_by_two<kInt8>(vf[2 * e] & keep0, even0, odd0);
                 codes_to_f16_by_two<kInt8>(vf[2 * e + 1] & keep1, even1, odd1);
 #pragma unroll
-                for (int nb = 0; nb < kRowBlocks; ++nb)
-                  mma_16816<true>(o[nb][ch + e], even0, odd0, even1, odd1, half ? pb[nb][1][0] : pb[nb][0][0], half ? pb[nb][1][1] : pb[nb][0][1]);
+                for (int nb = 0; nb < kRowBlocks; ++nb) mma_16816<true>(o[nb][ch + e], even0, odd0, even1, odd1, weights[nb][0], weights[nb][1]);
               }
             }
           };
           if (tok + kStepTokens <= r.len) {
-            add_half(0, ~0u, ~0u);
-            add_half(1, ~0u, ~0u);
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) add_half(half, ~0u, ~0u);
           } else {
             auto keep = [&](int j) { return (j < r.len ? 0xffffu : 0u) | (j + 1 < r.len ? 0xffff0000u : 0u); };
 #pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < kHalves; ++half) {
               const int j = tok + half * 16 + 2 * t;
               if (tok + half * 16 < r.len) add_half(half, keep(j), keep(j + 8));
             }
@@ -910,13 +932,15 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   p.shift = block_shift(c.block_size);
   p.rows = unit_rows(c);
   p.rows_shift = p.rows == 8 ? 3 : p.rows == 16 ? 4 : p.rows == 32 ? 5 : 6;
-  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - kTileTokens) + 1);
+  p.tile_shift = c.head_dim == 64 ? 8 : 7;
+  p.most_tiles = INT32_MAX / c.batch;
+  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - 256) + 1);
   p.causal = c.is_causal;
   p.f16 = c.dtype == SDPA_B200_F16;
   p.scale_log2 = c.softmax_scale * 1.4426950408889634f;
   // a CTA per tile, up to one wave
   const int64_t units = static_cast<int64_t>(c.batch) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
-  const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + kTileTokens - 1) / kTileTokens);
+  const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + (1 << p.tile_shift) - 1) >> p.tile_shift);
   p.grid = static_cast<int>(tiles < kCtasPerSm * sms ? tiles : kCtasPerSm * sms);
   const size_t rows = static_cast<size_t>(kCtasPerSm) * kMaxSms * 2 * p.rows;
   p.part_o = reinterpret_cast<float*>(workspace + kWorkspaceHeaderBytes);
@@ -954,7 +978,7 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
     return SDPA_B200_LAUNCH_FAILED;
   }
   count_launch();
-  if (p.grid == 1) return SDPA_B200_OK;  // nobody to share a unit with
+  if (p.grid == 1 || c.max_seqlen_k <= 1 << p.tile_shift) return SDPA_B200_OK;  // no unit is shared
   cudaLaunchConfig_t cfg = {};  // under this grid's tail, under stream capture too: what stands in front is a kernel of this call
   cfg.gridDim = dim3(p.grid - 1, p.rows / 4);
   cfg.blockDim = dim3(128);
