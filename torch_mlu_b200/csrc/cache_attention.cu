@@ -5,19 +5,25 @@
 // over the cached tokens j of the request, j <= i + len - rows of q where causal. Two paths:
 //
 // 1. Few rows per request (decode steps, drafted tokens): cache_stream_kernel, bound by the codes that come out of HBM. A unit is (request,
-//    kv head, chunk of up to 64 rows (query token, query head of the group)), whose codes are read once for all its rows: S^T = K Q^T and O^T = V^T W^T in
-//    mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 or 256 tokens,
-//    so that all SMs stream the same number of bytes however long each request is. A unit that several CTAs worked on leaves fp32 parts in the workspace,
-//    at most two per CTA, and a second kernel merges them.
-//    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a copy takes its warp about
-//    100 cycles, which one warp with 16 of them per tile of 16 KB - blocks of 16 tokens, head_dim 64 - could not keep up with); four do the arithmetic, as 1, 2 or 4 groups of 8 or 16
-//    rows by 4, 2 or 1 parts of a tile's tokens.
-//    Codes become f16, exactly. Q rows are brought to f16 by a power of two each (their largest element to 2^14..2^15: a bf16 element loses
-//    only what is 2^-39 of the row's largest). The scale of K goes onto the fp32 scores; that of V into the exponent, so that the weights w_j = 2^(s_j + log2 vs_j - m) with
-//    m their running maximum are f16 numbers of up to 2^15 which keep all 11 bits down to 2^-29 of the largest, whatever scales blocks have, and the products add up in the
-//    tensor core's fp32 accumulators without a pass over them. The sum of the softmax takes w_j / vs_j in fp32.
-// 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors in the
-//    workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest.
+//    kv head, chunk of up to 64 rows (query token, query head of the group)), whose codes are read once for all its rows: S^T = K Q^T and
+//    O^T = V^T W^T in mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an
+//    instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 or
+//    256 tokens, so that all SMs stream the same number of bytes however long each request is. A unit that several CTAs worked on leaves fp32
+//    parts in the workspace, at most two per CTA, and a second kernel merges them.
+//    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a
+//    copy takes its warp about 100 cycles, which one warp with 16 of them per tile of 16 KB - blocks of 16 tokens, head_dim 64 - could not keep
+//    up with); four do the arithmetic, as 1, 2 or 4 groups of 8 or 16 rows by 4, 2 or 1 parts of a tile's tokens.
+//    Codes become f16, exactly. Q rows are brought to f16 by a power of two each (their largest element to 2^14..2^15: a bf16 element loses only
+//    what is 2^-39 of the row's largest). The scale of K goes onto the fp32 scores; that of V into the exponent, so that the weights
+//    w_j = 2^(s_j + log2 vs_j - m) with m their running maximum are f16 numbers of up to 2^15 which keep all 11 bits down to 2^-29 of the
+//    largest, whatever scales blocks have, and the products add up in the tensor core's fp32 accumulators without a pass over them. The sum of
+//    the softmax takes w_j / vs_j in fp32.
+//    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
+//    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
+//    3 in the merge, and shares are whole tiles. 64 requests of 1000: 37 us, 3.3 TB/s; one of 1000: 8.8 us.
+// 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
+//    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
+//    2 requests, 32 heads of 128: 138 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -103,6 +109,7 @@ __host__ __device__ constexpr uint32_t stream_smem_bytes() {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 // barrier over the warps that do the arithmetic
 __device__ __forceinline__ void arithmetic_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
@@ -294,9 +301,15 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         const int n = __popc(__ballot_sync(0xffffffffu, lane < pages && mine >= 0));
         if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(n << p.shift) * kD);
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
-          const int block = __shfl_sync(0xffffffffu, mine, i);
-          if (elect_one()) tma_load_4d(dst + (i << p.shift) * kD, map, bar, 0, 0, cur.head, block);
+        for (int i = 0; i < n; i += 4) {  // their numbers come by four: one at a time cost a call with blocks of 16 tokens 3% more
+          int blocks[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, mine, (i + e) & 31);
+          if (elect_one()) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < n) tma_load_4d(dst + ((i + e) << p.shift) * kD, map, bar, 0, 0, cur.head, blocks[e]);
+          }
         }
       }
       if (done == 0) {  // the first copies are under way
@@ -347,6 +360,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     Request r = request_at(p, share.request);
     int unit = (share.first - share.before) / r.tiles;
     int tile = (share.first - share.before) - unit * r.tiles;
+    Request next_r = r;
+    int next = unit;  // the unit behind
     bool first_unit = true;
     for (int done = 0; done < n_tiles;) {
       const int seg_tiles = min(n_tiles - done, r.tiles - tile);
@@ -392,6 +407,16 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
       if constexpr (!kQInRegisters) arithmetic_sync();
+      if (done + seg_tiles < n_tiles) {  // where the next unit's rows of Q are: they come nearer while this one's tiles are worked on
+        next_unit(next_r, next);
+        const int next_row0 = next / p.heads_kv * p.rows + kRowsOfWarp * row_group;
+#pragma unroll
+        for (int nb = 0; nb < kRowBlocks; ++nb) {
+          const int row = next_row0 + 8 * nb + g, i = row / p.group;
+          if (t * 64 < kD && row < next_r.rows_q * p.group)
+            prefetch_l1(p.q + (next_r.q0 + i) * p.q_row + ((next - next / p.heads_kv * p.heads_kv) * p.group + row - i * p.group) * p.q_head + 64 * t);
+        }
+      }
       // tokens that all of the warp's rows see, and those that any of them does
       const int last_row = min(my_row0 + kRowsOfWarp - 1, row0 + n_rows - 1);
       const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.in_front) : r.len;
@@ -666,7 +691,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       done += seg_tiles;
       tile = 0;
       first_unit = false;
-      if (done < n_tiles) next_unit(r, unit);
+      r = next_r;
+      unit = next;
     }
   }
   if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
