@@ -182,6 +182,35 @@ def test_store_token_by_token(cuda_device, code):
         _same_cache(vc, vs, *want[1])
 
 
+@pytest.mark.parametrize("seed,block,tokens,most_left_out", [(0, 16, 1500, 31), (1, 32, 1500, 31), (2, 64, 2500, 3), (3, 128, 2500, 31), (4, 16, 40, 31), (5, 64, 300, 2), (6, 128, 5000, 0)])
+def test_store_runs_of_any_shape(cuda_device, seed, block, tokens, most_left_out):
+    """Runs of a block that begin and end anywhere, with tokens left out in them (-1, or behind the cache) and between them."""
+    heads, dim, g = 2, 64, torch.Generator().manual_seed(seed)
+    draw = lambda lo, hi: int(torch.randint(lo, hi + 1, (), generator=g))
+    slots, blocks = [-1] * draw(0, 40), 0
+    left_out = lambda n: slots.extend([-1 if draw(0, 1) else 1 << 29] * n)
+    while len(slots) < tokens:
+        place = draw(0, block - 1) if draw(0, 2) == 0 else 0
+        count = min(draw(1, block) if draw(0, 2) else block, block - place)
+        slot = blocks * block + place
+        for i in range(count):
+            if i and draw(0, 9) == 0:
+                left_out(draw(0, most_left_out))
+            slots.append(slot + i)
+        blocks += 1
+        if draw(0, 5) == 0:
+            left_out(draw(0, 100))
+    perm = torch.randperm(blocks, generator=g).tolist()
+    slots = [perm[s // block] * block + s % block if 0 <= s < blocks * block else s for s in slots]
+    k = torch.randn(len(slots), 2 * heads, dim, generator=torch.Generator(device=cuda_device).manual_seed(seed), device=cuda_device).bfloat16()
+    kc, ks = _cache(cuda_device, blocks, heads, block, dim, E4M3, 5)
+    vc, vs = _cache(cuda_device, blocks, heads, block, dim, E4M3, 6)
+    want = orc.store(k[:, :heads], torch.tensor(slots), kc, ks), orc.store(k[:, heads:], torch.tensor(slots), vc, vs)
+    kv_cache.store(k[:, :heads], k[:, heads:], _ints(cuda_device, slots), kc, vc, ks, vs)
+    _same_cache(kc, ks, *want[0])
+    _same_cache(vc, vs, *want[1])
+
+
 # ---------------------------------------------------------------------------------------------- attention
 def _batch(dev, lens, rows, hq, hkv, dim, block, code, dtype, seed=0, powers=True, poison=True, block_first=True, spare=2):
     """Queries, cache, table and lengths. What stands behind a request's last token is NaN (e4m3) or the largest code, free blocks have NaN scales."""

@@ -11,7 +11,9 @@
 // longer one all warps work, each thread with its elements in registers between the largest element and the codes, so that they are read once.
 // Measured (8192 tokens of 4 prompts, 8 heads of 128, bf16 beside their queries to e4m3): 57 us with a warp for each run, which found it by itself, and
 // elements looked at one by one; 21 with a warp that finds runs for the CTA and the largest element two at a time as integers; 16.5 with a path of its own for
-// runs without gaps (3 TB/s). Asking L2 for the window's rows while the runs are found gave nothing.
+// runs without gaps; 15.3 with all slots asked for before any is looked at; 14.2 with seven CTAs on an SM instead of six (3.5 TB/s; the few bytes spilled for it
+// cost the smallest calls 0.1 to 0.2). Of the 14.2, launch and runs are 4, and reading, codes and writing follow one another in a CTA. Rows held in
+// shared memory, those of the next head asked for ahead, one or eight warps instead of four, and asking L2 for the window's rows while the runs are found were no faster.
 #include "cache_common.cuh"
 
 namespace sdpa_b200 {
@@ -90,7 +92,7 @@ struct Run {
 };
 
 template <int kD, bool kInt8, bool kF16>
-__global__ void __launch_bounds__(kWarps * 32, 6) store_kernel(const StoreParams p) {
+__global__ void __launch_bounds__(kWarps * 32, 7) store_kernel(const StoreParams p) {
   constexpr int kLanes = kD / 8, kRows = 32 / kLanes;  // lanes per row, rows per step of a warp
   __shared__ Run runs[kMostWindow];
   __shared__ int num_runs;
@@ -105,68 +107,71 @@ __global__ void __launch_bounds__(kWarps * 32, 6) store_kernel(const StoreParams
     return slot < 0 || slot >= p.num_slots ? -1 : slot >> p.shift;
   };
 
-  if (warp == 0) {
-    // whether a token stands right behind the one in front of it
-    auto follows = [&](int t) { return t < p.tokens && t > 0 && p.slots[t] == p.slots[t - 1] + 1; };
-    // ---- the runs that begin in the window: where the nearest token with a place in front, within 32, is in another block
+  // by one warp: the runs that begin in the window whose first token is own0. All slots that it is likely to need are asked for at once
+  auto find_runs = [&](int own0) {
+    auto slot_at = [&](int t) { return t >= 0 && t < p.tokens ? p.slots[t] : -1; };
+    auto block_at = [&](int slot) { return slot < 0 || slot >= p.num_slots ? -1 : slot >> p.shift; };
+    const int front = slot_at(own0 - 32 + lane), end = own0 + p.window;
+    int slot = slot_at(own0 + lane), slot1 = slot_at(own0 + 32 + lane), slot2 = slot_at(own0 + 64 + lane);
+    const int front_block = block_at(front);
+    const unsigned front_placed = __ballot_sync(0xffffffffu, front_block >= 0);
+    int last = own0 - 1 - __clz(front_placed);  // the nearest token with a place, and its block
+    int last_block = __shfl_sync(0xffffffffu, front_block, front_placed ? 31 - __clz(front_placed) : 0);
+    int last_slot = __shfl_sync(0xffffffffu, front, 31);
     int found = 0;
-    int front = lane < own0 ? block_of(own0 - 1 - lane) : -1;
-    unsigned front_placed = __ballot_sync(0xffffffffu, front >= 0);
-    int last = front_placed ? own0 - __ffs(front_placed) : -64;  // the nearest token with a place, and its block
-    int last_block = __shfl_sync(0xffffffffu, front, front_placed ? __ffs(front_placed) - 1 : 0);
-    const int end = own0 + p.window;
-    int tail = block_of(end + lane), tail2 = block_of(end + 32 + lane);  // asked for early: the last run often goes on there
-    int next = own0 + lane < own0 + p.window || p.window >= 32 ? block_of(own0 + lane) : -1;
-    for (int base = own0; base < own0 + p.window; base += 32) {
-      const int b = lane < p.window ? next : -1;
-      next = base + 32 < own0 + p.window ? block_of(base + 32 + lane) : -1;
-      const unsigned placed = __ballot_sync(0xffffffffu, b >= 0), below = placed & ((1u << lane) - 1);
+    bool open = false;  // the run that goes on behind the 32 tokens looked at
+    Run run = {};
+    for (int base = own0;; base += 32) {
+      const int b = block_at(slot);
+      const unsigned placed = __ballot_sync(0xffffffffu, b >= 0), in_front = (1u << lane) - 1, below = placed & in_front;
       const int from_lane = __shfl_sync(0xffffffffu, b, below ? 31 - __clz(below) : 0);
+      const int slot_in_front = __shfl_up_sync(0xffffffffu, slot, 1);
+      // a run begins where the nearest token with a place in front, within 32, is in another block
       const int before = below ? from_lane : base + lane - last <= 32 ? last_block : -1;
-      const bool begins = b >= 0 && b != before;
-      const unsigned firsts = __ballot_sync(0xffffffffu, begins), parted = ~__ballot_sync(0xffffffffu, follows(base + lane));
-      // a run that has begun ends with the last token in front of the next one
-      if (placed != 0) {
-        const unsigned of_last = firsts ? placed & ((firsts & -firsts) - 1) : placed;
-        if (found > 0 && of_last != 0 && lane == 0) {
-          runs[found - 1].count = base + 32 - __clz(of_last) - runs[found - 1].first;
-          runs[found - 1].rows = runs[found - 1].rows && (parted << __clz(of_last)) == 0;
+      const unsigned firsts = __ballot_sync(0xffffffffu, b >= 0 && b != before);
+      const unsigned parted = __ballot_sync(0xffffffffu, slot != (lane == 0 ? last_slot : slot_in_front) + 1);
+      // the open run ends with the last token in front of the next one
+      if (open) {
+        const unsigned more = firsts ? placed & ((firsts & -firsts) - 1) : placed;
+        if (more != 0) {
+          run.count = base + 32 - __clz(more) - run.first;
+          run.rows = run.rows && parted << __clz(more) == 0;
+        }
+        if (firsts != 0) {
+          if (lane == 0) runs[found - 1] = run;
+          open = false;
         }
       }
-      if (begins) {
-        const unsigned behind = firsts & ~((2u << lane) - 1);
-        const unsigned mine = placed & ~((1u << lane) - 1) & (behind ? (behind & -behind) - 1 : ~0u);
+      const unsigned own = base + 32 <= end ? firsts : base < end ? firsts & ((1u << (end - base)) - 1) : 0u;
+      if (own != 0) {
+        const unsigned behind = firsts & ~(in_front << 1 | 1u);
+        const unsigned mine = placed & ~in_front & (behind ? (behind & -behind) - 1 : ~0u);
         const int n = 32 - __clz(mine) - lane;
-        // bits lane + 1 to lane + n - 1
-        const unsigned inside = (n >= 32 ? ~0u : (1u << n) - 1) << lane & ~(1u << lane);
-        runs[found + __popc(firsts & ((1u << lane) - 1))] = {base + lane, n, b, p.slots[base + lane] & mask, (parted & inside) == 0};
+        const unsigned inside = (n >= 32 ? ~0u : (1u << n) - 1) << lane & ~(1u << lane);  // bits lane + 1 to lane + n - 1
+        const Run r = {base + lane, n, b, slot & mask, (parted & inside) == 0};
+        if (own >> lane & 1) runs[found + __popc(own & in_front)] = r;
+        const int l = 31 - __clz(own);
+        run = {base + l, __shfl_sync(0xffffffffu, n, l), __shfl_sync(0xffffffffu, b, l), __shfl_sync(0xffffffffu, r.place, l), __shfl_sync(0xffffffffu, r.rows, l) != 0};
+        open = firsts >> l == 1u;
+        found += __popc(own);
       }
-      __syncwarp();
-      found += __popc(firsts);
       if (placed != 0) {
         last = base + 31 - __clz(placed);
         last_block = __shfl_sync(0xffffffffu, b, 31 - __clz(placed));
       }
+      if (base + 32 >= end && (!open || last < base)) break;  // no token behind is within 32
+      last_slot = __shfl_sync(0xffffffffu, slot, 31);
+      slot = slot1, slot1 = slot2;
+      slot2 = slot_at(base + 96 + lane);
     }
-    // the last one may go on behind the window
-    if (found > 0) {
-      Run run = runs[found - 1];
-      for (int base = end;; base += 32) {
-        const int b = tail;
-        tail = tail2;
-        const unsigned same = __ballot_sync(0xffffffffu, b == run.block), other = __ballot_sync(0xffffffffu, b >= 0 && b != run.block);
-        const unsigned more = same & (other == 0 ? ~0u : (other & -other) - 1);  // in front of the first token of another block
-        if (more == 0 || base + __ffs(more) - (run.first + run.count) > 32) break;
-        run.rows = run.rows && (~__ballot_sync(0xffffffffu, follows(base + lane)) << __clz(more)) == 0;
-        run.count = base + 32 - __clz(more) - run.first;
-        if (other != 0) break;
-        tail2 = block_of(base + 64 + lane);
-      }
-      __syncwarp();
-      if (lane == 0) runs[found - 1] = run;
+    __syncwarp();
+    if (lane == 0) {
+      if (open) runs[found - 1] = run;
+      num_runs = found;
     }
-    if (lane == 0) num_runs = found;
-  }
+  };
+
+  if (warp == 0) find_runs(own0);
   __syncthreads();
 
   const int count = num_runs;
