@@ -20,7 +20,7 @@
 //    the softmax takes w_j / vs_j in fp32.
 //    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
-//    3 in the merge, and shares are whole tiles. 64 requests of 1000: 37 us, 3.3 TB/s; one of 1000: 8.8 us.
+//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 1000: 37 us, 3.3 TB/s; one of 1000: 8.4 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 138 us.
@@ -701,9 +701,11 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 }
 
 // Merges the parts of the units that several CTAs worked on: block (i, j) those of the unit that CTA i began, rows 4j to 4j + 3, a warp each.
+// What it takes is a chain of latencies, behind a call whose own work is a few of them: with the first eight parts asked for beside their weights instead of
+// behind them 4 drafted tokens of 16 requests take 22.0 us and not 23.2, one token of 1000 8.4 and not 8.75. Sixteen took registers and were slower elsewhere.
 template <int kD>
 __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) {
-  constexpr int kPer = kD / 32;
+  constexpr int kPer = kD / 32, kEarly = 8;
   const int lane = threadIdx.x & 31, rr = blockIdx.y * 4 + (threadIdx.x >> 5), first = blockIdx.x;
   wait_for_previous_grid();
   launch_dependents();
@@ -717,6 +719,23 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) 
   for (int base = first; base <= u.last; base += 32) {
     const int n = min(32, u.last - base + 1);
     const float x = lane < n ? p.part_lse[part(base + lane)] : -INFINITY;
+    auto load = [&](int j, float (&v)[kPer]) {
+      const float* src = p.part_o + part(base + j) * kD + kPer * lane;
+      if constexpr (kPer == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(src);
+        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+      } else {
+        const float2 q = *reinterpret_cast<const float2*>(src);
+        v[0] = q.x, v[1] = q.y;
+      }
+    };
+    float early[kEarly][kPer];  // asked for beside their weights
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) early[j][e] = 0.f;
+      if (j < n) load(j, early[j]);
+    }
     nan = nan || __any_sync(0xffffffffu, isnan(x));
     float mn = x;
 #pragma unroll
@@ -730,18 +749,17 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) 
     sum = sum * a + s;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) acc[e] *= a;
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
+#pragma unroll
+    for (int j = 0; j < kEarly; ++j) {
       const float wj = __shfl_sync(0xffffffffu, w, j);
-      const float* src = p.part_o + part(base + j) * kD + kPer * lane;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wj, early[j][e], acc[e]);
+    }
+#pragma unroll 8
+    for (int j = kEarly; j < n; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
       float v[kPer];
-      if constexpr (kPer == 4) {
-        const float4 q = *reinterpret_cast<const float4*>(src);
-        v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
-      } else {
-        const float2 q = *reinterpret_cast<const float2*>(src);
-        v[0] = q.x, v[1] = q.y;
-      }
+      load(j, v);
 #pragma unroll
       for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wj, v[e], acc[e]);
     }
