@@ -301,7 +301,7 @@ typedef struct sdpa_b200_rotary_params {
   const void* k; /* NULL with heads_k == 0 */
   void* q_out;
   void* k_out;
-  const void* positions; /* int32, or int64 with positions_64; [axes][batch][length] by the strides below, in elements */
+  const void* positions; /* int32, or int64 with positions_64, aligned to them; [axes][batch][length] by the strides below, in elements */
   const float* inv_freq; /* [rotary_dim / 2] */
   int32_t batch, length, heads_q, heads_k;
   int32_t head_dim;    /* a multiple of 8, at most 256 */
@@ -395,13 +395,15 @@ typedef struct sdpa_b200_cache_params {
  * rounded again to a scale that has grown. A block whose first place is written starts anew. Tokens with a negative slot, or one behind the
  * cache, are left out. The tokens of one block stand next to each other, with rising slots, as sdpa_b200_plan_step gives them (the same slot
  * twice in a row: the later token stays; fewer than 32 tokens that are left out may stand between them); a block that comes up again
- * behind tokens of another one is not allowed, since the two parts are worked on at the same time. A NaN or infinite element becomes NaN in e4m3; int8 has none, there the scale becomes NaN until the
- * block starts anew. */
+ * behind tokens of another one is not allowed, since the two parts are worked on at the same time; keys and values have caches and scales of
+ * their own for the same reason. A NaN or infinite element becomes NaN in e4m3; int8 has none, there the scale becomes NaN until the block
+ * starts anew. */
 SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* stream);
 
 /* out, lse <- attention of each request's last rows of q over its tokens in the cache. A row without a visible key gets out = 0 and lse = +inf;
- * rows of q outside every request are left unwritten; a block number outside the cache makes the rows that see it NaN (with lse = +inf, as NaN rows have here). Nothing at or behind
- * seq_lens counts, whatever stands there. (A NaN among the values themselves may reach every row of its request, as 0 * NaN.) */
+ * rows of q outside every request are left unwritten; a block number outside the cache makes the rows that see it NaN (with lse = +inf, as
+ * NaN rows have here). Nothing at or behind seq_lens counts, whatever stands there. Where requests have many rows, codes * scales are brought to 16
+ * bits in the workspace: exact with scales that are powers of two, else rounded once. (A NaN among the values themselves may reach every row of its request, as 0 * NaN.) */
 SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);
 SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_params* p, void* workspace, size_t workspace_bytes, void* stream);
 

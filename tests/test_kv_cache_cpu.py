@@ -134,6 +134,13 @@ def test_refusals(native_lib, call, make, change, status, needle):
     assert got == status and needle in native_lib.sdpa_b200_last_error().decode(), native_lib.sdpa_b200_last_error()
 
 
+@pytest.mark.parametrize("change", [_set(positions=4098), _set(positions=4100, positions_64=1), _set(inv_freq=4097)])
+def test_rotary_refuses_unaligned_positions(native_lib, change):
+    p = _rotary()
+    change(p)
+    assert native_lib.sdpa_b200_rotary(ctypes.byref(p), None) == _cabi.INVALID_ARG and "aligned to their elements" in native_lib.sdpa_b200_last_error().decode()
+
+
 def test_workspaces(native_lib):
     """Few rows: parts for two CTAs per SM, whatever the lengths are. Many rows: 16-bit keys and values, every request's filled up to 128. Too small a one is refused."""
     n = ctypes.c_size_t(0)

@@ -373,6 +373,24 @@ def test_gradients_are_refused(cuda_device):
         assert not _run(b)[0].requires_grad
 
 
+def test_store_refuses_gradients_and_shared_caches(cuda_device):
+    k = torch.randn(2, 2, 64, device=cuda_device).bfloat16()
+    kc, ks = _cache(cuda_device, 3, 2, 16, 64, E4M3, 1)
+    vc, vs = _cache(cuda_device, 3, 2, 16, 64, E4M3, 2)
+    before, slots = [x.clone() for x in (kc.view(torch.int8), ks)], _ints(cuda_device, [0, 1])
+    for key, value in ((k.clone().requires_grad_(), k), (k, k.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="keeps no gradient"):
+            kv_cache.store(key, value, slots, kc, vc, ks, vs)
+    with pytest.raises(RuntimeError, match="of their own"):
+        kv_cache.store(k, k, slots, kc, kc, ks, vs)
+    with pytest.raises(RuntimeError, match="of their own"):
+        kv_cache.store(k, k, slots, kc, vc, ks, ks)
+    assert torch.equal(kc.view(torch.int8), before[0]) and torch.equal(ks, before[1])
+    with torch.no_grad():
+        kv_cache.store(k.clone().requires_grad_(), k, slots, kc, vc, ks, vs)
+    assert not torch.equal(kc.view(torch.int8), before[0])
+
+
 def test_rows_outside_every_request_are_left(cuda_device):
     """Offsets that begin behind the first row and end in front of the last; the outputs are read through the C ABI into buffers of a known filling."""
     import ctypes

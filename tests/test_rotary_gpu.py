@@ -158,6 +158,15 @@ def test_second_derivative_and_shared_inputs(cuda_device):
     _check(g1 / 2, w, pos, f, "shared", inverse=True)
 
 
+def test_learned_frequencies_are_refused(cuda_device):
+    pos, f = torch.arange(9, device=cuda_device), _freq(32, cuda_device).requires_grad_()
+    x = torch.randn(9, 2, 64, device=cuda_device).half()
+    with pytest.raises(RuntimeError, match="no gradient of inv_freq"):
+        rotary.rotary_embedding(x, None, pos, f)
+    with torch.no_grad():
+        assert torch.equal(rotary.rotary_embedding(x, None, pos, f)[0], rotary.rotary_embedding(x, None, pos, f.detach())[0])
+
+
 def test_autograd_refuses_what_it_would_get_wrong(cuda_device):
     pos, f = torch.arange(9, device=cuda_device), _freq(32, cuda_device)
     x = torch.randn(9, 2, 64, device=cuda_device).half()

@@ -182,8 +182,9 @@ extern "C" SDPA_B200_API int sdpa_b200_rotary(const sdpa_b200_rotary_params* p, 
     set_error("rotary: sections must not be negative and add up to rotary_dim / 2 = %d", p->rotary_dim / 2);
     return SDPA_B200_INVALID_ARG;
   }
-  if (p->positions == nullptr || p->inv_freq == nullptr) {
-    set_error("rotary: positions and inv_freq must be given");
+  if (p->positions == nullptr || p->inv_freq == nullptr || (reinterpret_cast<uintptr_t>(p->positions) & (p->positions_64 ? 7u : 3u)) != 0 ||
+      (reinterpret_cast<uintptr_t>(p->inv_freq) & 3u) != 0) {
+    set_error("rotary: positions and inv_freq must be given, aligned to their elements");
     return SDPA_B200_INVALID_ARG;
   }
   const int64_t qs[6] = {p->q_batch_stride, p->q_head_stride, p->q_row_stride, p->qo_batch_stride, p->qo_head_stride, p->qo_row_stride};

@@ -48,6 +48,8 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 }  // namespace
@@ -155,9 +157,11 @@ void cache_store(const Tensor& key, const Tensor& value, const Tensor& slots, co
   sdpa_b200_cache_params p = {};
   cache_params(p, key, "key", key_cache, value_cache, key_scale, value_scale);
   TORCH_CHECK(key.size(1) == key_cache.size(1), "the caches must have the heads of key and value");
+  TORCH_CHECK(!needs_grad(key) && !needs_grad(value), "the cache keeps no gradient: store keys and values under torch.no_grad()");
   check_ints(slots, "slots", key);
   TORCH_CHECK(slots.dim() == 1 && slots.size(0) == key.size(0), "slots must be [tokens]");
   if (key.size(0) == 0) return;
+  TORCH_CHECK(p.k_cache != p.v_cache && p.k_scale != p.v_scale, "keys and values need caches and scales of their own");
   p.key = key.data_ptr();
   p.value = value.data_ptr();
   p.slots = slots.data_ptr<int32_t>();
@@ -186,7 +190,7 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& ke
     check_ints(*cu_seqlens, "cu_seqlens", query);
     TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->size(0) == B + 1, "cu_seqlens must have requests + 1 entries");
   }
-  TORCH_CHECK(!(query.requires_grad() && at::GradMode::is_enabled()), "attention over the cache has no gradient: call it under torch.no_grad()");
+  TORCH_CHECK(!needs_grad(query), "attention over the cache has no gradient: call it under torch.no_grad()");
   c10::cuda::CUDAGuard guard(query.device());
   Tensor out = new_tensor({T, H, query.size(2)}, query.scalar_type(), query), lse = new_tensor({H, T}, at::kFloat, query);
   if (query.numel() == 0) return {out, lse};
@@ -295,8 +299,6 @@ Tensor readable(const Tensor& x) {
   return ok ? x : x.clone(at::MemoryFormat::Contiguous);
 }
 
-bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
-
 c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
 // The gradient of a turn is the turn backwards, itself an operator with a gradient.
@@ -353,6 +355,7 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& query, const Tensor& key, const 
   check_plain(inv_freq, "inv_freq");
   TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous() && inv_freq.device() == query.device(),
               "inv_freq must be a contiguous fp32 vector of rotary_dim / 2 frequencies on the device of query");
+  TORCH_CHECK(!needs_grad(inv_freq), "rotary positions have no gradient of inv_freq: detach it");
   check_plain(positions, "positions");
   TORCH_CHECK((positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) && positions.device() == query.device(),
               "positions must be int32 or int64, on the device of query");

@@ -44,7 +44,7 @@ def plan_step(cached_lens, new_tokens, block_table, ring, ring_state, *, block_s
     ``new_tokens[i]`` tokens are added to request i, which has ``cached_lens[i]``; a negative number takes tokens back (all of them when the request
     has ended). Blocks that a request needs are taken from the front of ``ring``, those that it gives back are put at its end:
     ring [num_blocks] holds ``ring_state[1]`` free block numbers from index ``ring_state[0]`` on, modulo its size. ``block_table`` and ``ring`` are
-    written; entries of the table behind a request's last block mean nothing. ``num_tokens`` is at least the number of new tokens.
+    written; entries of the table behind a request's last block mean nothing. ``num_tokens`` is at least the number of new tokens, and at least 1.
 
     All or nothing: a step that does not fit changes nothing and comes back without new tokens, and ``ring_state[2]`` of the result says why: the
     number of blocks that were lacking, or -1 - i for the first request i whose length would be negative or pass the table, or whose
@@ -61,8 +61,8 @@ def store(key, value, slots, key_cache, value_cache, key_scale, value_scale) -> 
     Every block and head that gets tokens has its scale raised to the smallest power of two at which the largest of them is a code (448 for
     e4m3, 127 for int8), unless it is as large already; tokens that the block holds are rounded again to a scale that has grown. A block
     whose first place is written starts anew. The tokens of a block stand next to each other, with rising slots, as plan_step gives them (fewer than 32
-    that are left out may stand between them). A NaN or
-    infinite element becomes a NaN of e4m3; in an int8 cache it makes the block's scale NaN until the block starts anew.
+    that are left out may stand between them; a block that came up again behind another would be worked on twice at a time). A NaN or
+    infinite element becomes a NaN of e4m3; in an int8 cache it makes the block's scale NaN until the block starts anew. There is no gradient.
     """
     _calls().cache_store(key, value, slots, key_cache, value_cache, key_scale, value_scale)
 
@@ -75,7 +75,8 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     ``seq_lens[i]`` tokens that the blocks of ``block_table[i]`` hold, up to its own with ``is_causal`` (bottom-right aligned). Without cu_seqlens every
     request has one row. ``max_seqlen_q`` and ``max_seqlen_k`` are at least the most rows and the longest request; without max_seqlen_k it is what
     the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace, which takes
-    4 * requests * max_seqlen_k * heads_kv * head_dim bytes, and the prefill kernel runs.
+    4 * requests * max_seqlen_k * heads_kv * head_dim bytes, and the prefill kernel runs. That is exact with scales that are powers of two, as store gives
+    them; with others every element is rounded once.
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package).
