@@ -23,7 +23,7 @@
 //    2 to 3 in the merge, and shares are whole tiles. 64 requests of 1000: 37 us, 3.3 TB/s; one of 1000: 8.4 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
-//    2 requests, 32 heads of 128: 138 us.
+//    2 requests, 32 heads of 128: 135 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -786,12 +786,12 @@ struct GatherParams {
   int batch, heads, max_blocks, num_blocks, shift, max_k;
 };
 
-constexpr int kGatherTokens = 64;
+constexpr int kGatherTokens = 32;  // of a block; with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
 constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, from a sequence's start
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
 
-// Block (i, h, b): tokens 64i to 64i + 63 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
+// Block (i, h, b): tokens 32i to 32i + 31 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
 // where a weight of 0 would meet another request's NaN, or whatever the workspace held. So every request's rows are filled up to a whole tile with zeros, and these
 // stand in the list of sequences as one of their own, without queries.
 template <int kD, bool kInt8, bool kF16>
@@ -819,27 +819,27 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       cu_k[2 * p.batch] = before + padded;
     }
   }
-  constexpr int kLanes = kD / 16, kTimes = kGatherTokens * kLanes / 256;  // 16 codes of K and of V a thread and time
+  constexpr int kLanes = kD / 8, kTimes = kGatherTokens * kLanes / 256;  // eight codes of K and of V a thread and time: the stores of a warp leave no gaps
   static_assert(kTimes >= 1, "a block has threads to spare");
-  const int tok0 = blockIdx.x * kGatherTokens + tid / kLanes, at = tid % kLanes * 16;
+  const int tok0 = blockIdx.x * kGatherTokens + tid / kLanes, at = tid % kLanes * 8;
   int id[kTimes];
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), page = tok >> p.shift;
     id[i] = tok < len && page < p.max_blocks ? p.block_table[b * p.table_stride + page] : -1;
   }
-  uint4 w[kTimes][2];
+  uint2 w[kTimes][2];
   float scale[kTimes][2];
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), place = tok & ((1 << p.shift) - 1);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      w[i][x] = make_uint4(0u, 0u, 0u, 0u);
+      w[i][x] = make_uint2(0u, 0u);
       // a block outside the cache: its scores are NaN, for those who see them
       scale[i][x] = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
-      w[i][x] = *reinterpret_cast<const uint4*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
+      w[i][x] = *reinterpret_cast<const uint2*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
       scale[i][x] = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
     }
   }
@@ -849,33 +849,31 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
     if (tok >= padded) break;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint32_t f[8], c[4] = {w[i][x].x, w[i][x].y, w[i][x].z, w[i][x].w};
+      uint32_t f[4], c[2] = {w[i][x].x, w[i][x].y};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 2; ++e) {
         uint32_t lo, hi;
         codes_to_f16<kInt8>(c[e], lo, hi);
         const float2 u = unpack_16x2<true>(lo), v = unpack_16x2<true>(hi);
         f[2 * e] = pack_16x2<kF16>(u.x * scale[i][x], u.y * scale[i][x]);
         f[2 * e + 1] = pack_16x2<kF16>(v.x * scale[i][x], v.y * scale[i][x]);
       }
-      uint4* dst = reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at);
-      dst[0] = make_uint4(f[0], f[1], f[2], f[3]);
-      dst[1] = make_uint4(f[4], f[5], f[6], f[7]);
+      *reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
     }
   }
 }
 
-// Path 1 costs its units of 64 rows, path 2 the gathering of every kv head's tokens and the prefill kernel's waves of units of up to 256 rows of a query head, all per token in
-// the cache. So the length does not decide, and in units of 64 rows a token's gathering is 0.9 and a wave 95 (head_dim 64: 135). Measured, 4 requests of 5000 tokens,
-// us, path 1 | 2: 32/8 heads of 128, 24 rows 59 | 91, 40 80 | 93, 64 101 | 93, 96 144 | 94; 16/16, 64 61 | 112, 96 101 | 113, 160 143 | 122; 64/8, 40 123 | 153,
-// 64 186 | 154; 16/4 of 64, 64 41 | 64, 96 54 | 65, 160 82.6 | 81.7.
+// Path 1 costs its units of 64 rows, path 2 the gathering of every kv head's tokens and the prefill kernel's waves of units of up to 256 rows of a query head, all per
+// token in the cache. So the length does not decide, and in units of 64 rows a token's gathering is 0.9 and a wave 95 (head_dim 64: 150). Measured, 4 requests of 5000
+// tokens, us, path 1 | 2: 32/8 heads of 128, 24 rows 58 | 86, 40 79 | 88, 56 99 | 88, 96 144 | 89; 16/16, 64 60 | 106, 128 101 | 107, 160 144 | 115; 64/8, 40 123 | 148,
+// 64 188 | 150; 16/4 of 64, 64 36 | 63, 128 61 | 64, 160 73 | 81. 16 requests of 1000, 32/8 of 128, 40 76 | 78, 64 95 | 79.
 bool streams(const sdpa_b200_cache_params& p) {
   const int64_t group = p.heads_q / p.heads_kv, batch = p.batch;
   if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64) return true;
   // requests of equal rows, or of any: half a unit each is empty then
   const double units = p.total_q == batch * p.max_seqlen_q ? static_cast<double>(batch * ((p.max_seqlen_q * group + 63) / 64)) : p.total_q * group / 64.0 + 0.5 * batch;
   const int64_t blocks = p.heads_q * std::max<int64_t>(batch, (p.total_q + 255) / 256);
-  return (units - 0.9 * batch) * p.heads_kv <= (p.head_dim == 64 ? 135.0 : 95.0) * static_cast<double>((blocks + 147) / 148);
+  return (units - 0.9 * batch) * p.heads_kv <= (p.head_dim == 64 ? 150.0 : 95.0) * static_cast<double>((blocks + 147) / 148);
 }
 
 int check_attention(const sdpa_b200_cache_params* p) {
