@@ -296,6 +296,18 @@ def test_some_rows_each(cuda_device, lens, rows, hq, hkv, dim, block, code, dtyp
     _compare(*_run(b, is_causal=causal, scale=0.05), b, causal, 0.05)
 
 
+@pytest.mark.parametrize("rows,hq,hkv,dim,code,dtype", [(1, 16, 8, 128, E4M3, torch.bfloat16), (1, 32, 8, 64, INT8, torch.float16), (3, 32, 8, 128, INT8, torch.bfloat16),
+                                                        (5, 32, 8, 128, E4M3, torch.float16), (9, 64, 8, 128, E4M3, torch.bfloat16)])
+def test_many_units_to_a_share(cuda_device, rows, hq, hkv, dim, code, dtype):
+    """Shares of many tiles and several units each, which count the hand-overs between units: short requests, some empty, one long."""
+    g = torch.Generator().manual_seed(rows)
+    lens = torch.randint(0, 1700 if dim == 64 else 900, (160,), generator=g).tolist()
+    lens[3], lens[7], lens[40], lens[159] = 0, 1, 7000, 129
+    b = _batch(cuda_device, lens, [rows if i % 5 else 1 for i in range(160)], hq, hkv, dim, 16, code, dtype, seed=rows)
+    _compare(*_run(b), b)
+    assert ops.device_status() == 0
+
+
 MANY_ROWS = [
     ([700, 600], [513, 520], 8, 2, 128, 64), ([1300, 130, 64], [600, 1, 0], 4, 4, 64, 16), ([300, 1000], [299, 300], 16, 2, 128, 128), ([520], [530], 1, 1, 64, 32),
     ([500, 0, 300], [490, 3, 300], 32, 2, 64, 16), ([257, 129, 128], [300, 129, 256], 32, 4, 64, 64), ([1000], [1000], 64, 8, 128, 32),

@@ -8,7 +8,7 @@
 //    kv head, chunk of up to 64 rows (query token, query head of the group)), whose codes are read once for all its rows: S^T = K Q^T and
 //    O^T = V^T W^T in mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an
 //    instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 or
-//    256 tokens, so that all SMs stream the same number of bytes however long each request is. A unit that several CTAs worked on leaves fp32
+//    256 tokens and of the hand-overs between units, so that all SMs are done at the same time however long each request is. A unit that several CTAs worked on leaves fp32
 //    parts in the workspace, at most two per CTA, and a second kernel merges them.
 //    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a
 //    copy takes its warp about 100 cycles, which one warp with 16 of them per tile of 16 KB - blocks of 16 tokens, head_dim 64 - could not keep
@@ -20,7 +20,7 @@
 //    the softmax takes w_j / vs_j in fp32.
 //    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
-//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 1000: 37 us, 3.3 TB/s; one of 1000: 8.4 us.
+//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000: 8.6 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 135 us.
@@ -36,6 +36,7 @@ constexpr int kWarps = 4;                  // those that do the arithmetic
 constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are dealt out as for six warps anyway
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
+constexpr int kPause = 2, kTilesToPause = 4;  // see Share
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
 constexpr float kSumUnit = 0x1p-40f;       // sums are kept in this unit, so that those over blocks of the least scale stay in range
 
@@ -55,6 +56,7 @@ struct StreamParams {
   int64_t q_row, q_head, o_row, o_head, table_stride;
   int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
   int tile_shift;  // log2 of a tile's tokens
+  int pause;       // see Share
   int most_tiles;  // that a request may have, so that the sum of all stays in 32 bits
   int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
   float scale_log2;
@@ -131,53 +133,79 @@ __device__ __forceinline__ float column_sum(float x) {
   return x;
 }
 
-// A CTA's share of the list of all tiles, [first, last), and the request that it begins in. Equal shares, the first of them one tile longer where they do not come out even.
+// A CTA's share of the list of all tiles. Places in the list: a unit has one for each tile, behind `pause` empty ones that stand for what the hand-over from unit
+// to unit takes, which is about that of two tiles (not so with 64 rows, whose warps have nothing to merge and more to do per tile: 59.5 us with it, 58.8 without, 4 requests
+// of 32 rows). Equal shares of the places, the first of them one longer where they do not come out even; a CTA works on the tiles whose places are in its own. Where a CTA
+// has fewer than four tiles it has few hand-overs, and the places are the tiles. Measured with equal shares of the tiles | of the places, one token each, us: 64 requests
+// of 200 to 1800 37.9 | 33.9, 128 of 100 to 900 52.8 | 39.9, 32 of 100 to 2000 with 32 kv heads 62 | 48.5, 64 of 500 to 4000 59.3 | 55.5; 4 tokens, 16 of 300 to 9000 at
+// head_dim 64 22.0 | 19.8. With pauses of one place the second took 43.9, with three the same, and 8 tokens of 32 requests 53.8 instead of 52.0.
 struct Share {
-  int first, last, request, before;  // before: tiles in front of the request's
-  int each, longer, ctas;            // tiles of a share, how many shares have one more, how many there are
-  __device__ __forceinline__ int cta_of(int tile) const {
+  int places;              // from the first tile of the CTA on; 0: it has none
+  Request request;         // where it begins
+  int unit, tile;
+  int unit_place;          // the place of that unit
+  int pause;
+  int each, longer;        // places of a share, how many shares have one more
+  __device__ __forceinline__ int cta_of(int place) const {
     const int in_longer = longer * (each + 1);
-    return tile < in_longer ? tile / (each + 1) : longer + (tile - in_longer) / each;
+    return place < in_longer ? place / (each + 1) : longer + (place - in_longer) / each;
   }
 };
 
 // Every warp finds it for itself, so that none waits for another.
 __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int lane) {
-  auto tiles_of = [&](int b) {
-    if (b >= p.batch) return 0;
+  auto add_tiles_of = [&](int b, int& tiles, int& units) {
+    if (b >= p.batch) return;
     const Request r = request_at(p, b);
-    return static_cast<int>(min(static_cast<int64_t>(r.tiles) * r.units, static_cast<int64_t>(p.most_tiles)));
+    units += static_cast<int>(min(static_cast<int64_t>(r.units), static_cast<int64_t>(p.most_tiles)));
+    tiles += static_cast<int>(min(static_cast<int64_t>(r.tiles) * r.units, static_cast<int64_t>(p.most_tiles)));
   };
-  const int of_first = tiles_of(lane);  // of the first 32 requests
-  int tiles = of_first;
+  int tiles_of_first = 0, units_of_first = 0;  // of the first 32 requests
+  add_tiles_of(lane, tiles_of_first, units_of_first);
+  int tiles = tiles_of_first, units = units_of_first;
 #pragma unroll 4
-  for (int b = lane + 32; b < p.batch; b += 32) tiles += tiles_of(b);
+  for (int b = lane + 32; b < p.batch; b += 32) add_tiles_of(b, tiles, units);
   tiles = __reduce_add_sync(0xffffffffu, tiles);
-  Share s = {0, 0, 0, 0, 0, 0, 0};
+  Share s = {};
   if (tiles == 0) return s;
-  s.ctas = min(tiles, p.grid);  // those that get a tile: the others would leave no part where the merge looks for one
-  s.each = tiles / s.ctas;
-  s.longer = tiles - s.each * s.ctas;
-  if (cta >= s.ctas) return s;
-  s.first = cta * s.each + min(cta, s.longer);
-  s.last = s.first + s.each + (cta < s.longer ? 1 : 0);
+  int places = tiles;
+  if (tiles >= kTilesToPause * p.grid) {
+    s.pause = p.pause;
+    places += p.pause * __reduce_add_sync(0xffffffffu, units);
+  }
+  const int ctas = min(tiles, p.grid);  // those that get a tile: the others would leave no part where the merge looks for one
+  s.each = places / ctas;
+  s.longer = places - s.each * ctas;
+  if (cta >= ctas) return s;
+  const int first = cta * s.each + min(cta, s.longer);
+  int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const int mine = b0 == 0 ? of_first : tiles_of(b0 + lane);
+    int mine = tiles_of_first, mine_units = units_of_first;
+    if (b0 != 0) {
+      mine = mine_units = 0;
+      add_tiles_of(b0 + lane, mine, mine_units);
+    }
+    mine += s.pause * mine_units;
     int run = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int x = __shfl_up_sync(0xffffffffu, run, d);
       if (lane >= d) run += x;
     }
-    const unsigned behind = __ballot_sync(0xffffffffu, s.first < s.before + run);
+    const unsigned behind = __ballot_sync(0xffffffffu, first < before + run);
     if (behind != 0) {
       const int at = __ffs(behind) - 1;
-      s.request = b0 + at;
-      s.before += __shfl_sync(0xffffffffu, run - mine, at);
+      s.request = request_at(p, b0 + at);
+      before += __shfl_sync(0xffffffffu, run - mine, at);
       break;
     }
-    s.before += __shfl_sync(0xffffffffu, run, 31);
+    before += __shfl_sync(0xffffffffu, run, 31);
   }
+  const int of_unit = s.request.tiles + s.pause;
+  s.unit = (first - before) / of_unit;
+  s.unit_place = before + s.unit * of_unit;
+  s.tile = max(first - s.unit_place - s.pause, 0);
+  s.places = s.each + (cta < s.longer ? 1 : 0) - max(s.pause - (first - s.unit_place), 0);
   return s;
 }
 
@@ -223,7 +251,6 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   wait_for_previous_grid();
   if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
   const Share share = share_of(p, blockIdx.x, lane);
-  const int n_tiles = share.last - share.first;
   // the next unit's request, or one without units behind the last
   auto next_unit = [&](Request& r, int& unit) {
     if (++unit < r.units) return;
@@ -238,7 +265,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     } while (r.units == 0);
   };
 
-  if (n_tiles > 0 && warp >= kWarps) {
+  if (share.places > 0 && warp >= kWarps) {
     // ================================================================ the loading warps, one for K and one for V
     // Lane i has page 32 * group + i of a unit: block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page) and scale. Three
     // groups are under way: the one that tiles are copied from, the next with its scales, and the block numbers of the one behind.
@@ -269,10 +296,10 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       return keys && id == p.num_blocks ? __int_as_float(0x7fffffff) : 0.f;  // none in the cache: the scores of those who see it are NaN
     };
     Place cur, nxt, far;
-    cur.r = request_at(p, share.request);
-    cur.unit = (share.first - share.before) / cur.r.tiles;
+    cur.r = share.request;
+    cur.unit = share.unit;
     cur.head = cur.unit % p.heads_kv;
-    int tile = (share.first - share.before) - cur.unit * cur.r.tiles;
+    int tile = share.tile;
     cur.group = ((tile * kTileTokens) >> p.shift) >> 5;
     nxt = far = cur;
     int id = block_at(cur), next_id = -1, far_id = -1;
@@ -287,7 +314,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int pages = kTileTokens >> p.shift;  // of a tile
     bool ok = true;
     int step = 0;
-    for (int done = 0; done < n_tiles; ++done) {
+    bool first = true;
+    for (int places = share.places; places > 0;) {
       const int page0 = (tile * kTileTokens) >> p.shift;
       if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
       const bool tokens = tile * kTileTokens < cur.r.len;
@@ -312,7 +340,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           }
         }
       }
-      if (done == 0) {  // the first copies are under way
+      if (first) {  // the first copies are under way
         advance(nxt);
         next_id = block_at(nxt);
         far = nxt;
@@ -336,16 +364,19 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (lane == 0) mbar_arrive(bar);
         ++step;
       }
-      if (done == 0) next_scale = scale_at(nxt, next_id);
+      if (first) next_scale = scale_at(nxt, next_id);
+      first = false;
+      --places;
       if (++tile == cur.r.tiles) {
         tile = 0;
+        places -= share.pause;
         next_group();
       }
     }
   }
 
   SharedUnit left = {-1, 0, 0, 0, 0, 0};
-  if (n_tiles > 0 && warp < kWarps) {
+  if (share.places > 0 && warp < kWarps) {
     // ================================================================ the arithmetic. Fragments: a thread has rows 2t and 2t + 1 of every 8
     const int g = lane >> 2;
     const int t = lane & 3;
@@ -357,14 +388,14 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     };
     bool ok = true;
     int step = 0;  // tiles read
-    Request r = request_at(p, share.request);
-    int unit = (share.first - share.before) / r.tiles;
-    int tile = (share.first - share.before) - unit * r.tiles;
+    Request r = share.request;
+    int unit = share.unit, tile = share.tile, unit_place = share.unit_place;
     Request next_r = r;
     int next = unit;  // the unit behind
     bool first_unit = true;
-    for (int done = 0; done < n_tiles;) {
-      const int seg_tiles = min(n_tiles - done, r.tiles - tile);
+    for (int places = share.places; places > 0;) {
+      const int seg_tiles = min(places, r.tiles - tile);
+      places -= seg_tiles + share.pause;
       const int row0 = unit / p.heads_kv * p.rows, head = unit - unit / p.heads_kv * p.heads_kv;
       const int n_rows = min(p.rows, r.rows_q * p.group - row0);
       const int my_row0 = row0 + kRowsOfWarp * row_group;
@@ -407,7 +438,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
       if constexpr (!kQInRegisters) arithmetic_sync();
-      if (done + seg_tiles < n_tiles) {  // where the next unit's rows of Q are: they come nearer while this one's tiles are worked on
+      if (places > 0) {  // where the next unit's rows of Q are: they come nearer while this one's tiles are worked on
         next_unit(next_r, next);
         const int next_row0 = next / p.heads_kv * p.rows + kRowsOfWarp * row_group;
 #pragma unroll
@@ -687,8 +718,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         ++step;
       }
       // begun here, ended by the CTA whose share holds its last tile
-      if (tile == 0 && !whole) left = {share.cta_of(share.first + done + r.tiles - 1), slot, head, row0, n_rows, r.q0};
-      done += seg_tiles;
+      if (tile == 0 && !whole) left = {share.cta_of(unit_place + share.pause + r.tiles - 1), slot, head, row0, n_rows, r.q0};
+      unit_place += share.pause + r.tiles;
       tile = 0;
       first_unit = false;
       r = next_r;
@@ -975,7 +1006,8 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   p.rows = unit_rows(c);
   p.rows_shift = p.rows == 8 ? 3 : p.rows == 16 ? 4 : p.rows == 32 ? 5 : 6;
   p.tile_shift = c.head_dim == 64 ? 8 : 7;
-  p.most_tiles = INT32_MAX / c.batch;
+  p.pause = p.rows == 64 ? 0 : kPause;
+  p.most_tiles = INT32_MAX / (1 + kPause) / c.batch;
   p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - 256) + 1);
   p.causal = c.is_causal;
   p.f16 = c.dtype == SDPA_B200_F16;
