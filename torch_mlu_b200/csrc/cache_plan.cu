@@ -31,7 +31,11 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_par
   __shared__ int first_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x, ranks = gridDim.x;
-  if (tid == 0) first_bad = p.batch;
+  if (tid == 0) {
+    first_bad = p.batch;
+    launch_dependents();
+  }
+  wait_for_previous_grid();
   const int first = p.ring_state[0], count = p.ring_state[1];
   __syncthreads();
 
@@ -186,7 +190,7 @@ extern "C" SDPA_B200_API int sdpa_b200_plan_step(const sdpa_b200_plan_params* p,
   }
   // one block for a decode step; for more tokens up to eight, the largest cluster that every device takes
   const int ranks = p->num_tokens <= kThreads && p->batch <= kThreads ? 1 : p->num_tokens <= 2 * kThreads ? 4 : 8;
-  const cudaError_t err = launch_behind(plan_kernel, dim3(ranks), kThreads, smem, static_cast<cudaStream_t>(stream), false, ranks, *p, shift);
+  const cudaError_t err = launch_behind(plan_kernel, dim3(ranks), kThreads, smem, static_cast<cudaStream_t>(stream), true, ranks, *p, shift);
   if (err != cudaSuccess) {
     set_error("plan_step: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;

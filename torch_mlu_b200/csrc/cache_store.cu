@@ -171,6 +171,8 @@ __global__ void __launch_bounds__(kWarps * 32, 7) store_kernel(const StoreParams
     }
   };
 
+  if (threadIdx.x == 0) launch_dependents();
+  wait_for_previous_grid();
   if (warp == 0) find_runs(own0);
   __syncthreads();
 
@@ -321,15 +323,14 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params*
   const unsigned grid = static_cast<unsigned>(ctas);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const bool f16 = p->dtype == SDPA_B200_F16;
+  cudaError_t err = cudaSuccess;
   auto launch = [&](auto dim, auto int8) {
     constexpr int kD = decltype(dim)::value;
     constexpr bool kInt8 = decltype(int8)::value;
-    if (f16) store_kernel<kD, kInt8, true><<<grid, kWarps * 32, 0, cs>>>(s);
-    else store_kernel<kD, kInt8, false><<<grid, kWarps * 32, 0, cs>>>(s);
+    err = launch_behind(f16 ? store_kernel<kD, kInt8, true> : store_kernel<kD, kInt8, false>, dim3(grid), kWarps * 32, 0, cs, true, 1, s);
   };
   auto launch_dim = [&](auto dim) { p->code == SDPA_B200_INT8 ? launch(dim, std::true_type{}) : launch(dim, std::false_type{}); };
   p->head_dim == 64 ? launch_dim(std::integral_constant<int, 64>{}) : launch_dim(std::integral_constant<int, 128>{});
-  const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) {
     set_error("cache_store: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;

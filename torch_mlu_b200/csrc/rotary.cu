@@ -56,6 +56,8 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const RotaryParams 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   const int64_t token = item / p.splits;
+  if (threadIdx.x == 0) launch_dependents();
+  wait_for_previous_grid();
   if (token >= p.tokens) return;
   const int split = static_cast<int>(item - token * p.splits);
   const int b = static_cast<int>(token / p.length), row = static_cast<int>(token - static_cast<int64_t>(b) * p.length);
@@ -233,8 +235,7 @@ extern "C" SDPA_B200_API int sdpa_b200_rotary(const sdpa_b200_rotary_params* p, 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool f16 = p->dtype == SDPA_B200_F16;
   auto kernel = p->interleaved ? (f16 ? rotary_kernel<true, true> : rotary_kernel<false, true>) : (f16 ? rotary_kernel<true, false> : rotary_kernel<false, false>);
-  kernel<<<static_cast<unsigned>(blocks), kWarps * 32, 0, s>>>(r);
-  const cudaError_t err = cudaGetLastError();
+  const cudaError_t err = launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kWarps * 32, 0, s, true, 1, r);
   if (err != cudaSuccess) {
     set_error("rotary: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;
