@@ -12,7 +12,7 @@
 // Measured (8192 tokens of 4 prompts, 8 heads of 128, bf16 beside their queries to e4m3): 57 us with a warp for each run, which found it by itself, and
 // elements looked at one by one; 21 with a warp that finds runs for the CTA and the largest element two at a time as integers; 16.5 with a path of its own for
 // runs without gaps; 15.3 with all slots asked for before any is looked at; 14.2 with seven CTAs on an SM instead of six (3.5 TB/s; the few bytes spilled for it
-// cost the smallest calls 0.1 to 0.2). Of the 14.2, launch and runs are 4, and reading, codes and writing follow one another in a CTA. Rows held in
+// cost the smallest calls 0.1 to 0.2). Of the 14.2 (14.0 a call back to back, under the tail of the one in front), launch and runs are 4, and reading, codes and writing follow one another in a CTA. Rows held in
 // shared memory, those of the next head asked for ahead, one or eight warps instead of four, and asking L2 for the window's rows while the runs are found were no faster.
 #include "cache_common.cuh"
 

@@ -3,8 +3,10 @@
 //
 // A warp takes a token and some of its heads: its lanes form the cosines and sines together, once, in its own part of shared memory, then each keeps those of
 // its eight pairs in registers and goes over the heads, four at a time, with 16-byte loads and stores. Bound by HBM: every element is read and written once.
-// The product of a position and a frequency is taken in 64 bits, where it is exact, and brought into [-1, 1] half turns there: at position 10^6 the 32-bit product is off by up to
-// 0.03 radians. The rest, in 32 bits, is off by 2e-7.
+// The product of a position and a frequency is taken in 64 bits, where it is exact, and brought into [-1, 1] half turns there: at position 10^6 the
+// 32-bit product is off by up to 0.03 radians. The rest, in 32 bits, is off by 2e-7.
+// Measured: 16384 tokens, 32 and 8 heads of 128, three axes 55.7 us, 6.0 TB/s, 92% of a copy's rate; a training step's two turns of 8 x 2048 tokens, 16 and 16
+// heads, 87.4 us, 6.1 TB/s; 64 tokens 2.6 us, a launch.
 #include "kernels.h"
 #include "ptx_sm100.cuh"
 
