@@ -308,6 +308,18 @@ def test_many_units_to_a_share(cuda_device, rows, hq, hkv, dim, code, dtype):
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("lens,rows,hq,hkv,dim,code,dtype", [
+    ([1000], 1, 32, 8, 128, E4M3, torch.bfloat16), ([4000, 130, 0, 1], 1, 16, 4, 64, INT8, torch.float16), ([257, 128, 3, 900, 1024], 4, 8, 2, 128, INT8, torch.bfloat16),
+    ([129, 256, 64, 255] * 4, 1, 32, 8, 128, E4M3, torch.float16), ([2, 5000], 2, 32, 4, 128, E4M3, torch.bfloat16), ([300] * 8, 16, 4, 4, 64, E4M3, torch.float16)])
+def test_few_short_units(cuda_device, lens, rows, hq, hkv, dim, code, dtype):
+    """Units that clusters of CTAs take, of every size, and the same calls with a bound on lengths at which they are shared out by tiles."""
+    b = _batch(cuda_device, lens, [min(rows, n) if i % 3 == 2 else rows for i, n in enumerate(lens)], hq, hkv, dim, 16, code, dtype, seed=len(lens), powers=False)
+    for most in (max(lens), 1 << 20):
+        for causal in (True, False):
+            _compare(*_run(b, max_k=most, is_causal=causal), b, causal)
+    assert ops.device_status() == 0
+
+
 MANY_ROWS = [
     ([700, 600], [513, 520], 8, 2, 128, 64), ([1300, 130, 64], [600, 1, 0], 4, 4, 64, 16), ([300, 1000], [299, 300], 16, 2, 128, 128), ([520], [530], 1, 1, 64, 32),
     ([500, 0, 300], [490, 3, 300], 32, 2, 64, 16), ([257, 129, 128], [300, 129, 256], 32, 4, 64, 64), ([1000], [1000], 64, 8, 128, 32),

@@ -9,7 +9,7 @@
 //    O^T = V^T W^T in mma.sync.m16n8k16, tokens and dimensions in M, 8 rows in N, so that the few rows of a decode step leave no part of an
 //    instruction empty. The lengths are on the GPU; every CTA sums them up and takes an equal contiguous share of all units' tiles of 128 or
 //    256 tokens and of the hand-overs between units, so that all SMs are done at the same time however long each request is. A unit that several CTAs worked on leaves fp32
-//    parts in the workspace, at most two per CTA, and a second kernel merges them.
+//    parts in the workspace, at most two per CTA, and a second kernel merges them. Few short units are taken by a cluster of CTAs each instead.
 //    Two warps of a CTA, one for K and one for V, look up blocks and scales, two groups of 32 pages ahead, and fill a ring of tiles by TMA (a
 //    copy takes its warp about 100 cycles, which one warp with 16 of them per tile of 16 KB - blocks of 16 tokens, head_dim 64 - could not keep
 //    up with); four do the arithmetic, as 1, 2 or 4 groups of 8 or 16 rows by 4, 2 or 1 parts of a tile's tokens.
@@ -20,7 +20,7 @@
 //    the softmax takes w_j / vs_j in fp32.
 //    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
-//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000: 8.6 us.
+//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.1 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 135 us.
@@ -37,6 +37,8 @@ constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
 constexpr int kPause = 2, kTilesToPause = 4;  // see Share
+constexpr int kTilesInCluster = 8;          // that a CTA of a cluster may get: see cluster_of
+constexpr int kMostClusterCtas = 256;       // clusters of eight find room for that many CTAs at once
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
 constexpr float kSumUnit = 0x1p-40f;       // sums are kept in this unit, so that those over blocks of the least scale stay in range
 
@@ -57,6 +59,7 @@ struct StreamParams {
   int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
   int tile_shift;  // log2 of a tile's tokens
   int pause;       // see Share
+  int cluster, units_each;  // CTAs that share a unit, units that each request has room for: see Share
   int most_tiles;  // that a request may have, so that the sum of all stays in 32 bits
   int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
   float scale_log2;
@@ -209,8 +212,31 @@ __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int la
   return s;
 }
 
+// A row out of its merged parts: kPer of its dimensions a lane, sums of the weights 2^(lse - top) and of the parts by them
+template <int kPer>
+__device__ __forceinline__ void write_row(const StreamParams& p, int q0, int head, int row, int lane, const float (&acc)[kPer], float sum, float top, bool nan) {
+  const int i = row / p.group, hq = head * p.group + row - i * p.group;
+  const float inv = nan ? __int_as_float(0x7fffffff) : sum > 0.f ? 1.f / sum : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (q0 + i) * p.o_row + hq * p.o_head + kPer * lane);
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = p.f16 ? pack_f16x2(acc[e] * inv, acc[e + 1] * inv) : pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+  if (lane == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + q0 + i] = !nan && sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : INFINITY;
+}
+
+// Where a cluster of CTAs takes a unit: each a stretch of its tiles. Nothing is looked up but the one request.
+__device__ __forceinline__ Share share_in_cluster(const StreamParams& p, int cta) {
+  const int unit = cta / p.cluster, rank = cta - unit * p.cluster, b = unit / p.units_each;
+  Share s = {};
+  s.request = request_at(p, b);
+  s.unit = unit - b * p.units_each;
+  s.each = (s.request.tiles + p.cluster - 1) / p.cluster;
+  s.tile = rank * s.each;
+  if (s.unit < s.request.units) s.places = max(min(s.each, s.request.tiles - s.tile), 0);
+  return s;
+}
+
 // kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
-template <int kRowBlocks, int kRowWarps, int kD, bool kInt8>
+template <int kRowBlocks, int kRowWarps, int kD, bool kInt8, bool kCluster>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
   constexpr int kChunks = kD / 16;                           // 16 dimensions each
@@ -236,8 +262,13 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t full = smem_u32(q_state + kQWords), empty = full + 8 * kSt;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(q_state + kQWords) + 2 * kSt);
 
+  // kCluster: this CTA's part of the unit
+  float* own_part = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(abort_flag) + 4 + 15) & ~static_cast<uintptr_t>(15));  // [row][dimension]
+  float* own_lse = own_part + kRowsOfWarp * kD;
+
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  if (kCluster && threadIdx.x < kRowsOfWarp) own_lse[threadIdx.x] = -INFINITY;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
       mbar_init(full + 8 * i, 2);
@@ -250,7 +281,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   __syncthreads();
   wait_for_previous_grid();
   if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
-  const Share share = share_of(p, blockIdx.x, lane);
+  const Share share = kCluster ? share_in_cluster(p, blockIdx.x) : share_of(p, blockIdx.x, lane);
   // the next unit's request, or one without units behind the last
   auto next_unit = [&](Request& r, int& unit) {
     if (++unit < r.units) return;
@@ -703,11 +734,11 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
             if (g == 0 && part == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum[x] > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
           } else {
-            const int64_t at = (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
-            float* dst = p.part_o + at * kD + dim0;
+            const int64_t at = kCluster ? row - row0 : (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
+            float* dst = (kCluster ? own_part : p.part_o) + at * kD + dim0;
 #pragma unroll
             for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + 16 * ch) = make_float2(acc[ch][x] * inv, acc[ch][2 + x] * inv);
-            if (g == 0 && part == 0) p.part_lse[at] = lse2;
+            if (g == 0 && part == 0) (kCluster ? own_lse : p.part_lse)[at] = lse2;
           }
         }
       }
@@ -726,7 +757,52 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       unit = next;
     }
   }
-  if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
+  if constexpr (kCluster) {
+    cluster_sync();  // every CTA's part is written
+    const Request& r = share.request;
+    const int row0 = share.unit / p.heads_kv * p.rows, head = share.unit - share.unit / p.heads_kv * p.heads_kv;
+    const int rank = blockIdx.x - blockIdx.x / p.cluster * p.cluster;
+    if (share.unit < r.units && share.each < r.tiles) {  // (a single CTA's unit is done)
+      const int n_rows = min(p.rows, r.rows_q * p.group - row0);
+      for (int rr = rank + p.cluster * warp; rr < n_rows; rr += p.cluster * (kWarps + 2)) {
+        constexpr int kPer = kD / 32;
+        float v[8][kPer];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t src = smem_u32(own_part + rr * kD + kPer * lane);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) v[c][e] = 0.f;
+          if (c * share.each >= r.tiles) continue;  // without tiles: its part was never written
+          if constexpr (kPer == 4) {
+            const float4 x = cluster_ld_f32x4(src, c);
+            v[c][0] = x.x, v[c][1] = x.y, v[c][2] = x.z, v[c][3] = x.w;
+          } else {
+            const float2 x = cluster_ld_f32x2(src, c);
+            v[c][0] = x.x, v[c][1] = x.y;
+          }
+        }
+        const float x = lane < p.cluster ? cluster_ld_f32(smem_u32(own_lse + rr), lane) : -INFINITY;
+        const bool nan = __any_sync(0xffffffffu, isnan(x));
+        float top = x;
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        top = __shfl_sync(0xffffffffu, top, 0);
+        const float w = x == -INFINITY ? 0.f : exp2f(x - top);
+        float sum = 0.f, acc[kPer] = {};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float wc = __shfl_sync(0xffffffffu, w, c);
+          sum += wc;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wc, v[c][e], acc[e]);
+        }
+        write_row<kPer>(p, r.q0, head, row0 + rr, lane, acc, sum, top, nan);
+      }
+    }
+    cluster_sync();  // the others have read this CTA's
+  } else {
+    if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
+  }
   if (lane == 0) drain_after_abort(abort_flag);
   if (threadIdx.x == 0 && *abort_flag != 0) atomicExch(p.status, static_cast<uint32_t>(SDPA_B200_DEVICE_TIMEOUT));
 }
@@ -795,12 +871,7 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) 
       for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wj, v[e], acc[e]);
     }
   }
-  const int row = u.row0 + rr, i = row / p.group, hq = u.head * p.group + row - i * p.group;
-  const float inv = nan ? __int_as_float(0x7fffffff) : sum > 0.f ? 1.f / sum : 0.f;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (u.q0 + i) * p.o_row + hq * p.o_head + kPer * lane);
-#pragma unroll
-  for (int e = 0; e < kPer; e += 2) dst[e / 2] = p.f16 ? pack_f16x2(acc[e] * inv, acc[e + 1] * inv) : pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
-  if (lane == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + u.q0 + i] = !nan && sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : INFINITY;
+  write_row<kPer>(p, u.q0, u.head, u.row0 + rr, lane, acc, sum, top, nan);
 }
 
 // ---- many rows: the codes of all requests as packed 16-bit K and V
@@ -974,6 +1045,19 @@ size_t gather_bytes(const sdpa_b200_cache_params& p) {
   return static_cast<size_t>(p.batch) * padded_keys(p.max_seqlen_k) * p.heads_kv * p.head_dim * 2;
 }
 
+// Where the units are few and short, a cluster of 2 to 8 CTAs takes each, the tiles in equal stretches, and merges its parts through distributed shared memory: no lengths to be
+// summed up in front and no second kernel behind. That leaves SMs idle where units are of many lengths, so it is for up to eight tiles a CTA of the longest. Measured, shares of
+// the list | clusters, one token each, 32/8 heads of 128, us: 1 request of 1000 8.6 | 6.1, of 4000 12.0 | 8.4, of 8000 17.4 | 11.5; 4 of 600 to 5000 15.2 | 10.1, of 8000
+// 21.8 | 17.9; 8 of 300 to 1000 9.6 | 7.9, of 600 to 4000 14.3 | 13.0; 16 of 100 to 500 12.2 | 7.9, of 100 to 2000 13.9 | 12.4, of 2000 21.0 | 17.9. Beyond: 1 of 32000
+// 24.2 | 31.0, 16 of 600 to 8000 28.0 | 34.4, 4 tokens of 16 of 300 to 9000 at head_dim 64 19.9 | 24.0.
+int cluster_of(const sdpa_b200_cache_params& c, int rows, int64_t units, int tile_shift) {
+  const int64_t tiles = (static_cast<int64_t>(c.max_seqlen_k) + (1 << tile_shift) - 1) >> tile_shift;
+  if (rows > 16 || tiles < 2) return 0;
+  int size = 8;
+  while (size > 1 && (units * size > kMostClusterCtas || size / 2 >= tiles)) size /= 2;
+  return size > 1 && tiles <= kTilesInCluster * size ? size : 0;
+}
+
 int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* status, cudaStream_t stream) {
   const int sms = sm_count();
   if (sms <= 0 || sms > kMaxSms) {
@@ -1016,6 +1100,10 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   const int64_t units = static_cast<int64_t>(c.batch) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
   const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + (1 << p.tile_shift) - 1) >> p.tile_shift);
   p.grid = static_cast<int>(tiles < kCtasPerSm * sms ? tiles : kCtasPerSm * sms);
+  // a cluster for each unit
+  p.units_each = static_cast<int>(units / c.batch);
+  p.cluster = cluster_of(c, p.rows, units, p.tile_shift);
+  if (p.cluster > 0) p.grid = static_cast<int>(units) * p.cluster;
   const size_t rows = static_cast<size_t>(kCtasPerSm) * kMaxSms * 2 * p.rows;
   p.part_o = reinterpret_cast<float*>(workspace + kWorkspaceHeaderBytes);
   p.part_lse = p.part_o + rows * c.head_dim;
@@ -1026,14 +1114,21 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
   st = make_cache_tensor_map(&tm_v, c.v_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.v_row_stride, c.v_head_stride, c.v_block_stride, c.block_size);
   if (st != SDPA_B200_OK) return st;
   cudaError_t err = cudaSuccess;
-  auto launch = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag) {
-    constexpr bool kInt8 = decltype(int8_tag)::value;
+  auto launch_as = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag, auto cluster_tag) {
+    constexpr bool kInt8 = decltype(int8_tag)::value, kCluster = decltype(cluster_tag)::value;
     constexpr int kRowBlocks = decltype(blocks_tag)::value, kRowWarps = decltype(rows_tag)::value, kD = decltype(dim_tag)::value;
-    constexpr uint32_t kSmem = stream_smem_bytes<kRowBlocks, kRowWarps, kD>();
+    constexpr uint32_t kSmem = stream_smem_bytes<kRowBlocks, kRowWarps, kD>() + (kCluster ? 32 + 8 * kRowBlocks * (kD + 1) * 4 : 0);
     static_assert(kCtasPerSm * (kSmem + 1024) <= 228 * 1024, "two CTAs do not fit an SM");
-    auto kernel = cache_stream_kernel<kRowBlocks, kRowWarps, kD, kInt8>;
+    auto kernel = cache_stream_kernel<kRowBlocks, kRowWarps, kD, kInt8, kCluster>;
     err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (err == cudaSuccess) err = launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, c.device_status != nullptr, 1, tm_k, tm_v, p);
+    if (err == cudaSuccess)
+      err = launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, c.device_status != nullptr, kCluster ? p.cluster : 1, tm_k, tm_v, p);
+  };
+  auto launch = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag) {
+    if constexpr (decltype(rows_tag)::value == 1) {
+      if (p.cluster > 0) return launch_as(blocks_tag, rows_tag, dim_tag, int8_tag, std::true_type{});
+    }
+    launch_as(blocks_tag, rows_tag, dim_tag, int8_tag, std::false_type{});
   };
   auto launch_code = [&](auto blocks_tag, auto rows_tag, auto dim_tag) {
     c.code == SDPA_B200_INT8 ? launch(blocks_tag, rows_tag, dim_tag, std::true_type{}) : launch(blocks_tag, rows_tag, dim_tag, std::false_type{});
@@ -1052,7 +1147,7 @@ int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* st
     return SDPA_B200_LAUNCH_FAILED;
   }
   count_launch();
-  if (p.grid == 1 || c.max_seqlen_k <= 1 << p.tile_shift) return SDPA_B200_OK;  // no unit is shared
+  if (p.cluster > 0 || p.grid == 1 || c.max_seqlen_k <= 1 << p.tile_shift) return SDPA_B200_OK;  // no unit is shared, or merged already
   cudaLaunchConfig_t cfg = {};  // under this grid's tail, under stream capture too: what stands in front is a kernel of this call
   cfg.gridDim = dim3(p.grid - 1, p.rows / 4);
   cfg.blockDim = dim3(128);
