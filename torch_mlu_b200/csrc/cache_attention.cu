@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "cache_common.cuh"
+#include "cache_shares.cuh"
 
 namespace sdpa_b200 {
 namespace {
@@ -36,7 +37,7 @@ constexpr int kWarps = 4;                  // those that do the arithmetic
 constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are dealt out as for six warps anyway
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
-constexpr int kPause = 2, kTilesToPause = 4;  // see Share
+constexpr int kPause = 2;  // see share_of
 constexpr int kTilesInCluster = 8;          // that a CTA of a cluster may get: see cluster_of
 constexpr int kMostClusterCtas = 256;       // clusters of eight find room for that many CTAs at once
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
@@ -58,9 +59,9 @@ struct StreamParams {
   int64_t q_row, q_head, o_row, o_head, table_stride;
   int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
   int tile_shift;  // log2 of a tile's tokens
-  int pause;       // see Share
-  int cluster, units_each;  // CTAs that share a unit, units that each request has room for: see Share
-  int most_tiles;  // that a request may have, so that the sum of all stays in 32 bits
+  int pause;       // see share_of
+  int first_q, max_rows;  // the first request's row of q where there are no offsets; rows that a request may have
+  int cluster, units_each;  // CTAs that share a unit, units that each request has room for: see share_in_cluster
   int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
   float scale_log2;
 };
@@ -69,27 +70,6 @@ struct StreamParams {
 struct SharedUnit {
   int last, slot, head, row0, rows, q0;  // the CTA that ends it; where the first CTA's part is; kv head, rows [row0, row0 + rows) of the request whose tokens begin at q0
 };
-
-// A request as units see it
-struct Request {
-  int index, len, rows_q, q0;  // tokens in the cache, rows of q, the first of them
-  int in_front;                // row i sees i + 1 + in_front tokens where causal
-  int tiles, units;            // per unit; 0 units: no rows
-};
-
-__device__ __forceinline__ Request request_at(const StreamParams& p, int b) {
-  Request r;
-  r.index = b;
-  const int len = p.seq_lens[b];
-  r.len = min(max(len, 0), p.max_len);
-  r.q0 = p.cu_q ? p.cu_q[b] : b;
-  r.rows_q = p.cu_q ? max(p.cu_q[b + 1] - r.q0, 0) : 1;
-  if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
-  r.in_front = len > p.max_len - 1 ? r.len : r.len - r.rows_q;  // longer than the table: all its rows see the block that there is none of
-  r.tiles = max((r.len + (1 << p.tile_shift) - 1) >> p.tile_shift, 1);  // an empty request has rows to write too
-  r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
-  return r;
-}
 
 // Tokens of a tile, 32 KB of K and V, and those that a warp handles at a time: its products, maxima over lanes, exponentials and products again are one long chain, in which the
 // blocks of 16 tokens run beside each other; as many as registers hold.
@@ -136,32 +116,19 @@ __device__ __forceinline__ float column_sum(float x) {
   return x;
 }
 
-// A CTA's share of the list of all tiles. Places in the list: a unit has one for each tile, behind `pause` empty ones that stand for what the hand-over from unit
+// A CTA's share of the list of all tiles (cache_shares.cuh). The empty places in front of a unit stand for what the hand-over from unit
 // to unit takes, which is about that of two tiles (not so with 64 rows, whose warps have nothing to merge and more to do per tile: 59.5 us with it, 58.8 without, 4 requests
-// of 32 rows). Equal shares of the places, the first of them one longer where they do not come out even; a CTA works on the tiles whose places are in its own. Where a CTA
-// has fewer than four tiles it has few hand-overs, and the places are the tiles. Measured with equal shares of the tiles | of the places, one token each, us: 64 requests
+// of 32 rows). Measured with equal shares of the tiles | of the places, one token each, us: 64 requests
 // of 200 to 1800 37.9 | 33.9, 128 of 100 to 900 52.8 | 39.9, 32 of 100 to 2000 with 32 kv heads 62 | 48.5, 64 of 500 to 4000 59.3 | 55.5; 4 tokens, 16 of 300 to 9000 at
 // head_dim 64 22.0 | 19.8. With pauses of one place the second took 43.9, with three the same, and 8 tokens of 32 requests 53.8 instead of 52.0.
-struct Share {
-  int places;              // from the first tile of the CTA on; 0: it has none
-  Request request;         // where it begins
-  int unit, tile;
-  int unit_place;          // the place of that unit
-  int pause;
-  int each, longer;        // places of a share, how many shares have one more
-  __device__ __forceinline__ int cta_of(int place) const {
-    const int in_longer = longer * (each + 1);
-    return place < in_longer ? place / (each + 1) : longer + (place - in_longer) / each;
-  }
-};
-
+//
 // Every warp finds it for itself, so that none waits for another.
 __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int lane) {
   auto add_tiles_of = [&](int b, int& tiles, int& units) {
     if (b >= p.batch) return;
     const Request r = request_at(p, b);
-    units += static_cast<int>(min(static_cast<int64_t>(r.units), static_cast<int64_t>(p.most_tiles)));
-    tiles += static_cast<int>(min(static_cast<int64_t>(r.tiles) * r.units, static_cast<int64_t>(p.most_tiles)));
+    units += r.units;
+    tiles += tiles_of(r);
   };
   int tiles_of_first = 0, units_of_first = 0;  // of the first 32 requests
   add_tiles_of(lane, tiles_of_first, units_of_first);
@@ -171,16 +138,8 @@ __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int la
   tiles = __reduce_add_sync(0xffffffffu, tiles);
   Share s = {};
   if (tiles == 0) return s;
-  int places = tiles;
-  if (tiles >= kTilesToPause * p.grid) {
-    s.pause = p.pause;
-    places += p.pause * __reduce_add_sync(0xffffffffu, units);
-  }
-  const int ctas = min(tiles, p.grid);  // those that get a tile: the others would leave no part where the merge looks for one
-  s.each = places / ctas;
-  s.longer = places - s.each * ctas;
-  if (cta >= ctas) return s;
-  const int first = cta * s.each + min(cta, s.longer);
+  const int first = deal(s, p, tiles, tiles >= kTilesToPause * p.grid ? __reduce_add_sync(0xffffffffu, units) : 0, cta);
+  if (first < 0) return s;
   int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     int mine = tiles_of_first, mine_units = units_of_first;
@@ -198,17 +157,12 @@ __device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int la
     const unsigned behind = __ballot_sync(0xffffffffu, first < before + run);
     if (behind != 0) {
       const int at = __ffs(behind) - 1;
-      s.request = request_at(p, b0 + at);
       before += __shfl_sync(0xffffffffu, run - mine, at);
+      begin_in(s, request_at(p, b0 + at), first - before, cta);
       break;
     }
     before += __shfl_sync(0xffffffffu, run, 31);
   }
-  const int of_unit = s.request.tiles + s.pause;
-  s.unit = (first - before) / of_unit;
-  s.unit_place = before + s.unit * of_unit;
-  s.tile = max(first - s.unit_place - s.pause, 0);
-  s.places = s.each + (cta < s.longer ? 1 : 0) - max(s.pause - (first - s.unit_place), 0);
   return s;
 }
 
@@ -282,20 +236,6 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   wait_for_previous_grid();
   if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
   const Share share = kCluster ? share_in_cluster(p, blockIdx.x) : share_of(p, blockIdx.x, lane);
-  // the next unit's request, or one without units behind the last
-  auto next_unit = [&](Request& r, int& unit) {
-    if (++unit < r.units) return;
-    unit = 0;
-    int b = r.index + 1;
-    do {
-      if (b >= p.batch) {
-        r = {b, 0, 0, 0, 0, 1, 0};
-        return;
-      }
-      r = request_at(p, b++);
-    } while (r.units == 0);
-  };
-
   if (share.places > 0 && warp >= kWarps) {
     // ================================================================ the loading warps, one for K and one for V
     // Lane i has page 32 * group + i of a unit: block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page) and scale. Three
@@ -312,7 +252,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         ++x.group;
       } else {
         x.group = 0;
-        if (x.r.units > 0) next_unit(x.r, x.unit);
+        if (x.r.units > 0) next_unit(p, x.r, x.unit);
         x.head = x.unit % p.heads_kv;
       }
     };
@@ -420,7 +360,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     bool ok = true;
     int step = 0;  // tiles read
     Request r = share.request;
-    int unit = share.unit, tile = share.tile, unit_place = share.unit_place;
+    int unit = share.unit, tile = share.tile;
     Request next_r = r;
     int next = unit;  // the unit behind
     bool first_unit = true;
@@ -470,7 +410,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
       if constexpr (!kQInRegisters) arithmetic_sync();
       if (places > 0) {  // where the next unit's rows of Q are: they come nearer while this one's tiles are worked on
-        next_unit(next_r, next);
+        next_unit(p, next_r, next);
         const int next_row0 = next / p.heads_kv * p.rows + kRowsOfWarp * row_group;
 #pragma unroll
         for (int nb = 0; nb < kRowBlocks; ++nb) {
@@ -748,9 +688,8 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         if (lane == 0) mbar_arrive(empty + 8 * st);
         ++step;
       }
-      // begun here, ended by the CTA whose share holds its last tile
-      if (tile == 0 && !whole) left = {share.cta_of(unit_place + share.pause + r.tiles - 1), slot, head, row0, n_rows, r.q0};
-      unit_place += share.pause + r.tiles;
+      // begun here, where the share ends; ended by the CTA whose share holds its last tile
+      if (tile == 0 && !whole) left = {share.cta_behind(blockIdx.x, r.tiles - seg_tiles - 1), slot, head, row0, n_rows, r.q0};
       tile = 0;
       first_unit = false;
       r = next_r;
@@ -1058,50 +997,62 @@ int cluster_of(const sdpa_b200_cache_params& c, int rows, int64_t units, int til
   return size > 1 && tiles <= kTilesInCluster * size ? size : 0;
 }
 
-int launch_stream(const sdpa_b200_cache_params& c, char* workspace, uint32_t* status, cudaStream_t stream) {
-  const int sms = sm_count();
-  if (sms <= 0 || sms > kMaxSms) {
-    set_error("cache_attention: cannot use a device with %d SMs", sms);
-    return SDPA_B200_NO_DEVICE;
-  }
-  StreamParams p;
-  p.q = static_cast<const uint16_t*>(c.q);
-  p.out = static_cast<uint16_t*>(c.out);
-  p.lse = c.lse;
-  p.k_scale = c.k_scale;
-  p.v_scale = c.v_scale;
+// What the list of tiles and its units depend on, of all requests; no device is asked
+StreamParams list_of(const sdpa_b200_cache_params& c) {
+  StreamParams p = {};
   p.block_table = c.block_table;
   p.seq_lens = c.seq_lens;
   p.cu_q = c.cu_seqlens_q;
-  p.status = status;
-  p.q_row = c.q_row_stride;
-  p.q_head = c.q_head_stride;
-  p.o_row = c.o_row_stride;
-  p.o_head = c.o_head_stride;
   p.table_stride = c.table_stride;
   p.batch = c.batch;
   p.heads_q = c.heads_q;
   p.heads_kv = c.heads_kv;
   p.group = c.heads_q / c.heads_kv;
   p.total_q = c.total_q;
+  p.max_rows = c.max_seqlen_q;
   p.max_blocks = c.max_blocks;
-  p.num_blocks = c.num_blocks;
-  p.shift = block_shift(c.block_size);
   p.rows = unit_rows(c);
   p.rows_shift = p.rows == 8 ? 3 : p.rows == 16 ? 4 : p.rows == 32 ? 5 : 6;
   p.tile_shift = c.head_dim == 64 ? 8 : 7;
   p.pause = p.rows == 64 ? 0 : kPause;
-  p.most_tiles = INT32_MAX / (1 + kPause) / c.batch;
   p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - 256) + 1);
+  return p;
+}
+
+// Requests [first, first + count)
+int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* workspace, uint32_t* status, cudaStream_t stream) {
+  const int sms = sm_count();
+  if (sms <= 0 || sms > kMaxSms) {
+    set_error("cache_attention: cannot use a device with %d SMs", sms);
+    return SDPA_B200_NO_DEVICE;
+  }
+  StreamParams p = list_of(c);
+  p.batch = count;
+  p.block_table += first * p.table_stride;
+  p.seq_lens += first;
+  if (p.cu_q != nullptr) p.cu_q += first;
+  p.first_q = first;
+  p.q = static_cast<const uint16_t*>(c.q);
+  p.out = static_cast<uint16_t*>(c.out);
+  p.lse = c.lse;
+  p.k_scale = c.k_scale;
+  p.v_scale = c.v_scale;
+  p.status = status;
+  p.q_row = c.q_row_stride;
+  p.q_head = c.q_head_stride;
+  p.o_row = c.o_row_stride;
+  p.o_head = c.o_head_stride;
+  p.num_blocks = c.num_blocks;
+  p.shift = block_shift(c.block_size);
   p.causal = c.is_causal;
   p.f16 = c.dtype == SDPA_B200_F16;
   p.scale_log2 = c.softmax_scale * 1.4426950408889634f;
   // a CTA per tile, up to one wave
-  const int64_t units = static_cast<int64_t>(c.batch) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
+  const int64_t units = static_cast<int64_t>(count) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
   const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + (1 << p.tile_shift) - 1) >> p.tile_shift);
   p.grid = static_cast<int>(tiles < kCtasPerSm * sms ? tiles : kCtasPerSm * sms);
   // a cluster for each unit
-  p.units_each = static_cast<int>(units / c.batch);
+  p.units_each = static_cast<int>(units / count);
   p.cluster = cluster_of(c, p.rows, units, p.tile_shift);
   if (p.cluster > 0) p.grid = static_cast<int>(units) * p.cluster;
   const size_t rows = static_cast<size_t>(kCtasPerSm) * kMaxSms * 2 * p.rows;
@@ -1267,6 +1218,11 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
     set_error("cache_attention: the workspace must be a device pointer aligned to 256 bytes, of %zu bytes (got %zu)", need, workspace_bytes);
     return SDPA_B200_INVALID_ARG;
   }
+  if (streams(*p) && requests_at_once(list_of(*p)) == 0) {
+    set_error("cache_attention: a request of %d rows of %d heads and the %lld tokens of its table is too long", p->max_seqlen_q, p->heads_q,
+              static_cast<long long>(p->max_blocks) * p->block_size);
+    return SDPA_B200_UNSUPPORTED;
+  }
   if (!streams(*p) && (p->batch > 65535 || p->heads_kv > 65535)) {
     set_error("cache_attention: many rows per request come in batches of up to 65535, with up to 65535 heads (got %d, %d)", p->batch, p->heads_kv);
     return SDPA_B200_UNSUPPORTED;
@@ -1283,6 +1239,13 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
     return SDPA_B200_LAUNCH_FAILED;
   }
   uint32_t* status = p->device_status != nullptr ? p->device_status : static_cast<uint32_t*>(workspace);
-  if (streams(*p)) return launch_stream(*p, static_cast<char*>(workspace), status, s);
+  if (streams(*p)) {
+    const int at_once = requests_at_once(list_of(*p));
+    for (int first = 0; first < p->batch; first += at_once) {
+      st = launch_stream(*p, first, std::min(at_once, p->batch - first), static_cast<char*>(workspace), status, s);
+      if (st != SDPA_B200_OK) return st;
+    }
+    return SDPA_B200_OK;
+  }
   return launch_gathered(*p, static_cast<char*>(workspace), status, s);
 }
