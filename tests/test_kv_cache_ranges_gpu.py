@@ -42,3 +42,70 @@ def test_a_list_that_takes_several_launches(cuda_device):
         assert launched == 2 * (_cabi.launch_count() - before)
         # which CTAs share a unit differs, and so the order of the sums
         _compare(*again, b)
+
+
+def _gathers(b, **kw):
+    """Whether a call brings keys and values to 16 bits in its workspace, by the names of its kernels; and its results."""
+    torch.cuda.synchronize()
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        out, lse = _run(b, **kw)
+        torch.cuda.synchronize()
+    names = [e.key for e in prof.key_averages()]
+    gathers, streams = (any(n in name for name in names) for n in ("cache_gather_kernel", "cache_stream_kernel"))
+    assert gathers != streams, names
+    return gathers, out, lse
+
+
+@pytest.mark.parametrize("code,values", [(E4M3, (63488.0, 64000.0, 65504.0)), (INT8, (65024.0, 65280.0, 65504.0))])
+@pytest.mark.parametrize("rows", [2, 1000])
+def test_f16_elements_whose_codes_are_65536(cuda_device, rows, code, values):
+    """On both paths. The keys' large elements meet queries of 2^-10: a score has 8 to 11 of each. Where they are clamped to 65504 it is off by 2^-11 of that, 2^-11 * 11.4 * 3 for
+    the three of a key at most, and a weight by twice as much of itself; a value by 2^-11 of itself; the logsumexp by as much as a score."""
+    n, hq, hkv, dim, block = 1300, 64, 8, 128, 64
+    g = torch.Generator(device=cuda_device).manual_seed(rows)
+    k, v = (torch.randn(n, hkv, dim, generator=g, device=cuda_device).half() for _ in range(2))
+    for i, x in enumerate(values):
+        k[i::7, :, i] = x * (1 if i % 2 else -1)
+        v[i::11, i % hkv, i::5] = x
+    kc, ks = _cache(cuda_device, 24, hkv, block, dim, code, 1)
+    vc, vs = _cache(cuda_device, 24, hkv, block, dim, code, 2)
+    pages = torch.randperm(24, generator=torch.Generator().manual_seed(1))[:-(-n // block)]
+    slots = _ints(cuda_device, [int(pages[t // block]) * block + t % block for t in range(n)])
+    want = orc.store(k, slots, kc, ks), orc.store(v, slots, vc, vs)
+    kv_cache.store(k, v, slots, kc, vc, ks, vs)
+    _same_cache(kc, ks, *want[0])
+    _same_cache(vc, vs, *want[1])
+    for c, scale in ((kc, ks), (vc, vs)):  # (the last block has more than the tokens)
+        largest = float((c[pages[:-1]].float() * scale[pages[:-1]][..., None, None]).abs().max())
+        assert largest == 65536
+    q = torch.randn(rows, hq, dim, generator=g, device=cuda_device).half()
+    q[..., :3] = 2.0 ** -10 * q[..., :3].sign()
+    b = (q, kc, vc, ks, vs, _ints(cuda_device, [pages.tolist()]), _ints(cuda_device, [n]), _ints(cuda_device, [0, rows]))
+    gathers, out, lse = _gathers(b)
+    assert gathers == (rows == 1000)
+    ref, ref_lse, size, most = orc.attention(*b)
+    clamped = gathers * 2.0 ** -11
+    score = clamped * 65536 * 2.0 ** -10 * 3 * dim ** -0.5
+    # v is up to 65536 in few places, so that the result stays below 65504
+    assert float(ref.abs().max()) < 60000 and bool(out.isfinite().all())
+    tol = 2.0 ** -11 * ref.abs() + (2.0 ** -11 + 1e-4 + clamped + 2 * score) * size
+    assert bool(((out.double() - ref).abs() <= tol).all()), float(((out.double() - ref).abs() - tol).max())
+    ltol = 2.0 ** -24 * (n / 128 * 9 + 40) + 2.0 ** -21 * most.clamp_min(1) + 2.0 ** -23 * ref_lse.abs() + score
+    assert bool(((lse.double() - ref_lse).abs() <= ltol).all())
+
+
+def test_f16_queries_over_a_cache_of_bf16_elements(cuda_device):
+    """Values beyond f16's range count as 65504 where they are brought to 16 bits, and as they are where they are not; NaN stays what it is."""
+    n, dim, block = 1100, 64, 64
+    for rows, hq in ((1, 4), (1000, 64)):
+        b = list(_batch(cuda_device, [n, 64], [rows, 1], hq, 2, dim, block, E4M3, torch.float16, poison=False))
+        b[2] = (torch.ones_like(b[2], dtype=torch.float32) * 256).to(E4M3)
+        b[4] = torch.full_like(b[4], 2.0 ** 9)  # 131072 everywhere
+        gathers, out, lse = _gathers(b)
+        assert gathers == (rows == 1000)
+        # 131072 does not fit the result and is +inf. A mean of numbers that are all 65504, with weights rounded to f16, is off by up to (2^-11 + 1e-4) * 65504 = 38.6: 65465 to
+        # 65543, of which the nearest f16 numbers are 65472 and, from 65520 on, +inf
+        assert bool((out >= (65472 if gathers else math.inf)).all()) and bool(lse.isfinite().all()) and bool(out.isfinite().any()) == gathers
+        b[2][int(b[5][0, 3]), 0, 5] = torch.tensor(math.nan, device=cuda_device).to(E4M3)
+        out, lse = _run(b)
+        assert bool(out[:rows, :hq // 2].isnan().any()) and not bool(out[rows:].isnan().any())

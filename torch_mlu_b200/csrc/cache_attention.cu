@@ -22,7 +22,7 @@
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
 //    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.1 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
-//    in the workspace (exact with the powers of two that the store kernel chooses), and the prefill kernel does the rest. 512 tokens behind 7680,
+//    in the workspace (exact with the powers of two that the store kernel chooses, within the type's range), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 135 us.
 #include <algorithm>
 #include <type_traits>
@@ -832,6 +832,16 @@ constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, 
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
 
+// two elements in 16 bits, the largest number of the type where they are beyond it: a code is rounded, and the elements 65504 of f16 or 3.39e38 of bf16 come back as
+// 2^16 or 2^128. NaN stays.
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack_16x2_finite(float lo, float hi) {
+  uint32_t r;
+  if constexpr (kF16) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // Block (i, h, b): tokens 32i to 32i + 31 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
 // where a weight of 0 would meet another request's NaN, or whatever the workspace held. So every request's rows are filled up to a whole tile with zeros, and these
 // stand in the list of sequences as one of their own, without queries.
@@ -881,7 +891,8 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       scale[i][x] = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
       w[i][x] = *reinterpret_cast<const uint2*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
-      scale[i][x] = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
+      const float own = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
+      scale[i][x] = fabsf(own) == INFINITY ? __int_as_float(0x7fffffff) : own;  // nor are elements of such a block numbers on the other path
     }
   }
 #pragma unroll
@@ -896,8 +907,8 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
         uint32_t lo, hi;
         codes_to_f16<kInt8>(c[e], lo, hi);
         const float2 u = unpack_16x2<true>(lo), v = unpack_16x2<true>(hi);
-        f[2 * e] = pack_16x2<kF16>(u.x * scale[i][x], u.y * scale[i][x]);
-        f[2 * e + 1] = pack_16x2<kF16>(v.x * scale[i][x], v.y * scale[i][x]);
+        f[2 * e] = pack_16x2_finite<kF16>(u.x * scale[i][x], u.y * scale[i][x]);
+        f[2 * e + 1] = pack_16x2_finite<kF16>(v.x * scale[i][x], v.y * scale[i][x]);
       }
       *reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
     }

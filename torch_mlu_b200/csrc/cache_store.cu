@@ -3,7 +3,7 @@
 // Per (block, head) that gets tokens: need = the smallest power of two at which the largest new element is a code, scale = max(old, need) where
 // the block holds earlier tokens, code = round(x / scale). Decoding raises the scale of a block that fills up token by token; earlier tokens are then
 // read, multiplied by old / scale and rounded again. With powers of two that costs e4m3 only what falls below its smallest numbers, and a
-// dequantised element is exact in 16 bits.
+// dequantised element is exact in 16 bits within their range (the code of f16's 65504 is 65536).
 //
 // Bound by HBM for prompts (two bytes read and one written per element), by latency for decode steps. The tokens of one block stand next to each other,
 // so a run of them is found from the slots alone: it begins where a token's block is not that of the token with a place in front. A CTA takes a window of

@@ -76,7 +76,8 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     request has one row. ``max_seqlen_q`` and ``max_seqlen_k`` are at least the most rows and the longest request; without max_seqlen_k it is what
     the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace, which takes
     4 * requests * max_seqlen_k * heads_kv * head_dim bytes, and the prefill kernel runs. That is exact with scales that are powers of two, as store gives
-    them; with others every element is rounded once.
+    them; with others every element is rounded once. Elements beyond the largest number of query's type are that number there (fp16: 65504, of which the code may be 65536),
+    and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24.
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package).
