@@ -118,7 +118,7 @@ static void walk(const char* name, const std::vector<int32_t>& lens, const std::
   std::vector<int32_t> offsets(1, 0);
   for (int r : rows_q) offsets.push_back(offsets.back() + r);
   Lists all = {lens.data(), cu ? offsets.data() : nullptr, static_cast<int>(lens.size()), heads_kv, group, offsets.back(), unit_rows,
-               unit_rows == 8 ? 3 : unit_rows == 16 ? 4 : unit_rows == 32 ? 5 : 6, tile_shift, capacity + 1, 2 * sms, unit_rows == 64 ? 0 : 2, 0,
+               unit_rows == 8 ? 3 : unit_rows == 16 ? 4 : unit_rows == 32 ? 5 : 6, tile_shift, capacity, 2 * sms, unit_rows == 64 ? 0 : 2, 0,
                std::max(1, *std::max_element(rows_q.begin(), rows_q.end()))};
   const int at_once = requests_at_once(all);
   CHECK(at_once > 0, "%s: too long", name);

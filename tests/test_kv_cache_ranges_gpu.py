@@ -109,3 +109,33 @@ def test_f16_queries_over_a_cache_of_bf16_elements(cuda_device):
         b[2][int(b[5][0, 3]), 0, 5] = torch.tensor(math.nan, device=cuda_device).to(E4M3)
         out, lse = _run(b)
         assert bool(out[:rows, :hq // 2].isnan().any()) and not bool(out[rows:].isnan().any())
+
+
+@pytest.mark.parametrize("rows,dim,width,max_k", [(1, 128, 8, None), (1, 64, 16, None), (3, 128, 8, 128), (1, 128, 90, None), (5, 64, 90, 1440), (1100, 128, 90, None), (1100, 64, 90, 1440),
+                                                  (1500, 128, 90, None), (1500, 128, 90, 1000)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_request_longer_than_its_table(cuda_device, rows, dim, width, max_k, causal):
+    """All of its rows are NaN, on both paths, whatever the bound on lengths, also where the call has no more tiles than requests, or the request more rows than the table tokens;
+    the requests beside it are as they would be."""
+    lens, each = [90, 60, 100, 128, 70], [2, 1, rows, 1, 3] if rows > 1 else [1] * 5
+    hq, hkv = (64, 8) if rows > 500 else (8, 2)
+    if width * 16 >= 1300:
+        lens = [1000, 60, 700, 900, 1300]
+    for length in (width * 16 + 1, 10 ** 9, 2 ** 31 - 1):
+        b = list(_batch(cuda_device, lens, each, hq, hkv, dim, 16, E4M3, torch.bfloat16, seed=rows))
+        table = torch.full((5, width), -5, dtype=torch.int32, device=cuda_device)
+        n = min(width, b[5].size(1))
+        table[:, :n] = b[5][:, :n]
+        b[5] = table
+        lens_given = b[6].clone()
+        lens_given[2] = length
+        q, kc, vc, ks, vs, _, _, cu = b
+        kw = dict(is_causal=causal)
+        out, lse = kv_cache.attention(q, kc, vc, ks, vs, table, lens_given, cu, max(each), max_k, **kw) if rows > 1 else kv_cache.attention(q, kc, vc, ks, vs, table, lens_given, max_seqlen_k=max_k, **kw)
+        lo, hi = int(cu[2]), int(cu[3])
+        assert bool(out[lo:hi].isnan().all()) and bool((lse[:, lo:hi] == math.inf).all())
+        out[lo:hi], lse[:, lo:hi] = 0, math.inf  # as of a request without tokens
+        b[6] = b[6].clone()
+        b[6][2] = 0
+        _compare(out, lse, b, causal, many=rows > 500)
+    assert ops.device_status() == 0

@@ -62,7 +62,7 @@ struct StreamParams {
   int pause;       // see share_of
   int first_q, max_rows;  // the first request's row of q where there are no offsets; rows that a request may have
   int cluster, units_each;  // CTAs that share a unit, units that each request has room for: see share_in_cluster
-  int max_len;  // one more than the table holds: a longer request's rows are NaN all the same
+  int max_len;  // tokens that a table's row holds
   float scale_log2;
 };
 
@@ -259,7 +259,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto block_at = [&](const Place& x) {
       const int page = x.group * 32 + lane;
       if ((static_cast<int64_t>(page) << p.shift) >= x.r.len) return -1;
-      const int id = page < p.max_blocks ? p.block_table[x.r.index * p.table_stride + page] : -1;
+      const int id = page < p.max_blocks && !longer_than_table(x.r) ? p.block_table[x.r.index * p.table_stride + page] : -1;
       return id >= 0 && id < p.num_blocks ? id : p.num_blocks;
     };
     auto scale_at = [&](const Place& x, int id) {
@@ -824,7 +824,8 @@ struct GatherParams {
   const int32_t* block_table;
   const int32_t* seq_lens;
   int64_t table_stride;
-  int batch, heads, max_blocks, num_blocks, shift, max_k;
+  int batch, heads, max_blocks, num_blocks, shift;
+  int max_k, max_len;  // tokens that a request has here at most, that a table's row holds
 };
 
 constexpr int kGatherTokens = 32;  // of a block; with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
@@ -844,21 +845,23 @@ __device__ __forceinline__ uint32_t pack_16x2_finite(float lo, float hi) {
 
 // Block (i, h, b): tokens 32i to 32i + 31 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
 // where a weight of 0 would meet another request's NaN, or whatever the workspace held. So every request's rows are filled up to a whole tile with zeros, and these
-// stand in the list of sequences as one of their own, without queries.
+// stand in the list of sequences as one of their own, without queries. A request that is longer than its table has the most tokens here that any may have, which
+// are no fewer than its rows, so that each of them sees the first; all are in a block that there is none of.
 template <int kD, bool kInt8, bool kF16>
 __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p) {
   __shared__ int sums[8];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
-  auto len_of = [&](int i) { return min(max(p.seq_lens[i], 0), p.max_k); };
+  auto len_of = [&](int given) { return given > p.max_len ? p.max_k : min(max(given, 0), p.max_k); };
+  const int given = p.seq_lens[b], len = len_of(given), padded = static_cast<int>(padded_keys(len));
+  const int max_blocks = given > p.max_len ? 0 : p.max_blocks;
   int before = 0;
-  for (int i = tid; i < b; i += 256) before += static_cast<int>(padded_keys(len_of(i)));
+  for (int i = tid; i < b; i += 256) before += static_cast<int>(padded_keys(len_of(p.seq_lens[i])));
 #pragma unroll
   for (int d = 1; d < 32; d *= 2) before += __shfl_xor_sync(0xffffffffu, before, d);
   if ((tid & 31) == 0) sums[tid >> 5] = before;
   __syncthreads();
   before = 0;
   for (int w = 0; w < 8; ++w) before += sums[w];
-  const int len = len_of(b), padded = static_cast<int>(padded_keys(len));
   if (blockIdx.x == 0 && h == 0 && tid == 0) {
     int32_t* cu_k = p.cu + 2 * p.batch + 1;
     p.cu[2 * b] = p.cu_q[b];
@@ -877,7 +880,7 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), page = tok >> p.shift;
-    id[i] = tok < len && page < p.max_blocks ? p.block_table[b * p.table_stride + page] : -1;
+    id[i] = tok < len && page < max_blocks ? p.block_table[b * p.table_stride + page] : -1;
   }
   uint2 w[kTimes][2];
   float scale[kTimes][2];
@@ -891,8 +894,7 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       scale[i][x] = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
       w[i][x] = *reinterpret_cast<const uint2*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
-      const float own = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
-      scale[i][x] = fabsf(own) == INFINITY ? __int_as_float(0x7fffffff) : own;  // nor are elements of such a block numbers on the other path
+      scale[i][x] = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
     }
   }
 #pragma unroll
@@ -902,13 +904,14 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       uint32_t f[4], c[2] = {w[i][x].x, w[i][x].y};
+      const float own = fabsf(scale[i][x]) == INFINITY ? __int_as_float(0x7fffffff) : scale[i][x];  // nor are elements of such a block numbers on the other path
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         uint32_t lo, hi;
         codes_to_f16<kInt8>(c[e], lo, hi);
         const float2 u = unpack_16x2<true>(lo), v = unpack_16x2<true>(hi);
-        f[2 * e] = pack_16x2_finite<kF16>(u.x * scale[i][x], u.y * scale[i][x]);
-        f[2 * e + 1] = pack_16x2_finite<kF16>(v.x * scale[i][x], v.y * scale[i][x]);
+        f[2 * e] = pack_16x2_finite<kF16>(u.x * own, u.y * own);
+        f[2 * e + 1] = pack_16x2_finite<kF16>(v.x * own, v.y * own);
       }
       *reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
     }
@@ -991,8 +994,14 @@ int unit_rows(const sdpa_b200_cache_params& p) {
 
 size_t round_256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Tokens that a table's row holds
+int table_tokens(const sdpa_b200_cache_params& p) { return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.max_blocks) * p.block_size, INT32_MAX - 256)); }
+
+// Tokens of the longest request among the 16-bit copies, no fewer than any has rows
+int most_gathered(const sdpa_b200_cache_params& p) { return std::max(p.max_seqlen_k, p.max_seqlen_q); }
+
 size_t gather_bytes(const sdpa_b200_cache_params& p) {
-  return static_cast<size_t>(p.batch) * padded_keys(p.max_seqlen_k) * p.heads_kv * p.head_dim * 2;
+  return static_cast<size_t>(p.batch) * padded_keys(most_gathered(p)) * p.heads_kv * p.head_dim * 2;
 }
 
 // Where the units are few and short, a cluster of 2 to 8 CTAs takes each, the tiles in equal stretches, and merges its parts through distributed shared memory: no lengths to be
@@ -1026,7 +1035,7 @@ StreamParams list_of(const sdpa_b200_cache_params& c) {
   p.rows_shift = p.rows == 8 ? 3 : p.rows == 16 ? 4 : p.rows == 32 ? 5 : 6;
   p.tile_shift = c.head_dim == 64 ? 8 : 7;
   p.pause = p.rows == 64 ? 0 : kPause;
-  p.max_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(c.max_blocks) * c.block_size, INT32_MAX - 256) + 1);
+  p.max_len = table_tokens(c);
   return p;
 }
 
@@ -1151,8 +1160,9 @@ int launch_gathered(const sdpa_b200_cache_params& c, char* workspace, uint32_t* 
   g.max_blocks = c.max_blocks;
   g.num_blocks = c.num_blocks;
   g.shift = block_shift(c.block_size);
-  g.max_k = c.max_seqlen_k;
-  const dim3 grid(static_cast<unsigned>(padded_keys(c.max_seqlen_k) / kGatherTokens), c.heads_kv, c.batch);
+  g.max_k = most_gathered(c);
+  g.max_len = table_tokens(c);
+  const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / kGatherTokens), c.heads_kv, c.batch);
   const bool f16 = c.dtype == SDPA_B200_F16;
   auto launch = [&](auto dim, auto int8) {
     constexpr int kD = decltype(dim)::value;
@@ -1180,9 +1190,9 @@ int launch_gathered(const sdpa_b200_cache_params& c, char* workspace, uint32_t* 
   f.heads_kv = c.heads_kv;
   f.head_dim = c.head_dim;
   f.max_seqlen_q = c.max_seqlen_q;
-  f.max_seqlen_k = c.max_seqlen_k;
+  f.max_seqlen_k = g.max_k;
   f.total_q = c.total_q;
-  f.total_k = static_cast<int32_t>(c.batch * padded_keys(c.max_seqlen_k));
+  f.total_k = static_cast<int32_t>(c.batch * padded_keys(g.max_k));
   f.q_row_stride = c.q_row_stride;
   f.q_head_stride = c.q_head_stride;
   f.o_row_stride = c.o_row_stride;
@@ -1238,7 +1248,7 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
     set_error("cache_attention: many rows per request come in batches of up to 65535, with up to 65535 heads (got %d, %d)", p->batch, p->heads_kv);
     return SDPA_B200_UNSUPPORTED;
   }
-  if (!streams(*p) && p->batch * padded_keys(p->max_seqlen_k) > INT32_MAX) {
+  if (!streams(*p) && p->batch * padded_keys(most_gathered(*p)) > INT32_MAX) {
     set_error("cache_attention: batch * max_seqlen_k must be below 2^31 for long requests");
     return SDPA_B200_INVALID_ARG;
   }

@@ -11,7 +11,7 @@ namespace sdpa_b200 {
 
 constexpr int kTilesToPause = 4;  // a CTA with fewer tiles than that has few hand-overs: the places are the tiles
 
-// A request as units see it
+// A request as units see it. One that is longer than its table has one token, in a block that there is none of, which all its rows see.
 struct Request {
   int index, len, rows_q, q0;  // tokens in the cache, rows of q, the first of them
   int in_front;                // row i sees i + 1 + in_front tokens where causal
@@ -23,18 +23,22 @@ __host__ __device__ __forceinline__ Request request_at(const P& p, int b) {
   Request r;
   r.index = b;
   const int len = p.seq_lens[b];
-  r.len = len < 0 ? 0 : len < p.max_len ? len : p.max_len;
+  const bool too_long = len > p.max_len;
+  r.len = too_long ? 1 : len < 0 ? 0 : len;
   r.q0 = p.cu_q ? p.cu_q[b] : p.first_q + b;
   r.rows_q = 1;
   if (p.cu_q) r.rows_q = p.cu_q[b + 1] > r.q0 ? p.cu_q[b + 1] - r.q0 : 0;
   if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
   if (r.rows_q > p.max_rows) r.rows_q = p.max_rows;  // what the places were counted with
-  r.in_front = len > p.max_len - 1 ? r.len : r.len - r.rows_q;  // longer than the table: all its rows see the block that there is none of
+  r.in_front = too_long ? r.len : r.len - r.rows_q;
   r.tiles = (r.len + (1 << p.tile_shift) - 1) >> p.tile_shift;
   if (r.tiles < 1) r.tiles = 1;  // an empty request has rows to write too
   r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
   return r;
 }
+
+// (those of others see less than their length in front of their first row)
+__host__ __device__ __forceinline__ bool longer_than_table(const Request& r) { return r.in_front == r.len; }
 
 __host__ __device__ __forceinline__ int tiles_of(const Request& r) { return r.tiles * r.units; }
 

@@ -80,7 +80,7 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24.
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
-    cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package).
+    cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package), a length that passes the table's row all rows of its request.
     """
     return _calls().cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k,
                                     is_causal, scale)
