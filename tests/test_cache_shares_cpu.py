@@ -200,3 +200,21 @@ def test_a_request_whose_tiles_do_not_fit_is_refused(native_lib):
             assert got == status and "is too long" in native_lib.sdpa_b200_last_error().decode(), native_lib.sdpa_b200_last_error()
         elif not torch.cuda.is_available():  # fits: only the device is missing
             assert got == status
+
+
+def test_workspace_of_many_requests_at_a_large_bound(native_lib):
+    """16-bit copies are made for as many requests at a time as fit 4 GiB, and not at all where one does not: a bound on lengths never decides whether a call can be made."""
+    import ctypes
+    from test_kv_cache_cpu import _cache, _set
+    from torch_mlu_b200 import _cabi
+    n = ctypes.c_size_t(0)
+    sizes = []
+    for batch, rows, bound in ((32, 2048, 8192), (32, 2048, 131072), (256, 2048, 131072), (1, 2048, 1 << 20), (1, 2048, (1 << 20) + 1), (100000, 512, 4096)):
+        p = _cache()
+        _set(heads_kv=8, heads_q=32, q_row_stride=4096, o_row_stride=4096, batch=batch, total_q=rows * min(batch, 32), max_seqlen_q=rows, max_seqlen_k=bound, max_blocks=1 << 14, table_stride=1 << 14)(p)
+        assert native_lib.sdpa_b200_cache_attention_workspace_bytes(ctypes.byref(p), ctypes.byref(n)) == 0
+        sizes.append(n.value)
+        assert n.value <= (4 << 30) + (1 << 20)
+        got = native_lib.sdpa_b200_cache_attention(ctypes.byref(p), 4096, n.value, None)
+        assert torch.cuda.is_available() or got == _cabi.NO_DEVICE  # nothing else is in the way
+    assert 32 * 8192 * 8 * 128 * 4 <= sizes[0] < sizes[1] and sizes[3] >= 4 << 30 and sizes[4] < 1 << 27

@@ -139,3 +139,27 @@ def test_a_request_longer_than_its_table(cuda_device, rows, dim, width, max_k, c
         b[6][2] = 0
         _compare(out, lse, b, causal, many=rows > 500)
     assert ops.device_status() == 0
+
+
+def test_requests_gathered_in_several_launches(cuda_device):
+    """A bound on lengths at which the 16-bit copies of all requests would take 9.7 GB: they are made for a few at a time, and where those of one would take more than 4 GiB not at
+    all; rows outside every request stay as they are."""
+    lens, rows = [1300, 300, 1, 0, 700, 1500, 1024, 64, 900], [1000, 300, 1, 2, 700, 1, 1024, 40, 900]
+    b = _batch(cuda_device, lens, rows, 64, 8, 128, 64, E4M3, torch.bfloat16)
+    for bound, many in ((1500, True), (1 << 18, True), ((1 << 20) + 1, False)):
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        gathers, out, lse = _gathers(b, max_k=bound)
+        assert gathers == many and torch.cuda.max_memory_allocated() < 9 << 30
+        _compare(out, lse, b, many=many)
+    # replayed from a graph, on a workspace that is full of NaN
+    keep = _run(b, max_k=1500)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = _run(b, max_q=1024, max_k=1 << 18)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    _compare(out, lse, b, many=True)
+    assert torch.equal(out[:1000], keep[0][:1000])  # the same tiles, whoever is beside them
+    assert ops.device_status() == 0

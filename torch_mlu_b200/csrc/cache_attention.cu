@@ -829,6 +829,7 @@ struct GatherParams {
 };
 
 constexpr int kGatherTokens = 32;  // of a block; with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
+constexpr int64_t kMostGatheredBytes = int64_t(4) << 30;  // of the 16-bit copies in the workspace
 constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, from a sequence's start
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
@@ -918,13 +919,29 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
   }
 }
 
+// Tokens that a table's row holds
+int table_tokens(const sdpa_b200_cache_params& p) { return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.max_blocks) * p.block_size, INT32_MAX - 256)); }
+
+// Tokens of the longest request among the 16-bit copies, no fewer than any has rows
+int most_gathered(const sdpa_b200_cache_params& p) { return std::max(p.max_seqlen_k, p.max_seqlen_q); }
+
+// Keys and values of one request among the 16-bit copies, at its longest
+int64_t gathered_bytes(const sdpa_b200_cache_params& p) { return 4 * padded_keys(most_gathered(p)) * p.heads_kv * p.head_dim; }
+
+// Requests that are gathered at a time. What they hold is not known here: by the bound on lengths, which may be the table's, the copies of a large batch would take more memory than
+// the cache itself. 64 requests of 512 rows behind 32768 tokens, 32/8 heads of 128, in two launches of each kernel instead of one: 16.8 instead of 16.7 ms.
+int gathered_at_once(const sdpa_b200_cache_params& p) {
+  const int64_t most = std::min<int64_t>(kMostGatheredBytes / gathered_bytes(p), 32767), launches = (p.batch + most - 1) / most;
+  return static_cast<int>((p.batch + launches - 1) / launches);  // launches of equal size
+}
+
 // Path 1 costs its units of 64 rows, path 2 the gathering of every kv head's tokens and the prefill kernel's waves of units of up to 256 rows of a query head, all per
 // token in the cache. So the length does not decide, and in units of 64 rows a token's gathering is 0.9 and a wave 95 (head_dim 64: 150). Measured, 4 requests of 5000
 // tokens, us, path 1 | 2: 32/8 heads of 128, 24 rows 58 | 86, 40 79 | 88, 56 99 | 88, 96 144 | 89; 16/16, 64 60 | 106, 128 101 | 107, 160 144 | 115; 64/8, 40 123 | 148,
 // 64 188 | 150; 16/4 of 64, 64 36 | 63, 128 61 | 64, 160 73 | 81. 16 requests of 1000, 32/8 of 128, 40 76 | 78, 64 95 | 79.
 bool streams(const sdpa_b200_cache_params& p) {
   const int64_t group = p.heads_q / p.heads_kv, batch = p.batch;
-  if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64) return true;
+  if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64 || gathered_bytes(p) > kMostGatheredBytes) return true;
   // requests of equal rows, or of any: half a unit each is empty then
   const double units = p.total_q == batch * p.max_seqlen_q ? static_cast<double>(batch * ((p.max_seqlen_q * group + 63) / 64)) : p.total_q * group / 64.0 + 0.5 * batch;
   const int64_t blocks = p.heads_q * std::max<int64_t>(batch, (p.total_q + 255) / 256);
@@ -993,16 +1010,6 @@ int unit_rows(const sdpa_b200_cache_params& p) {
 }
 
 size_t round_256(size_t n) { return (n + 255) / 256 * 256; }
-
-// Tokens that a table's row holds
-int table_tokens(const sdpa_b200_cache_params& p) { return static_cast<int>(std::min<int64_t>(static_cast<int64_t>(p.max_blocks) * p.block_size, INT32_MAX - 256)); }
-
-// Tokens of the longest request among the 16-bit copies, no fewer than any has rows
-int most_gathered(const sdpa_b200_cache_params& p) { return std::max(p.max_seqlen_k, p.max_seqlen_q); }
-
-size_t gather_bytes(const sdpa_b200_cache_params& p) {
-  return static_cast<size_t>(p.batch) * padded_keys(most_gathered(p)) * p.heads_kv * p.head_dim * 2;
-}
 
 // Where the units are few and short, a cluster of 2 to 8 CTAs takes each, the tiles in equal stretches, and merges its parts through distributed shared memory: no lengths to be
 // summed up in front and no second kernel behind. That leaves SMs idle where units are of many lengths, so it is for up to eight tiles a CTA of the longest. Measured, shares of
@@ -1137,32 +1144,34 @@ int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* w
   return SDPA_B200_OK;
 }
 
-int launch_gathered(const sdpa_b200_cache_params& c, char* workspace, uint32_t* status, cudaStream_t stream) {
-  // the prefill kernel's own workspace in front, then K, V and the offsets
+// Requests [first, first + count)
+int launch_gathered(const sdpa_b200_cache_params& c, int first, int count, char* workspace, uint32_t* status, cudaStream_t stream) {
+  // behind the header the prefill kernel's own one, then K, V and the offsets
   sdpa_b200_params f = {};
   GatherParams g;
-  char* at = workspace + kWorkspaceHeaderBytes;
+  char* at = workspace + 2 * kWorkspaceHeaderBytes;
+  const int64_t copies = count * gathered_bytes(c);
   g.out[0] = reinterpret_cast<uint16_t*>(at);
-  g.out[1] = reinterpret_cast<uint16_t*>(at + gather_bytes(c));
-  g.cu = reinterpret_cast<int32_t*>(at + 2 * gather_bytes(c));
-  g.cu_q = c.cu_seqlens_q;
+  g.out[1] = reinterpret_cast<uint16_t*>(at + copies / 2);
+  g.cu = reinterpret_cast<int32_t*>(at + copies);
+  g.cu_q = c.cu_seqlens_q + first;
   g.cache[0] = static_cast<const uint8_t*>(c.k_cache);
   g.cache[1] = static_cast<const uint8_t*>(c.v_cache);
   g.scale[0] = c.k_scale;
   g.scale[1] = c.v_scale;
   g.block[0] = c.k_block_stride, g.head[0] = c.k_head_stride, g.row[0] = c.k_row_stride;
   g.block[1] = c.v_block_stride, g.head[1] = c.v_head_stride, g.row[1] = c.v_row_stride;
-  g.block_table = c.block_table;
-  g.seq_lens = c.seq_lens;
+  g.block_table = c.block_table + first * c.table_stride;
+  g.seq_lens = c.seq_lens + first;
   g.table_stride = c.table_stride;
-  g.batch = c.batch;
+  g.batch = count;
   g.heads = c.heads_kv;
   g.max_blocks = c.max_blocks;
   g.num_blocks = c.num_blocks;
   g.shift = block_shift(c.block_size);
   g.max_k = most_gathered(c);
   g.max_len = table_tokens(c);
-  const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / kGatherTokens), c.heads_kv, c.batch);
+  const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / kGatherTokens), c.heads_kv, count);
   const bool f16 = c.dtype == SDPA_B200_F16;
   auto launch = [&](auto dim, auto int8) {
     constexpr int kD = decltype(dim)::value;
@@ -1184,15 +1193,15 @@ int launch_gathered(const sdpa_b200_cache_params& c, char* workspace, uint32_t* 
   f.out = c.out;
   f.lse = c.lse;
   f.cu_seqlens_q = g.cu;
-  f.cu_seqlens_k = g.cu + 2 * c.batch + 1;
-  f.batch = 2 * c.batch;
+  f.cu_seqlens_k = g.cu + 2 * count + 1;
+  f.batch = 2 * count;
   f.heads_q = c.heads_q;
   f.heads_kv = c.heads_kv;
   f.head_dim = c.head_dim;
   f.max_seqlen_q = c.max_seqlen_q;
   f.max_seqlen_k = g.max_k;
   f.total_q = c.total_q;
-  f.total_k = static_cast<int32_t>(c.batch * padded_keys(g.max_k));
+  f.total_k = static_cast<int32_t>(count * padded_keys(g.max_k));
   f.q_row_stride = c.q_row_stride;
   f.q_head_stride = c.q_head_stride;
   f.o_row_stride = c.o_row_stride;
@@ -1206,11 +1215,14 @@ int launch_gathered(const sdpa_b200_cache_params& c, char* workspace, uint32_t* 
   f.device_status = status;
   const int st = validate_forward_args(&f);
   if (st != SDPA_B200_OK) return st;
-  return launch_fwd_prefill(f, workspace, stream);
+  return launch_fwd_prefill(f, workspace + kWorkspaceHeaderBytes, stream);
 }
 
 size_t workspace_bytes_of(const sdpa_b200_cache_params& p) {
-  if (!streams(p)) return kWorkspaceHeaderBytes + 2 * gather_bytes(p) + round_256((4 * static_cast<size_t>(p.batch) + 2) * 4);
+  if (!streams(p)) {
+    const size_t n = gathered_at_once(p);
+    return 2 * kWorkspaceHeaderBytes + n * gathered_bytes(p) + round_256((4 * n + 2) * 4);
+  }
   const size_t ctas = static_cast<size_t>(kCtasPerSm) * kMaxSms;
   return kWorkspaceHeaderBytes + round_256(ctas * 2 * unit_rows(p) * (p.head_dim + 1) * 4 + ctas * sizeof(SharedUnit));
 }
@@ -1244,13 +1256,9 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
               static_cast<long long>(p->max_blocks) * p->block_size);
     return SDPA_B200_UNSUPPORTED;
   }
-  if (!streams(*p) && (p->batch > 65535 || p->heads_kv > 65535)) {
-    set_error("cache_attention: many rows per request come in batches of up to 65535, with up to 65535 heads (got %d, %d)", p->batch, p->heads_kv);
+  if (!streams(*p) && p->heads_kv > 65535) {
+    set_error("cache_attention: many rows per request come with up to 65535 heads of the cache (got %d)", p->heads_kv);
     return SDPA_B200_UNSUPPORTED;
-  }
-  if (!streams(*p) && p->batch * padded_keys(most_gathered(*p)) > INT32_MAX) {
-    set_error("cache_attention: batch * max_seqlen_k must be below 2^31 for long requests");
-    return SDPA_B200_INVALID_ARG;
   }
   st = check_device();
   if (st != SDPA_B200_OK) return st;
@@ -1260,13 +1268,12 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
     return SDPA_B200_LAUNCH_FAILED;
   }
   uint32_t* status = p->device_status != nullptr ? p->device_status : static_cast<uint32_t*>(workspace);
-  if (streams(*p)) {
-    const int at_once = requests_at_once(list_of(*p));
-    for (int first = 0; first < p->batch; first += at_once) {
-      st = launch_stream(*p, first, std::min(at_once, p->batch - first), static_cast<char*>(workspace), status, s);
-      if (st != SDPA_B200_OK) return st;
-    }
-    return SDPA_B200_OK;
+  const bool few_rows = streams(*p);
+  const int at_once = few_rows ? requests_at_once(list_of(*p)) : gathered_at_once(*p);
+  for (int first = 0; first < p->batch; first += at_once) {
+    const int count = std::min(at_once, p->batch - first);
+    st = few_rows ? launch_stream(*p, first, count, static_cast<char*>(workspace), status, s) : launch_gathered(*p, first, count, static_cast<char*>(workspace), status, s);
+    if (st != SDPA_B200_OK) return st;
   }
-  return launch_gathered(*p, static_cast<char*>(workspace), status, s);
+  return SDPA_B200_OK;
 }

@@ -74,8 +74,8 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     query is packed [tokens, heads_q, head_dim]; request i owns rows cu_seqlens[i] to cu_seqlens[i + 1] - 1, its last tokens, and sees the
     ``seq_lens[i]`` tokens that the blocks of ``block_table[i]`` hold, up to its own with ``is_causal`` (bottom-right aligned). Without cu_seqlens every
     request has one row. ``max_seqlen_q`` and ``max_seqlen_k`` are at least the most rows and the longest request; without max_seqlen_k it is what
-    the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace, which takes
-    4 * requests * max_seqlen_k * heads_kv * head_dim bytes, and the prefill kernel runs. That is exact with scales that are powers of two, as store gives
+    the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace and the prefill
+    kernel runs: 4 * max_seqlen_k * heads_kv * head_dim bytes a request, for as many requests at a time as fit 4 GiB (where not even one does, the codes are streamed). That is exact with scales that are powers of two, as store gives
     them; with others every element is rounded once. Elements beyond the largest number of query's type are that number there (fp16: 65504, of which the code may be 65536),
     and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24.
 
