@@ -1,10 +1,15 @@
 // The serving operators from tensors to launched kernels: bookkeeping of a step, the 8-bit paged cache, rotary positions with their gradient. Called by
 // py_calls.cpp for kv_cache.py and rotary.py: a decode step's kernels run for a few microseconds each, and filling the parameter blocks through ctypes took
-// the host 25 to 45 us a call.
+// the host 25 to 45 us a call. They are operators of b200_sdpa too, through which a call goes while somebody wants to see it (a tracer, a dispatch mode): what launched
+// kernels beside a tracer would leave its results in the traced program as constants.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/library.h>
 
 #include "torch_glue.h"
 
@@ -50,12 +55,33 @@ void written(const Tensor& t) {
 
 bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
+// Whether a tracer, a dispatch mode, a functional transform or code below autograd is to see the operators of this thread. (Autocast has nothing to do with them, and inference
+// mode, which switches autograd off too, is what servers run in.)
+bool calls_are_seen() {
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  return !(c10::default_included_set | c10::autocast_dispatch_keyset).has_all(tls.included_) ||
+         (tls.excluded_.has(c10::DispatchKey::AutogradFunctionality) && !c10::InferenceMode::is_enabled()) ||
+         c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing();
+}
+
+// What wraps a tensor (a functional transform, a fake tensor) has no rule for these operators
+void check_all_plain(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors) check_plain(*t, "every argument");
+}
+
+template <class F>
+auto operator_named(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
 void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 }  // namespace
 
-std::vector<Tensor> plan_step(const Tensor& cached_lens, const Tensor& new_tokens, const Tensor& block_table, const Tensor& ring, const Tensor& ring_state,
-                              int64_t block_size, int64_t num_tokens, bool in_place) {
+namespace {
+
+std::vector<Tensor> launch_plan(const Tensor& cached_lens, const Tensor& new_tokens, const Tensor& block_table, const Tensor& ring, const Tensor& ring_state,
+                                int64_t block_size, int64_t num_tokens, bool in_place) {
   check_ints(cached_lens, "cached_lens", cached_lens);
   check_ints(new_tokens, "new_tokens", cached_lens);
   check_ints(ring, "ring", cached_lens);
@@ -110,6 +136,34 @@ std::vector<Tensor> plan_step(const Tensor& cached_lens, const Tensor& new_token
   return step;
 }
 
+using PlanResult = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>;
+PlanResult plan_operator(const Tensor& cached_lens, const Tensor& new_tokens, const Tensor& block_table, const Tensor& ring, const Tensor& ring_state, int64_t block_size,
+                         int64_t num_tokens) {
+  const auto r = launch_plan(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens, false);
+  return {r[0], r[1], r[2], r[3], r[4]};
+}
+std::tuple<Tensor, Tensor, Tensor> plan_operator_in_place(const Tensor& cached_lens, const Tensor& new_tokens, const Tensor& block_table, const Tensor& ring,
+                                                          const Tensor& ring_state, int64_t block_size, int64_t num_tokens) {
+  const auto r = launch_plan(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens, true);
+  return {r[1], r[2], r[3]};
+}
+
+}  // namespace
+
+std::vector<Tensor> plan_step(const Tensor& cached_lens, const Tensor& new_tokens, const Tensor& block_table, const Tensor& ring, const Tensor& ring_state,
+                              int64_t block_size, int64_t num_tokens, bool in_place) {
+  if (!calls_are_seen()) return launch_plan(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens, in_place);
+  check_all_plain({&cached_lens, &new_tokens, &block_table, &ring, &ring_state});
+  if (!in_place) {
+    static auto op = operator_named<decltype(plan_operator)>("b200_sdpa::plan_step");
+    const auto r = op.call(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens);
+    return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), std::get<4>(r)};
+  }
+  static auto op = operator_named<decltype(plan_operator_in_place)>("b200_sdpa::plan_step_");
+  const auto r = op.call(cached_lens, new_tokens, block_table, ring, ring_state, block_size, num_tokens);
+  return {cached_lens, std::get<0>(r), std::get<1>(r), std::get<2>(r), ring_state};
+}
+
 namespace {
 
 void cache_params(sdpa_b200_cache_params& p, const Tensor& x, const char* name, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs) {
@@ -146,9 +200,7 @@ void cache_params(sdpa_b200_cache_params& p, const Tensor& x, const char* name, 
   p.dtype = x.scalar_type() == at::kHalf ? SDPA_B200_F16 : SDPA_B200_BF16;
 }
 
-}  // namespace
-
-void cache_store(const Tensor& key, const Tensor& value, const Tensor& slots, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
+void launch_store(const Tensor& key, const Tensor& value, const Tensor& slots, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
                  const Tensor& value_scale) {
   TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes(), "key and value must both be [tokens, heads_kv, head_dim]");
   TORCH_CHECK(key.scalar_type() == value.scalar_type() && key.device() == value.device() && key.stride(2) == 1 && value.stride(2) == 1,
@@ -175,7 +227,7 @@ void cache_store(const Tensor& key, const Tensor& value, const Tensor& slots, co
   for (const Tensor* t : {&key_cache, &value_cache, &key_scale, &value_scale}) written(*t);
 }
 
-std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
+std::tuple<Tensor, Tensor> launch_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
                                            const Tensor& value_scale, const Tensor& block_table, const Tensor& seq_lens,
                                            const c10::optional<Tensor>& cu_seqlens, int64_t max_seqlen_q, c10::optional<int64_t> max_seqlen_k, bool causal,
                                            c10::optional<double> scale) {
@@ -219,6 +271,28 @@ std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& ke
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);  // back to torch's stream-ordered pool at the end of this call
   check_status(sdpa_b200_cache_attention(&p, ws.get(), bytes, stream_of(query)), "sdpa_b200_cache_attention");
   return {out, lse};
+}
+
+}  // namespace
+
+void cache_store(const Tensor& key, const Tensor& value, const Tensor& slots, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
+                 const Tensor& value_scale) {
+  if (!calls_are_seen()) return launch_store(key, value, slots, key_cache, value_cache, key_scale, value_scale);
+  check_all_plain({&key, &value, &slots, &key_cache, &value_cache, &key_scale, &value_scale});
+  static auto op = operator_named<decltype(launch_store)>("b200_sdpa::cache_store_");
+  op.call(key, value, slots, key_cache, value_cache, key_scale, value_scale);
+}
+
+std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
+                                           const Tensor& value_scale, const Tensor& block_table, const Tensor& seq_lens,
+                                           const c10::optional<Tensor>& cu_seqlens, int64_t max_seqlen_q, c10::optional<int64_t> max_seqlen_k, bool causal,
+                                           c10::optional<double> scale) {
+  if (!calls_are_seen())
+    return launch_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k, causal, scale);
+  check_all_plain({&query, &key_cache, &value_cache, &key_scale, &value_scale, &block_table, &seq_lens});
+  if (cu_seqlens.has_value()) check_plain(*cu_seqlens, "cu_seqlens");
+  static auto op = operator_named<decltype(launch_attention)>("b200_sdpa::cache_attention");
+  return op.call(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k, causal, scale);
 }
 
 // ------------------------------------------------------------------------- rotary positions
@@ -301,53 +375,7 @@ Tensor readable(const Tensor& x) {
 
 c10::optional<Tensor> if_defined(const Tensor& t) { return t.defined() ? c10::optional<Tensor>(t) : c10::nullopt; }
 
-// The gradient of a turn is the turn backwards, itself an operator with a gradient.
-struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
-  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& other,
-                                                const Tensor& positions, const Tensor& inv_freq, std::vector<int64_t> sections, bool interleaved, bool inverse, double scaling) {
-    ctx->set_materialize_grads(false);
-    ctx->save_for_backward({positions, inv_freq});
-    ctx->saved_data["sections"] = sections;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["inverse"] = inverse;
-    ctx->saved_data["scaling"] = scaling;
-    at::AutoDispatchBelowADInplaceOrView guard;
-    const Tensor y = other.value_or(Tensor());
-    auto r = turn(x, y, positions, inv_freq, {std::move(sections), interleaved, inverse, scaling}, false);
-    if (!y.defined()) return {std::get<0>(r)};
-    return {std::get<0>(r), std::get<1>(r)};
-  }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
-    const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool(),
-                          ctx->saved_data["scaling"].toDouble()};
-    torch::autograd::variable_list result(8);
-    std::vector<size_t> wanted;
-    for (size_t i = 0; i < grads.size(); ++i)
-      if (grads[i].defined() && ctx->needs_input_grad(i)) wanted.push_back(i);
-    if (wanted.empty()) return result;
-    Tensor g[2];
-    for (size_t i = 0; i < wanted.size(); ++i) {
-      check_plain(grads[wanted[i]], "an incoming gradient");
-      g[i] = readable(grads[wanted[i]]);
-    }
-    std::tuple<Tensor, Tensor> r;
-    if (needs_grad(g[0]) || needs_grad(g[1])) {
-      const auto v = RotaryFunction::apply(g[0], if_defined(g[1]), saved[0], saved[1], c.sections, c.interleaved, c.inverse, c.scaling);
-      r = {v[0], v.size() > 1 ? v[1] : Tensor()};
-    } else {
-      r = turn(g[0], g[1], saved[0], saved[1], c, false);
-    }
-    result[wanted[0]] = std::get<0>(r);
-    if (wanted.size() > 1) result[wanted[1]] = std::get<1>(r);
-    return result;
-  }
-};
-
-}  // namespace
-
-std::tuple<Tensor, Tensor> rotary(const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& inv_freq, const std::vector<int64_t>& sections,
-                                  bool interleaved, double scaling, bool in_place) {
+void check_rotary(const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& inv_freq, const std::vector<int64_t>& sections) {
   TORCH_CHECK(query.dim() == 3 || query.dim() == 4, "query must be packed [tokens, heads, head_dim] or [batch, heads, seq_len, head_dim]");
   rotary_tensor(query, "query", query);
   if (key.defined()) rotary_tensor(key, "key", query);
@@ -376,26 +404,147 @@ std::tuple<Tensor, Tensor> rotary(const Tensor& query, const Tensor& key, const 
     TORCH_CHECK((dims == 1 || (dims == 2 && (positions.size(first) == 1 || positions.size(first) == query.size(0)))) && positions.size(-1) == query.size(2),
                 "positions must be ", first ? "[axes, length] or [axes, batch, length]" : "[length] or [batch, length]", " (got shape ", positions.sizes(), ")");
   }
-  const RotaryCall c = {sections, interleaved, false, scaling};
-  if (in_place) {
-    TORCH_CHECK(!needs_grad(query) && !needs_grad(key), "rotary positions in place have no gradient: use rotary_embedding");
-    TORCH_CHECK(!key.defined() || query.numel() == 0 || key.data_ptr() != query.data_ptr(), "rotary positions in place: query and key are the same memory");
-    for (const Tensor* t : {&query, &key}) {
-      for (int64_t i = 0; t->defined() && i < t->dim(); ++i)
-        TORCH_CHECK(t->size(i) <= 1 || t->stride(i) != 0, "rotary positions in place need elements of their own (a stride is 0)");
+}
+
+// An operator has no results that may be missing: one, or two with a key
+std::vector<Tensor> rotary_operator(const Tensor& query, const c10::optional<Tensor>& key, const Tensor& positions, const Tensor& inv_freq, at::OptionalIntArrayRef sections,
+                                    bool interleaved, double scaling, bool inverse) {
+  const Tensor k = key.value_or(Tensor());
+  const std::vector<int64_t> parts = sections.has_value() ? sections->vec() : std::vector<int64_t>();
+  check_rotary(query, k, positions, inv_freq, parts);
+  const auto r = turn(query, k, positions, inv_freq, {parts, interleaved, inverse, scaling}, false);
+  if (!k.defined()) return {std::get<0>(r)};
+  return {std::get<0>(r), std::get<1>(r)};
+}
+
+// turn() into new tensors, below autograd, seen by those who want to see it
+std::tuple<Tensor, Tensor> turned(const Tensor& x, const Tensor& y, const Tensor& positions, const Tensor& inv_freq, const RotaryCall& c) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  if (!c10::impl::TorchDispatchModeTLS::any_modes_set() && !torch::jit::tracer::isTracing()) return turn(x, y, positions, inv_freq, c, false);
+  static auto op = operator_named<decltype(rotary_operator)>("b200_sdpa::rotary_embedding");
+  const auto r = op.call(x, if_defined(y), positions, inv_freq, c.sections.empty() ? at::OptionalIntArrayRef() : at::OptionalIntArrayRef(c.sections), c.interleaved, c.scaling, c.inverse);
+  return {r[0], r.size() > 1 ? r[1] : Tensor()};
+}
+
+// The gradient of a turn is the turn backwards, itself an operator with a gradient.
+struct RotaryFunction : torch::autograd::Function<RotaryFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const c10::optional<Tensor>& other,
+                                                const Tensor& positions, const Tensor& inv_freq, std::vector<int64_t> sections, bool interleaved, bool inverse, double scaling) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({positions, inv_freq});
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["scaling"] = scaling;
+    const Tensor y = other.value_or(Tensor());
+    auto r = turned(x, y, positions, inv_freq, {std::move(sections), interleaved, inverse, scaling});
+    if (!y.defined()) return {std::get<0>(r)};
+    return {std::get<0>(r), std::get<1>(r)};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const RotaryCall c = {ctx->saved_data["sections"].toIntVector(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["inverse"].toBool(),
+                          ctx->saved_data["scaling"].toDouble()};
+    torch::autograd::variable_list result(8);
+    std::vector<size_t> wanted;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined() && ctx->needs_input_grad(i)) wanted.push_back(i);
+    if (wanted.empty()) return result;
+    Tensor g[2];
+    for (size_t i = 0; i < wanted.size(); ++i) {
+      check_plain(grads[wanted[i]], "an incoming gradient");
+      g[i] = readable(grads[wanted[i]]);
     }
-    auto r = turn(query, key, positions, inv_freq, c, true);
-    for (const Tensor* t : {&query, &key})
-      if (t->defined()) written(*t);
-    return r;
+    std::tuple<Tensor, Tensor> r;
+    if (needs_grad(g[0]) || needs_grad(g[1])) {
+      const auto v = RotaryFunction::apply(g[0], if_defined(g[1]), saved[0], saved[1], c.sections, c.interleaved, c.inverse, c.scaling);
+      r = {v[0], v.size() > 1 ? v[1] : Tensor()};
+    } else {
+      r = turned(g[0], g[1], saved[0], saved[1], c);
+    }
+    result[wanted[0]] = std::get<0>(r);
+    if (wanted.size() > 1) result[wanted[1]] = std::get<1>(r);
+    return result;
   }
-  if (!needs_grad(query) && !needs_grad(key)) {
-    for (const Tensor* t : {&query, &key})
-      TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "forward-mode differentiation of rotary positions is not implemented");
-    return turn(query, key, positions, inv_freq, c, false);
+};
+
+std::vector<Tensor> rotary_with_grad(const Tensor& query, const c10::optional<Tensor>& key, const Tensor& positions, const Tensor& inv_freq, at::OptionalIntArrayRef sections,
+                                     bool interleaved, double scaling, bool inverse) {
+  const Tensor k = key.value_or(Tensor());
+  const std::vector<int64_t> parts = sections.has_value() ? sections->vec() : std::vector<int64_t>();
+  check_rotary(query, k, positions, inv_freq, parts);
+  if (needs_grad(query) || needs_grad(k)) return RotaryFunction::apply(query, key, positions, inv_freq, parts, interleaved, inverse, scaling);
+  for (const Tensor* t : {&query, &k})
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "forward-mode differentiation of rotary positions is not implemented");
+  const auto r = turned(query, k, positions, inv_freq, {parts, interleaved, inverse, scaling});
+  if (!k.defined()) return {std::get<0>(r)};
+  return {std::get<0>(r), std::get<1>(r)};
+}
+
+void rotary_operator_in_place(const Tensor& query, const c10::optional<Tensor>& key, const Tensor& positions, const Tensor& inv_freq, at::OptionalIntArrayRef sections,
+                              bool interleaved, double scaling) {
+  const Tensor k = key.value_or(Tensor());
+  const std::vector<int64_t> parts = sections.has_value() ? sections->vec() : std::vector<int64_t>();
+  check_rotary(query, k, positions, inv_freq, parts);
+  TORCH_CHECK(!needs_grad(query) && !needs_grad(k), "rotary positions in place have no gradient: use rotary_embedding");
+  TORCH_CHECK(!k.defined() || query.numel() == 0 || k.data_ptr() != query.data_ptr(), "rotary positions in place: query and key are the same memory");
+  for (const Tensor* t : {&query, &k}) {
+    for (int64_t i = 0; t->defined() && i < t->dim(); ++i)
+      TORCH_CHECK(t->size(i) <= 1 || t->stride(i) != 0, "rotary positions in place need elements of their own (a stride is 0)");
   }
-  const auto v = RotaryFunction::apply(query, if_defined(key), positions, inv_freq, sections, interleaved, false, scaling);
-  return {v[0], v.size() > 1 ? v[1] : Tensor()};
+  turn(query, k, positions, inv_freq, {parts, interleaved, false, scaling}, true);
+  for (const Tensor* t : {&query, &k})
+    if (t->defined()) written(*t);
+}
+
+}  // namespace
+
+std::tuple<Tensor, Tensor> rotary(const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& inv_freq, const std::vector<int64_t>& sections,
+                                  bool interleaved, double scaling, bool in_place) {
+  const bool seen = calls_are_seen();
+  const at::OptionalIntArrayRef parts = sections.empty() ? at::OptionalIntArrayRef() : at::OptionalIntArrayRef(sections);
+  if (in_place) {
+    if (seen) {
+      static auto op = operator_named<decltype(rotary_operator_in_place)>("b200_sdpa::rotary_embedding_");
+      check_rotary(query, key, positions, inv_freq, sections);
+      op.call(query, if_defined(key), positions, inv_freq, parts, interleaved, scaling);
+    } else {
+      rotary_operator_in_place(query, if_defined(key), positions, inv_freq, parts, interleaved, scaling);
+    }
+    return {query, key};
+  }
+  std::vector<Tensor> r;
+  if (seen) {
+    static auto op = operator_named<decltype(rotary_operator)>("b200_sdpa::rotary_embedding");
+    check_rotary(query, key, positions, inv_freq, sections);  // a wrapped tensor has no rule here
+    r = op.call(query, if_defined(key), positions, inv_freq, parts, interleaved, scaling, false);
+  } else {
+    r = rotary_with_grad(query, if_defined(key), positions, inv_freq, parts, interleaved, scaling, false);
+  }
+  return {r[0], r.size() > 1 ? r[1] : Tensor()};
 }
 
 }  // namespace b200_glue
+
+TORCH_LIBRARY_FRAGMENT(b200_sdpa, m) {
+  m.def("rotary_embedding(Tensor query, Tensor? key, Tensor positions, Tensor inv_freq, int[]? sections, bool interleaved, float scaling, bool inverse) -> Tensor[]");
+  m.def("rotary_embedding_(Tensor(a!) query, Tensor(b!)? key, Tensor positions, Tensor inv_freq, int[]? sections, bool interleaved, float scaling) -> ()");
+  m.def("plan_step(Tensor cached_lens, Tensor new_tokens, Tensor(a!) block_table, Tensor(b!) ring, Tensor ring_state, int block_size, int num_tokens) -> "
+        "(Tensor seq_lens, Tensor cu_seqlens, Tensor positions, Tensor slots, Tensor next_state)");
+  m.def("plan_step_(Tensor(a!) cached_lens, Tensor new_tokens, Tensor(b!) block_table, Tensor(c!) ring, Tensor(d!) ring_state, int block_size, int num_tokens) -> "
+        "(Tensor cu_seqlens, Tensor positions, Tensor slots)");
+  m.def("cache_store_(Tensor key, Tensor value, Tensor slots, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor(c!) key_scale, Tensor(d!) value_scale) -> ()");
+  m.def("cache_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
+        "int max_seqlen_q, int? max_seqlen_k, bool is_causal, float? scale) -> (Tensor, Tensor)");
+}
+
+TORCH_LIBRARY_IMPL(b200_sdpa, CUDA, m) {
+  m.impl("rotary_embedding", b200_glue::rotary_operator);
+  m.impl("rotary_embedding_", b200_glue::rotary_operator_in_place);
+  m.impl("plan_step", b200_glue::plan_operator);
+  m.impl("plan_step_", b200_glue::plan_operator_in_place);
+  m.impl("cache_store_", b200_glue::launch_store);
+  m.impl("cache_attention", b200_glue::launch_attention);
+}
+
+TORCH_LIBRARY_IMPL(b200_sdpa, AutogradCUDA, m) { m.impl("rotary_embedding", b200_glue::rotary_with_grad); }
