@@ -358,7 +358,7 @@ typedef struct sdpa_b200_cache_params {
   /* codes by (block, head, token) strides in bytes, multiples of 16, head_dim contiguous; 16-byte aligned */
   void* k_cache;
   void* v_cache;
-  float* k_scale; /* [num_blocks][heads_kv] */
+  float* k_scale; /* [num_blocks][heads_kv]; those of V not negative */
   float* v_scale;
   int64_t k_block_stride, k_head_stride, k_row_stride;
   int64_t v_block_stride, v_head_stride, v_row_stride;
@@ -402,7 +402,8 @@ SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* s
 
 /* out, lse <- attention of each request's last rows of q over its tokens in the cache. A row without a visible key gets out = 0 and lse = +inf;
  * rows of q outside every request are left unwritten; a block number outside the cache makes the rows that see it NaN (with lse = +inf, as
- * NaN rows have here), a length that passes the table's row all rows of its request. Nothing at or behind seq_lens counts, whatever stands there. Where requests have many rows, codes * scales are brought to 16
+ * NaN rows have here), a length that passes the table's row all rows of its request. Nothing at or behind seq_lens counts, whatever stands there. A scale of K
+ * or V that is infinite or NaN, or a negative one of V, makes the rows that see its block NaN; one of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few. Where requests have many rows, codes * scales are brought to 16
  * bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range: beyond its largest number (f16 65504; the
  * code of an element from 63488 on may be 65536) they are that number, and f16 loses what is below 2^-24, as of a cache that was filled from bf16. (A NaN among the values themselves may reach every row of its request, as 0 * NaN.) */
 SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);

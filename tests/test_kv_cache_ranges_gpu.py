@@ -163,3 +163,87 @@ def test_requests_gathered_in_several_launches(cuda_device):
     _compare(out, lse, b, many=True)
     assert torch.equal(out[:1000], keep[0][:1000])  # the same tiles, whoever is beside them
     assert ops.device_status() == 0
+
+
+def _far_apart(b, exponents, block):
+    """Scales of V by the place of a block in its request: 2^e for the exponents in turn, None: a block of zeros with the least scale. Scores are of N(0,1) queries and keys."""
+    q, kc, vc, ks, vs, table, lens, cu = b
+    if kc.dtype == E4M3:  # drawn codes beyond 448 are NaN, which is not what is looked at here
+        for c in (kc, vc):
+            c.copy_(c.float().nan_to_num(448.0).to(E4M3))
+    for i, n in enumerate(lens.tolist()):
+        for page in range(-(-n // block)):
+            at, e = int(table[i, page]), exponents[page % len(exponents)]
+            if e is None:
+                vc[at] = torch.zeros((), device=vc.device).to(vc.dtype)
+                vs[at] = 2.0 ** -100
+            else:
+                vs[at] = 2.0 ** e
+    return b
+
+
+def _compare_far(out, lse, b, causal):
+    """As _compare; a score carries log2 of V's scale, up to 127, in 32 bits, and so does the running maximum: each off by 2^-18, of the logsumexp (times ln 2) 2^-17 together."""
+    want, want_lse, size, most = orc.attention(*b[:7], b[7], causal)
+    half = torch.finfo(b[0].dtype).eps / 2
+    assert float(most.max()) < 60
+    tol = half * want.abs() + (2.0 ** -11 + 1e-4) * size
+    off = (out.double() - want).abs()
+    assert bool((off <= tol).all()), (int((off > tol).sum()), float((off / size.clamp_min(1e-300)).max()))
+    ltol = 2.0 ** -24 * (int(b[6].max()) / 128 * 9 + 40) + 2.0 ** -21 * most.clamp_min(1) + 2.0 ** -23 * want_lse.abs() + 2.0 ** -17
+    assert bool(((lse.double() - want_lse).abs() <= ltol).all()), float((lse.double() - want_lse).abs().max())
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("exponents", [(100,), (119,), (96, 110), (None, 60), (60, None), (None, None, None, 100, -20), (110, None, 0, -90), (-90, -60, 20, 70)])
+@pytest.mark.parametrize("lens,rows,hq,hkv,dim", [([300], 1, 8, 2, 64), ([1000, 77, 640], 1, 32, 8, 128), ([700, 65, 900], 3, 16, 4, 64), ([500, 400], 12, 8, 2, 128), ([3000] * 40, 1, 16, 4, 128)])
+def test_values_of_the_whole_range_of_bf16(cuda_device, lens, rows, hq, hkv, dim, exponents, code):
+    """Values of up to 2^127, beside blocks of zeros and small ones: every key has its weight, whatever the scales of V are."""
+    b = list(_batch(cuda_device, lens, [rows] * len(lens), hq, hkv, dim, 16, code, torch.bfloat16, seed=len(lens), poison=False))
+    top = 119 if code == E4M3 else 120
+    if code == E4M3:  # codes of up to 448
+        b[2] = (b[2].float() / 4).to(E4M3)
+    else:
+        b[2] = b[2] // 4
+    b = _far_apart(b, [e if e is None else min(e, top - 2) for e in exponents], 16)
+    for causal in (True, False):
+        _compare_far(*_run(b, is_causal=causal), b, causal)
+        _compare_far(*_run(b, max_k=1 << 20, is_causal=causal), b, causal)  # by shares of the list where clusters would take the units
+
+
+def test_stored_values_of_the_whole_range_of_bf16(cuda_device):
+    """Through the store, whose scales go from 2^-100 to 2^119, and on both paths. (The prefill kernel sums weights times values in 32 bits before it divides by the sum of the
+    weights, as for any value: 600 of 2^124 would not fit.)"""
+    n, dim, block = 600, 128, 64
+    for rows, hq in ((1, 16), (500, 64)):
+        g = torch.Generator(device=cuda_device).manual_seed(rows)
+        k, v = (torch.randn(n, 8, dim, generator=g, device=cuda_device).bfloat16() for _ in range(2))
+        v *= 2.0 ** (122 if rows == 1 else 110)
+        v[64:128] = 0
+        kc, ks = _cache(cuda_device, 12, 8, block, dim, E4M3, 1)
+        vc, vs = _cache(cuda_device, 12, 8, block, dim, E4M3, 2)
+        table = _ints(cuda_device, [[3, 1, 4, 7, 5, 9, 2, 6, 11, 0]])
+        kv_cache.store(k, v, _ints(cuda_device, [int(table[0, t // block]) * block + t % block for t in range(n)]), kc, vc, ks, vs)
+        assert float(vs[1].max()) == 2.0 ** -100 and float(vs[3].max()) >= 2.0 ** (115 if rows == 1 else 103)
+        q = torch.randn(rows, hq, dim, generator=g, device=cuda_device).bfloat16()
+        b = (q, kc, vc, ks, vs, table, _ints(cuda_device, [n]), _ints(cuda_device, [0, rows]))
+        gathers, out, lse = _gathers(b)
+        assert gathers == (rows == 500)
+        if gathers:
+            _compare(out, lse, b, many=True)
+        else:
+            _compare_far(out, lse, b, True)
+
+
+@pytest.mark.parametrize("rows,hq", [(1, 16), (500, 64)])
+def test_scales_that_no_element_can_have(cuda_device, rows, hq):
+    """Infinite ones of K and V, NaN, and negative ones of V: the rows that see their blocks are NaN on both paths, those of other requests as they are."""
+    for which, value in ((3, math.inf), (3, -math.inf), (3, math.nan), (4, math.inf), (4, math.nan), (4, -1.0), (4, -math.inf)):
+        b = list(_batch(cuda_device, [600, 200], [rows, 1], hq, 8, 128, 64, INT8, torch.bfloat16, poison=False))
+        want = _run(b)
+        b[which][int(b[5][0, 0])] = value
+        gathers, out, lse = _gathers(b)
+        assert gathers == (rows == 500)
+        assert bool(out[:rows].isnan().all()), (which, value)
+        assert which == 4 or bool((lse[:, :rows] == math.inf).all())  # (the logsumexp has no part of V)
+        assert torch.equal(out[rows:], want[0][rows:]) and torch.equal(lse[:, rows:], want[1][:, rows:])

@@ -17,7 +17,8 @@
 //    what is 2^-39 of the row's largest). The scale of K goes onto the fp32 scores; that of V into the exponent, so that the weights
 //    w_j = 2^(s_j + log2 vs_j - m) with m their running maximum are f16 numbers of up to 2^15 which keep all 11 bits down to 2^-29 of the
 //    largest, whatever scales blocks have, and the products add up in the tensor core's fp32 accumulators without a pass over them. The sum of
-//    the softmax takes w_j / vs_j in fp32.
+//    the softmax takes w_j / vs_j in fp32; from the first tile on that has a scale of V above 1 it takes 2^(s_j - m), another exponential, since w_j may then be too small
+//    for 32 bits beside a key whose value is 2^100 times as large (in a loop of its own: within the one for all calls it cost 2 to 5%).
 //    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
 //    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.1 us.
@@ -41,7 +42,11 @@ constexpr int kPause = 2;  // see share_of
 constexpr int kTilesInCluster = 8;          // that a CTA of a cluster may get: see cluster_of
 constexpr int kMostClusterCtas = 256;       // clusters of eight find room for that many CTAs at once
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
-constexpr float kSumUnit = 0x1p-40f;       // sums are kept in this unit, so that those over blocks of the least scale stay in range
+// Sums are kept in this unit: they are up to 2^100 a token where the largest weight is that of a block of the least scale, and no less than 2^-121 where it is that of bf16's largest
+constexpr float kSumUnit = 0x1p-15f;
+// Scales of V above it are far from the least one: a weight times its scale, or what such products are multiplied by when their maximum moves, may then be too small for 32 bits
+// though the weight itself counts. Up to it, what is lost is 2^-25 of the sum.
+constexpr float kFarScale = 1.f;
 
 struct StreamParams {
   const uint16_t* q;
@@ -209,7 +214,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t ring = (raw_addr + 1023u) & ~1023u;
   uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
-  float4* slot_scales = reinterpret_cast<float4*>(ring_ptr + kSt * kStageBytes);  // [stage][16 tokens]: of K, log2 of that of V, kSumUnit over that of V
+  float4* slot_scales = reinterpret_cast<float4*>(ring_ptr + kSt * kStageBytes);  // [stage][16 tokens]: of K, log2 of that of V, kSumUnit over that of V, 1 where one of V's is far
   float2* row_state = reinterpret_cast<float2*>(slot_scales + kSt * kSlots);      // [warp][row]: maximum and sum
   uint2* q_state = reinterpret_cast<uint2*>(row_state + kWarps * 16);             // [row group][block of 8 rows][chunk][lane]: B fragments
   constexpr int kQWords = kQInRegisters ? 0 : kRowWarps * kRowBlocks * kChunks * 32;
@@ -283,7 +288,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       far_id = block_at(far);
     };
     const int pages = kTileTokens >> p.shift;  // of a tile
-    bool ok = true;
+    bool ok = true, far_scales = false;  // a scale of V above kFarScale has been seen, in this tile or before
     int step = 0;
     bool first = true;
     for (int places = share.places; places > 0;) {
@@ -324,11 +329,13 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         float* slot = reinterpret_cast<float*>(slot_scales + st * kSlots + lane);
         if (lane < kSlots) {
           if (keys) {
-            slot[0] = own;
+            slot[0] = fabsf(own) == INFINITY ? __int_as_float(0x7fffffff) : own;
           } else {
-            const float used = isnan(own) ? own : fmaxf(own, kLeastScale);
+            const float used = own >= 0.f ? fmaxf(own, kLeastScale) : __int_as_float(0x7fffffff);
             slot[1] = log2f(used);
             slot[2] = kSumUnit / used;
+            if (__any_sync((1u << kSlots) - 1, used > kFarScale)) far_scales = true;
+            slot[3] = far_scales ? 1.f : 0.f;
           }
         }
         __syncwarp();
@@ -480,10 +487,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
           }
         };
-#pragma unroll 1
-        for (int c = 0; c < kPartTokens; c += kStepTokens) {
+        auto work_on = [&](int c, auto far_tag) {
+          constexpr bool kFar = decltype(far_tag)::value;
           const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
-          if (tok >= seen_by_any) break;
           const uint32_t v_smem = ring + st * kStageBytes + in_tile * kD + kTileTokens * kD;
           float s[kRowBlocks][kHalves][4];
           scores(c, s);
@@ -525,18 +531,33 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             my = fmaxf(m[nb].y, column_max(my));
             // a row that has seen no key has o = l = 0: any finite factor will do
             a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
+            if constexpr (kFar) {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
+              const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
+              const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
+              l[nb].x = l[nb].x * hx * hx;
+              l[nb].y = l[nb].y * hy * hy;
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                const float lv = sc[half].y;
+                l[nb].x += exp2f(s[nb][half][0] - lv - vx) + exp2f(s[nb][half][2] - lv - vx);
+                l[nb].y += exp2f(s[nb][half][1] - lv - vy) + exp2f(s[nb][half][3] - lv - vy);
+              }
+            } else {
+              l[nb].x *= a[nb].x;
+              l[nb].y *= a[nb].y;
+            }
             moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
             m[nb] = make_float2(mx, my);
             const float ux = mx == -INFINITY ? 0.f : mx - kBias, uy = my == -INFINITY ? 0.f : my - kBias;
-            l[nb].x *= a[nb].x;
-            l[nb].y *= a[nb].y;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
               const float rv = sc[half].z;
               const float x0 = ex2_approx(s[nb][half][0] - ux), y0 = ex2_approx(s[nb][half][1] - uy);
               const float x1 = ex2_approx(s[nb][half][2] - ux), y1 = ex2_approx(s[nb][half][3] - uy);
-              l[nb].x = fmaf(x0 + x1, rv, l[nb].x);
-              l[nb].y = fmaf(y0 + y1, rv, l[nb].y);
+              if constexpr (!kFar) {
+                l[nb].x = fmaf(x0 + x1, rv, l[nb].x);
+                l[nb].y = fmaf(y0 + y1, rv, l[nb].y);
+              }
               pb[nb][half][0] = transpose_8x8(pack_f16x2(x0, y0));
               pb[nb][half][1] = transpose_8x8(pack_f16x2(x1, y1));
             }
@@ -588,6 +609,14 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
               if (tok + half * 16 < r.len) add_half(half, keep(j), keep(j + 8));
             }
           }
+        };
+        const int end = min(kPartTokens, seen_by_any - tile_tok - part * kPartTokens);
+        if (slot_scales[st * kSlots].w == 0.f) {
+#pragma unroll 1
+          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::false_type{});
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::true_type{});
         }
         // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
         if (i + 1 < seg_tiles) {
@@ -643,8 +672,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             float f[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              f[x] = others[x][w].x == -INFINITY ? 0.f : ex2_approx(others[x][w].x - mm[x]);
-              sum[x] = fmaf(others[x][w].y, f[x], sum[x]);
+              const float h = others[x][w].x == -INFINITY ? 0.f : ex2_approx(0.5f * (others[x][w].x - mm[x]));
+              f[x] = h * h;
+              sum[x] = fmaf(others[x][w].y * h, h, sum[x]);
             }
 #pragma unroll
             for (int ch = 0; ch < kMine; ++ch)
@@ -905,7 +935,7 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       uint32_t f[4], c[2] = {w[i][x].x, w[i][x].y};
-      const float own = fabsf(scale[i][x]) == INFINITY ? __int_as_float(0x7fffffff) : scale[i][x];  // nor are elements of such a block numbers on the other path
+      const float own = fabsf(scale[i][x]) == INFINITY || (x == 1 && scale[i][x] < 0.f) ? __int_as_float(0x7fffffff) : scale[i][x];  // as on the other path
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         uint32_t lo, hi;
