@@ -188,3 +188,30 @@ def test_functional_transforms_are_refused(cuda_device):
         torch.func.functionalize(lambda t: kv_cache.store(t, k, lens * 0, kc, vc, ks, vs))(k)
     with pytest.raises(RuntimeError, match="ordinary tensor"):
         torch.func.vmap(lambda t: kv_cache.plan_step(lens, t, table, lens, _ints(cuda_device, [0, 0, 0]), block_size=16, num_tokens=4).slots)(torch.stack([lens, lens]))
+
+
+def test_what_would_be_left_out_of_a_derivative_is_refused(cuda_device):
+    """Scales and caches that need gradients, and tangents of any argument."""
+    import torch.autograd.forward_ad as fwAD
+    q, kc, vc, ks, vs, table, lens, cu = _batch(cuda_device, [100, 90], [1, 1], 4, 2, 64, 16, E4M3, torch.bfloat16, poison=False)
+    k, slots, f, pos = torch.ones(2, 2, 64, device=cuda_device, dtype=torch.bfloat16), _ints(cuda_device, [0, 1]), _freq(32, cuda_device), _ints(cuda_device, [3, 4])
+    attend = lambda *a: kv_cache.attention(*a, table, lens)
+    store = lambda *a: kv_cache.store(a[0], a[1], slots, *a[2:])
+    before = [x.clone() for x in (kc.view(torch.int8), vc.view(torch.int8), ks, vs)]
+    for call, args, text in ((attend, (q, kc, vc, ks, vs), "has no gradient"), (store, (k, k.clone(), kc, vc, ks, vs), "keeps no gradient")):
+        for i, x in enumerate(args):
+            if x.dtype == E4M3:
+                continue
+            with pytest.raises(RuntimeError, match=text):
+                call(*(y.detach().requires_grad_() if j == i else y for j, y in enumerate(args)))
+            with torch.no_grad():
+                call(*(y.detach().clone().requires_grad_() if j == i else y.clone() for j, y in enumerate(args)))
+            with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                call(*(fwAD.make_dual(y, torch.ones_like(y)) if j == i else y for j, y in enumerate(args)))
+    for call in (rotary.rotary_embedding, rotary.rotary_embedding_):
+        for i in (0, 1, 3):
+            args = [q.clone(), k.clone(), pos, f]
+            with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+                args[i] = fwAD.make_dual(args[i], torch.ones_like(args[i]))
+                call(*args)
+    assert all(torch.equal(x, y) for x, y in zip(before, (kc.view(torch.int8), vc.view(torch.int8), ks, vs)))

@@ -53,6 +53,11 @@ void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
+// What is differentiated forwards, or backwards, would be left out silently.
+void check_no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "forward-mode differentiation of ", what, " is not implemented");
+}
+
 bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
 // Whether a tracer, a dispatch mode, a functional transform or code below autograd is to see the operators of this thread. (Autocast has nothing to do with them, and inference
@@ -209,7 +214,10 @@ void launch_store(const Tensor& key, const Tensor& value, const Tensor& slots, c
   sdpa_b200_cache_params p = {};
   cache_params(p, key, "key", key_cache, value_cache, key_scale, value_scale);
   TORCH_CHECK(key.size(1) == key_cache.size(1), "the caches must have the heads of key and value");
-  TORCH_CHECK(!needs_grad(key) && !needs_grad(value), "the cache keeps no gradient: store keys and values under torch.no_grad()");
+  for (const Tensor* t : {&key, &value, &key_cache, &value_cache, &key_scale, &value_scale}) {
+    TORCH_CHECK(!needs_grad(*t), "the cache keeps no gradient: store keys and values under torch.no_grad()");
+    check_no_tangent(*t, "the cache");
+  }
   check_ints(slots, "slots", key);
   TORCH_CHECK(slots.dim() == 1 && slots.size(0) == key.size(0), "slots must be [tokens]");
   if (key.size(0) == 0) return;
@@ -242,7 +250,10 @@ std::tuple<Tensor, Tensor> launch_attention(const Tensor& query, const Tensor& k
     check_ints(*cu_seqlens, "cu_seqlens", query);
     TORCH_CHECK(cu_seqlens->dim() == 1 && cu_seqlens->size(0) == B + 1, "cu_seqlens must have requests + 1 entries");
   }
-  TORCH_CHECK(!needs_grad(query), "attention over the cache has no gradient: call it under torch.no_grad()");
+  for (const Tensor* t : {&query, &key_cache, &value_cache, &key_scale, &value_scale}) {
+    TORCH_CHECK(!needs_grad(*t), "attention over the cache has no gradient: call it under torch.no_grad()");
+    check_no_tangent(*t, "attention over the cache");
+  }
   c10::cuda::CUDAGuard guard(query.device());
   Tensor out = new_tensor({T, H, query.size(2)}, query.scalar_type(), query), lse = new_tensor({H, T}, at::kFloat, query);
   if (query.numel() == 0) return {out, lse};
@@ -384,6 +395,7 @@ void check_rotary(const Tensor& query, const Tensor& key, const Tensor& position
   TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous() && inv_freq.device() == query.device(),
               "inv_freq must be a contiguous fp32 vector of rotary_dim / 2 frequencies on the device of query");
   TORCH_CHECK(!needs_grad(inv_freq), "rotary positions have no gradient of inv_freq: detach it");
+  for (const Tensor* t : {&query, &key, &inv_freq}) check_no_tangent(*t, "rotary positions");
   check_plain(positions, "positions");
   TORCH_CHECK((positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong) && positions.device() == query.device(),
               "positions must be int32 or int64, on the device of query");
@@ -474,8 +486,6 @@ std::vector<Tensor> rotary_with_grad(const Tensor& query, const c10::optional<Te
   const std::vector<int64_t> parts = sections.has_value() ? sections->vec() : std::vector<int64_t>();
   check_rotary(query, k, positions, inv_freq, parts);
   if (needs_grad(query) || needs_grad(k)) return RotaryFunction::apply(query, key, positions, inv_freq, parts, interleaved, inverse, scaling);
-  for (const Tensor* t : {&query, &k})
-    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), "forward-mode differentiation of rotary positions is not implemented");
   const auto r = turned(query, k, positions, inv_freq, {parts, interleaved, inverse, scaling});
   if (!k.defined()) return {std::get<0>(r)};
   return {std::get<0>(r), std::get<1>(r)};
