@@ -247,3 +247,20 @@ def test_scales_that_no_element_can_have(cuda_device, rows, hq):
         assert bool(out[:rows].isnan().all()), (which, value)
         assert which == 4 or bool((lse[:, :rows] == math.inf).all())  # (the logsumexp has no part of V)
         assert torch.equal(out[rows:], want[0][rows:]) and torch.equal(lse[:, rows:], want[1][:, rows:])
+
+
+def test_plan_of_the_most_tokens(cuda_device):
+    """2^30 tokens in a step, the most that are counted: with twice as many the second request is the one that does not fit, however many blocks there are."""
+    most, width, blocks = 1 << 30, 1 << 23, (1 << 24) - 1
+    table = torch.full((2, width), -1, dtype=torch.int32, device=cuda_device)
+    ring = torch.arange(blocks, dtype=torch.int32, device=cuda_device)
+    state, none = _ints(cuda_device, [0, blocks, 0]), _ints(cuda_device, [0, 0])
+    plan = lambda new: kv_cache.plan_step(none, _ints(cuda_device, new), table, ring, state, block_size=128, num_tokens=most)
+    step = plan([most, most])
+    assert step.ring_state.tolist() == [0, blocks, -2] and step.seq_lens.tolist() == [0, 0] and step.cu_seqlens.tolist() == [0, 0, 0]
+    assert int(step.slots[-1]) == -1 and int(table[0, 0]) == -1
+    del step
+    step = plan([most - 5, 5])
+    assert step.ring_state.tolist() == [width + 1, blocks - width - 1, 0] and step.cu_seqlens.tolist() == [0, most - 5, most]
+    assert step.positions[-7:].tolist() == [most - 7, most - 6, 0, 1, 2, 3, 4] and step.slots[-5:].tolist() == [width * 128 + i for i in range(5)]
+    assert int(step.slots[most - 6]) == most - 6 and int(table[1, 0]) == width

@@ -18,7 +18,8 @@ constexpr int kThreads = 1024;
 constexpr int kMaxBatch = 16384;  // three running sums of it fit a block's shared memory
 
 struct Sums {
-  int tokens, need, freed;
+  unsigned tokens;
+  int need, freed;
 };
 
 __device__ __forceinline__ int pages_of(int n, int shift) { return (n + (1 << shift) - 1) >> shift; }
@@ -53,13 +54,14 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_par
       bad = c < 0 || c > most || len < 0 || len > most || n > p.num_tokens;
       if (!bad) {
         const int had = pages_of(c, shift), has = pages_of(static_cast<int>(len), shift);
-        mine = {n > 0 ? n : 0, has > had ? has - had : 0, had > has ? had - has : 0};
+        mine = {n > 0 ? static_cast<unsigned>(n) : 0u, has > had ? has - had : 0, had > has ? had - has : 0};
       }
     }
     Sums run = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-      const int a = __shfl_up_sync(0xffffffffu, run.tokens, d), b = __shfl_up_sync(0xffffffffu, run.need, d), c = __shfl_up_sync(0xffffffffu, run.freed, d);
+      const unsigned a = __shfl_up_sync(0xffffffffu, run.tokens, d);
+      const int b = __shfl_up_sync(0xffffffffu, run.need, d), c = __shfl_up_sync(0xffffffffu, run.freed, d);
       if (lane >= d) {
         run.tokens += a;
         run.need += b;
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(const sdpa_b200_plan_par
     }
     __syncthreads();
   }
-  // No sum has passed 32 bits in front of the first bad request: tokens end at 2 * num_tokens at most, pages at batch * max_blocks (checked by the host).
+  // No sum has passed 32 bits in front of the first bad request: tokens end at 2 * num_tokens at most, 2^31, pages at batch * max_blocks (checked by the host).
   const int refused = first_bad < p.batch ? -1 - first_bad : all_need > count ? static_cast<int>(all_need - count) : 0;
   const bool fine = refused == 0;
   const int total = fine ? static_cast<int>(all_tokens) : 0;
