@@ -11,6 +11,9 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cstdlib>
+
 #include "torch_glue.h"
 
 namespace b200_glue {
@@ -330,6 +333,37 @@ void strides_of(const Tensor& t, int64_t& batch, int64_t& head, int64_t& row) {
   row = t.stride(t.dim() == 4 ? 2 : 0);
 }
 
+// Whether two tensors whose elements are a row apart by the same strides have any in common: slices of one projection do not, overlapping ones do. (Other strides are not
+// looked at.)
+bool rows_overlap(const Tensor& x, const Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  int64_t xs[3], ys[3];  // batch, head, row
+  strides_of(x, xs[0], xs[1], xs[2]);
+  strides_of(y, ys[0], ys[1], ys[2]);
+  const bool packed = x.dim() == 3;
+  const int64_t xn[3] = {packed ? 1 : x.size(0), x.size(1), x.size(packed ? 0 : 2)}, yn[3] = {xn[0], y.size(1), xn[2]}, width = x.size(-1);
+  // where an element of x and one of y are the same, the distance of the tensors is a sum of n * stride with n from -(y's size - 1) to x's size - 1, and of less than a row
+  struct Step {
+    int64_t stride, least, most;
+  };
+  Step steps[3];
+  int n_steps = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (xn[i] == 1 && yn[i] == 1) continue;
+    if (xn[i] > 1 && yn[i] > 1 && xs[i] != ys[i]) return false;
+    steps[n_steps++] = {xn[i] > 1 ? xs[i] : ys[i], 1 - yn[i], xn[i] - 1};
+  }
+  std::sort(steps, steps + n_steps, [](const Step& a, const Step& b) { return a.stride > b.stride; });
+  auto reaches = [&](auto&& self, int i, int64_t distance) -> bool {
+    if (i == n_steps) return std::abs(distance) < width;
+    const int64_t n = distance / steps[i].stride;  // strides are positive here; the nearest two and one on either side
+    for (int64_t k = std::max(n - 1, steps[i].least); k <= std::min(n + 1, steps[i].most); ++k)
+      if (self(self, i + 1, distance - k * steps[i].stride)) return true;
+    return false;
+  };
+  return reaches(reaches, 0, (reinterpret_cast<intptr_t>(y.data_ptr()) - reinterpret_cast<intptr_t>(x.data_ptr())) / 2);
+}
+
 Tensor new_turned(const Tensor& x) {
   if (x.dim() == 3) return new_tensor(x.sizes(), x.scalar_type(), x);
   return new_tensor({x.size(0), x.size(2), x.size(1), x.size(3)}, x.scalar_type(), x).transpose(1, 2);
@@ -497,11 +531,11 @@ void rotary_operator_in_place(const Tensor& query, const c10::optional<Tensor>& 
   const std::vector<int64_t> parts = sections.has_value() ? sections->vec() : std::vector<int64_t>();
   check_rotary(query, k, positions, inv_freq, parts);
   TORCH_CHECK(!needs_grad(query) && !needs_grad(k), "rotary positions in place have no gradient: use rotary_embedding");
-  TORCH_CHECK(!k.defined() || query.numel() == 0 || k.data_ptr() != query.data_ptr(), "rotary positions in place: query and key are the same memory");
   for (const Tensor* t : {&query, &k}) {
     for (int64_t i = 0; t->defined() && i < t->dim(); ++i)
       TORCH_CHECK(t->size(i) <= 1 || t->stride(i) != 0, "rotary positions in place need elements of their own (a stride is 0)");
   }
+  TORCH_CHECK(!k.defined() || !rows_overlap(query, k), "rotary positions in place: query and key are the same memory, or share some");
   turn(query, k, positions, inv_freq, {parts, interleaved, false, scaling}, true);
   for (const Tensor* t : {&query, &k})
     if (t->defined()) written(*t);

@@ -29,6 +29,6 @@ def rotary_embedding(query, key, positions, inv_freq, *, sections: Optional[Sequ
 
 def rotary_embedding_(query, key, positions, inv_freq, *, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
                       scaling: float = 1.0):
-    """``rotary_embedding`` in place, for tensors that need no gradient."""
+    """``rotary_embedding`` in place, for tensors that need no gradient and share no elements."""
     calls = torch_glue.calls or torch_glue.load()
     return calls.rotary(query, key, positions, inv_freq, sections, interleaved, scaling, True)
