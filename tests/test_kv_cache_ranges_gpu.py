@@ -264,3 +264,15 @@ def test_plan_of_the_most_tokens(cuda_device):
     assert step.ring_state.tolist() == [width + 1, blocks - width - 1, 0] and step.cu_seqlens.tolist() == [0, most - 5, most]
     assert step.positions[-7:].tolist() == [most - 7, most - 6, 0, 1, 2, 3, 4] and step.slots[-5:].tolist() == [width * 128 + i for i in range(5)]
     assert int(step.slots[most - 6]) == most - 6 and int(table[1, 0]) == width
+
+
+@pytest.mark.parametrize("rows,bound,dim", [(20, 4, 64), (9, 2, 128), (100, 30, 128)])
+def test_more_rows_than_the_bound_says(cuda_device, rows, bound, dim):
+    """Those behind the bound may stay unwritten; those in front of it, and other requests, are as they should be."""
+    b = _batch(cuda_device, [900, 400, 70], [2, rows, 1], 8, 2, dim, 32, INT8, torch.float16)
+    for max_k in (900, 1 << 20):
+        out, lse = _run(b, max_q=bound, max_k=max_k)
+        whole, whole_lse = _run(b)
+        for i in range(2 + bound, 2 + rows):
+            out[i], lse[:, i] = whole[i], whole_lse[:, i]
+        _compare(out, lse, b)

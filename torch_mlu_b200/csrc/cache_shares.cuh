@@ -29,8 +29,8 @@ __host__ __device__ __forceinline__ Request request_at(const P& p, int b) {
   r.rows_q = 1;
   if (p.cu_q) r.rows_q = p.cu_q[b + 1] > r.q0 ? p.cu_q[b + 1] - r.q0 : 0;
   if (r.q0 < 0 || r.q0 + static_cast<int64_t>(r.rows_q) > p.total_q) r.rows_q = 0;  // offsets that leave q: no rows
-  if (r.rows_q > p.max_rows) r.rows_q = p.max_rows;  // what the places were counted with
   r.in_front = too_long ? r.len : r.len - r.rows_q;
+  if (r.rows_q > p.max_rows) r.rows_q = p.max_rows;  // what the places were counted with: those behind are not walked
   r.tiles = (r.len + (1 << p.tile_shift) - 1) >> p.tile_shift;
   if (r.tiles < 1) r.tiles = 1;  // an empty request has rows to write too
   r.units = p.heads_kv * ((r.rows_q * p.group + p.rows - 1) >> p.rows_shift);
