@@ -405,7 +405,8 @@ SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* s
  * NaN rows have here), a length that passes the table's row all rows of its request. Nothing at or behind seq_lens counts, whatever stands there. A scale of K
  * or V that is infinite or NaN, or a negative one of V, makes the rows that see its block NaN; one of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few. Where requests have many rows, codes * scales are brought to 16
  * bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range: beyond its largest number (f16 65504; the
- * code of an element from 63488 on may be 65536) they are that number, and f16 loses what is below 2^-24, as of a cache that was filled from bf16. (A NaN among the values themselves may reach every row of its request, as 0 * NaN.) */
+ * code of an element from 63488 on may be 65536) they are that number, and f16 loses what is below 2^-24, as of a cache that was filled from bf16. (A NaN among the values themselves, or a scale of V that is NaN, may reach every row of its
+ * request and kv head, as 0 * NaN.) */
 SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);
 SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_params* p, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -276,3 +276,30 @@ def test_more_rows_than_the_bound_says(cuda_device, rows, bound, dim):
         for i in range(2 + bound, 2 + rows):
             out[i], lse[:, i] = whole[i], whole_lse[:, i]
         _compare(out, lse, b)
+
+
+@pytest.mark.parametrize("code", [E4M3, INT8])
+@pytest.mark.parametrize("rows,hq", [(4, 8), (600, 64)])
+def test_nan_among_the_last_drafted_tokens(cuda_device, code, rows, hq):
+    """What a key, or a value, that is no number reaches: the rows that see the key; of a value any row of its request; in int8, which marks the block's scale, the same of the
+    block's keys and values. Other requests are as they are, and so are the request's other kv heads."""
+    for which in (0, 1):
+        lens = [640, 500]
+        b = list(_batch(cuda_device, lens, [rows, 3], hq, 2 if rows < 100 else 8, 128, 64, code, torch.bfloat16, poison=False))
+        if code == E4M3:
+            for c in (b[1], b[2]):
+                c.copy_(c.float().nan_to_num(448.0).to(E4M3))
+        hkv = b[1].shape[1]
+        want = _run(b)
+        k, v = (torch.randn(2, hkv, 128, device=cuda_device).bfloat16() * 1e-3 for _ in range(2))
+        block = int(b[5][0, 9])
+        (k, v)[which][1, 0, 7] = math.nan
+        kv_cache.store(k, v, _ints(cuda_device, [block * 64 + 62, block * 64 + 63]), *b[1:5])  # the last two tokens of the first request
+        out, lse = _run(b)
+        group = hq // hkv
+        other = slice(group, None)
+        assert bool(out[:, other].isfinite().all()) and torch.equal(out[rows:], want[0][rows:]) and torch.equal(lse[:, rows:], want[1][:, rows:])
+        assert bool(out[rows - 1, :group].isnan().any())  # the last row sees it
+        if which == 0:
+            sees = torch.arange(640 - rows, 640, device=cuda_device) >= (639 if code == E4M3 else 576)
+            assert bool(out[:rows, :group][sees].isnan().all()) and bool(out[:rows, :group][~sees].isfinite().all())

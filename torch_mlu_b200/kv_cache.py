@@ -81,6 +81,7 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package), a length that passes the table's row all rows of its request.
+    A key that is NaN reaches the rows that see it, a value any row of its request and kv head (in an int8 cache, whose block has the scale NaN then: the block's keys, the block's values).
     """
     return _calls().cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_seqlen_q, max_seqlen_k,
                                     is_causal, scale)

@@ -4,7 +4,8 @@ After ``load()``:
 * ``torch.ops.b200_sdpa._scaled_dot_product_flash_attention`` (+ ``_backward``) and
   ``torch.ops.b200_sdpa._flash_attention_forward`` (+ ``_backward``) exist with the reference's
   schemas (codegen/mlu_functions.yaml:1313-1316) and differentiate through autograd.
-* so do ``rotary_embedding``, ``plan_step``, ``cache_store_`` and ``cache_attention`` (kv_cache.py, rotary.py), through which their calls go under tracers and dispatch modes;
+* ``torch.ops.b200_sdpa.rotary_embedding`` (which differentiates), ``plan_step``, ``cache_store_`` and ``cache_attention`` exist too (and ``rotary_embedding_``, ``plan_step_``):
+  calls of kv_cache.py and rotary.py go through them under tracers and dispatch modes.
 * ``install_aten_overrides()`` additionally points the CUDA kernels of the same four ``aten``
   operators at this library, so ``F.scaled_dot_product_attention`` under the flash backend runs
   here. It is opt-in because it changes those operators for the whole process.
