@@ -1,5 +1,6 @@
 """The ends of the serving operators' ranges: long lists, the types' largest values, lengths and bounds that do not fit, against the restatements in 64 bits.
 Tolerances as in test_kv_cache_gpu.py, from which the helpers come."""
+import ctypes
 import math
 
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 from oracle import cache_oracle as orc
 from test_kv_cache_gpu import E4M3, INT8, _batch, _cache, _compare, _ints, _run, _same_cache
-from torch_mlu_b200 import kv_cache, ops
+from torch_mlu_b200 import _cabi, kv_cache, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -24,7 +25,6 @@ def test_one_long_chunk_among_many_requests(cuda_device, requests, at):
 
 def test_a_list_that_takes_several_launches(cuda_device):
     """Tables so wide that the tiles of all requests at their longest would not be counted in 32 bits."""
-    from torch_mlu_b200 import _cabi
     requests, heads, block = 70, 128, 128
     for rows in (1, 2):
         lens = [1 + 37 * i % 300 for i in range(requests)]
@@ -44,16 +44,27 @@ def test_a_list_that_takes_several_launches(cuda_device):
         _compare(*again, b)
 
 
-def _gathers(b, **kw):
-    """Whether a call brings keys and values to 16 bits in its workspace, by the names of its kernels; and its results."""
-    torch.cuda.synchronize()
-    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
-        out, lse = _run(b, **kw)
-        torch.cuda.synchronize()
-    names = [e.key for e in prof.key_averages()]
-    gathers, streams = (any(n in name for name in names) for n in ("cache_gather_kernel", "cache_stream_kernel"))
-    assert gathers != streams, names
-    return gathers, out, lse
+def _gathers(b, max_q=None, max_k=None, **kw):
+    """Whether a call brings keys and values to 16 bits in its workspace, by the size of that (without copies it is one of four, for parts of 8 to 64 rows); and its results."""
+    q, kc, vc, ks, vs, table, lens, cu = b
+    max_q = max_q or max(1, int((cu[1:] - cu[:-1]).max()))
+    max_k = max_k or max(1, int(lens.max()))
+    p = _cabi.CacheParams()
+    p.k_cache, p.v_cache, p.k_scale, p.v_scale = (x.data_ptr() for x in (kc, vc, ks, vs))
+    for x, c in (("k", kc), ("v", vc)):
+        for f, stride in zip(("block", "head", "row"), c.stride()):
+            setattr(p, f"{x}_{f}_stride", stride)
+    p.num_blocks, p.heads_kv, p.block_size, p.head_dim = kc.shape
+    p.code, p.dtype = _cabi.CODE_INT8 if kc.dtype == INT8 else _cabi.CODE_E4M3, _cabi.DTYPE_F16 if q.dtype == torch.float16 else _cabi.DTYPE_BF16
+    p.q = p.out = p.lse = q.data_ptr()  # (only asked for sizes)
+    p.block_table, p.seq_lens, p.cu_seqlens_q = (t.data_ptr() for t in (table, lens, cu))
+    p.q_row_stride, p.q_head_stride, _ = p.o_row_stride, p.o_head_stride, _ = q.stride()
+    p.table_stride, p.max_blocks, p.batch, p.total_q, p.heads_q = table.stride(0), table.size(1), table.size(0), q.shape[0], q.shape[1]
+    p.max_seqlen_q, p.max_seqlen_k, p.is_causal, p.softmax_scale = max_q, max_k, 1, 0.1
+    n = ctypes.c_size_t(0)
+    assert _cabi.load().sdpa_b200_cache_attention_workspace_bytes(ctypes.byref(p), ctypes.byref(n)) == 0
+    parts = [256 + -(-320 * (2 * rows * (kc.shape[3] + 1) * 4 + 24) // 256) * 256 for rows in (8, 16, 32, 64)]
+    return (n.value not in parts, *_run(b, max_q, max_k, **kw))
 
 
 @pytest.mark.parametrize("code,values", [(E4M3, (63488.0, 64000.0, 65504.0)), (INT8, (65024.0, 65280.0, 65504.0))])
