@@ -218,3 +218,19 @@ def test_workspace_of_many_requests_at_a_large_bound(native_lib):
         got = native_lib.sdpa_b200_cache_attention(ctypes.byref(p), 4096, n.value, None)
         assert torch.cuda.is_available() or got == _cabi.NO_DEVICE  # nothing else is in the way
     assert 32 * 8192 * 8 * 128 * 4 <= sizes[0] < sizes[1] and sizes[3] >= 4 << 30 and sizes[4] < 1 << 27
+
+
+def test_sizes_whose_product_passes_64_bits(native_lib):
+    """4 * 2^31 tokens * 2^24 heads * 128 is 2^64: answered as any other size, by streaming or by a refusal."""
+    import ctypes
+    from test_kv_cache_cpu import _cache, _set
+    from torch_mlu_b200 import _cabi
+    n = ctypes.c_size_t(0)
+    for heads in (1 << 22, (1 << 23) - 5, 1 << 23):
+        for bound in (2 ** 31 - 1, 1 << 30, 1 << 20):
+            p = _cache()
+            _set(heads_kv=heads, heads_q=heads, q_row_stride=heads * 128, o_row_stride=heads * 128, k_block_stride=heads * 64 * 128, v_block_stride=heads * 64 * 128,
+                 max_seqlen_q=100, total_q=200, max_seqlen_k=bound, batch=2)(p)
+            assert native_lib.sdpa_b200_cache_attention_workspace_bytes(ctypes.byref(p), ctypes.byref(n)) == 0 and 0 < n.value < 1 << 27
+            got = native_lib.sdpa_b200_cache_attention(ctypes.byref(p), 4096, n.value, None)
+            assert got in (_cabi.UNSUPPORTED, _cabi.NO_DEVICE) or torch.cuda.is_available()

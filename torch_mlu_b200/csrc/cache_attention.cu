@@ -955,8 +955,11 @@ int table_tokens(const sdpa_b200_cache_params& p) { return static_cast<int>(std:
 // Tokens of the longest request among the 16-bit copies, no fewer than any has rows
 int most_gathered(const sdpa_b200_cache_params& p) { return std::max(p.max_seqlen_k, p.max_seqlen_q); }
 
-// Keys and values of one request among the 16-bit copies, at its longest
-int64_t gathered_bytes(const sdpa_b200_cache_params& p) { return 4 * padded_keys(most_gathered(p)) * p.heads_kv * p.head_dim; }
+// Keys and values of one request among the 16-bit copies, at its longest; one more than fits where they do not
+int64_t gathered_bytes(const sdpa_b200_cache_params& p) {
+  const int64_t rows = padded_keys(most_gathered(p)) * p.heads_kv, row_bytes = 4 * p.head_dim;
+  return rows <= kMostGatheredBytes / row_bytes ? rows * row_bytes : kMostGatheredBytes + 1;
+}
 
 // Requests that are gathered at a time. What they hold is not known here: by the bound on lengths, which may be the table's, the copies of a large batch would take more memory than
 // the cache itself. 64 requests of 512 rows behind 32768 tokens, 32/8 heads of 128, in two launches of each kernel instead of one: 16.8 instead of 16.7 ms.
