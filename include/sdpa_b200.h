@@ -401,12 +401,15 @@ typedef struct sdpa_b200_cache_params {
 SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* stream);
 
 /* out, lse <- attention of each request's last rows of q over its tokens in the cache. A row without a visible key gets out = 0 and lse = +inf;
- * rows of q outside every request are left unwritten; a block number outside the cache makes the rows that see it NaN (with lse = +inf, as
- * NaN rows have here), a length that passes the table's row all rows of its request. Nothing at or behind seq_lens counts, whatever stands there. A scale of K
- * or V that is infinite or NaN, or a negative one of V, makes the rows that see its block NaN; one of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few. Where requests have many rows, codes * scales are brought to 16
- * bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range: beyond its largest number (f16 65504; the
- * code of an element from 63488 on may be 65536) they are that number, and f16 loses what is below 2^-24, as of a cache that was filled from bf16. (A NaN among the values themselves, or a scale of V that is NaN, may reach every row of its
- * request and kv head, as 0 * NaN.) */
+ * rows of q outside every request are left unwritten. NaN (with lse = +inf, as NaN rows have here): the rows that see a block number outside the
+ * cache, or a scale of K that is infinite or NaN, and all rows of a request whose length passes the table's row. Nothing at or behind seq_lens
+ * counts, whatever stands there. A NaN among the values, or a scale of V that is negative, infinite or NaN, may reach every row of its request
+ * and kv head, as 0 * NaN. A scale of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few; there a value counts down to
+ * 2^-39 of the largest product of a weight and a scale of V in its row.
+ * Where requests have many rows, codes * scales are brought to 16 bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB
+ * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range. What is beyond its
+ * largest number is that number (f16: 65504; the code of an element from 63488 on may be 65536), and f16 loses what is below 2^-24, as of a
+ * cache that was filled from bf16. */
 SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);
 SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_params* p, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -21,7 +21,7 @@
 //    for 32 bits beside a key whose value is 2^100 times as large (in a loop of its own: within the one for all calls it cost 2 to 5%).
 //    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
-//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.1 us.
+//    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.2 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses, within the type's range), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 135 us.
@@ -45,7 +45,7 @@ constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a 
 // Sums are kept in this unit: they are up to 2^100 a token where the largest weight is that of a block of the least scale, and no less than 2^-121 where it is that of bf16's largest
 constexpr float kSumUnit = 0x1p-15f;
 // Scales of V above it are far from the least one: a weight times its scale, or what such products are multiplied by when their maximum moves, may then be too small for 32 bits
-// though the weight itself counts. Up to it, what is lost is 2^-25 of the sum.
+// though the weight itself counts. Up to it, a key that is lost has less than 2^-26 of the largest weight.
 constexpr float kFarScale = 1.f;
 
 struct StreamParams {
@@ -1303,10 +1303,9 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_attention(const sdpa_b200_cache_par
   uint32_t* status = p->device_status != nullptr ? p->device_status : static_cast<uint32_t*>(workspace);
   const bool few_rows = streams(*p);
   const int at_once = few_rows ? requests_at_once(list_of(*p)) : gathered_at_once(*p);
-  for (int first = 0; first < p->batch; first += at_once) {
-    const int count = std::min(at_once, p->batch - first);
-    st = few_rows ? launch_stream(*p, first, count, static_cast<char*>(workspace), status, s) : launch_gathered(*p, first, count, static_cast<char*>(workspace), status, s);
-    if (st != SDPA_B200_OK) return st;
+  for (int64_t first = 0; first < p->batch && st == SDPA_B200_OK; first += at_once) {
+    const int count = static_cast<int>(std::min<int64_t>(at_once, p->batch - first));
+    st = (few_rows ? launch_stream : launch_gathered)(*p, static_cast<int>(first), count, static_cast<char*>(workspace), status, s);
   }
-  return SDPA_B200_OK;
+  return st;
 }
