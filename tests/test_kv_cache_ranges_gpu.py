@@ -314,3 +314,42 @@ def test_nan_among_the_last_drafted_tokens(cuda_device, code, rows, hq):
         if which == 0:
             sees = torch.arange(640 - rows, 640, device=cuda_device) >= (639 if code == E4M3 else 576)
             assert bool(out[:rows, :group][sees].isnan().all()) and bool(out[:rows, :group][~sees].isfinite().all())
+
+
+@pytest.mark.parametrize("rows,hq,hkv", [(3, 8, 2), (40, 16, 2), (1000, 64, 8)])
+def test_offsets_that_leave_q(cuda_device, rows, hq, hkv):
+    """A step's offsets beside fewer rows of q, or offsets of less than 0: nothing is written outside out and lse, and requests whose rows are all there are as they should be."""
+    dim = 64
+    b = _batch(cuda_device, [1100, 300, 200, 70], [rows, 2, rows // 2 + 1, 1], hq, hkv, dim, 32, INT8, torch.bfloat16)
+    q, kc, vc, ks, vs, table, lens, cu = b
+    for shift, total in ((0, int(cu[3]) - 1), (0, int(cu[2])), (-1, int(cu[4])), (-(1 << 30), int(cu[4])), (5, int(cu[4])), (1 << 30, int(cu[4]))):
+        given = cu + shift
+        guard = 4096
+        out_all = torch.full((2 * guard + total * hq * dim,), 7.0, dtype=q.dtype, device=cuda_device)
+        lse_all = torch.full((2 * guard + hq * total,), 7.0, device=cuda_device)
+        out, lse = out_all[guard:-guard].view(total, hq, dim), lse_all[guard:-guard].view(hq, total)
+        p = _cabi.CacheParams()
+        p.k_cache, p.v_cache, p.k_scale, p.v_scale = (x.data_ptr() for x in (kc, vc, ks, vs))
+        for x, c in (("k", kc), ("v", vc)):
+            for f, stride in zip(("block", "head", "row"), c.stride()):
+                setattr(p, f"{x}_{f}_stride", stride)
+        p.num_blocks, p.heads_kv, p.block_size, p.head_dim = kc.shape
+        p.code, p.dtype = _cabi.CODE_INT8, _cabi.DTYPE_BF16
+        part = q[:total].contiguous()
+        p.q, p.out, p.lse, p.block_table, p.seq_lens, p.cu_seqlens_q = (t.data_ptr() for t in (part, out, lse, table, lens, given))
+        p.q_row_stride = p.o_row_stride = hq * dim
+        p.q_head_stride = p.o_head_stride = dim
+        p.table_stride, p.max_blocks, p.batch, p.total_q, p.heads_q = table.stride(0), table.size(1), 4, total, hq
+        p.max_seqlen_q, p.max_seqlen_k, p.is_causal, p.softmax_scale = max(2, rows), 1100, 1, 0.125
+        n = ctypes.c_size_t(0)
+        lib = _cabi.load()
+        assert lib.sdpa_b200_cache_attention_workspace_bytes(ctypes.byref(p), ctypes.byref(n)) == 0
+        ws = torch.full((n.value,), 255, dtype=torch.uint8, device=cuda_device)
+        assert lib.sdpa_b200_cache_attention(ctypes.byref(p), ws.data_ptr(), n.value, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        for x in (out_all, lse_all):
+            assert bool((x[:guard] == 7).all()) and bool((x[-guard:] == 7).all())
+        if shift == 0:  # those whose rows are all there
+            end = int(cu[2])
+            _compare(out[:end], lse[:, :end], (q[:end], kc, vc, ks, vs, table[:2], lens[:2], cu[:3]), many=rows > 500)
+    assert ops.device_status() == 0

@@ -854,7 +854,7 @@ struct GatherParams {
   const int32_t* block_table;
   const int32_t* seq_lens;
   int64_t table_stride;
-  int batch, heads, max_blocks, num_blocks, shift;
+  int batch, total_q, heads, max_blocks, num_blocks, shift;
   int max_k, max_len;  // tokens that a request has here at most, that a table's row holds
 };
 
@@ -895,12 +895,13 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
   for (int w = 0; w < 8; ++w) before += sums[w];
   if (blockIdx.x == 0 && h == 0 && tid == 0) {
     int32_t* cu_k = p.cu + 2 * p.batch + 1;
-    p.cu[2 * b] = p.cu_q[b];
-    p.cu[2 * b + 1] = p.cu_q[b + 1];
+    auto offset = [&](int i) { return min(max(p.cu_q[i], 0), p.total_q); };  // the prefill kernel writes where they say
+    p.cu[2 * b] = offset(b);
+    p.cu[2 * b + 1] = offset(b + 1);
     cu_k[2 * b] = before;
     cu_k[2 * b + 1] = before + len;
     if (b == p.batch - 1) {
-      p.cu[2 * p.batch] = p.cu_q[p.batch];
+      p.cu[2 * p.batch] = offset(p.batch);
       cu_k[2 * p.batch] = before + padded;
     }
   }
@@ -1198,6 +1199,7 @@ int launch_gathered(const sdpa_b200_cache_params& c, int first, int count, char*
   g.seq_lens = c.seq_lens + first;
   g.table_stride = c.table_stride;
   g.batch = count;
+  g.total_q = c.total_q;
   g.heads = c.heads_kv;
   g.max_blocks = c.max_blocks;
   g.num_blocks = c.num_blocks;
