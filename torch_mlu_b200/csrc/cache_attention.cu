@@ -19,12 +19,12 @@
 //    largest, whatever scales blocks have, and the products add up in the tensor core's fp32 accumulators without a pass over them. The sum of
 //    the softmax takes w_j / vs_j in fp32; from the first tile on that has a scale of V above 1 it takes 2^(s_j - m), another exponential, since w_j may then be too small
 //    for 32 bits beside a key whose value is 2^100 times as large (in a loop of its own: within the one for all calls it cost 2 to 5%).
-//    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 296 us, 6.42 TB/s, 98% of a
+//    Measured, one token per request, head_dim 128: 64 requests of 2048 to 32768 tokens, 8 kv heads, 1.9 GB of codes: 292 to 300 us, 6.3 to 6.5 TB/s, 97 to 99% of a
 //    copy's rate. What is small does not get there: about 4 us go by before the first tile is there, 2 to 3 in a unit's hand-over between warps,
 //    2 to 3 in the merge, and shares are whole tiles. 64 requests of 200 to 1800: 34 us, 3.7 TB/s; one of 1000, in clusters: 6.2 us.
 // 2. Many rows (chunks of prompts): the tensor cores bound it. cache_gather_kernel brings the request's codes * scales into 16-bit packed tensors
 //    in the workspace (exact with the powers of two that the store kernel chooses, within the type's range), and the prefill kernel does the rest. 512 tokens behind 7680,
-//    2 requests, 32 heads of 128: 135 us.
+//    2 requests, 32 heads of 128: 134 to 139 us.
 #include <algorithm>
 #include <type_traits>
 
