@@ -321,12 +321,14 @@ typedef struct sdpa_b200_rotary_params {
 
 SDPA_B200_API int sdpa_b200_rotary(const sdpa_b200_rotary_params* p, void* stream);
 
-/* ---- the 8-bit paged cache ---------------------------------------------------------------------------------------------
- * Keys and values live in blocks of block_size tokens: codes [num_blocks][heads_kv][block_size][head_dim], e4m3 or int8, with one
- * fp32 scale per block and head; an element is code * scale. A request's token at position p is in the block block_table[request]
+/* ---- the paged cache --------------------------------------------------------------------------------------------------
+ * Keys and values live in blocks of block_size tokens: codes [num_blocks][heads_kv][block_size][head_dim]; an element is code * scale.
+ * 8 bits: e4m3 or int8, with one fp32 scale per block and head. 4 bits: whole numbers from -8 to 7, two in a byte, the even element in the low
+ * half, with a bf16 scale for every 32 elements of a token and head, [num_blocks][heads_kv][block_size][head_dim / 32].
+ * A request's token at position p is in the block block_table[request]
  * [p / block_size], at p % block_size; that place in the cache, block * block_size + p % block_size, is called its slot. No
  * counterpart in the reference, which has no paged cache. */
-enum { SDPA_B200_E4M3 = 0, SDPA_B200_INT8 = 1 };
+enum { SDPA_B200_E4M3 = 0, SDPA_B200_INT8 = 1, SDPA_B200_INT4 = 4 };
 
 /* One serving step's bookkeeping. new_tokens[i] tokens are added to request i (negative: that many are taken back), and what it needs
  * or no longer needs of blocks moves between block_table and a ring of free ones. The ring holds ring_state[1] free blocks from index
@@ -358,12 +360,12 @@ typedef struct sdpa_b200_cache_params {
   /* codes by (block, head, token) strides in bytes, multiples of 16, head_dim contiguous; 16-byte aligned */
   void* k_cache;
   void* v_cache;
-  float* k_scale; /* [num_blocks][heads_kv]; those of V not negative */
-  float* v_scale;
+  void* k_scale; /* 8 bits: fp32 [num_blocks][heads_kv], those of V not negative; 4 bits: bf16 [num_blocks][heads_kv][block_size][head_dim / 32], 16-byte aligned */
+  void* v_scale;
   int64_t k_block_stride, k_head_stride, k_row_stride;
   int64_t v_block_stride, v_head_stride, v_row_stride;
   int32_t num_blocks, block_size, heads_kv, head_dim; /* block_size: 16, 32, 64 or 128; head_dim: 64 or 128 */
-  int32_t code;  /* SDPA_B200_E4M3 or SDPA_B200_INT8 */
+  int32_t code;  /* SDPA_B200_E4M3, SDPA_B200_INT8 or SDPA_B200_INT4 */
   int32_t dtype; /* of key, value, q, out: SDPA_B200_BF16 or SDPA_B200_F16 */
   /* store */
   const void* key; /* [num_tokens][heads_kv][head_dim] by strides in elements, multiples of 8 */
@@ -388,24 +390,39 @@ typedef struct sdpa_b200_cache_params {
   int32_t is_causal;                  /* bottom-right aligned, as everywhere here */
   float softmax_scale;
   uint32_t* device_status; /* as in sdpa_b200_params */
+  /* load */
+  void* key_out; /* [num_tokens][heads_kv][head_dim], contiguous, 16-byte aligned */
+  void* value_out;
+  const int32_t* first; /* [batch]: each request's first token; NULL: 0 */
+  const int32_t* cu_seqlens_k; /* [batch + 1]: offsets of the requests' rows of key_out and value_out */
 } sdpa_b200_cache_params;
 
-/* Puts the keys and values of a step into the cache. Every (block, head) that gets tokens has its scale raised to the smallest power of two
+/* Puts the keys and values of a step into the cache. 8 bits: every (block, head) that gets tokens has its scale raised to the smallest power of two
  * at which the largest of them is a code (448 for e4m3, 127 for int8), unless it is that large already; earlier tokens of the block are
  * rounded again to a scale that has grown. A block whose first place is written starts anew. Tokens with a negative slot, or one behind the
  * cache, are left out. The tokens of one block stand next to each other, with rising slots, as sdpa_b200_plan_step gives them (the same slot
  * twice in a row: the later token stays; fewer than 32 tokens that are left out may stand between them); a block that comes up again
  * behind tokens of another one is not allowed, since the two parts are worked on at the same time; keys and values have caches and scales of
  * their own for the same reason. A NaN or infinite element becomes NaN in e4m3; int8 has none, there the scale becomes NaN until the block
- * starts anew. */
+ * starts anew.
+ * 4 bits: every 32 elements of a token and head get the smallest scale of five significant bits, 2^-100 at least, at which the largest of them is no more than 7 (a code times
+ * such a scale is exact in 16 bits within the type's range); the code is the nearest whole number, the even one of two. A scale depends on nothing but its 32 elements. With a
+ * NaN or infinite one among them it is NaN and the codes are 0. */
 SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* stream);
+
+/* key_out, value_out <- tokens of the requests: row cu_seqlens_k[b] + i is token first[b] + i of request b, found through block_table, max_blocks blocks a row. code * scale
+ * is rounded once to dtype; what is beyond its largest number is that number. NaN: a token in front of 0 or behind the table's row, a block number outside the cache, an
+ * infinite or NaN scale. Rows in front of cu_seqlens_k[0] and behind the last request are filled with zeros. Offsets that fall, or leave the outputs, write nothing outside
+ * them; a row that several requests claim belongs to one of them. */
+SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* p, void* stream);
 
 /* out, lse <- attention of each request's last rows of q over its tokens in the cache. A row without a visible key gets out = 0 and lse = +inf;
  * rows of q outside every request are left unwritten. NaN (with lse = +inf, as NaN rows have here): the rows that see a block number outside the
  * cache, or a scale of K that is infinite or NaN, and all rows of a request whose length passes the table's row. Nothing at or behind seq_lens
  * counts, whatever stands there. A NaN among the values, or a scale of V that is negative, infinite or NaN, may reach every row of its request
  * and kv head, as 0 * NaN. A scale of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few; there a value counts down to
- * 2^-39 of the largest product of a weight and a scale of V in its row.
+ * 2^-39 of the largest product of a weight and a scale of V in its row. In a 4-bit cache scales of V may be negative, and a scale of K or V that is infinite or NaN reaches
+ * only the rows that see its token.
  * Where requests have many rows, codes * scales are brought to 16 bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB
  * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range. What is beyond its
  * largest number is that number (f16: 65504; the code of an element from 63488 on may be 65536), and f16 loses what is below 2^-24, as of a

@@ -1,4 +1,4 @@
-"""Plain restatements, in 64 bits and request by request, of the serving operators: bookkeeping of a step, the 8-bit paged cache, attention over it,
+"""Plain restatements, in 64 bits and request by request, of the serving operators: bookkeeping of a step, the paged cache, attention over it,
 rotary positions. Test infrastructure only."""
 import math
 
@@ -89,11 +89,69 @@ def store(x, slots, codes, scales):
     return values, scales
 
 
+def store4(x, slots, codes, scales):
+    """(whole numbers [blocks, heads, block, dim], scales [blocks, heads, block, dim / 32]), fp64, after tokens x [tokens, heads, dim] went to `slots` of a 4-bit cache."""
+    size = codes.shape[2]
+    values, scales, x = numbers4(codes.cpu()).double(), scales.cpu().double().clone(), x.cpu().double()
+    allowed = torch.tensor([m * 2.0 ** -4 for m in range(16, 32)], dtype=torch.float64)  # five significant bits
+    for t, slot in enumerate(slots.tolist()):
+        if not 0 <= slot < codes.shape[0] * size:
+            continue
+        groups = x[t].reshape(x.shape[1], -1, 32)
+        for h in range(x.shape[1]):
+            for g, part in enumerate(groups[h]):
+                at = (slot // size, h, slot % size)
+                if not bool(part.isfinite().all()):
+                    scales[at][g] = math.nan
+                    values[at][32 * g:32 * g + 32] = 0
+                    continue
+                most, scale = float(part.abs().max()), 2.0 ** -100
+                if most > 7 * scale:
+                    unit = 2.0 ** math.floor(math.log2(most / 7))
+                    fits = [float(a) * u for u in (unit / 2, unit, 2 * unit) for a in allowed if 7 * float(a) * u >= most]
+                    scale = min(fits)
+                scales[at][g] = scale
+                values[at][32 * g:32 * g + 32] = torch.round(part / scale)
+    return values, scales
+
+
+def numbers4(codes):
+    """What bytes [..., n] of a 4-bit cache hold: [..., 2n] int8."""
+    x = codes.to(torch.int16)
+    x = torch.stack([x % 16, x // 16], -1).flatten(-2)
+    return torch.where(x > 7, x - 16, x).to(torch.int8)
+
+
+def elements(codes, scales):
+    """The elements of a cache's blocks, fp64, and whether each is one: a scale that is infinite makes NaN."""
+    scales = torch.where(scales.double().isinf(), math.nan, scales.double())
+    if codes.dtype == torch.uint8:
+        return numbers4(codes).double() * scales.repeat_interleave(32, -1)
+    return codes.view(torch.uint8).view(codes.dtype).double() * scales[:, :, None, None]
+
+
+def load(key_cache, value_cache, key_scale, value_scale, table, cu, num_tokens, first=None):
+    """(keys, values) [num_tokens, heads, dim] in 64 bits."""
+    S, outs = key_cache.shape[2], []
+    for codes, scales in ((key_cache, key_scale), (value_cache, value_scale)):
+        x = elements(codes, scales)
+        out = torch.zeros(num_tokens, x.shape[1], x.shape[3], dtype=torch.float64, device=x.device)
+        for b in range(table.shape[0]):
+            lo = 0 if first is None else int(first[b])
+            for i, row in enumerate(range(int(cu[b]), int(cu[b + 1]))):
+                token = lo + i
+                block = int(table[b, token // S]) if 0 <= token < table.shape[1] * S else -1
+                out[row] = x[block, :, token % S] if 0 <= block < codes.shape[0] else math.nan
+        outs.append(out)
+    return outs
+
+
 def attention(q, key_cache, value_cache, key_scale, value_scale, table, seq_lens, cu, causal=True, scale=None):
     """(out [tokens, heads, dim], lse [heads, tokens], mean |v| by the weights [tokens, heads, dim], largest |score| [heads, tokens]) in 64 bits; NaN where nothing is written."""
     T, Hq, D = q.shape
     H, S = key_cache.shape[1], key_cache.shape[2]
     scale = D ** -0.5 if scale is None else scale
+    four = key_cache.dtype == torch.uint8
     out = torch.full((T, Hq, D), math.nan, dtype=torch.float64, device=q.device)
     size = out.clone()
     lse = torch.full((Hq, T), math.nan, dtype=torch.float64, device=q.device)
@@ -106,9 +164,12 @@ def attention(q, key_cache, value_cache, key_scale, value_scale, table, seq_lens
         bad = (ids < 0) | (ids >= key_cache.shape[0])
         ids = torch.where(bad, 0, ids)
         # a block outside the cache: its scores are NaN, its values 0
-        whole = lambda c, s, spoilt: torch.where(bad[:, None, None, None], spoilt, c.view(torch.uint8)[ids].view(c.dtype).double() * s[ids].double()[:, :, None, None]
-                                                 ).permute(1, 0, 2, 3).reshape(H, -1, D)[:, :n]
+        of = lambda c, s: elements(c.view(torch.uint8)[ids].view(c.dtype), s[ids]) if four else c.view(torch.uint8)[ids].view(c.dtype).double() * s[ids].double()[:, :, None, None]
+        whole = lambda c, s, spoilt: torch.where(bad[:, None, None, None], spoilt, of(c, s)).permute(1, 0, 2, 3).reshape(H, -1, D)[:, :n]
         k, v = whole(key_cache, key_scale, math.nan), whole(value_cache, value_scale, 0.0)
+        if four:  # a token with a value that is NaN: who sees it is NaN, who does not is not
+            spoilt = v.isnan().any(-1, keepdim=True)
+            k, v = torch.where(spoilt, math.nan, k), torch.where(v.isnan(), 0, v)
         rows = q[lo:hi].double().permute(1, 0, 2).reshape(H, Hq // H, hi - lo, D)
         s = torch.einsum("hgmd,hnd->hgmn", rows, k) * scale
         seen = torch.ones(hi - lo, n, dtype=torch.bool, device=q.device)

@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libsdpa_b200.so")
 OK, INVALID_ARG, UNSUPPORTED, LAUNCH_FAILED, DEVICE_TIMEOUT, NO_DEVICE = range(6)
 KERNEL_AUTO, KERNEL_PREFILL, KERNEL_DECODE = 0, 1, 2
 DTYPE_BF16, DTYPE_F16 = 0, 1
-CODE_E4M3, CODE_INT8 = 0, 1
+CODE_E4M3, CODE_INT8, CODE_INT4 = 0, 1, 4
 
 # every symbol include/sdpa_b200.h declares
 EXPORTED_SYMBOLS = (
@@ -41,6 +41,7 @@ EXPORTED_SYMBOLS = (
     "sdpa_b200_rotary",
     "sdpa_b200_plan_step",
     "sdpa_b200_cache_store",
+    "sdpa_b200_cache_load",
     "sdpa_b200_cache_attention_workspace_bytes",
     "sdpa_b200_cache_attention",
     "sdpa_b200_launch_count",
@@ -115,6 +116,7 @@ class CacheParams(ctypes.Structure):
         ("block_table", c_void_p), ("seq_lens", c_void_p), ("cu_seqlens_q", c_void_p), ("table_stride", c_int64),
         ("max_blocks", c_int32), ("heads_q", c_int32), ("total_q", c_int32), ("max_seqlen_q", c_int32), ("max_seqlen_k", c_int32),
         ("is_causal", c_int32), ("softmax_scale", c_float), ("device_status", c_void_p),
+        ("key_out", c_void_p), ("value_out", c_void_p), ("first", c_void_p), ("cu_seqlens_k", c_void_p),
     ]
 
 
@@ -182,7 +184,8 @@ def load() -> ctypes.CDLL:
     lib.sdpa_b200_sum_bias_grad.restype = c_int
     lib.sdpa_b200_sum_bias_grad.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                             c_int32, c_void_p]
-    for name, struct in (("sdpa_b200_rotary", RotaryParams), ("sdpa_b200_plan_step", PlanParams), ("sdpa_b200_cache_store", CacheParams)):
+    for name, struct in (("sdpa_b200_rotary", RotaryParams), ("sdpa_b200_plan_step", PlanParams), ("sdpa_b200_cache_store", CacheParams),
+                         ("sdpa_b200_cache_load", CacheParams)):
         fn = getattr(lib, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(struct), c_void_p]

@@ -19,7 +19,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 SOURCES = ["sdpa_api.cu", "fwd_prefill_sm100.cu", "decode_splitkv.cu", "bwd_sm100.cu", "bwd_fused_sm100.cu", "bwd_ds_gemm_sm100.cu",
            "merge_partials.cu", "dropout_mask.cu", "bias_transpose.cu", "d256_sm100.cu", "rotary.cu", "cache_plan.cu", "cache_store.cu",
-           "cache_attention.cu"]
+           "cache_attention.cu", "cache4_store.cu", "cache4_attention.cu", "cache_load.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",

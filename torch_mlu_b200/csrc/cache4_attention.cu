@@ -1,0 +1,748 @@
+// Attention of few rows per request over the 4-bit paged cache: the kernel behind cache_attention.cu's list of tiles. No counterpart in the reference, which has no paged cache.
+//
+//   s_ij = scale * sum_g ks[j, g] <q_ig, kc_jg>,  out_id = sum_j softmax_j(s_i) * vs[j, g(d)] * vc_jd
+//
+// over groups g of 32 dimensions, each with a bf16 scale of its own for every token and kv head; codes are whole numbers from -8 to 7. Units, shares, ring of tiles, loading warps and
+// the merge are those of the 8-bit kernel (cache_attention.cu); what differs is what a byte costs: with 4.5 bits an element, twice the products and conversions per byte that
+// comes out of HBM. So:
+// * Codes of K become f16 with one AND-XOR each two: the low bits of a 16-bit word are the f16 subnormal u * 2^-24, u = code + 8, of the even nibbles, those of the odd
+//   ones 16 times that, for which Q is divided by 16. The 8 comes off in the accumulators, which begin with -8 * 2^-24 * sum of the group's q instead of 0: u is small, so
+//   that the sums lose three of fp32's bits to it.
+// * The scale of K goes onto the group's fp32 sums: 4 multiply-adds for each 32 x 16 codes a warp converts, where scaling the codes would take 8.
+// * Codes of V become whole f16 numbers (0x6400 | u is 1024 + u): sums over tens of thousands of tokens would lose too much to an offset.
+// * The scale of V is taken apart: 2^e, the power of two above the token's largest, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
+//   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of the token's largest has its products' full 11 bits only where the weight is that much above
+//   the smallest normal one.
+// * The loading warps bring the scales into these forms once for all, a tile ahead: fp32 of K's, e, 2^-e and the rests of V's, NaN where a scale is no finite number, zeros behind the
+//   last token, whose codes (any byte is a finite number) therefore need no mask.
+#include <type_traits>
+
+#include "cache_stream.cuh"
+
+namespace sdpa_b200 {
+namespace {
+
+constexpr float kBias = 14.f;      // weights are kept times 2^14: times the rest of V's scale they fit f16
+constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
+constexpr int kFarExponents = 100;   // e of two tokens that are further apart: the smaller one's weight may not fit 32 bits though it counts
+
+template <int kD>
+__host__ __device__ constexpr int tile_tokens() { return kD == 64 ? 256 : 128; }
+template <int kD>
+__host__ __device__ constexpr int step_tokens() { return kD == 64 ? 64 : 32; }
+template <int kD>
+__host__ __device__ constexpr uint32_t stage_bytes() { return tile_tokens<kD>() * kD; }  // codes of K and of V
+// fp32 scales of K, e and 2^-e of each token's V, the rests by pairs of tokens, whether exponents are far apart
+template <int kD>
+__host__ __device__ constexpr uint32_t scale_bytes() { return tile_tokens<kD>() * (kD / 32 * 4 + 8 + kD / 32 * 2) + 16; }
+// B fragments of Q: in registers where there is room; else in shared memory, with their sums
+template <int kRowBlocks, int kD>
+__host__ __device__ constexpr bool q_in_registers() { return kRowBlocks == 1 || kD == 64; }
+template <int kRowBlocks, int kRowWarps, int kD>
+__host__ __device__ constexpr uint32_t q_bytes() { return q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 32) * (512 + 32); }
+template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
+__host__ __device__ constexpr uint32_t smem_bytes(int stages) {
+  return 1024 + stages * (stage_bytes<kD>() + scale_bytes<kD>() + 16) + 16 + kWarps * 8 * 8 + q_bytes<kRowBlocks, kRowWarps, kD>() +
+         (kCluster ? 32 + 8 * kRowBlocks * (kD + 1) * 4 : 0);
+}
+// Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB
+template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
+__host__ __device__ constexpr int ring_stages() {
+  int n = 5;
+  while (kCtasPerSm * (smem_bytes<kRowBlocks, kRowWarps, kD, kCluster>(n) + 1024) > 228 * 1024) --n;
+  return n;
+}
+
+// Eight codes as f16 pairs (n, n + 4), n = 0..3: u * 2^-24 for even n, 16 times that for odd n, u = code + 8
+__device__ __forceinline__ void codes_to_subnormal(uint32_t w, uint32_t (&x)[4]) {
+  const uint32_t v = w >> 8;
+  x[0] = (w & 0x000f000fu) ^ 0x00080008u;
+  x[1] = (w & 0x00f000f0u) ^ 0x00800080u;
+  x[2] = (v & 0x000f000fu) ^ 0x00080008u;
+  x[3] = (v & 0x00f000f0u) ^ 0x00800080u;
+}
+// The same as the codes' values: 0x6400 | u is 1024 + u, with 16 u in its place 64 times 16 + u / 4
+__device__ __forceinline__ void codes_to_numbers(uint32_t w, uint32_t (&x)[4]) {
+  const uint32_t v = w >> 8;
+  auto low = [](uint32_t y) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((y & 0x000f000fu) ^ 0x64086408u), "r"(0x64086408u));  // - 1032
+    return r;
+  };
+  auto high = [](uint32_t y) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"((y & 0x00f000f0u) ^ 0x64806480u), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
+    return r;
+  };
+  x[0] = low(w);
+  x[1] = high(w);
+  x[2] = low(v);
+  x[3] = high(v);
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
+template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
+  constexpr int kGroups = kD / 32;
+  constexpr int kChunks = kD / 16;                           // of 16 dimensions, an MMA each
+  constexpr int kRowBytes = kD / 2;
+  constexpr int kSt = ring_stages<kRowBlocks, kRowWarps, kD, kCluster>();
+  constexpr bool kQInRegisters = q_in_registers<kRowBlocks, kD>();
+  constexpr uint32_t kStageBytes = stage_bytes<kD>();
+  constexpr int kParts = kWarps / kRowWarps;                 // of a tile's tokens
+  constexpr int kTileTokens = tile_tokens<kD>(), kStepTokens = step_tokens<kD>(), kHalves = kStepTokens / 16;
+  constexpr int kPartTokens = kTileTokens / kParts;
+  constexpr int kRowsOfWarp = 8 * kRowBlocks;
+  constexpr int kState = kChunks * 4 * 32;                   // floats of a warp's accumulators, of 8 rows
+  static_assert(kWarps * kState * 4 <= kStageBytes, "the warps' states do not fit a tile's place");
+  static_assert(kSt >= 3, "too few tiles under way");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t ring = (raw_addr + 1023u) & ~1023u;
+  uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
+  float* k_scales = reinterpret_cast<float*>(ring_ptr + kSt * kStageBytes);             // [stage][token][group]
+  float2* v_tokens = reinterpret_cast<float2*>(k_scales + kSt * kTileTokens * kGroups);  // [stage][token]: e of its scales, kSumUnit * 2^-e
+  uint32_t* v_rests = reinterpret_cast<uint32_t*>(v_tokens + kSt * kTileTokens);         // [stage][pair of tokens][group]: f16 scales over 2^e
+  uint4* stage_far = reinterpret_cast<uint4*>(v_rests + kSt * kTileTokens / 2 * kGroups);  // [stage]
+  float2* row_state = reinterpret_cast<float2*>(stage_far + kSt);                         // [warp][row of 8]: maximum and sum
+  uint4* q_state = reinterpret_cast<uint4*>(row_state + kWarps * 8);                      // [row group][block of 8 rows][group][lane]: B fragments
+  constexpr int kQWords = kQInRegisters ? 0 : kRowWarps * kRowBlocks * kGroups * 32;
+  float2* q_sums = reinterpret_cast<float2*>(q_state + kQWords);                           // [row group][block of 8 rows][group][t]
+  const uint32_t full = smem_u32(q_sums + kQWords / 8), empty = full + 8 * kSt;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(q_sums + kQWords / 8) + 2 * kSt);
+
+  // kCluster: this CTA's part of the unit
+  float* own_part = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(abort_flag) + 4 + 15) & ~static_cast<uintptr_t>(15));  // [row][dimension]
+  float* own_lse = own_part + kRowsOfWarp * kD;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (kCluster && threadIdx.x < kRowsOfWarp) own_lse[threadIdx.x] = -INFINITY;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(full + 8 * i, 2);
+      mbar_init(empty + 8 * i, kWarps);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp >= kWarps && elect_one()) tma_prefetch_desc(warp == kWarps ? &tm_k : &tm_v);
+  __syncthreads();
+  wait_for_previous_grid();
+  if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
+  const Share share = kCluster ? share_in_cluster(p, blockIdx.x) : share_of(p, blockIdx.x, lane);
+  if (share.places > 0 && warp >= kWarps) {
+    // ================================================================ the loading warps, one for K and one for V
+    // Lane i has page 32 * group + i of a unit: its block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page). Three groups are under
+    // way: the one that tiles are copied from, the next, and the one behind. Scales come a tile ahead, those of two neighbouring tokens (never of two pages) a load.
+    const bool keys = warp == kWarps;
+    const CUtensorMap* map = keys ? &tm_k : &tm_v;
+    const uint16_t* scales = static_cast<const uint16_t*>(keys ? p.k_scale : p.v_scale);
+    struct Place {
+      Request r;
+      int unit, group, head;
+    };
+    auto advance = [&](Place& x) {
+      if (static_cast<int64_t>((x.group + 1) * 32) << p.shift < x.r.len) {
+        ++x.group;
+      } else {
+        x.group = 0;
+        if (x.r.units > 0) next_unit(p, x.r, x.unit);
+        x.head = x.unit % p.heads_kv;
+      }
+    };
+    auto block_at = [&](const Place& x) {
+      const int page = x.group * 32 + lane;
+      if ((static_cast<int64_t>(page) << p.shift) >= x.r.len) return -1;
+      const int id = page < p.max_blocks && !longer_than_table(x.r) ? p.block_table[x.r.index * p.table_stride + page] : -1;
+      return id >= 0 && id < p.num_blocks ? id : p.num_blocks;
+    };
+    constexpr int kTimes = kTileTokens / 64;  // pairs of tokens of a lane
+    using Pair = std::conditional_t<kD == 128, uint4, uint2>;
+    struct Raw {
+      Pair pair[kTimes];
+    };
+    // bf16 scales of the pairs lane, lane + 32, ... of the tile whose first page is lane page0's
+    auto load_scales = [&](Raw& raw, int page0, int ids, int head) {
+#pragma unroll
+      for (int i = 0; i < kTimes; ++i) {
+        const int tok = 2 * (lane + 32 * i), id = __shfl_sync(0xffffffffu, ids, (page0 + (tok >> p.shift)) & 31);
+        const uint32_t none = keys && id == p.num_blocks ? 0x7fc07fc0u : 0u;  // no such block: the scores of those who see it are NaN
+        if constexpr (kD == 128) raw.pair[i] = make_uint4(none, none, none, none);
+        else raw.pair[i] = make_uint2(none, none);
+        if (id >= 0 && id < p.num_blocks)
+          raw.pair[i] = *reinterpret_cast<const Pair*>(scales + (((static_cast<int64_t>(id) * p.heads_kv + head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups);
+      }
+    };
+    Place cur, nxt, far;
+    cur.r = share.request;
+    cur.unit = share.unit;
+    cur.head = cur.unit % p.heads_kv;
+    int tile = share.tile;
+    cur.group = ((tile * kTileTokens) >> p.shift) >> 5;
+    nxt = far = cur;
+    int id = block_at(cur), next_id = -1, far_id = -1;
+    auto next_group = [&]() {
+      cur = nxt, id = next_id;
+      nxt = far, next_id = far_id;
+      advance(far);
+      far_id = block_at(far);
+    };
+    const int pages = kTileTokens >> p.shift;  // of a tile
+    bool ok = true, far_apart = false;
+    int least_e = 1000, largest_e = -1000;     // of V's scales so far
+    int step = 0;
+    bool first = true;
+    Raw raw, ahead;
+    for (int places = share.places; places > 0;) {
+      const int page0 = (tile * kTileTokens) >> p.shift;
+      if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
+      const int tile_tok = tile * kTileTokens;
+      const bool tokens = tile_tok < cur.r.len;
+      const uint32_t st = step % kSt, bar = full + 8 * st;
+      if (first) load_scales(raw, page0, id, cur.head);
+      if (tokens) {
+        const uint32_t dst = ring + st * kStageBytes + (keys ? 0u : kTileTokens * kRowBytes);
+        if (ok && step >= kSt) ok = mbar_wait(empty + 8 * st, (step / kSt + 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int mine = __shfl_sync(0xffffffffu, id, ((page0 & 31) + lane) & 31);
+        const int n = __popc(__ballot_sync(0xffffffffu, lane < pages && mine >= 0));
+        if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(n << p.shift) * kRowBytes);
+#pragma unroll 1
+        for (int i = 0; i < n; i += 4) {
+          int blocks[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, mine, (i + e) & 31);
+          if (elect_one()) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e < n) tma_load_4d(dst + ((i + e) << p.shift) * kRowBytes, map, bar, 0, 0, cur.head, blocks[e]);
+          }
+        }
+      }
+      if (first) {  // the first copies are under way
+        advance(nxt);
+        next_id = block_at(nxt);
+        far = nxt;
+        advance(far);
+        far_id = block_at(far);
+        first = false;
+      }
+      {  // the next tile's scales: it is the unit's next, in this group or the next one, or the first of the unit behind
+        const int next_page0 = ((tile + 1) * kTileTokens) >> p.shift;
+        const bool more = tile + 1 < cur.r.tiles, here = more && next_page0 >> 5 == cur.group;
+        load_scales(ahead, more ? next_page0 : 0, here ? id : next_id, here ? cur.head : nxt.head);
+      }
+      if (tokens) {
+#pragma unroll
+        for (int i = 0; i < kTimes; ++i) {
+          const int pair = lane + 32 * i;
+          uint32_t words[kGroups];  // the first token's, then the second's
+          words[0] = raw.pair[i].x, words[1] = raw.pair[i].y;
+          if constexpr (kD == 128) words[2] = raw.pair[i].z, words[3] = raw.pair[i].w;
+          if (keys) {
+            float f[2 * kGroups];
+#pragma unroll
+            for (int e = 0; e < kGroups; ++e) {
+              f[2 * e] = __uint_as_float(words[e] << 16);
+              f[2 * e + 1] = __uint_as_float(words[e] & 0xffff0000u);
+            }
+#pragma unroll
+            for (int e = 0; e < 2 * kGroups; ++e)
+              if (fabsf(f[e]) == INFINITY) f[e] = __int_as_float(0x7fffffff);
+            float4* dst = reinterpret_cast<float4*>(k_scales + (st * kTileTokens + 2 * pair) * kGroups);
+#pragma unroll
+            for (int e = 0; e < kGroups / 2; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          } else {
+            float2 of_token[2];
+            uint32_t rests[kGroups] = {};
+#pragma unroll
+            for (int tok = 0; tok < 2; ++tok) {
+              const bool there = tile_tok + 2 * pair + tok < cur.r.len;
+              uint32_t bits[kGroups], top = 0u;
+#pragma unroll
+              for (int e = 0; e < kGroups; ++e) {
+                const uint32_t w = words[tok * kGroups / 2 + e / 2];
+                bits[e] = there ? e & 1 ? w >> 16 : w & 0xffffu : 0u;
+                top = max(top, bits[e] & 0x7fffu);
+              }
+              const bool bad = top >= 0x7f80u;
+              if (bad) top = 0u;
+              const int e2 = top == 0u ? 0 : min(max(static_cast<int>(top >> 7) - 126, kLeastExponent), 126);
+              if (top != 0u) {
+                least_e = min(least_e, e2);
+                largest_e = max(largest_e, e2);
+              }
+              const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);  // 2^-e
+              of_token[tok] = make_float2(bad ? __int_as_float(0x7fffffff) : static_cast<float>(e2), kSumUnit * down);
+#pragma unroll
+              for (int e = 0; e < kGroups; ++e) {
+                const uint32_t h = pack_f16x2(bad ? 0.f : __uint_as_float(bits[e] << 16) * down, 0.f) & 0xffffu;
+                rests[e] |= tok ? h << 16 : h;
+              }
+            }
+            *reinterpret_cast<float4*>(v_tokens + st * kTileTokens + 2 * pair) = make_float4(of_token[0].x, of_token[0].y, of_token[1].x, of_token[1].y);
+            uint32_t* dst = v_rests + (st * (kTileTokens / 2) + pair) * kGroups;
+            if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(rests[0], rests[1], rests[2], rests[3]);
+            else *reinterpret_cast<uint2*>(dst) = make_uint2(rests[0], rests[1]);
+          }
+        }
+        if (!keys) {
+          least_e = __reduce_min_sync(0xffffffffu, least_e);
+          largest_e = __reduce_max_sync(0xffffffffu, largest_e);
+          far_apart = far_apart || largest_e - least_e > kFarExponents;
+          if (lane == 0) stage_far[st].x = far_apart;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        ++step;
+      }
+      raw = ahead;
+      --places;
+      if (++tile == cur.r.tiles) {
+        tile = 0;
+        places -= share.pause;
+        next_group();
+      }
+    }
+  }
+
+  SharedUnit left = {-1, 0, 0, 0, 0, 0};
+  if (share.places > 0 && warp < kWarps) {
+    // ================================================================ the arithmetic. Fragments: a thread has rows 2t and 2t + 1 of every 8
+    const int g = lane >> 2;
+    const int t = lane & 3;
+    const int row_group = warp / kParts, part = warp % kParts;
+    const int mrow = lane & 7, mat = lane >> 3;
+    auto chunk_at = [&](int row, int chunk) -> uint32_t {  // byte offset of a 16-byte chunk (32 dimensions) of a row in a swizzled tile
+      if constexpr (kD == 128) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+      return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
+    };
+    bool ok = true;
+    int step = 0;  // tiles read
+    Request r = share.request;
+    int unit = share.unit, tile = share.tile;
+    Request next_r = r;
+    int next = unit;  // the unit behind
+    bool first_unit = true;
+    for (int places = share.places; places > 0;) {
+      const int seg_tiles = min(places, r.tiles - tile);
+      places -= seg_tiles + share.pause;
+      const int row0 = unit / p.heads_kv * p.rows, head = unit - unit / p.heads_kv * p.heads_kv;
+      const int n_rows = min(p.rows, r.rows_q * p.group - row0);
+      const int my_row0 = row0 + kRowsOfWarp * row_group;
+      // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 8t..8t+7 of every 32: pairs (n, n + 4), those of odd n over 16
+      uint4 qb[kRowBlocks][kQInRegisters ? kGroups : 1];
+      float2 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit
+      uint4* my_q = q_state + row_group * kRowBlocks * kGroups * 32 + lane;
+      float2* my_sums = q_sums + row_group * kRowBlocks * kGroups * 4;
+      float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale and the 2^24 that the products lack
+      int2 limit[kRowBlocks];     // how many tokens they see
+      bool huge = false;          // queries whose factor has no room for the 2^24: the scores take it
+#pragma unroll
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        const int row = my_row0 + 8 * nb + g, i = row / p.group;
+        const bool have = row < row0 + n_rows;
+        const uint16_t* src = p.q + (r.q0 + i) * p.q_row + (head * p.group + row - i * p.group) * p.q_head + 8 * t;
+        uint4 w[kGroups];
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) w[k] = have ? *reinterpret_cast<const uint4*>(src + 32 * k) : make_uint4(0u, 0u, 0u, 0u);
+        auto floats = [&](const uint4& q, float (&x)[8]) {
+          const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = p.f16 ? unpack_16x2<true>(words[e]) : unpack_16x2<false>(words[e]);
+            x[2 * e] = f.x, x[2 * e + 1] = f.y;
+          }
+        };
+        float largest = 0.f;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          float x[8];
+          floats(w[k], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[e]));
+        }
+        largest = quad_max(largest);
+        const int e2 = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -100), 127);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e2) << 23);
+        const float down = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e2) << 23);
+        huge = huge || e2 > 90;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          float x[8];
+          floats(w[k], x);
+          const float odd = up * 0.0625f;
+          const uint4 packed = make_uint4(pack_f16x2(x[0] * up, x[4] * up), pack_f16x2(x[1] * odd, x[5] * odd), pack_f16x2(x[2] * up, x[6] * up),
+                                          pack_f16x2(x[3] * odd, x[7] * odd));
+          const float2 a = unpack_16x2<true>(packed.x), b = unpack_16x2<true>(packed.y), c = unpack_16x2<true>(packed.z), d = unpack_16x2<true>(packed.w);
+          float sum = (a.x + a.y + c.x + c.y) + 16.f * (b.x + b.y + d.x + d.y);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          sum *= -0x1p-21f;
+          const float2 sums = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
+          if constexpr (kQInRegisters) {
+            qb[nb][k] = packed;
+            qs[nb][k] = sums;
+          } else if (part == 0) {
+            my_q[(nb * kGroups + k) * 32] = packed;
+            if (g == 0) my_sums[(nb * kGroups + k) * 4 + t] = sums;
+          }
+        }
+        const int sees = p.causal ? min(r.len, i + 1 + r.in_front) : r.len;
+        factor[nb] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
+        limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
+      }
+      huge = __any_sync(0xffffffffu, huge);
+      if (!huge) {
+#pragma unroll
+        for (int nb = 0; nb < kRowBlocks; ++nb) factor[nb] = make_float2(factor[nb].x * 0x1p24f, factor[nb].y * 0x1p24f);
+      }
+      if constexpr (!kQInRegisters) arithmetic_sync();
+      if (places > 0) {  // where the next unit's rows of Q are: they come nearer while this one's tiles are worked on
+        next_unit(p, next_r, next);
+        const int next_row0 = next / p.heads_kv * p.rows + kRowsOfWarp * row_group;
+#pragma unroll
+        for (int nb = 0; nb < kRowBlocks; ++nb) {
+          const int row = next_row0 + 8 * nb + g, i = row / p.group;
+          if (t * 64 < kD && row < next_r.rows_q * p.group)
+            prefetch_l1(p.q + (next_r.q0 + i) * p.q_row + ((next - next / p.heads_kv * p.heads_kv) * p.group + row - i * p.group) * p.q_head + 64 * t);
+        }
+      }
+      // tokens that all of the warp's rows see, and those that any of them does
+      const int last_row = min(my_row0 + kRowsOfWarp - 1, row0 + n_rows - 1);
+      const int seen_by_all = p.causal ? min(r.len, my_row0 / p.group + 1 + r.in_front) : r.len;
+      const int seen_by_any = my_row0 >= row0 + n_rows ? 0 : p.causal ? min(r.len, last_row / p.group + 1 + r.in_front) : r.len;
+
+      float o[kRowBlocks][kChunks][4];  // [2c + j]: dimensions 32c + 4g + 2j, the same, the next, the next; rows 2t, 2t + 1, 2t, 2t + 1
+      float2 m[kRowBlocks], l[kRowBlocks];  // running maximum of score + e; this thread's share of the sums, in units of kSumUnit
+#pragma unroll
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        m[nb] = make_float2(-INFINITY, -INFINITY);
+        l[nb] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) o[nb][ch][0] = o[nb][ch][1] = o[nb][ch][2] = o[nb][ch][3] = 0.f;
+      }
+
+      for (int i = 0; i < seg_tiles; ++i) {
+        const int tile_tok = (tile + i) * kTileTokens;
+        if (tile_tok >= r.len) break;  // a request without tokens
+        const uint32_t st = step % kSt;
+        if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        __syncwarp();
+        auto work_on = [&](int c, auto far_tag) {
+          constexpr bool kFar = decltype(far_tag)::value;
+          const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
+          // ---- S^T = K Q^T, 16 tokens and 32 dimensions at a time
+          // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
+          const uint32_t k_smem = ring + st * kStageBytes + in_tile * kRowBytes;
+          const float* ks = k_scales + (st * kTileTokens + in_tile + g) * kGroups;
+          float s[kRowBlocks][kHalves][4];
+#pragma unroll
+          for (int ch = 0; ch < kGroups; ch += 2) {
+            uint4 q[2][kRowBlocks];
+            float2 begin[2][kRowBlocks];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int nb = 0; nb < kRowBlocks; ++nb) {
+                if constexpr (kQInRegisters) {
+                  q[e][nb] = qb[nb][ch + e];
+                  begin[e][nb] = qs[nb][ch + e];
+                } else {
+                  q[e][nb] = my_q[(nb * kGroups + ch + e) * 32];
+                  begin[e][nb] = my_sums[(nb * kGroups + ch + e) * 4 + t];
+                }
+              }
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              uint32_t kf[4];  // tokens 0-7 and 8-15 of a group, the same of the next
+              ldmatrix_x4(k_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), kf);
+              const float2 near = *reinterpret_cast<const float2*>(ks + half * 16 * kGroups + ch), behind = *reinterpret_cast<const float2*>(ks + (half * 16 + 8) * kGroups + ch);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t x[4], y[4];
+                codes_to_subnormal(kf[2 * e], x);
+                codes_to_subnormal(kf[2 * e + 1], y);
+                const float kg = e ? near.y : near.x, kg8 = e ? behind.y : behind.x;
+#pragma unroll
+                for (int nb = 0; nb < kRowBlocks; ++nb) {
+                  float a[4] = {begin[e][nb].x, begin[e][nb].y, begin[e][nb].x, begin[e][nb].y};
+                  mma_16816<true>(a, x[0], y[0], x[1], y[1], q[e][nb].x, q[e][nb].y);
+                  mma_16816<true>(a, x[2], y[2], x[3], y[3], q[e][nb].z, q[e][nb].w);
+                  if (ch + e == 0) {
+                    s[nb][half][0] = a[0] * kg, s[nb][half][1] = a[1] * kg, s[nb][half][2] = a[2] * kg8, s[nb][half][3] = a[3] * kg8;
+                  } else {
+                    s[nb][half][0] = fmaf(a[0], kg, s[nb][half][0]), s[nb][half][1] = fmaf(a[1], kg, s[nb][half][1]);
+                    s[nb][half][2] = fmaf(a[2], kg8, s[nb][half][2]), s[nb][half][3] = fmaf(a[3], kg8, s[nb][half][3]);
+                  }
+                }
+              }
+            }
+          }
+          if (huge) {
+#pragma unroll
+            for (int nb = 0; nb < kRowBlocks; ++nb)
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nb][half][e] *= 0x1p24f;
+          }
+          float2 near[kHalves], behind[kHalves];  // e and kSumUnit * 2^-e of tokens g, g + 8
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+            near[half] = v_tokens[st * kTileTokens + in_tile + half * 16 + g];
+            behind[half] = v_tokens[st * kTileTokens + in_tile + half * 16 + 8 + g];
+          }
+          uint32_t pb[kRowBlocks][kHalves][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
+          bool moved = false;
+          float2 a[kRowBlocks];
+#pragma unroll
+          for (int nb = 0; nb < kRowBlocks; ++nb) {
+            // scores and e, masked where a row ends inside the step
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              s[nb][half][0] = fmaf(s[nb][half][0], factor[nb].x, near[half].x);
+              s[nb][half][1] = fmaf(s[nb][half][1], factor[nb].y, near[half].x);
+              s[nb][half][2] = fmaf(s[nb][half][2], factor[nb].x, behind[half].x);
+              s[nb][half][3] = fmaf(s[nb][half][3], factor[nb].y, behind[half].x);
+            }
+            if (tok + kStepTokens > seen_by_all) {
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                const int j = tok + half * 16 + g;
+                if (j >= limit[nb].x) s[nb][half][0] = -INFINITY;
+                if (j >= limit[nb].y) s[nb][half][1] = -INFINITY;
+                if (j + 8 >= limit[nb].x) s[nb][half][2] = -INFINITY;
+                if (j + 8 >= limit[nb].y) s[nb][half][3] = -INFINITY;
+              }
+            }
+            float mx = s[nb][0][0], my = s[nb][0][1];
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              mx = max3(mx, s[nb][half][0], s[nb][half][2]);
+              my = max3(my, s[nb][half][1], s[nb][half][3]);
+            }
+            mx = fmaxf(m[nb].x, column_max(mx));
+            my = fmaxf(m[nb].y, column_max(my));
+            // a row that has seen no key has o = l = 0: any finite factor will do
+            a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
+            if constexpr (kFar) {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
+              const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
+              const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
+              l[nb].x = l[nb].x * hx * hx;
+              l[nb].y = l[nb].y * hy * hy;
+              constexpr float kUp = 0x1p14f * kSumUnit;  // what the other sums are multiplied by
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                l[nb].x = fmaf(kUp, exp2f(s[nb][half][0] - near[half].x - vx) + exp2f(s[nb][half][2] - behind[half].x - vx), l[nb].x);
+                l[nb].y = fmaf(kUp, exp2f(s[nb][half][1] - near[half].x - vy) + exp2f(s[nb][half][3] - behind[half].x - vy), l[nb].y);
+              }
+            } else {
+              l[nb].x *= a[nb].x;
+              l[nb].y *= a[nb].y;
+            }
+            moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
+            m[nb] = make_float2(mx, my);
+            const float ux = mx == -INFINITY ? 0.f : mx - kBias, uy = my == -INFINITY ? 0.f : my - kBias;
+#pragma unroll
+            for (int half = 0; half < kHalves; ++half) {
+              const float x0 = ex2_approx(s[nb][half][0] - ux), y0 = ex2_approx(s[nb][half][1] - uy);
+              const float x1 = ex2_approx(s[nb][half][2] - ux), y1 = ex2_approx(s[nb][half][3] - uy);
+              if constexpr (!kFar) {
+                l[nb].x = fmaf(x1, behind[half].y, fmaf(x0, near[half].y, l[nb].x));
+                l[nb].y = fmaf(y1, behind[half].y, fmaf(y0, near[half].y, l[nb].y));
+              }
+              pb[nb][half][0] = transpose_8x8(pack_f16x2(x0, y0));
+              pb[nb][half][1] = transpose_8x8(pack_f16x2(x1, y1));
+            }
+          }
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int nb = 0; nb < kRowBlocks; ++nb)
+#pragma unroll
+              for (int ch = 0; ch < kChunks; ++ch) {
+                o[nb][ch][0] *= a[nb].x;
+                o[nb][ch][1] *= a[nb].y;
+                o[nb][ch][2] *= a[nb].x;
+                o[nb][ch][3] *= a[nb].y;
+              }
+          }
+          // ---- O^T += V^T W^T, 16 tokens and 32 dimensions at a time
+          const uint32_t v_smem = ring + st * kStageBytes + (kTileTokens + in_tile) * kRowBytes;
+          const uint32_t* rests = v_rests + (st * (kTileTokens / 2) + in_tile / 2 + t) * kGroups;
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+#pragma unroll
+            for (int ch = 0; ch < kGroups; ch += 2) {
+              uint32_t vf[4];
+              ldmatrix_x4_trans(v_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), vf);
+              const uint2 rest = *reinterpret_cast<const uint2*>(rests + half * 8 * kGroups + ch), rest8 = *reinterpret_cast<const uint2*>(rests + (half * 8 + 4) * kGroups + ch);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                uint32_t x[4], y[4];  // f16 pairs of two tokens: dimensions 4g to 4g + 3
+                codes_to_numbers(vf[2 * e], x);
+                codes_to_numbers(vf[2 * e + 1], y);
+#pragma unroll
+                for (int nb = 0; nb < kRowBlocks; ++nb) {
+                  const uint32_t w0 = mul_f16x2(pb[nb][half][0], e ? rest.y : rest.x), w1 = mul_f16x2(pb[nb][half][1], e ? rest8.y : rest8.x);
+                  mma_16816<true>(o[nb][2 * (ch + e)], x[0], x[1], y[0], y[1], w0, w1);
+                  mma_16816<true>(o[nb][2 * (ch + e) + 1], x[2], x[3], y[2], y[3], w0, w1);
+                }
+              }
+            }
+          }
+        };
+        const int end = min(kPartTokens, seen_by_any - tile_tok - part * kPartTokens);
+        if (stage_far[st].x == 0u) {
+#pragma unroll 1
+          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::false_type{});
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::true_type{});
+        }
+        // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
+        if (i + 1 < seg_tiles) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * st);
+          ++step;
+        }
+      }
+      const bool tokens = r.len > 0;
+      const uint32_t st = step % kSt;
+#pragma unroll
+      for (int nb = 0; nb < kRowBlocks; ++nb) l[nb] = make_float2(column_sum(l[nb].x), column_sum(l[nb].y));
+      // ---- the parts of a tile's tokens come together, 8 rows at a time: every warp takes some of the dimensions, of all parts
+      constexpr int kMine = kChunks / kParts;
+      float* states = reinterpret_cast<float*>(ring_ptr + st * kStageBytes) + row_group * kParts * kState + lane;
+      const bool whole = seg_tiles == r.tiles;
+      const int slot = first_unit ? 0 : 1;
+#pragma unroll
+      for (int nb = 0; nb < kRowBlocks; ++nb) {
+        float acc[kMine][4];
+        float mm[2] = {m[nb].x, m[nb].y}, sum[2] = {l[nb].x, l[nb].y};
+        if (kParts > 1 && tokens) {
+          arithmetic_sync();
+#pragma unroll
+          for (int ch = 0; ch < kChunks; ++ch)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) states[part * kState + (ch * 4 + e) * 32] = o[nb][ch][e];
+          if (g == 0) {
+            row_state[warp * 8 + 2 * t] = make_float2(m[nb].x, l[nb].x);
+            row_state[warp * 8 + 2 * t + 1] = make_float2(m[nb].y, l[nb].y);
+          }
+          arithmetic_sync();
+          float2 others[2][kParts];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            mm[x] = -INFINITY;
+            sum[x] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kParts; ++w) {
+              others[x][w] = row_state[(row_group * kParts + w) * 8 + 2 * t + x];
+              mm[x] = fmaxf(mm[x], others[x][w].x);
+            }
+          }
+#pragma unroll
+          for (int ch = 0; ch < kMine; ++ch) acc[ch][0] = acc[ch][1] = acc[ch][2] = acc[ch][3] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kParts; ++w) {
+            float f[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float h = others[x][w].x == -INFINITY ? 0.f : ex2_approx(0.5f * (others[x][w].x - mm[x]));
+              f[x] = h * h;
+              sum[x] = fmaf(others[x][w].y * h, h, sum[x]);
+            }
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[ch][e] = fmaf(states[w * kState + ((part * kMine + ch) * 4 + e) * 32], f[e & 1], acc[ch][e]);
+          }
+        } else {
+#pragma unroll
+          for (int ch = 0; ch < kMine; ++ch)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[ch][e] = o[nb][ch][e];  // all of them, or zeros
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int row = my_row0 + 8 * nb + 2 * t + x;
+          if (row >= row0 + n_rows) continue;
+          const float inv = sum[x] > 0.f ? kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN
+          const float lse2 = sum[x] == 0.f ? -INFINITY : mm[x] - kBias - log2f(kSumUnit) + log2f(sum[x]);
+          auto dim_of = [&](int ch) { return 32 * ((part * kMine + ch) >> 1) + 4 * g + 2 * ((part * kMine + ch) & 1); };
+          if (whole) {
+            const int i = row / p.group, hq = head * p.group + row - i * p.group;
+            uint16_t* dst = p.out + (r.q0 + i) * p.o_row + hq * p.o_head;
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch) {
+              const float even = acc[ch][x] * inv, odd = acc[ch][2 + x] * inv;
+              *reinterpret_cast<uint32_t*>(dst + dim_of(ch)) = p.f16 ? pack_f16x2(even, odd) : pack_bf16x2(even, odd);
+            }
+            if (g == 0 && part == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum[x] > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
+          } else {
+            const int64_t at = kCluster ? row - row0 : (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
+            float* dst = (kCluster ? own_part : p.part_o) + at * kD;
+#pragma unroll
+            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + dim_of(ch)) = make_float2(acc[ch][x] * inv, acc[ch][2 + x] * inv);
+            if (g == 0 && part == 0) (kCluster ? own_lse : p.part_lse)[at] = lse2;
+          }
+        }
+      }
+      if (tokens) {
+        fence_proxy_async_smem();  // what was handed over goes before the copy into the same place
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + 8 * st);
+        ++step;
+      }
+      // begun here, where the share ends; ended by the CTA whose share holds its last tile
+      if (tile == 0 && !whole) left = {share.cta_behind(blockIdx.x, r.tiles - seg_tiles - 1), slot, head, row0, n_rows, r.q0};
+      tile = 0;
+      first_unit = false;
+      r = next_r;
+      unit = next;
+    }
+  }
+  if constexpr (kCluster) {
+    cluster_sync();  // every CTA's part is written
+    merge_in_cluster<kD>(p, share, own_part, own_lse, warp, lane);
+    cluster_sync();  // the others have read this CTA's
+  } else {
+    if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
+  }
+  if (lane == 0) drain_after_abort(abort_flag);
+  if (threadIdx.x == 0 && *abort_flag != 0) atomicExch(p.status, static_cast<uint32_t>(SDPA_B200_DEVICE_TIMEOUT));
+}
+
+template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
+cudaError_t launch_as(const StreamParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream, bool overlap) {
+  constexpr uint32_t kSmem = smem_bytes<kRowBlocks, kRowWarps, kD, kCluster>(ring_stages<kRowBlocks, kRowWarps, kD, kCluster>());
+  auto kernel = cache4_stream_kernel<kRowBlocks, kRowWarps, kD, kCluster>;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (err != cudaSuccess) return err;
+  return launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, overlap, kCluster ? p.cluster : 1, tm_k, tm_v, p);
+}
+
+template <int kD>
+cudaError_t launch_dim(const StreamParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, cudaStream_t stream, bool overlap) {
+  if (p.rows == 8) return (p.cluster > 0 ? launch_as<1, 1, kD, true> : launch_as<1, 1, kD, false>)(p, tm_k, tm_v, stream, overlap);
+  if (p.rows == 16) return (p.cluster > 0 ? launch_as<2, 1, kD, true> : launch_as<2, 1, kD, false>)(p, tm_k, tm_v, stream, overlap);
+  return (p.rows == 32 ? launch_as<2, 2, kD, false> : launch_as<2, 4, kD, false>)(p, tm_k, tm_v, stream, overlap);
+}
+
+}  // namespace
+
+cudaError_t launch_stream4(const StreamParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int head_dim, cudaStream_t stream, bool overlap) {
+  return (head_dim == 64 ? launch_dim<64> : launch_dim<128>)(p, tm_k, tm_v, stream, overlap);
+}
+
+}  // namespace sdpa_b200

@@ -1,0 +1,123 @@
+// Keys and values of a serving step into the 4-bit paged cache. No counterpart in the reference, which has no paged cache.
+//
+// For every 32 elements of a token and head: scale = the smallest number of five significant bits, 2^-100 at least, with 7 * scale >= max |x|, code = round(x / scale), ties to even.
+// Five bits, since 7 * 31 < 2^8: a code times its scale is then exact in bf16 (and f16, within its range), so that what attention streams, gathers and reads back is one number; that
+// costs a step of 1/32 more on average. x has at most 11 bits, a scale 5: no quotient but a tie itself comes nearer than 2^-12 to the middle of two codes, so x * (1 / scale) with one
+// correction step, which gives quotients of few bits exactly, rounds as the exact quotient does.
+//
+// A scale depends on its own 32 elements only: no runs to find, nothing read back, no order among tokens. A thread has eight elements, four threads a scale.
+#include <type_traits>
+
+#include "cache_common.cuh"
+
+namespace sdpa_b200 {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Store4Side {
+  const uint16_t* in;
+  uint8_t* cache;
+  uint16_t* scale;
+  int64_t in_row, in_head, block, head, row;
+};
+
+struct Store4Params {
+  Store4Side side[2];  // keys, values
+  const int32_t* slots;
+  int tokens, heads, num_slots, shift;
+};
+
+// kRows: rows (a head of a token) that a thread has a part of
+template <int kD, bool kF16, int kRows>
+__global__ void __launch_bounds__(kThreads) store4_kernel(const Store4Params p) {
+  constexpr int kLanes = kD / 8, kRowsAtOnce = kThreads / kLanes;
+  constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
+  const Store4Side& x = p.side[blockIdx.x & 1];
+  const int at = threadIdx.x % kLanes * 8;
+  const int row0 = static_cast<int>(blockIdx.x >> 1) * (kRowsAtOnce * kRows) + threadIdx.x / kLanes;
+  launch_dependents();
+  wait_for_previous_grid();
+  uint4 held[kRows];
+  int slot[kRows], head[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const int row = row0 + i * kRowsAtOnce, t = row / p.heads;
+    head[i] = row - t * p.heads;
+    held[i] = make_uint4(0u, 0u, 0u, 0u);
+    slot[i] = -1;
+    if (t < p.tokens) {
+      slot[i] = p.slots[t];
+      if (t + 1 < p.tokens && p.slots[t + 1] == slot[i]) slot[i] = -1;  // the same slot again with the next token: the later stays
+      held[i] = *reinterpret_cast<const uint4*>(x.in + t * x.in_row + head[i] * x.in_head + at);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    // 16-bit floats without their signs are ordered as integers, infinity and NaN behind all numbers
+    uint32_t top = __vmaxu2(__vmaxu2(held[i].x & 0x7fff7fffu, held[i].y & 0x7fff7fffu), __vmaxu2(held[i].z & 0x7fff7fffu, held[i].w & 0x7fff7fffu));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = max(top & 0xffffu, top >> 16);
+    const bool bad = top >= kInf;
+    const float most = unpack_16x2<kF16>(top).x;
+    float scale = __uint_as_float((__float_as_uint(__fdiv_rn(most, 7.f)) + 0x7ffffu) & 0xfff80000u);
+    scale = bad ? 1.f : fmaxf(scale, 0x1p-100f);
+    const float inv = __frcp_rn(scale);
+    const uint32_t words[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+    uint32_t code[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = unpack_16x2<kF16>(words[e]);
+      const float2 q = mul2(v, make_float2(inv, inv));
+      const float2 off = fma2(q, make_float2(-scale, -scale), v);
+      const float2 n = add2(fma2(off, make_float2(inv, inv), q), make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23 + x has x, rounded, in its low bits
+      code[2 * e] = __float_as_uint(n.x);
+      code[2 * e + 1] = __float_as_uint(n.y);
+    }
+    auto bytes = [&](int e) { return __byte_perm(__byte_perm(code[e], code[e + 2], 0x0040), __byte_perm(code[e + 4], code[e + 6], 0x0040), 0x5410); };
+    uint32_t packed = (bytes(0) & 0x0f0f0f0fu) | (bytes(1) << 4 & 0xf0f0f0f0u);
+    if (bad) packed = 0u;
+    if (slot[i] < 0 || slot[i] >= p.num_slots) continue;
+    const int block = slot[i] >> p.shift, place = slot[i] & ((1 << p.shift) - 1);
+    *reinterpret_cast<uint32_t*>(x.cache + block * x.block + head[i] * x.head + place * x.row + at / 2) = packed;
+    if (at % kScaleGroup == 0)
+      x.scale[((((static_cast<int64_t>(block) * p.heads + head[i]) << p.shift) + place) * kD + at) / kScaleGroup] = bad ? 0x7fc0u : static_cast<uint16_t>(__float_as_uint(scale) >> 16);
+  }
+}
+
+}  // namespace
+
+int launch_store4(const sdpa_b200_cache_params& p, cudaStream_t stream) {
+  Store4Params s;
+  s.side[0] = {static_cast<const uint16_t*>(p.key), static_cast<uint8_t*>(p.k_cache), static_cast<uint16_t*>(p.k_scale), p.key_row_stride, p.key_head_stride,
+               p.k_block_stride, p.k_head_stride, p.k_row_stride};
+  s.side[1] = {static_cast<const uint16_t*>(p.value), static_cast<uint8_t*>(p.v_cache), static_cast<uint16_t*>(p.v_scale), p.value_row_stride, p.value_head_stride,
+               p.v_block_stride, p.v_head_stride, p.v_row_stride};
+  s.slots = p.slots;
+  s.tokens = p.num_tokens;
+  s.heads = p.heads_kv;
+  s.shift = block_shift(p.block_size);
+  s.num_slots = p.num_blocks << s.shift;
+  const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads_kv;
+  const bool f16 = p.dtype == SDPA_B200_F16;
+  cudaError_t err = cudaSuccess;
+  auto launch = [&](auto dim, auto each) {
+    constexpr int kD = decltype(dim)::value, kRows = decltype(each)::value, kRowsOfCta = kThreads / (kD / 8) * kRows;
+    const unsigned grid = static_cast<unsigned>(2 * ((rows + kRowsOfCta - 1) / kRowsOfCta));
+    err = launch_behind(f16 ? store4_kernel<kD, true, kRows> : store4_kernel<kD, false, kRows>, dim3(grid), kThreads, 0, stream, true, 1, s);
+  };
+  auto launch_rows = [&](auto dim) {
+    // few rows: a thread has one, whose loads are all that there is to wait for
+    rows * p.head_dim <= 148 * 2048 * 8 ? launch(dim, std::integral_constant<int, 1>{}) : launch(dim, std::integral_constant<int, 4>{});
+  };
+  p.head_dim == 64 ? launch_rows(std::integral_constant<int, 64>{}) : launch_rows(std::integral_constant<int, 128>{});
+  if (err != cudaSuccess) {
+    set_error("cache_store: launch failed: %s", cudaGetErrorString(err));
+    return SDPA_B200_LAUNCH_FAILED;
+  }
+  count_launch();
+  return SDPA_B200_OK;
+}
+
+}  // namespace sdpa_b200

@@ -28,53 +28,17 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "cache_common.cuh"
-#include "cache_shares.cuh"
+#include "cache_stream.cuh"
 
 namespace sdpa_b200 {
 namespace {
 
-constexpr int kWarps = 4;                  // those that do the arithmetic
-constexpr int kThreads = (kWarps + 2) * 32;  // and two that load: registers are dealt out as for six warps anyway
-constexpr int kCtasPerSm = 2;
-constexpr int kMaxSms = 160;  // workspace sizes do not ask the device: an upper bound of its SMs (148)
-constexpr int kPause = 2;  // see share_of
 constexpr int kTilesInCluster = 8;          // that a CTA of a cluster may get: see cluster_of
 constexpr int kMostClusterCtas = 256;       // clusters of eight find room for that many CTAs at once
 constexpr float kLeastScale = 0x1p-100f;   // of V: a block of zeros may have a scale of 0, which has no logarithm
-// Sums are kept in this unit: they are up to 2^100 a token where the largest weight is that of a block of the least scale, and no less than 2^-121 where it is that of bf16's largest
-constexpr float kSumUnit = 0x1p-15f;
 // Scales of V above it are far from the least one: a weight times its scale, or what such products are multiplied by when their maximum moves, may then be too small for 32 bits
 // though the weight itself counts. Up to it, a key that is lost has less than 2^-26 of the largest weight.
 constexpr float kFarScale = 1.f;
-
-struct StreamParams {
-  const uint16_t* q;
-  uint16_t* out;
-  float* lse;
-  const float* k_scale;
-  const float* v_scale;
-  const int32_t* block_table;
-  const int32_t* seq_lens;
-  const int32_t* cu_q;
-  float* part_o;    // [2 per CTA][rows][head_dim], normalised
-  float* part_lse;  // [2 per CTA][rows], log2 domain; -inf: no key seen, NaN: a NaN row
-  struct SharedUnit* shared_units;  // one per CTA
-  uint32_t* status;
-  int64_t q_row, q_head, o_row, o_head, table_stride;
-  int batch, heads_q, heads_kv, group, total_q, max_blocks, num_blocks, shift, rows, rows_shift, grid, causal, f16;
-  int tile_shift;  // log2 of a tile's tokens
-  int pause;       // see share_of
-  int first_q, max_rows;  // the first request's row of q where there are no offsets; rows that a request may have
-  int cluster, units_each;  // CTAs that share a unit, units that each request has room for: see share_in_cluster
-  int max_len;  // tokens that a table's row holds
-  float scale_log2;
-};
-
-// The unit that begins in a CTA's share and ends in a later one's: what the merge kernel needs to know. `last` < 0: there is none.
-struct SharedUnit {
-  int last, slot, head, row0, rows, q0;  // the CTA that ends it; where the first CTA's part is; kv head, rows [row0, row0 + rows) of the request whose tokens begin at q0
-};
 
 // Tokens of a tile, 32 KB of K and V, and those that a warp handles at a time: its products, maxima over lanes, exponentials and products again are one long chain, in which the
 // blocks of 16 tokens run beside each other; as many as registers hold.
@@ -94,104 +58,6 @@ template <int kRowBlocks, int kRowWarps, int kD>
 __host__ __device__ constexpr uint32_t stream_smem_bytes() {
   return 1024 + ring_stages<kRowWarps, kD>() * (stage_bytes<kD>() + tile_tokens<kD>() + 16) + 16 + kWarps * 16 * 8 +
          (q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 16) * 2 * 128);
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
-// barrier over the warps that do the arithmetic
-__device__ __forceinline__ void arithmetic_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
-
-// One 8 x 8 matrix of 16-bit elements: row g, columns 2t and 2t + 1 in, row 2t and 2t + 1, column g out
-__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-// over the eight lanes that share t = lane % 4
-__device__ __forceinline__ float column_max(float x) {
-#pragma unroll
-  for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-  return x;
-}
-__device__ __forceinline__ float column_sum(float x) {
-#pragma unroll
-  for (int d = 4; d < 32; d *= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
-  return x;
-}
-
-// A CTA's share of the list of all tiles (cache_shares.cuh). The empty places in front of a unit stand for what the hand-over from unit
-// to unit takes, which is about that of two tiles (not so with 64 rows, whose warps have nothing to merge and more to do per tile: 59.5 us with it, 58.8 without, 4 requests
-// of 32 rows). Measured with equal shares of the tiles | of the places, one token each, us: 64 requests
-// of 200 to 1800 37.9 | 33.9, 128 of 100 to 900 52.8 | 39.9, 32 of 100 to 2000 with 32 kv heads 62 | 48.5, 64 of 500 to 4000 59.3 | 55.5; 4 tokens, 16 of 300 to 9000 at
-// head_dim 64 22.0 | 19.8. With pauses of one place the second took 43.9, with three the same, and 8 tokens of 32 requests 53.8 instead of 52.0.
-//
-// Every warp finds it for itself, so that none waits for another.
-__device__ __forceinline__ Share share_of(const StreamParams& p, int cta, int lane) {
-  auto add_tiles_of = [&](int b, int& tiles, int& units) {
-    if (b >= p.batch) return;
-    const Request r = request_at(p, b);
-    units += r.units;
-    tiles += tiles_of(r);
-  };
-  int tiles_of_first = 0, units_of_first = 0;  // of the first 32 requests
-  add_tiles_of(lane, tiles_of_first, units_of_first);
-  int tiles = tiles_of_first, units = units_of_first;
-#pragma unroll 4
-  for (int b = lane + 32; b < p.batch; b += 32) add_tiles_of(b, tiles, units);
-  tiles = __reduce_add_sync(0xffffffffu, tiles);
-  Share s = {};
-  if (tiles == 0) return s;
-  const int first = deal(s, p, tiles, tiles >= kTilesToPause * p.grid ? __reduce_add_sync(0xffffffffu, units) : 0, cta);
-  if (first < 0) return s;
-  int before = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int mine = tiles_of_first, mine_units = units_of_first;
-    if (b0 != 0) {
-      mine = mine_units = 0;
-      add_tiles_of(b0 + lane, mine, mine_units);
-    }
-    mine += s.pause * mine_units;
-    int run = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int x = __shfl_up_sync(0xffffffffu, run, d);
-      if (lane >= d) run += x;
-    }
-    const unsigned behind = __ballot_sync(0xffffffffu, first < before + run);
-    if (behind != 0) {
-      const int at = __ffs(behind) - 1;
-      before += __shfl_sync(0xffffffffu, run - mine, at);
-      begin_in(s, request_at(p, b0 + at), first - before, cta);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, run, 31);
-  }
-  return s;
-}
-
-// A row out of its merged parts: kPer of its dimensions a lane, sums of the weights 2^(lse - top) and of the parts by them
-template <int kPer>
-__device__ __forceinline__ void write_row(const StreamParams& p, int q0, int head, int row, int lane, const float (&acc)[kPer], float sum, float top, bool nan) {
-  const int i = row / p.group, hq = head * p.group + row - i * p.group;
-  const float inv = nan ? __int_as_float(0x7fffffff) : sum > 0.f ? 1.f / sum : 0.f;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + (q0 + i) * p.o_row + hq * p.o_head + kPer * lane);
-#pragma unroll
-  for (int e = 0; e < kPer; e += 2) dst[e / 2] = p.f16 ? pack_f16x2(acc[e] * inv, acc[e + 1] * inv) : pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
-  if (lane == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + q0 + i] = !nan && sum > 0.f ? (top + log2f(sum)) * 0.6931471805599453f : INFINITY;
-}
-
-// Where a cluster of CTAs takes a unit: each a stretch of its tiles. Nothing is looked up but the one request.
-__device__ __forceinline__ Share share_in_cluster(const StreamParams& p, int cta) {
-  const int unit = cta / p.cluster, rank = cta - unit * p.cluster, b = unit / p.units_each;
-  Share s = {};
-  s.request = request_at(p, b);
-  s.unit = unit - b * p.units_each;
-  s.each = (s.request.tiles + p.cluster - 1) / p.cluster;
-  s.tile = rank * s.each;
-  if (s.unit < s.request.units) s.places = max(min(s.each, s.request.tiles - s.tile), 0);
-  return s;
 }
 
 // kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
@@ -247,7 +113,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     // groups are under way: the one that tiles are copied from, the next with its scales, and the block numbers of the one behind.
     const bool keys = warp == kWarps;
     const CUtensorMap* map = keys ? &tm_k : &tm_v;
-    const float* scales = keys ? p.k_scale : p.v_scale;
+    const float* scales = static_cast<const float*>(keys ? p.k_scale : p.v_scale);
     struct Place {
       Request r;
       int unit, group, head;
@@ -728,46 +594,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   }
   if constexpr (kCluster) {
     cluster_sync();  // every CTA's part is written
-    const Request& r = share.request;
-    const int row0 = share.unit / p.heads_kv * p.rows, head = share.unit - share.unit / p.heads_kv * p.heads_kv;
-    const int rank = blockIdx.x - blockIdx.x / p.cluster * p.cluster;
-    if (share.unit < r.units && share.each < r.tiles) {  // (a single CTA's unit is done)
-      const int n_rows = min(p.rows, r.rows_q * p.group - row0);
-      for (int rr = rank + p.cluster * warp; rr < n_rows; rr += p.cluster * (kWarps + 2)) {
-        constexpr int kPer = kD / 32;
-        float v[8][kPer];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t src = smem_u32(own_part + rr * kD + kPer * lane);
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) v[c][e] = 0.f;
-          if (c * share.each >= r.tiles) continue;  // without tiles: its part was never written
-          if constexpr (kPer == 4) {
-            const float4 x = cluster_ld_f32x4(src, c);
-            v[c][0] = x.x, v[c][1] = x.y, v[c][2] = x.z, v[c][3] = x.w;
-          } else {
-            const float2 x = cluster_ld_f32x2(src, c);
-            v[c][0] = x.x, v[c][1] = x.y;
-          }
-        }
-        const float x = lane < p.cluster ? cluster_ld_f32(smem_u32(own_lse + rr), lane) : -INFINITY;
-        const bool nan = __any_sync(0xffffffffu, isnan(x));
-        float top = x;
-#pragma unroll
-        for (int d = 1; d < 8; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        top = __shfl_sync(0xffffffffu, top, 0);
-        const float w = x == -INFINITY ? 0.f : exp2f(x - top);
-        float sum = 0.f, acc[kPer] = {};
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float wc = __shfl_sync(0xffffffffu, w, c);
-          sum += wc;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) acc[e] = fmaf(wc, v[c][e], acc[e]);
-        }
-        write_row<kPer>(p, r.q0, head, row0 + rr, lane, acc, sum, top, nan);
-      }
-    }
+    merge_in_cluster<kD>(p, share, own_part, own_lse, warp, lane);
     cluster_sync();  // the others have read this CTA's
   } else {
     if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
@@ -846,7 +673,7 @@ __global__ void __launch_bounds__(128) cache_merge_kernel(const StreamParams p) 
 // ---- many rows: the codes of all requests as packed 16-bit K and V
 struct GatherParams {
   const uint8_t* cache[2];
-  const float* scale[2];
+  const void* scale[2];
   uint16_t* out[2];
   const int32_t* cu_q;
   int32_t* cu;  // offsets of queries [2 * batch + 1], then of keys
@@ -864,21 +691,11 @@ constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, 
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
 
-// two elements in 16 bits, the largest number of the type where they are beyond it: a code is rounded, and the elements 65504 of f16 or 3.39e38 of bf16 come back as
-// 2^16 or 2^128. NaN stays.
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack_16x2_finite(float lo, float hi) {
-  uint32_t r;
-  if constexpr (kF16) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // Block (i, h, b): tokens 32i to 32i + 31 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
 // where a weight of 0 would meet another request's NaN, or whatever the workspace held. So every request's rows are filled up to a whole tile with zeros, and these
 // stand in the list of sequences as one of their own, without queries. A request that is longer than its table has the most tokens here that any may have, which
 // are no fewer than its rows, so that each of them sees the first; all are in a block that there is none of.
-template <int kD, bool kInt8, bool kF16>
+template <int kD, int kCode, bool kF16>
 __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p) {
   __shared__ int sums[8];
   const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x;
@@ -914,37 +731,38 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
     const int tok = tok0 + i * (256 / kLanes), page = tok >> p.shift;
     id[i] = tok < len && page < max_blocks ? p.block_table[b * p.table_stride + page] : -1;
   }
-  uint2 w[kTimes][2];
-  float scale[kTimes][2];
+  Eight<kCode> w[kTimes][2];
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), place = tok & ((1 << p.shift) - 1);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      w[i][x] = make_uint2(0u, 0u);
+      w[i][x].codes = make_uint2(0u, 0u);
       // a block outside the cache: its scores are NaN, for those who see them
-      scale[i][x] = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
+      w[i][x].scale = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
-      w[i][x] = *reinterpret_cast<const uint2*>(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + at);
-      scale[i][x] = p.scale[x][static_cast<int64_t>(id[i]) * p.heads + h];
+      w[i][x].load(p.cache[x], p.scale[x], p.block[x], p.head[x], p.row[x], id[i], p.heads, h, place, p.shift, kD, at);
     }
   }
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes);
     if (tok >= padded) break;
+    float own[2];  // as on the other path
+#pragma unroll
+    for (int x = 0; x < 2; ++x) own[x] = fabsf(w[i][x].scale) == INFINITY ? __int_as_float(0x7fffffff) : w[i][x].scale;
+    if constexpr (kCode == SDPA_B200_INT4) {  // a scale of V that is no number is its token's: who sees the token is NaN, not who has the weight 0 for it
+      if (isnan(own[1])) own[0] = own[1], own[1] = 0.f;
+    } else if (own[1] < 0.f) {
+      own[1] = __int_as_float(0x7fffffff);
+    }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      uint32_t f[4], c[2] = {w[i][x].x, w[i][x].y};
-      const float own = fabsf(scale[i][x]) == INFINITY || (x == 1 && scale[i][x] < 0.f) ? __int_as_float(0x7fffffff) : scale[i][x];  // as on the other path
+      float v[8];
+      w[i][x].values(v);
+      uint32_t f[4];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t lo, hi;
-        codes_to_f16<kInt8>(c[e], lo, hi);
-        const float2 u = unpack_16x2<true>(lo), v = unpack_16x2<true>(hi);
-        f[2 * e] = pack_16x2_finite<kF16>(u.x * own, u.y * own);
-        f[2 * e + 1] = pack_16x2_finite<kF16>(v.x * own, v.y * own);
-      }
+      for (int e = 0; e < 4; ++e) f[e] = pack_16x2_finite<kF16>(v[2 * e] * own[x], v[2 * e + 1] * own[x]);
       *reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
     }
   }
@@ -1121,9 +939,9 @@ int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* w
   p.part_lse = p.part_o + rows * c.head_dim;
   p.shared_units = reinterpret_cast<SharedUnit*>(p.part_lse + rows);
   CUtensorMap tm_k, tm_v;
-  int st = make_cache_tensor_map(&tm_k, c.k_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.k_row_stride, c.k_head_stride, c.k_block_stride, c.block_size);
+  int st = make_cache_tensor_map(&tm_k, c.k_cache, row_bytes(c), c.block_size, c.heads_kv, c.num_blocks, c.k_row_stride, c.k_head_stride, c.k_block_stride, c.block_size);
   if (st != SDPA_B200_OK) return st;
-  st = make_cache_tensor_map(&tm_v, c.v_cache, c.head_dim, c.block_size, c.heads_kv, c.num_blocks, c.v_row_stride, c.v_head_stride, c.v_block_stride, c.block_size);
+  st = make_cache_tensor_map(&tm_v, c.v_cache, row_bytes(c), c.block_size, c.heads_kv, c.num_blocks, c.v_row_stride, c.v_head_stride, c.v_block_stride, c.block_size);
   if (st != SDPA_B200_OK) return st;
   cudaError_t err = cudaSuccess;
   auto launch_as = [&](auto blocks_tag, auto rows_tag, auto dim_tag, auto int8_tag, auto cluster_tag) {
@@ -1150,7 +968,8 @@ int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* w
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (p.rows == 8) launch_dim(One{}, One{});
+  if (c.code == SDPA_B200_INT4) err = launch_stream4(p, tm_k, tm_v, c.head_dim, stream, c.device_status != nullptr);
+  else if (p.rows == 8) launch_dim(One{}, One{});
   else if (p.rows == 16) launch_dim(Two{}, One{});
   else if (p.rows == 32) launch_dim(Two{}, Two{});
   else launch_dim(Two{}, std::integral_constant<int, 4>{});
@@ -1208,13 +1027,16 @@ int launch_gathered(const sdpa_b200_cache_params& c, int first, int count, char*
   g.max_len = table_tokens(c);
   const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / kGatherTokens), c.heads_kv, count);
   const bool f16 = c.dtype == SDPA_B200_F16;
-  auto launch = [&](auto dim, auto int8) {
-    constexpr int kD = decltype(dim)::value;
-    constexpr bool kInt8 = decltype(int8)::value;
-    if (f16) cache_gather_kernel<kD, kInt8, true><<<grid, 256, 0, stream>>>(g);
-    else cache_gather_kernel<kD, kInt8, false><<<grid, 256, 0, stream>>>(g);
+  auto launch = [&](auto dim, auto code) {
+    constexpr int kD = decltype(dim)::value, kCode = decltype(code)::value;
+    if (f16) cache_gather_kernel<kD, kCode, true><<<grid, 256, 0, stream>>>(g);
+    else cache_gather_kernel<kD, kCode, false><<<grid, 256, 0, stream>>>(g);
   };
-  auto launch_dim = [&](auto dim) { c.code == SDPA_B200_INT8 ? launch(dim, std::true_type{}) : launch(dim, std::false_type{}); };
+  auto launch_dim = [&](auto dim) {
+    if (c.code == SDPA_B200_INT8) launch(dim, std::integral_constant<int, SDPA_B200_INT8>{});
+    else if (c.code == SDPA_B200_INT4) launch(dim, std::integral_constant<int, SDPA_B200_INT4>{});
+    else launch(dim, std::integral_constant<int, SDPA_B200_E4M3>{});
+  };
   c.head_dim == 64 ? launch_dim(std::integral_constant<int, 64>{}) : launch_dim(std::integral_constant<int, 128>{});
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) {

@@ -1,4 +1,4 @@
-// The 8-bit codes of the paged cache (include/sdpa_b200.h): conversions from and to 16-bit and 32-bit values, argument checks.
+// The codes of the paged cache (include/sdpa_b200.h): conversions from and to 16-bit and 32-bit values, argument checks.
 #pragma once
 
 #include "kernels.h"
@@ -30,6 +30,59 @@ __device__ __forceinline__ void codes_to_f16_by_two(uint32_t codes, uint32_t& ev
   } else {
     codes_to_f16<false>(__byte_perm(codes, 0u, 0x3120), even, odd);
   }
+}
+
+// Four bits: eight codes, the even element in the low half of its byte, as their values
+__device__ __forceinline__ void codes4_to_floats(uint32_t codes, float (&x)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(static_cast<int>(codes << (28 - 4 * e)) >> 28);
+}
+
+constexpr int kScaleGroup = 32;  // elements of a token and head that share a scale in a 4-bit cache
+
+// Eight elements of a cache of any code, out of 64-bit or 32-bit words of codes and their scale
+template <int kCode>
+struct Eight {
+  uint2 codes;
+  float scale;
+
+  __device__ __forceinline__ void load(const uint8_t* cache, const void* scales, int64_t block_stride, int64_t head_stride, int64_t row_stride, int block, int heads, int head,
+                                       int place, int shift, int head_dim, int at) {
+    const uint8_t* row = cache + block * block_stride + head * head_stride + place * row_stride;
+    const int64_t of_head = static_cast<int64_t>(block) * heads + head;
+    if constexpr (kCode == SDPA_B200_INT4) {
+      codes = make_uint2(*reinterpret_cast<const uint32_t*>(row + at / 2), 0u);
+      scale = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[((of_head << shift) + place) * (head_dim / kScaleGroup) + at / kScaleGroup]) << 16);
+    } else {
+      codes = *reinterpret_cast<const uint2*>(row + at);
+      scale = static_cast<const float*>(scales)[of_head];
+    }
+  }
+  __device__ __forceinline__ void values(float (&x)[8]) const {
+    if constexpr (kCode == SDPA_B200_INT4) {
+      codes4_to_floats(codes.x, x);
+    } else {
+      uint32_t h[4];
+      codes_to_f16<kCode == SDPA_B200_INT8>(codes.x, h[0], h[1]);
+      codes_to_f16<kCode == SDPA_B200_INT8>(codes.y, h[2], h[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = unpack_16x2<true>(h[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+      }
+    }
+  }
+};
+
+// two elements in 16 bits, the largest number of the type where they are beyond it: a code is rounded, and the elements 65504 of f16 or 3.39e38 of bf16 come back as
+// 2^16 or 2^128. NaN stays.
+template <bool kF16>
+__device__ __forceinline__ uint32_t pack_16x2_finite(float lo, float hi) {
+  uint32_t r;
+  if constexpr (kF16) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 // The smallest power of two 2^k, k >= -100, at which `largest` (finite, not negative) is a code: at most 448 = 1.75 * 2^8 of e4m3, 127 = 1.984375 * 2^6 of int8.
@@ -82,14 +135,20 @@ inline int block_shift(int block_size) {
   return -1;
 }
 
-// What store and attention want of the cache itself. Touches no device.
+// Store of 4-bit codes (cache4_store.cu), of arguments that have been checked
+int launch_store4(const sdpa_b200_cache_params& p, cudaStream_t stream);
+
+// Bytes of a token's codes of one head
+inline int row_bytes(const sdpa_b200_cache_params& p) { return p.code == SDPA_B200_INT4 ? p.head_dim / 2 : p.head_dim; }
+
+// What store, load and attention want of the cache itself. Touches no device.
 inline int check_cache(const sdpa_b200_cache_params* p, const char* who) {
   if (p == nullptr) {
     set_error("%s: params is NULL", who);
     return SDPA_B200_INVALID_ARG;
   }
-  if (p->code != SDPA_B200_E4M3 && p->code != SDPA_B200_INT8) {
-    set_error("%s: codes must be e4m3 or int8 (code %d)", who, p->code);
+  if (p->code != SDPA_B200_E4M3 && p->code != SDPA_B200_INT8 && p->code != SDPA_B200_INT4) {
+    set_error("%s: codes must be e4m3 or int8, or int4 (code %d)", who, p->code);
     return SDPA_B200_UNSUPPORTED;
   }
   if (p->dtype != SDPA_B200_BF16 && p->dtype != SDPA_B200_F16) {
@@ -97,7 +156,7 @@ inline int check_cache(const sdpa_b200_cache_params* p, const char* who) {
     return SDPA_B200_UNSUPPORTED;
   }
   if (p->head_dim != 64 && p->head_dim != 128) {
-    set_error("%s: the 8-bit cache is built for head_dim 64 and 128 (got %d)", who, p->head_dim);
+    set_error("%s: the %d-bit cache is built for head_dim 64 and 128 (got %d)", who, p->code == SDPA_B200_INT4 ? 4 : 8, p->head_dim);
     return SDPA_B200_UNSUPPORTED;
   }
   if (block_shift(p->block_size) < 0) {
@@ -117,15 +176,17 @@ inline int check_cache(const sdpa_b200_cache_params* p, const char* who) {
       return SDPA_B200_INVALID_ARG;
     }
     for (int i = 0; i < 3; ++i) {
-      if (sizes[i] > 1 && (strides[x][i] < p->head_dim || strides[x][i] % 16 != 0 || strides[x][i] >= (int64_t(1) << 40))) {
-        set_error("%s: %s_cache needs block / head / token strides that are multiples of 16 bytes and at least head_dim (got %lld)", who, x ? "v" : "k",
+      if (sizes[i] > 1 && (strides[x][i] < row_bytes(*p) || strides[x][i] % 16 != 0 || strides[x][i] >= (int64_t(1) << 40))) {
+        set_error("%s: %s_cache needs block / head / token strides that are multiples of 16 bytes and at least head_dim%s (got %lld)", who, x ? "v" : "k",
+                  p->code == SDPA_B200_INT4 ? " / 2" : "",
                   static_cast<long long>(strides[x][i]));
         return SDPA_B200_INVALID_ARG;
       }
     }
   }
-  if (p->k_scale == nullptr || p->v_scale == nullptr || ((reinterpret_cast<uintptr_t>(p->k_scale) | reinterpret_cast<uintptr_t>(p->v_scale)) & 3u) != 0) {
-    set_error("%s: k_scale and v_scale must be 4-byte aligned device pointers", who);
+  const unsigned scale_align = p->code == SDPA_B200_INT4 ? 16 : 4;
+  if (p->k_scale == nullptr || p->v_scale == nullptr || ((reinterpret_cast<uintptr_t>(p->k_scale) | reinterpret_cast<uintptr_t>(p->v_scale)) & (scale_align - 1)) != 0) {
+    set_error("%s: k_scale and v_scale must be %u-byte aligned device pointers", who, scale_align);
     return SDPA_B200_INVALID_ARG;
   }
   return SDPA_B200_OK;

@@ -300,12 +300,17 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params*
   st = check_input("key", p->key, p->key_row_stride, p->key_head_stride, p->num_tokens, p->heads_kv);
   if (st == SDPA_B200_OK) st = check_input("value", p->value, p->value_row_stride, p->value_head_stride, p->num_tokens, p->heads_kv);
   if (st != SDPA_B200_OK) return st;
+  if (p->code == SDPA_B200_INT4 && static_cast<int64_t>(p->num_tokens) * p->heads_kv > INT32_MAX / 2) {  // rows are counted in 32 bits there
+    set_error("cache_store: too many tokens (%d) for %d heads", p->num_tokens, p->heads_kv);
+    return SDPA_B200_INVALID_ARG;
+  }
   st = check_device();
   if (st != SDPA_B200_OK) return st;
+  if (p->code == SDPA_B200_INT4) return launch_store4(*p, static_cast<cudaStream_t>(stream));
   StoreParams s;
-  s.side[0] = {static_cast<const uint16_t*>(p->key), static_cast<uint8_t*>(p->k_cache), p->k_scale, p->key_row_stride, p->key_head_stride, p->k_block_stride,
+  s.side[0] = {static_cast<const uint16_t*>(p->key), static_cast<uint8_t*>(p->k_cache), static_cast<float*>(p->k_scale), p->key_row_stride, p->key_head_stride, p->k_block_stride,
                p->k_head_stride, p->k_row_stride};
-  s.side[1] = {static_cast<const uint16_t*>(p->value), static_cast<uint8_t*>(p->v_cache), p->v_scale, p->value_row_stride, p->value_head_stride,
+  s.side[1] = {static_cast<const uint16_t*>(p->value), static_cast<uint8_t*>(p->v_cache), static_cast<float*>(p->v_scale), p->value_row_stride, p->value_head_stride,
                p->v_block_stride, p->v_head_stride, p->v_row_stride};
   s.slots = p->slots;
   s.tokens = p->num_tokens;

@@ -3,6 +3,7 @@
 // decode step, a short prompt), and building the 90-field parameter block field by field through ctypes took the host
 // 50 to 60 us per call; here a call costs 5 to 10 us, most of it the CUDA launches.
 #include <ATen/PythonTorchFunctionTLS.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
@@ -242,6 +243,21 @@ PyObject* py_cache_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// cache_load(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, num_tokens, first or None, dtype)
+PyObject* py_cache_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect_args(n, 9);
+  const Tensor &kc = tensor_arg(a[0], "key_cache"), &vc = tensor_arg(a[1], "value_cache"), &ks = tensor_arg(a[2], "key_scale"), &vs = tensor_arg(a[3], "value_scale"),
+               &table = tensor_arg(a[4], "block_table"), &cu = tensor_arg(a[5], "cu_seqlens");
+  const int64_t num_tokens = int_arg(a[6]);
+  const c10::optional<Tensor> first = optional_tensor(a[7], "first");
+  if (!THPDtype_Check(a[8])) throw torch::TypeError("dtype must be a torch.dtype");
+  const at::ScalarType dtype = reinterpret_cast<THPDtype*>(a[8])->scalar_type;
+  auto r = call([&] { return cache_load(kc, vc, ks, vs, table, cu, num_tokens, first, dtype); });
+  return tuple_of({std::get<0>(r), std::get<1>(r)});
+  END_HANDLE_TH_ERRORS
+}
+
 // cache_attention(query, key_cache, value_cache, key_scale, value_scale, block_table, seq_lens, cu_seqlens, max_q, max_k, is_causal, scale)
 PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -311,6 +327,7 @@ PyMethodDef g_methods[] = {
     FAST("sdpa", py_sdpa),
     FAST("plan_step", py_plan_step),
     FAST("cache_store", py_cache_store),
+    FAST("cache_load", py_cache_load),
     FAST("cache_attention", py_cache_attention),
     FAST("rotary", py_rotary),
     FAST("status_word", py_status_word),

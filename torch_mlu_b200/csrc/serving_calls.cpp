@@ -1,4 +1,4 @@
-// The serving operators from tensors to launched kernels: bookkeeping of a step, the 8-bit paged cache, rotary positions with their gradient. Called by
+// The serving operators from tensors to launched kernels: bookkeeping of a step, the paged cache, rotary positions with their gradient. Called by
 // py_calls.cpp for kv_cache.py and rotary.py: a decode step's kernels run for a few microseconds each, and filling the parameter blocks through ctypes took
 // the host 25 to 45 us a call. They are operators of b200_sdpa too, through which a call goes while somebody wants to see it (a tracer, a dispatch mode): what launched
 // kernels beside a tracer would leave its results in the traced program as constants.
@@ -174,26 +174,33 @@ std::vector<Tensor> plan_step(const Tensor& cached_lens, const Tensor& new_token
 
 namespace {
 
-void cache_params(sdpa_b200_cache_params& p, const Tensor& x, const char* name, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs) {
-  check_plain(x, name);
-  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "16-bit tensors must be fp16 or bf16 (got ", x.scalar_type(), ")");
+// The cache: 8 bits, or 4 with two codes in a byte, on the device of `x`
+void cache_params(sdpa_b200_cache_params& p, const Tensor& x, at::ScalarType dtype, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs) {
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "16-bit tensors must be fp16 or bf16 (got ", dtype, ")");
   check_plain(kc, "key_cache");
   check_plain(vc, "value_cache");
   TORCH_CHECK(kc.dim() == 4 && kc.sizes() == vc.sizes(), "key_cache and value_cache must both be [num_blocks, heads_kv, block_size, head_dim]");
-  TORCH_CHECK((kc.scalar_type() == at::kFloat8_e4m3fn || kc.scalar_type() == at::kChar) && vc.scalar_type() == kc.scalar_type(),
-              "the caches must both be float8_e4m3fn or int8");
-  TORCH_CHECK(x.size(-1) == kc.size(3), "the caches must have the head_dim of the other tensors");
+  const bool four = kc.scalar_type() == at::kByte;
+  TORCH_CHECK((kc.scalar_type() == at::kFloat8_e4m3fn || kc.scalar_type() == at::kChar || (four && ks.dim() == 4)) && vc.scalar_type() == kc.scalar_type(),
+              "the caches must both be float8_e4m3fn or int8, or uint8 with a scale for every 32 of their 4-bit codes");
   for (const Tensor* t : {&kc, &vc})
     TORCH_CHECK(t->device() == x.device() && t->stride(3) == 1, "the caches must have a contiguous last dimension, on the device of the other tensors");
+  const int64_t head_dim = four ? 2 * kc.size(3) : kc.size(3);
   for (const Tensor* t : {&ks, &vs}) {
     check_plain(*t, "a scale");
-    TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == kc.size(0) && t->size(1) == kc.size(1) && t->is_contiguous() && t->device() == x.device(),
-                "key_scale and value_scale must be contiguous fp32 [num_blocks, heads_kv] on the device of the other tensors");
+    if (four) {
+      TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 4 && t->size(0) == kc.size(0) && t->size(1) == kc.size(1) && t->size(2) == kc.size(2) &&
+                      t->size(3) * 32 == head_dim && t->is_contiguous() && t->device() == x.device(),
+                  "key_scale and value_scale of 4-bit caches must be contiguous bf16 [num_blocks, heads_kv, block_size, head_dim / 32] on the device of the other tensors");
+    } else {
+      TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) == kc.size(0) && t->size(1) == kc.size(1) && t->is_contiguous() && t->device() == x.device(),
+                  "key_scale and value_scale must be contiguous fp32 [num_blocks, heads_kv] on the device of the other tensors");
+    }
   }
   p.k_cache = kc.data_ptr();
   p.v_cache = vc.data_ptr();
-  p.k_scale = ks.data_ptr<float>();
-  p.v_scale = vs.data_ptr<float>();
+  p.k_scale = ks.data_ptr();
+  p.v_scale = vs.data_ptr();
   p.k_block_stride = kc.stride(0);
   p.k_head_stride = kc.stride(1);
   p.k_row_stride = kc.stride(2);
@@ -203,9 +210,15 @@ void cache_params(sdpa_b200_cache_params& p, const Tensor& x, const char* name, 
   p.num_blocks = to_int32(kc.size(0), "num_blocks");
   p.heads_kv = to_int32(kc.size(1), "heads_kv");
   p.block_size = to_int32(kc.size(2), "block_size");
-  p.head_dim = to_int32(kc.size(3), "head_dim");
-  p.code = kc.scalar_type() == at::kChar ? SDPA_B200_INT8 : SDPA_B200_E4M3;
-  p.dtype = x.scalar_type() == at::kHalf ? SDPA_B200_F16 : SDPA_B200_BF16;
+  p.head_dim = to_int32(head_dim, "head_dim");
+  p.code = four ? SDPA_B200_INT4 : kc.scalar_type() == at::kChar ? SDPA_B200_INT8 : SDPA_B200_E4M3;
+  p.dtype = dtype == at::kHalf ? SDPA_B200_F16 : SDPA_B200_BF16;
+}
+// The same beside 16-bit rows with the cache's head_dim
+void cache_params(sdpa_b200_cache_params& p, const Tensor& x, const char* name, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs) {
+  check_plain(x, name);
+  cache_params(p, x, x.scalar_type(), kc, vc, ks, vs);
+  TORCH_CHECK(x.size(-1) == p.head_dim, "the caches must have the head_dim of the other tensors");
 }
 
 void launch_store(const Tensor& key, const Tensor& value, const Tensor& slots, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
@@ -236,6 +249,40 @@ void launch_store(const Tensor& key, const Tensor& value, const Tensor& slots, c
   c10::cuda::CUDAGuard guard(key.device());
   check_status(sdpa_b200_cache_store(&p, stream_of(key)), "sdpa_b200_cache_store");
   for (const Tensor* t : {&key_cache, &value_cache, &key_scale, &value_scale}) written(*t);
+}
+
+std::tuple<Tensor, Tensor> launch_load(const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale, const Tensor& value_scale, const Tensor& block_table,
+                                      const Tensor& cu_seqlens, int64_t num_tokens, const c10::optional<Tensor>& first, at::ScalarType dtype) {
+  sdpa_b200_cache_params p = {};
+  check_plain(key_cache, "key_cache");
+  cache_params(p, key_cache, dtype, key_cache, value_cache, key_scale, value_scale);
+  check_table(block_table, key_cache);
+  const int64_t B = block_table.size(0);
+  check_ints(cu_seqlens, "cu_seqlens", key_cache);
+  TORCH_CHECK(cu_seqlens.dim() == 1 && cu_seqlens.size(0) == B + 1, "cu_seqlens must have requests + 1 entries");
+  if (first.has_value()) {
+    check_ints(*first, "first", key_cache);
+    TORCH_CHECK(first->dim() == 1 && first->size(0) == B, "first must be [requests]");
+  }
+  for (const Tensor* t : {&key_cache, &value_cache, &key_scale, &value_scale}) {
+    TORCH_CHECK(!needs_grad(*t), "what a cache holds has no gradient: load it under torch.no_grad()");
+    check_no_tangent(*t, "the cache");
+  }
+  TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative (got ", num_tokens, ")");
+  p.num_tokens = to_int32(num_tokens, "num_tokens");
+  c10::cuda::CUDAGuard guard(key_cache.device());
+  Tensor key = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache), value = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache);
+  if (num_tokens == 0) return {key, value};
+  p.block_table = block_table.data_ptr<int32_t>();
+  p.table_stride = table_stride(block_table);
+  p.max_blocks = to_int32(block_table.size(1), "max_blocks");
+  p.batch = to_int32(B, "requests");
+  p.cu_seqlens_k = cu_seqlens.data_ptr<int32_t>();
+  p.first = first.has_value() ? first->data_ptr<int32_t>() : nullptr;
+  p.key_out = key.data_ptr();
+  p.value_out = value.data_ptr();
+  check_status(sdpa_b200_cache_load(&p, stream_of(key_cache)), "sdpa_b200_cache_load");
+  return {key, value};
 }
 
 std::tuple<Tensor, Tensor> launch_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
@@ -295,6 +342,15 @@ void cache_store(const Tensor& key, const Tensor& value, const Tensor& slots, co
   check_all_plain({&key, &value, &slots, &key_cache, &value_cache, &key_scale, &value_scale});
   static auto op = operator_named<decltype(launch_store)>("b200_sdpa::cache_store_");
   op.call(key, value, slots, key_cache, value_cache, key_scale, value_scale);
+}
+
+std::tuple<Tensor, Tensor> cache_load(const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale, const Tensor& value_scale, const Tensor& block_table,
+                                      const Tensor& cu_seqlens, int64_t num_tokens, const c10::optional<Tensor>& first, at::ScalarType dtype) {
+  if (!calls_are_seen()) return launch_load(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, num_tokens, first, dtype);
+  check_all_plain({&key_cache, &value_cache, &key_scale, &value_scale, &block_table, &cu_seqlens});
+  if (first.has_value()) check_plain(*first, "first");
+  static auto op = operator_named<decltype(launch_load)>("b200_sdpa::cache_load");
+  return op.call(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, num_tokens, first, dtype);
 }
 
 std::tuple<Tensor, Tensor> cache_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
@@ -578,6 +634,8 @@ TORCH_LIBRARY_FRAGMENT(b200_sdpa, m) {
   m.def("plan_step_(Tensor(a!) cached_lens, Tensor new_tokens, Tensor(b!) block_table, Tensor(c!) ring, Tensor(d!) ring_state, int block_size, int num_tokens) -> "
         "(Tensor cu_seqlens, Tensor positions, Tensor slots)");
   m.def("cache_store_(Tensor key, Tensor value, Tensor slots, Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor(c!) key_scale, Tensor(d!) value_scale) -> ()");
+  m.def("cache_load(Tensor key_cache, Tensor value_cache, Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor cu_seqlens, int num_tokens, Tensor? first, "
+        "ScalarType dtype) -> (Tensor, Tensor)");
   m.def("cache_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor key_scale, Tensor value_scale, Tensor block_table, Tensor seq_lens, Tensor? cu_seqlens, "
         "int max_seqlen_q, int? max_seqlen_k, bool is_causal, float? scale) -> (Tensor, Tensor)");
 }
@@ -588,6 +646,7 @@ TORCH_LIBRARY_IMPL(b200_sdpa, CUDA, m) {
   m.impl("plan_step", b200_glue::plan_operator);
   m.impl("plan_step_", b200_glue::plan_operator_in_place);
   m.impl("cache_store_", b200_glue::launch_store);
+  m.impl("cache_load", b200_glue::launch_load);
   m.impl("cache_attention", b200_glue::launch_attention);
 }
 

@@ -98,11 +98,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> varlen_backward_with_dropout(
 at::Tensor sdpa(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& attn_mask,
                 double dropout_p, bool is_causal, c10::optional<double> scale);
 
-// serving_calls.cpp: rotary positions, the 8-bit paged cache (kv_cache.py, rotary.py)
+// serving_calls.cpp: rotary positions, the paged cache (kv_cache.py, rotary.py)
 std::vector<at::Tensor> plan_step(const at::Tensor& cached_lens, const at::Tensor& new_tokens, const at::Tensor& block_table, const at::Tensor& ring,
                                   const at::Tensor& ring_state, int64_t block_size, int64_t num_tokens, bool in_place);
 void cache_store(const at::Tensor& key, const at::Tensor& value, const at::Tensor& slots, const at::Tensor& key_cache, const at::Tensor& value_cache,
                  const at::Tensor& key_scale, const at::Tensor& value_scale);
+std::tuple<at::Tensor, at::Tensor> cache_load(const at::Tensor& key_cache, const at::Tensor& value_cache, const at::Tensor& key_scale, const at::Tensor& value_scale,
+                                             const at::Tensor& block_table, const at::Tensor& cu_seqlens, int64_t num_tokens,
+                                             const c10::optional<at::Tensor>& first, at::ScalarType dtype);
 std::tuple<at::Tensor, at::Tensor> cache_attention(const at::Tensor& query, const at::Tensor& key_cache, const at::Tensor& value_cache,
                                                    const at::Tensor& key_scale, const at::Tensor& value_scale, const at::Tensor& block_table,
                                                    const at::Tensor& seq_lens, const c10::optional<at::Tensor>& cu_seqlens, int64_t max_seqlen_q,
