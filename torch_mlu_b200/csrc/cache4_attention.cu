@@ -13,8 +13,8 @@
 // * The scale of V is taken apart: 2^e, the power of two above the token's largest, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
 //   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of the token's largest has its products' full 11 bits only where the weight is that much above
 //   the smallest normal one.
-// * The loading warps bring the scales into these forms once for all, a tile ahead: fp32 of K's, e, 2^-e and the rests of V's, NaN where a scale is no finite number, zeros behind the
-//   last token, whose codes (any byte is a finite number) therefore need no mask.
+// * The loading warps only issue copies, codes by TMA and scales by cp.async, and wait for nothing but room. A warp of the arithmetic brings the scales of V of its own tokens into these
+//   forms, a token or two a lane, beside its products with K.
 #include <type_traits>
 
 #include "cache_stream.cuh"
@@ -24,7 +24,7 @@ namespace {
 
 constexpr float kBias = 14.f;      // weights are kept times 2^14: times the rest of V's scale they fit f16
 constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
-constexpr int kFarExponents = 100;   // e of two tokens that are further apart: the smaller one's weight may not fit 32 bits though it counts
+constexpr int kFarExponents = 50;    // e that is further from the first one seen: of two tokens 2^100 apart the smaller one's weight may not fit 32 bits though it counts
 
 template <int kD>
 __host__ __device__ constexpr int tile_tokens() { return kD == 64 ? 256 : 128; }
@@ -32,9 +32,11 @@ template <int kD>
 __host__ __device__ constexpr int step_tokens() { return kD == 64 ? 64 : 32; }
 template <int kD>
 __host__ __device__ constexpr uint32_t stage_bytes() { return tile_tokens<kD>() * kD; }  // codes of K and of V
-// fp32 scales of K, e and 2^-e of each token's V, the rests by pairs of tokens, whether exponents are far apart
 template <int kD>
-__host__ __device__ constexpr uint32_t scale_bytes() { return tile_tokens<kD>() * (kD / 32 * 4 + 8 + kD / 32 * 2) + 16; }
+__host__ __device__ constexpr uint32_t scale_bytes() { return tile_tokens<kD>() * (kD / 32) * 2 * 2; }  // their scales
+// What a warp keeps of a step's scales of V, for two steps in turn: e and 2^-e of each token, the rests by pairs of tokens
+template <int kD>
+__host__ __device__ constexpr uint32_t step_scale_bytes() { return step_tokens<kD>() * (8 + kD / 32 * 2); }
 // B fragments of Q: in registers where there is room; else in shared memory, with their sums
 template <int kRowBlocks, int kD>
 __host__ __device__ constexpr bool q_in_registers() { return kRowBlocks == 1 || kD == 64; }
@@ -42,7 +44,7 @@ template <int kRowBlocks, int kRowWarps, int kD>
 __host__ __device__ constexpr uint32_t q_bytes() { return q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 32) * (512 + 32); }
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
 __host__ __device__ constexpr uint32_t smem_bytes(int stages) {
-  return 1024 + stages * (stage_bytes<kD>() + scale_bytes<kD>() + 16) + 16 + kWarps * 8 * 8 + q_bytes<kRowBlocks, kRowWarps, kD>() +
+  return 1024 + stages * (stage_bytes<kD>() + scale_bytes<kD>() + 16) + 16 + kWarps * (2 * step_scale_bytes<kD>() + 8 * 8) + q_bytes<kRowBlocks, kRowWarps, kD>() +
          (kCluster ? 32 + 8 * kRowBlocks * (kD + 1) * 4 : 0);
 }
 // Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB
@@ -85,6 +87,15 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
+__device__ __forceinline__ void copy_16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// This thread's arrival, when its copies so far are there
+__device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ const uint4 no_scales[1] = {{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}};
+
 // kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
@@ -106,11 +117,10 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t ring = (raw_addr + 1023u) & ~1023u;
   uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
-  float* k_scales = reinterpret_cast<float*>(ring_ptr + kSt * kStageBytes);             // [stage][token][group]
-  float2* v_tokens = reinterpret_cast<float2*>(k_scales + kSt * kTileTokens * kGroups);  // [stage][token]: e of its scales, kSumUnit * 2^-e
-  uint32_t* v_rests = reinterpret_cast<uint32_t*>(v_tokens + kSt * kTileTokens);         // [stage][pair of tokens][group]: f16 scales over 2^e
-  uint4* stage_far = reinterpret_cast<uint4*>(v_rests + kSt * kTileTokens / 2 * kGroups);  // [stage]
-  float2* row_state = reinterpret_cast<float2*>(stage_far + kSt);                         // [warp][row of 8]: maximum and sum
+  uint16_t* tile_scales = reinterpret_cast<uint16_t*>(ring_ptr + kSt * kStageBytes);     // [stage][K, V][token][group]
+  float2* v_tokens = reinterpret_cast<float2*>(tile_scales + kSt * 2 * kTileTokens * kGroups);  // [warp][step in turn][token]: e of its scales, kSumUnit * 2^-e
+  uint32_t* v_rests = reinterpret_cast<uint32_t*>(v_tokens + kWarps * 2 * kStepTokens);  // [warp][step in turn][pair of tokens][group]: f16 scales over 2^e
+  float2* row_state = reinterpret_cast<float2*>(v_rests + kWarps * kStepTokens * kGroups);  // [warp][row of 8]: maximum and sum
   uint4* q_state = reinterpret_cast<uint4*>(row_state + kWarps * 8);                      // [row group][block of 8 rows][group][lane]: B fragments
   constexpr int kQWords = kQInRegisters ? 0 : kRowWarps * kRowBlocks * kGroups * 32;
   float2* q_sums = reinterpret_cast<float2*>(q_state + kQWords);                           // [row group][block of 8 rows][group][t]
@@ -126,7 +136,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   if (kCluster && threadIdx.x < kRowsOfWarp) own_lse[threadIdx.x] = -INFINITY;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
-      mbar_init(full + 8 * i, 2);
+      mbar_init(full + 8 * i, 64);  // every lane of the loading warps, when its scales are there
       mbar_init(empty + 8 * i, kWarps);
     }
     *abort_flag = 0;
@@ -140,7 +150,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   if (share.places > 0 && warp >= kWarps) {
     // ================================================================ the loading warps, one for K and one for V
     // Lane i has page 32 * group + i of a unit: its block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page). Three groups are under
-    // way: the one that tiles are copied from, the next, and the one behind. Scales come a tile ahead, those of two neighbouring tokens (never of two pages) a load.
+    // way: the one that tiles are copied from, the next, and the one behind.
     const bool keys = warp == kWarps;
     const CUtensorMap* map = keys ? &tm_k : &tm_v;
     const uint16_t* scales = static_cast<const uint16_t*>(keys ? p.k_scale : p.v_scale);
@@ -163,23 +173,6 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       const int id = page < p.max_blocks && !longer_than_table(x.r) ? p.block_table[x.r.index * p.table_stride + page] : -1;
       return id >= 0 && id < p.num_blocks ? id : p.num_blocks;
     };
-    constexpr int kTimes = kTileTokens / 64;  // pairs of tokens of a lane
-    using Pair = std::conditional_t<kD == 128, uint4, uint2>;
-    struct Raw {
-      Pair pair[kTimes];
-    };
-    // bf16 scales of the pairs lane, lane + 32, ... of the tile whose first page is lane page0's
-    auto load_scales = [&](Raw& raw, int page0, int ids, int head) {
-#pragma unroll
-      for (int i = 0; i < kTimes; ++i) {
-        const int tok = 2 * (lane + 32 * i), id = __shfl_sync(0xffffffffu, ids, (page0 + (tok >> p.shift)) & 31);
-        const uint32_t none = keys && id == p.num_blocks ? 0x7fc07fc0u : 0u;  // no such block: the scores of those who see it are NaN
-        if constexpr (kD == 128) raw.pair[i] = make_uint4(none, none, none, none);
-        else raw.pair[i] = make_uint2(none, none);
-        if (id >= 0 && id < p.num_blocks)
-          raw.pair[i] = *reinterpret_cast<const Pair*>(scales + (((static_cast<int64_t>(id) * p.heads_kv + head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups);
-      }
-    };
     Place cur, nxt, far;
     cur.r = share.request;
     cur.unit = share.unit;
@@ -195,20 +188,13 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       far_id = block_at(far);
     };
     const int pages = kTileTokens >> p.shift;  // of a tile
-    bool ok = true, far_apart = false;
-    int least_e = 1000, largest_e = -1000;     // of V's scales so far
+    bool ok = true, first = true;
     int step = 0;
-    bool first = true;
-    Raw raw, ahead;
     for (int places = share.places; places > 0;) {
       const int page0 = (tile * kTileTokens) >> p.shift;
       if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
-      const int tile_tok = tile * kTileTokens;
-      const bool tokens = tile_tok < cur.r.len;
-      const uint32_t st = step % kSt, bar = full + 8 * st;
-      if (first) load_scales(raw, page0, id, cur.head);
-      if (tokens) {
-        const uint32_t dst = ring + st * kStageBytes + (keys ? 0u : kTileTokens * kRowBytes);
+      if (tile * kTileTokens < cur.r.len) {
+        const uint32_t st = step % kSt, bar = full + 8 * st, dst = ring + st * kStageBytes + (keys ? 0u : kTileTokens * kRowBytes);
         if (ok && step >= kSt) ok = mbar_wait(empty + 8 * st, (step / kSt + 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -226,6 +212,18 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               if (i + e < n) tma_load_4d(dst + ((i + e) << p.shift) * kRowBytes, map, bar, 0, 0, cur.head, blocks[e]);
           }
         }
+        // 16 bytes of scales at a time, of one page; those of a block that is not there are NaN, those behind the last page stay what they are
+        constexpr int kTokensAtOnce = 8 / kGroups;
+        const uint32_t scale_dst = smem_u32(tile_scales + (2 * st + (keys ? 0 : 1)) * kTileTokens * kGroups);
+#pragma unroll
+        for (int i = 0; i < kTileTokens / kTokensAtOnce / 32; ++i) {
+          const int tok = (lane + 32 * i) * kTokensAtOnce, block = __shfl_sync(0xffffffffu, mine, tok >> p.shift);
+          const uint16_t* src = scales + (((static_cast<int64_t>(block) * p.heads_kv + cur.head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups;
+          if (block == p.num_blocks) src = reinterpret_cast<const uint16_t*>(no_scales);
+          if (block >= 0) copy_16_async(scale_dst + (lane + 32 * i) * 16, src);
+        }
+        arrive_behind_copies(bar);
+        ++step;
       }
       if (first) {  // the first copies are under way
         advance(nxt);
@@ -235,76 +233,6 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         far_id = block_at(far);
         first = false;
       }
-      {  // the next tile's scales: it is the unit's next, in this group or the next one, or the first of the unit behind
-        const int next_page0 = ((tile + 1) * kTileTokens) >> p.shift;
-        const bool more = tile + 1 < cur.r.tiles, here = more && next_page0 >> 5 == cur.group;
-        load_scales(ahead, more ? next_page0 : 0, here ? id : next_id, here ? cur.head : nxt.head);
-      }
-      if (tokens) {
-#pragma unroll
-        for (int i = 0; i < kTimes; ++i) {
-          const int pair = lane + 32 * i;
-          uint32_t words[kGroups];  // the first token's, then the second's
-          words[0] = raw.pair[i].x, words[1] = raw.pair[i].y;
-          if constexpr (kD == 128) words[2] = raw.pair[i].z, words[3] = raw.pair[i].w;
-          if (keys) {
-            float f[2 * kGroups];
-#pragma unroll
-            for (int e = 0; e < kGroups; ++e) {
-              f[2 * e] = __uint_as_float(words[e] << 16);
-              f[2 * e + 1] = __uint_as_float(words[e] & 0xffff0000u);
-            }
-#pragma unroll
-            for (int e = 0; e < 2 * kGroups; ++e)
-              if (fabsf(f[e]) == INFINITY) f[e] = __int_as_float(0x7fffffff);
-            float4* dst = reinterpret_cast<float4*>(k_scales + (st * kTileTokens + 2 * pair) * kGroups);
-#pragma unroll
-            for (int e = 0; e < kGroups / 2; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-          } else {
-            float2 of_token[2];
-            uint32_t rests[kGroups] = {};
-#pragma unroll
-            for (int tok = 0; tok < 2; ++tok) {
-              const bool there = tile_tok + 2 * pair + tok < cur.r.len;
-              uint32_t bits[kGroups], top = 0u;
-#pragma unroll
-              for (int e = 0; e < kGroups; ++e) {
-                const uint32_t w = words[tok * kGroups / 2 + e / 2];
-                bits[e] = there ? e & 1 ? w >> 16 : w & 0xffffu : 0u;
-                top = max(top, bits[e] & 0x7fffu);
-              }
-              const bool bad = top >= 0x7f80u;
-              if (bad) top = 0u;
-              const int e2 = top == 0u ? 0 : min(max(static_cast<int>(top >> 7) - 126, kLeastExponent), 126);
-              if (top != 0u) {
-                least_e = min(least_e, e2);
-                largest_e = max(largest_e, e2);
-              }
-              const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);  // 2^-e
-              of_token[tok] = make_float2(bad ? __int_as_float(0x7fffffff) : static_cast<float>(e2), kSumUnit * down);
-#pragma unroll
-              for (int e = 0; e < kGroups; ++e) {
-                const uint32_t h = pack_f16x2(bad ? 0.f : __uint_as_float(bits[e] << 16) * down, 0.f) & 0xffffu;
-                rests[e] |= tok ? h << 16 : h;
-              }
-            }
-            *reinterpret_cast<float4*>(v_tokens + st * kTileTokens + 2 * pair) = make_float4(of_token[0].x, of_token[0].y, of_token[1].x, of_token[1].y);
-            uint32_t* dst = v_rests + (st * (kTileTokens / 2) + pair) * kGroups;
-            if constexpr (kGroups == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(rests[0], rests[1], rests[2], rests[3]);
-            else *reinterpret_cast<uint2*>(dst) = make_uint2(rests[0], rests[1]);
-          }
-        }
-        if (!keys) {
-          least_e = __reduce_min_sync(0xffffffffu, least_e);
-          largest_e = __reduce_max_sync(0xffffffffu, largest_e);
-          far_apart = far_apart || largest_e - least_e > kFarExponents;
-          if (lane == 0) stage_far[st].x = far_apart;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
-        ++step;
-      }
-      raw = ahead;
       --places;
       if (++tile == cur.r.tiles) {
         tile = 0;
@@ -325,8 +253,10 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       if constexpr (kD == 128) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
       return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
     };
-    bool ok = true;
+    bool ok = true, far_apart = false;
+    int first_e = 1000;  // of V's scales, the first that this warp has seen
     int step = 0;  // tiles read
+    int turn = 0;  // of the places for a step's scales
     Request r = share.request;
     int unit = share.unit, tile = share.tile;
     Request next_r = r;
@@ -438,13 +368,61 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         __syncwarp();
+        // ---- the scales of V of a step: a lane has one token, or two with half as many groups
+        auto take_scales = [&](int c) {
+          const int in_tile = part * kPartTokens + c;
+          constexpr int kOfLane = kStepTokens / 32;
+          const uint16_t* src = tile_scales + ((2 * st + 1) * kTileTokens + in_tile + kOfLane * lane) * kGroups;
+          const uint2 raw = *reinterpret_cast<const uint2*>(src);
+          const uint32_t words[2] = {raw.x, raw.y};
+          uint32_t rest[2];
+          float2 of_token[kOfLane];
+          int e2s[kOfLane];
+#pragma unroll
+          for (int x = 0; x < kOfLane; ++x) {
+            uint32_t w[2 / kOfLane], top = 0u;
+            const bool there = tile_tok + in_tile + kOfLane * lane + x < r.len;
+#pragma unroll
+            for (int e = 0; e < 2 / kOfLane; ++e) {
+              w[e] = there ? words[kOfLane == 1 ? e : x] : 0u;
+              top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+            }
+            top = max(top & 0xffffu, top >> 16);
+            const bool bad = top >= 0x7f80u;
+            const int e2 = bad || top == 0u ? 0 : min(max(static_cast<int>(top >> 7) - 126, kLeastExponent), 126);
+            e2s[x] = e2;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);  // 2^-e
+            of_token[x] = make_float2(bad ? __int_as_float(0x7fffffff) : static_cast<float>(e2), kSumUnit * down);
+#pragma unroll
+            for (int e = 0; e < 2 / kOfLane; ++e)
+              rest[kOfLane == 1 ? e : x] = bad ? 0u : pack_f16x2(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
+          }
+          float2* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
+          uint32_t* rests = v_rests + (2 * warp + turn) * (kStepTokens / 2) * kGroups;
+          if constexpr (kOfLane == 1) {
+            tokens[0] = of_token[0];
+            // lanes of a pair of tokens: the even one has groups 0 and 1 of both, the odd one 2 and 3
+            const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? rest[0] : rest[1], 1);
+            const uint32_t near = lane & 1 ? other : rest[0], behind = lane & 1 ? rest[1] : other;
+            *reinterpret_cast<uint2*>(rests + 2 * lane) = make_uint2(__byte_perm(near, behind, 0x5410), __byte_perm(near, behind, 0x7632));
+          } else {
+            *reinterpret_cast<float4*>(tokens) = make_float4(of_token[0].x, of_token[0].y, of_token[kOfLane - 1].x, of_token[kOfLane - 1].y);
+            *reinterpret_cast<uint2*>(rests + 2 * lane) = make_uint2(__byte_perm(rest[0], rest[1], 0x5410), __byte_perm(rest[0], rest[1], 0x7632));
+          }
+          if (first_e == 1000) first_e = __shfl_sync(0xffffffffu, e2s[0], 0);
+          bool is_far = false;
+#pragma unroll
+          for (int x = 0; x < kOfLane; ++x) is_far = is_far || abs(e2s[x] - first_e) > kFarExponents;
+          far_apart = __any_sync(0xffffffffu, is_far) || far_apart;
+          __syncwarp();
+        };
         auto work_on = [&](int c, auto far_tag) {
           constexpr bool kFar = decltype(far_tag)::value;
           const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
           // ---- S^T = K Q^T, 16 tokens and 32 dimensions at a time
           // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
           const uint32_t k_smem = ring + st * kStageBytes + in_tile * kRowBytes;
-          const float* ks = k_scales + (st * kTileTokens + in_tile + g) * kGroups;
+          const uint16_t* ks = tile_scales + (2 * st * kTileTokens + in_tile + g) * kGroups;
           float s[kRowBlocks][kHalves][4];
 #pragma unroll
           for (int ch = 0; ch < kGroups; ch += 2) {
@@ -466,13 +444,13 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             for (int half = 0; half < kHalves; ++half) {
               uint32_t kf[4];  // tokens 0-7 and 8-15 of a group, the same of the next
               ldmatrix_x4(k_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), kf);
-              const float2 near = *reinterpret_cast<const float2*>(ks + half * 16 * kGroups + ch), behind = *reinterpret_cast<const float2*>(ks + (half * 16 + 8) * kGroups + ch);
+              const uint32_t near = *reinterpret_cast<const uint32_t*>(ks + half * 16 * kGroups + ch), behind = *reinterpret_cast<const uint32_t*>(ks + (half * 16 + 8) * kGroups + ch);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t x[4], y[4];
                 codes_to_subnormal(kf[2 * e], x);
                 codes_to_subnormal(kf[2 * e + 1], y);
-                const float kg = e ? near.y : near.x, kg8 = e ? behind.y : behind.x;
+                const float kg = __uint_as_float(e ? near & 0xffff0000u : near << 16), kg8 = __uint_as_float(e ? behind & 0xffff0000u : behind << 16);
 #pragma unroll
                 for (int nb = 0; nb < kRowBlocks; ++nb) {
                   float a[4] = {begin[e][nb].x, begin[e][nb].y, begin[e][nb].x, begin[e][nb].y};
@@ -499,8 +477,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           float2 near[kHalves], behind[kHalves];  // e and kSumUnit * 2^-e of tokens g, g + 8
 #pragma unroll
           for (int half = 0; half < kHalves; ++half) {
-            near[half] = v_tokens[st * kTileTokens + in_tile + half * 16 + g];
-            behind[half] = v_tokens[st * kTileTokens + in_tile + half * 16 + 8 + g];
+            near[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + g];
+            behind[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + 8 + g];
           }
           uint32_t pb[kRowBlocks][kHalves][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
           bool moved = false;
@@ -510,6 +488,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             // scores and e, masked where a row ends inside the step
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[nb][half][e] = fmaf(s[nb][half][e], 0.f, s[nb][half][e]);  // an infinite scale: NaN
               s[nb][half][0] = fmaf(s[nb][half][0], factor[nb].x, near[half].x);
               s[nb][half][1] = fmaf(s[nb][half][1], factor[nb].y, near[half].x);
               s[nb][half][2] = fmaf(s[nb][half][2], factor[nb].x, behind[half].x);
@@ -578,7 +558,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           }
           // ---- O^T += V^T W^T, 16 tokens and 32 dimensions at a time
           const uint32_t v_smem = ring + st * kStageBytes + (kTileTokens + in_tile) * kRowBytes;
-          const uint32_t* rests = v_rests + (st * (kTileTokens / 2) + in_tile / 2 + t) * kGroups;
+          const uint32_t* rests = v_rests + ((2 * warp + turn) * (kStepTokens / 2) + t) * kGroups;
 #pragma unroll
           for (int half = 0; half < kHalves; ++half) {
 #pragma unroll
@@ -602,12 +582,12 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           }
         };
         const int end = min(kPartTokens, seen_by_any - tile_tok - part * kPartTokens);
-        if (stage_far[st].x == 0u) {
 #pragma unroll 1
-          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::false_type{});
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < end; c += kStepTokens) work_on(c, std::true_type{});
+        for (int c = 0; c < end; c += kStepTokens) {
+          take_scales(c);
+          if (!far_apart) work_on(c, std::false_type{});
+          else work_on(c, std::true_type{});
+          turn ^= 1;
         }
         // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
         if (i + 1 < seg_tiles) {
