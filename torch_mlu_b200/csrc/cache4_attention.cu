@@ -9,7 +9,7 @@
 //   ones 16 times that, for which Q is divided by 16. The 8 comes off in the accumulators, which begin with -8 * 2^-24 * sum of the group's q instead of 0: u is small, so
 //   that the sums lose three of fp32's bits to it.
 // * The scale of K goes onto the group's fp32 sums: 4 multiply-adds for each 32 x 16 codes a warp converts, where scaling the codes would take 8.
-// * Codes of V become whole f16 numbers (0x6400 | u is 1024 + u): sums over tens of thousands of tokens would lose too much to an offset.
+// * Codes of V become code * 2^-9 by one multiply-add each two more: sums over tens of thousands of tokens would lose too much to an offset.
 // * The scale of V is taken apart: 2^e, the power of two above the token's largest, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
 //   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of the token's largest has its products' full 11 bits only where the weight is that much above
 //   the smallest normal one.
@@ -55,31 +55,25 @@ __host__ __device__ constexpr int ring_stages() {
   return n;
 }
 
-// Eight codes as f16 pairs (n, n + 4), n = 0..3: u * 2^-24 for even n, 16 times that for odd n, u = code + 8
-__device__ __forceinline__ void codes_to_subnormal(uint32_t w, uint32_t (&x)[4]) {
-  const uint32_t v = w >> 8;
-  x[0] = (w & 0x000f000fu) ^ 0x00080008u;
-  x[1] = (w & 0x00f000f0u) ^ 0x00800080u;
-  x[2] = (v & 0x000f000fu) ^ 0x00080008u;
-  x[3] = (v & 0x00f000f0u) ^ 0x00800080u;
+// Eight codes as f16 pairs (n, n + 4), n = 0..3: the subnormals u * 2^-24 for even n, 16 times that for odd n, u = code + 8. `eights` are 0x00080008 and 0x00800080, in registers: with
+// the mask as an immediate operand a pair is one instruction then.
+__device__ __forceinline__ void codes_to_subnormal(uint32_t w, const uint32_t (&eights)[2], uint32_t (&x)[4]) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n)  // (w & mask) ^ eights
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(x[n]) : "r"(n < 2 ? w : w >> 8), "r"(n & 1 ? 0x00f000f0u : 0x000f000fu), "r"(eights[n & 1]));
 }
-// The same as the codes' values: 0x6400 | u is 1024 + u, with 16 u in its place 64 times 16 + u / 4
-__device__ __forceinline__ void codes_to_numbers(uint32_t w, uint32_t (&x)[4]) {
-  const uint32_t v = w >> 8;
-  auto low = [](uint32_t y) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"((y & 0x000f000fu) ^ 0x64086408u), "r"(0x64086408u));  // - 1032
-    return r;
-  };
-  auto high = [](uint32_t y) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"((y & 0x00f000f0u) ^ 0x64806480u), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
-    return r;
-  };
-  x[0] = low(w);
-  x[1] = high(w);
-  x[2] = low(v);
-  x[3] = high(v);
+// The same as normal numbers, code * 2^-9
+__device__ __forceinline__ void codes_to_numbers(uint32_t w, const uint32_t (&eights)[2], uint32_t (&x)[4]) {
+  codes_to_subnormal(w, eights, x);
+#pragma unroll
+  for (int n = 0; n < 4; ++n)  // times 2^15 or 2^11, minus 8 * 2^-9
+    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x[n]) : "r"(n & 1 ? 0x68006800u : 0x78007800u), "r"(0xa400a400u));
+}
+// D = A B + C, C elsewhere than D
+__device__ __forceinline__ void mma_16816_from(float (&d)[4], const float4& c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -257,6 +251,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     int first_e = 1000;  // of V's scales, the first that this warp has seen
     int step = 0;  // tiles read
     int turn = 0;  // of the places for a step's scales
+    const uint32_t none = *abort_flag & 0x40000000u;  // 0, which the compiler does not know: so that these stay in registers
+    const uint32_t eights[2] = {0x00080008u | none, 0x00800080u | none};
     Request r = share.request;
     int unit = share.unit, tile = share.tile;
     Request next_r = r;
@@ -270,7 +266,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       const int my_row0 = row0 + kRowsOfWarp * row_group;
       // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 8t..8t+7 of every 32: pairs (n, n + 4), those of odd n over 16
       uint4 qb[kRowBlocks][kQInRegisters ? kGroups : 1];
-      float2 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit
+      float4 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1, 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit
       uint4* my_q = q_state + row_group * kRowBlocks * kGroups * 32 + lane;
       float2* my_sums = q_sums + row_group * kRowBlocks * kGroups * 4;
       float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale and the 2^24 that the products lack
@@ -320,7 +316,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           const float2 sums = make_float2(__shfl_sync(0xffffffffu, sum, 8 * t), __shfl_sync(0xffffffffu, sum, 8 * t + 4));
           if constexpr (kQInRegisters) {
             qb[nb][k] = packed;
-            qs[nb][k] = sums;
+            qs[nb][k] = make_float4(sums.x, sums.y, sums.x, sums.y);
           } else if (part == 0) {
             my_q[(nb * kGroups + k) * 32] = packed;
             if (g == 0) my_sums[(nb * kGroups + k) * 4 + t] = sums;
@@ -427,7 +423,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
           for (int ch = 0; ch < kGroups; ch += 2) {
             uint4 q[2][kRowBlocks];
-            float2 begin[2][kRowBlocks];
+            float4 begin[2][kRowBlocks];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -437,7 +433,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                   begin[e][nb] = qs[nb][ch + e];
                 } else {
                   q[e][nb] = my_q[(nb * kGroups + ch + e) * 32];
-                  begin[e][nb] = my_sums[(nb * kGroups + ch + e) * 4 + t];
+                  const float2 sums = my_sums[(nb * kGroups + ch + e) * 4 + t];
+                  begin[e][nb] = make_float4(sums.x, sums.y, sums.x, sums.y);
                 }
               }
 #pragma unroll
@@ -448,13 +445,13 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t x[4], y[4];
-                codes_to_subnormal(kf[2 * e], x);
-                codes_to_subnormal(kf[2 * e + 1], y);
+                codes_to_subnormal(kf[2 * e], eights, x);
+                codes_to_subnormal(kf[2 * e + 1], eights, y);
                 const float kg = __uint_as_float(e ? near & 0xffff0000u : near << 16), kg8 = __uint_as_float(e ? behind & 0xffff0000u : behind << 16);
 #pragma unroll
                 for (int nb = 0; nb < kRowBlocks; ++nb) {
-                  float a[4] = {begin[e][nb].x, begin[e][nb].y, begin[e][nb].x, begin[e][nb].y};
-                  mma_16816<true>(a, x[0], y[0], x[1], y[1], q[e][nb].x, q[e][nb].y);
+                  float a[4];
+                  mma_16816_from(a, begin[e][nb], x[0], y[0], x[1], y[1], q[e][nb].x, q[e][nb].y);
                   mma_16816<true>(a, x[2], y[2], x[3], y[3], q[e][nb].z, q[e][nb].w);
                   if (ch + e == 0) {
                     s[nb][half][0] = a[0] * kg, s[nb][half][1] = a[1] * kg, s[nb][half][2] = a[2] * kg8, s[nb][half][3] = a[3] * kg8;
@@ -569,8 +566,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t x[4], y[4];  // f16 pairs of two tokens: dimensions 4g to 4g + 3
-                codes_to_numbers(vf[2 * e], x);
-                codes_to_numbers(vf[2 * e + 1], y);
+                codes_to_numbers(vf[2 * e], eights, x);
+                codes_to_numbers(vf[2 * e + 1], eights, y);
 #pragma unroll
                 for (int nb = 0; nb < kRowBlocks; ++nb) {
                   const uint32_t w0 = mul_f16x2(pb[nb][half][0], e ? rest.y : rest.x), w1 = mul_f16x2(pb[nb][half][1], e ? rest8.y : rest8.x);
@@ -657,7 +654,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         for (int x = 0; x < 2; ++x) {
           const int row = my_row0 + 8 * nb + 2 * t + x;
           if (row >= row0 + n_rows) continue;
-          const float inv = sum[x] > 0.f ? kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN
+          const float inv = sum[x] > 0.f ? 0x1p9f * kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN; codes were over 2^9
           const float lse2 = sum[x] == 0.f ? -INFINITY : mm[x] - kBias - log2f(kSumUnit) + log2f(sum[x]);
           auto dim_of = [&](int ch) { return 32 * ((part * kMine + ch) >> 1) + 4 * g + 2 * ((part * kMine + ch) & 1); };
           if (whole) {
