@@ -26,6 +26,11 @@ constexpr float kBias = 14.f;      // weights are kept times 2^14: times the res
 constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
 constexpr int kFarExponents = 50;    // e that is further from the first one seen: of two tokens 2^100 apart the smaller one's weight may not fit 32 bits though it counts
 
+// Loading warps: one for K and one for V, or, where an SM has three CTAs and each of them more time for a tile, one for both
+template <int kRowBlocks>
+__host__ __device__ constexpr int loading_warps() { return stream4_ctas_per_sm(8 * kRowBlocks) > 2 ? 1 : 2; }
+template <int kRowBlocks>
+__host__ __device__ constexpr int threads() { return (kWarps + loading_warps<kRowBlocks>()) * 32; }
 template <int kD>
 __host__ __device__ constexpr int tile_tokens() { return kD == 64 ? 256 : 128; }
 template <int kD>
@@ -37,9 +42,9 @@ __host__ __device__ constexpr uint32_t scale_bytes() { return tile_tokens<kD>() 
 // What a warp keeps of a step's scales of V, for two steps in turn: e and 2^-e of each token, the rests by pairs of tokens
 template <int kD>
 __host__ __device__ constexpr uint32_t step_scale_bytes() { return step_tokens<kD>() * (8 + kD / 32 * 2); }
-// B fragments of Q: in registers where there is room; else in shared memory, with their sums
+// B fragments of Q: in registers where there is room; else in shared memory, with their sums (8 rows, head_dim 128: 332 us so, 339 from registers that spill, 64 requests of 2048 to 32768)
 template <int kRowBlocks, int kD>
-__host__ __device__ constexpr bool q_in_registers() { return kRowBlocks == 1 || kD == 64; }
+__host__ __device__ constexpr bool q_in_registers() { return kD == 64; }
 template <int kRowBlocks, int kRowWarps, int kD>
 __host__ __device__ constexpr uint32_t q_bytes() { return q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 32) * (512 + 32); }
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
@@ -47,11 +52,11 @@ __host__ __device__ constexpr uint32_t smem_bytes(int stages) {
   return 1024 + stages * (stage_bytes<kD>() + scale_bytes<kD>() + 16) + 16 + kWarps * (2 * step_scale_bytes<kD>() + 8 * 8) + q_bytes<kRowBlocks, kRowWarps, kD>() +
          (kCluster ? 32 + 8 * kRowBlocks * (kD + 1) * 4 : 0);
 }
-// Tiles in a CTA's ring: what lets two CTAs share an SM's 228 KB
+// Tiles in a CTA's ring: what lets an SM's CTAs share its 228 KB
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
 __host__ __device__ constexpr int ring_stages() {
   int n = 5;
-  while (kCtasPerSm * (smem_bytes<kRowBlocks, kRowWarps, kD, kCluster>(n) + 1024) > 228 * 1024) --n;
+  while (stream4_ctas_per_sm(8 * kRowBlocks) * (smem_bytes<kRowBlocks, kRowWarps, kD, kCluster>(n) + 1024) > 228 * 1024) --n;
   return n;
 }
 
@@ -92,8 +97,9 @@ __device__ const uint4 no_scales[1] = {{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0
 
 // kRowBlocks: blocks of 8 rows of a warp. kRowWarps: groups of that many rows of a unit; the warps of a group share the tile's tokens.
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+__global__ void __launch_bounds__(threads<kRowBlocks>(), stream4_ctas_per_sm(8 * kRowBlocks))
 cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StreamParams p) {
+  constexpr int kLoaders = loading_warps<kRowBlocks>();
   constexpr int kGroups = kD / 32;
   constexpr int kChunks = kD / 16;                           // of 16 dimensions, an MMA each
   constexpr int kRowBytes = kD / 2;
@@ -130,24 +136,22 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   if (kCluster && threadIdx.x < kRowsOfWarp) own_lse[threadIdx.x] = -INFINITY;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSt; ++i) {
-      mbar_init(full + 8 * i, 64);  // every lane of the loading warps, when its scales are there
+      mbar_init(full + 8 * i, 32 * kLoaders);  // every lane of the loading warps, when its scales are there
       mbar_init(empty + 8 * i, kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp >= kWarps && elect_one()) tma_prefetch_desc(warp == kWarps ? &tm_k : &tm_v);
+  if (warp == kWarps && elect_one()) tma_prefetch_desc(&tm_k);
+  if (warp == kWarps + kLoaders - 1 && elect_one()) tma_prefetch_desc(&tm_v);
   __syncthreads();
   wait_for_previous_grid();
   if (threadIdx.x == 0) launch_dependents();  // behind the wait: the merge kernel's blocks wait for this grid only
   const Share share = kCluster ? share_in_cluster(p, blockIdx.x) : share_of(p, blockIdx.x, lane);
   if (share.places > 0 && warp >= kWarps) {
-    // ================================================================ the loading warps, one for K and one for V
+    // ================================================================ the loading warps
     // Lane i has page 32 * group + i of a unit: its block number (num_blocks: none in the cache, behind which the copy finds zeros; -1: no such page). Three groups are under
     // way: the one that tiles are copied from, the next, and the one behind.
-    const bool keys = warp == kWarps;
-    const CUtensorMap* map = keys ? &tm_k : &tm_v;
-    const uint16_t* scales = static_cast<const uint16_t*>(keys ? p.k_scale : p.v_scale);
     struct Place {
       Request r;
       int unit, group, head;
@@ -188,13 +192,15 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       const int page0 = (tile * kTileTokens) >> p.shift;
       if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
       if (tile * kTileTokens < cur.r.len) {
-        const uint32_t st = step % kSt, bar = full + 8 * st, dst = ring + st * kStageBytes + (keys ? 0u : kTileTokens * kRowBytes);
+        const uint32_t st = step % kSt, bar = full + 8 * st;
         if (ok && step >= kSt) ok = mbar_wait(empty + 8 * st, (step / kSt + 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         const int mine = __shfl_sync(0xffffffffu, id, ((page0 & 31) + lane) & 31);
         const int n = __popc(__ballot_sync(0xffffffffu, lane < pages && mine >= 0));
-        if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(n << p.shift) * kRowBytes);
+        const int sides = kLoaders == 1 ? 2 : 1;
+        if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(sides * n << p.shift) * kRowBytes);
+        const uint32_t dst = ring + st * kStageBytes;
 #pragma unroll 1
         for (int i = 0; i < n; i += 4) {
           int blocks[4];
@@ -202,19 +208,26 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, mine, (i + e) & 31);
           if (elect_one()) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e < n) tma_load_4d(dst + ((i + e) << p.shift) * kRowBytes, map, bar, 0, 0, cur.head, blocks[e]);
+            for (int e = 0; e < 4; ++e) {
+              if (i + e >= n) continue;
+              const uint32_t page_dst = dst + ((i + e) << p.shift) * kRowBytes;
+              if (warp == kWarps) tma_load_4d(page_dst, &tm_k, bar, 0, 0, cur.head, blocks[e]);
+              if (warp == kWarps + kLoaders - 1) tma_load_4d(page_dst + kTileTokens * kRowBytes, &tm_v, bar, 0, 0, cur.head, blocks[e]);
+            }
           }
         }
         // 16 bytes of scales at a time, of one page; those of a block that is not there are NaN, those behind the last page stay what they are
         constexpr int kTokensAtOnce = 8 / kGroups;
-        const uint32_t scale_dst = smem_u32(tile_scales + (2 * st + (keys ? 0 : 1)) * kTileTokens * kGroups);
+        const uint32_t scale_dst = smem_u32(tile_scales + 2 * st * kTileTokens * kGroups);
 #pragma unroll
         for (int i = 0; i < kTileTokens / kTokensAtOnce / 32; ++i) {
           const int tok = (lane + 32 * i) * kTokensAtOnce, block = __shfl_sync(0xffffffffu, mine, tok >> p.shift);
-          const uint16_t* src = scales + (((static_cast<int64_t>(block) * p.heads_kv + cur.head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups;
-          if (block == p.num_blocks) src = reinterpret_cast<const uint16_t*>(no_scales);
-          if (block >= 0) copy_16_async(scale_dst + (lane + 32 * i) * 16, src);
+          const int64_t at = (((static_cast<int64_t>(block) * p.heads_kv + cur.head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups;
+          const bool none = block == p.num_blocks;
+          if (block < 0) continue;
+          if (warp == kWarps) copy_16_async(scale_dst + (lane + 32 * i) * 16, none ? no_scales : static_cast<const void*>(static_cast<const uint16_t*>(p.k_scale) + at));
+          if (warp == kWarps + kLoaders - 1)
+            copy_16_async(scale_dst + kTileTokens * kGroups * 2 + (lane + 32 * i) * 16, none ? no_scales : static_cast<const void*>(static_cast<const uint16_t*>(p.v_scale) + at));
         }
         arrive_behind_copies(bar);
         ++step;
@@ -691,7 +704,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   }
   if constexpr (kCluster) {
     cluster_sync();  // every CTA's part is written
-    merge_in_cluster<kD>(p, share, own_part, own_lse, warp, lane);
+    merge_in_cluster<kD, kWarps + kLoaders>(p, share, own_part, own_lse, warp, lane);
     cluster_sync();  // the others have read this CTA's
   } else {
     if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
@@ -706,7 +719,7 @@ cudaError_t launch_as(const StreamParams& p, const CUtensorMap& tm_k, const CUte
   auto kernel = cache4_stream_kernel<kRowBlocks, kRowWarps, kD, kCluster>;
   const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return err;
-  return launch_behind(kernel, dim3(p.grid), kThreads, kSmem, stream, overlap, kCluster ? p.cluster : 1, tm_k, tm_v, p);
+  return launch_behind(kernel, dim3(p.grid), threads<kRowBlocks>(), kSmem, stream, overlap, kCluster ? p.cluster : 1, tm_k, tm_v, p);
 }
 
 template <int kD>

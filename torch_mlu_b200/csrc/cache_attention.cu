@@ -594,7 +594,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   }
   if constexpr (kCluster) {
     cluster_sync();  // every CTA's part is written
-    merge_in_cluster<kD>(p, share, own_part, own_lse, warp, lane);
+    merge_in_cluster<kD, kWarps + 2>(p, share, own_part, own_lse, warp, lane);
     cluster_sync();  // the others have read this CTA's
   } else {
     if (threadIdx.x == 0) p.shared_units[blockIdx.x] = left;
@@ -861,6 +861,8 @@ int unit_rows(const sdpa_b200_cache_params& p) {
   return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
+int ctas_per_sm(const sdpa_b200_cache_params& p) { return p.code == SDPA_B200_INT4 ? stream4_ctas_per_sm(unit_rows(p)) : kCtasPerSm; }
+
 size_t round_256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Where the units are few and short, a cluster of 2 to 8 CTAs takes each, the tiles in equal stretches, and merges its parts through distributed shared memory: no lengths to be
@@ -929,12 +931,13 @@ int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* w
   // a CTA per tile, up to one wave
   const int64_t units = static_cast<int64_t>(count) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
   const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + (1 << p.tile_shift) - 1) >> p.tile_shift);
-  p.grid = static_cast<int>(tiles < kCtasPerSm * sms ? tiles : kCtasPerSm * sms);
+  const int ctas = ctas_per_sm(c);
+  p.grid = static_cast<int>(tiles < ctas * sms ? tiles : ctas * sms);
   // a cluster for each unit
   p.units_each = static_cast<int>(units / count);
   p.cluster = cluster_of(c, p.rows, units, p.tile_shift);
   if (p.cluster > 0) p.grid = static_cast<int>(units) * p.cluster;
-  const size_t rows = static_cast<size_t>(kCtasPerSm) * kMaxSms * 2 * p.rows;
+  const size_t rows = static_cast<size_t>(ctas) * kMaxSms * 2 * p.rows;
   p.part_o = reinterpret_cast<float*>(workspace + kWorkspaceHeaderBytes);
   p.part_lse = p.part_o + rows * c.head_dim;
   p.shared_units = reinterpret_cast<SharedUnit*>(p.part_lse + rows);
@@ -1080,7 +1083,7 @@ size_t workspace_bytes_of(const sdpa_b200_cache_params& p) {
     const size_t n = gathered_at_once(p);
     return 2 * kWorkspaceHeaderBytes + n * gathered_bytes(p) + round_256((4 * n + 2) * 4);
   }
-  const size_t ctas = static_cast<size_t>(kCtasPerSm) * kMaxSms;
+  const size_t ctas = static_cast<size_t>(ctas_per_sm(p)) * kMaxSms;
   return kWorkspaceHeaderBytes + round_256(ctas * 2 * unit_rows(p) * (p.head_dim + 1) * 4 + ctas * sizeof(SharedUnit));
 }
 

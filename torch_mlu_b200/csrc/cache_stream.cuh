@@ -35,6 +35,8 @@ struct StreamParams {
   float scale_log2;
 };
 
+// CTAs of the kernel for 4-bit codes on an SM, by the rows of a unit
+__host__ __device__ constexpr int stream4_ctas_per_sm(int rows) { return rows == 8 ? 3 : 2; }
 // The kernel for 4-bit codes (cache4_attention.cu), with p.grid CTAs
 cudaError_t launch_stream4(const StreamParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v, int head_dim, cudaStream_t stream, bool overlap);
 
@@ -147,14 +149,14 @@ __device__ __forceinline__ Share share_in_cluster(const StreamParams& p, int cta
 }
 
 // Behind a cluster barrier: the CTAs' parts of the cluster's unit become its rows, dealt out to all warps of the cluster.
-template <int kD>
+template <int kD, int kAllWarps>
 __device__ __forceinline__ void merge_in_cluster(const StreamParams& p, const Share& share, const float* own_part, const float* own_lse, int warp, int lane) {
   const Request& r = share.request;
   const int row0 = share.unit / p.heads_kv * p.rows, head = share.unit - share.unit / p.heads_kv * p.heads_kv;
   const int rank = blockIdx.x - blockIdx.x / p.cluster * p.cluster;
   if (share.unit < r.units && share.each < r.tiles) {  // (a single CTA's unit is done)
     const int n_rows = min(p.rows, r.rows_q * p.group - row0);
-    for (int rr = rank + p.cluster * warp; rr < n_rows; rr += p.cluster * (kWarps + 2)) {
+    for (int rr = rank + p.cluster * warp; rr < n_rows; rr += p.cluster * kAllWarps) {
       constexpr int kPer = kD / 32;
       float v[8][kPer];
 #pragma unroll
