@@ -24,6 +24,8 @@ namespace {
 
 constexpr float kBias = 14.f;      // weights are kept times 2^14: times the rest of V's scale they fit f16
 constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
+constexpr int kNoExponent = 1000;
+constexpr int kPlainExponents = 10;  // e of a step's tokens up to that far below the largest: the rests of V's scales stay normal f16 numbers, or the groups' own distance makes them less
 constexpr int kFarExponents = 50;    // e that is further from the first one seen: of two tokens 2^100 apart the smaller one's weight may not fit 32 bits though it counts
 
 // Loading warps: one for K and one for V, or, where an SM has three CTAs and each of them more time for a tile, one for both
@@ -39,14 +41,14 @@ template <int kD>
 __host__ __device__ constexpr uint32_t stage_bytes() { return tile_tokens<kD>() * kD; }  // codes of K and of V
 template <int kD>
 __host__ __device__ constexpr uint32_t scale_bytes() { return tile_tokens<kD>() * (kD / 32) * 2 * 2; }  // their scales
-// What a warp keeps of a step's scales of V, for two steps in turn: e and 2^-e of each token, the rests by pairs of tokens
+// What a warp keeps of a step's scales of V, for two steps in turn: e of each token, the rests by pairs of tokens
 template <int kD>
-__host__ __device__ constexpr uint32_t step_scale_bytes() { return step_tokens<kD>() * (8 + kD / 32 * 2); }
+__host__ __device__ constexpr uint32_t step_scale_bytes() { return step_tokens<kD>() * (4 + kD / 32 * 2); }
 // B fragments of Q: in registers where there is room; else in shared memory, with their sums (8 rows, head_dim 128: 332 us so, 339 from registers that spill, 64 requests of 2048 to 32768)
 template <int kRowBlocks, int kD>
 __host__ __device__ constexpr bool q_in_registers() { return kD == 64; }
 template <int kRowBlocks, int kRowWarps, int kD>
-__host__ __device__ constexpr uint32_t q_bytes() { return q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 32) * (512 + 32); }
+__host__ __device__ constexpr uint32_t q_bytes() { return q_in_registers<kRowBlocks, kD>() ? 0 : kRowWarps * kRowBlocks * (kD / 32) * (512 + 64); }
 template <int kRowBlocks, int kRowWarps, int kD, bool kCluster>
 __host__ __device__ constexpr uint32_t smem_bytes(int stages) {
   return 1024 + stages * (stage_bytes<kD>() + scale_bytes<kD>() + 16) + 16 + kWarps * (2 * step_scale_bytes<kD>() + 8 * 8) + q_bytes<kRowBlocks, kRowWarps, kD>() +
@@ -67,12 +69,11 @@ __device__ __forceinline__ void codes_to_subnormal(uint32_t w, const uint32_t (&
   for (int n = 0; n < 4; ++n)  // (w & mask) ^ eights
     asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(x[n]) : "r"(n < 2 ? w : w >> 8), "r"(n & 1 ? 0x00f000f0u : 0x000f000fu), "r"(eights[n & 1]));
 }
-// The same as normal numbers, code * 2^-9
-__device__ __forceinline__ void codes_to_numbers(uint32_t w, const uint32_t (&eights)[2], uint32_t (&x)[4]) {
+// The same as normal numbers, code * 2^-9. `parts`: 2^15 and 2^11, minus 8 * 2^-9
+__device__ __forceinline__ void codes_to_numbers(uint32_t w, const uint32_t (&eights)[2], const uint32_t (&parts)[3], uint32_t (&x)[4]) {
   codes_to_subnormal(w, eights, x);
 #pragma unroll
-  for (int n = 0; n < 4; ++n)  // times 2^15 or 2^11, minus 8 * 2^-9
-    asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x[n]) : "r"(n & 1 ? 0x68006800u : 0x78007800u), "r"(0xa400a400u));
+  for (int n = 0; n < 4; ++n) asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(x[n]) : "r"(parts[n & 1]), "r"(parts[2]));
 }
 // D = A B + C, C elsewhere than D
 __device__ __forceinline__ void mma_16816_from(float (&d)[4], const float4& c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -110,6 +111,10 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   constexpr int kTileTokens = tile_tokens<kD>(), kStepTokens = step_tokens<kD>(), kHalves = kStepTokens / 16;
   constexpr int kPartTokens = kTileTokens / kParts;
   constexpr int kRowsOfWarp = 8 * kRowBlocks;
+  // Codes of V less their offset: by a multiply-add each two (64 for 32 tokens), or, where rows are few, off the step's products, by products of the weights with the offset (8) and 16
+  // additions, which leaves 16 u of odd dimensions. Either in every step, so that no sum ever holds the offset of more than a step's tokens.
+  constexpr bool kOffsetOnTensorCores = kRowBlocks == 1;
+  constexpr float kEven = kOffsetOnTensorCores ? 0x1p24f : 0x1p9f, kOdd = kOffsetOnTensorCores ? 0x1p20f : 0x1p9f;  // what accumulators lack
   constexpr int kState = kChunks * 4 * 32;                   // floats of a warp's accumulators, of 8 rows
   static_assert(kWarps * kState * 4 <= kStageBytes, "the warps' states do not fit a tile's place");
   static_assert(kSt >= 3, "too few tiles under way");
@@ -118,12 +123,12 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   const uint32_t ring = (raw_addr + 1023u) & ~1023u;
   uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
   uint16_t* tile_scales = reinterpret_cast<uint16_t*>(ring_ptr + kSt * kStageBytes);     // [stage][K, V][token][group]
-  float2* v_tokens = reinterpret_cast<float2*>(tile_scales + kSt * 2 * kTileTokens * kGroups);  // [warp][step in turn][token]: e of its scales, kSumUnit * 2^-e
+  float* v_tokens = reinterpret_cast<float*>(tile_scales + kSt * 2 * kTileTokens * kGroups);  // [warp][step in turn][token]: e of its scales, where a step has several
   uint32_t* v_rests = reinterpret_cast<uint32_t*>(v_tokens + kWarps * 2 * kStepTokens);  // [warp][step in turn][pair of tokens][group]: f16 scales over 2^e
   float2* row_state = reinterpret_cast<float2*>(v_rests + kWarps * kStepTokens * kGroups);  // [warp][row of 8]: maximum and sum
   uint4* q_state = reinterpret_cast<uint4*>(row_state + kWarps * 8);                      // [row group][block of 8 rows][group][lane]: B fragments
   constexpr int kQWords = kQInRegisters ? 0 : kRowWarps * kRowBlocks * kGroups * 32;
-  float2* q_sums = reinterpret_cast<float2*>(q_state + kQWords);                           // [row group][block of 8 rows][group][t]
+  float4* q_sums = reinterpret_cast<float4*>(q_state + kQWords);                           // [row group][block of 8 rows][group][t]: twice those of two rows
   const uint32_t full = smem_u32(q_sums + kQWords / 8), empty = full + 8 * kSt;
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(reinterpret_cast<uint64_t*>(q_sums + kQWords / 8) + 2 * kSt);
 
@@ -261,11 +266,13 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
     };
     bool ok = true, far_apart = false;
-    int first_e = 1000;  // of V's scales, the first that this warp has seen
+    int first_e = kNoExponent, step_e = 0;  // of V's scales, the first that this warp has seen; that of a step that goes the plain way
     int step = 0;  // tiles read
     int turn = 0;  // of the places for a step's scales
     const uint32_t none = *abort_flag & 0x40000000u;  // 0, which the compiler does not know: so that these stay in registers
     const uint32_t eights[2] = {0x00080008u | none, 0x00800080u | none};
+    const uint32_t parts[3] = {0x78007800u | none, 0x68006800u | none, 0xa400a400u | none};
+    const uint32_t less[2] = {0x80088008u | none, 0x80808080u | none};  // -8 and -128 in the subnormals' unit
     Request r = share.request;
     int unit = share.unit, tile = share.tile;
     Request next_r = r;
@@ -281,7 +288,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       uint4 qb[kRowBlocks][kQInRegisters ? kGroups : 1];
       float4 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1, 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit
       uint4* my_q = q_state + row_group * kRowBlocks * kGroups * 32 + lane;
-      float2* my_sums = q_sums + row_group * kRowBlocks * kGroups * 4;
+      float4* my_sums = q_sums + row_group * kRowBlocks * kGroups * 4;
       float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale and the 2^24 that the products lack
       int2 limit[kRowBlocks];     // how many tokens they see
       bool huge = false;          // queries whose factor has no room for the 2^24: the scores take it
@@ -332,7 +339,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             qs[nb][k] = make_float4(sums.x, sums.y, sums.x, sums.y);
           } else if (part == 0) {
             my_q[(nb * kGroups + k) * 32] = packed;
-            if (g == 0) my_sums[(nb * kGroups + k) * 4 + t] = sums;
+            if (g == 0) my_sums[(nb * kGroups + k) * 4 + t] = make_float4(sums.x, sums.y, sums.x, sums.y);
           }
         }
         const int sees = p.causal ? min(r.len, i + 1 + r.in_front) : r.len;
@@ -377,56 +384,72 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         __syncwarp();
-        // ---- the scales of V of a step: a lane has one token, or two with half as many groups
+        // ---- the scales of a step: a lane has one token, or two with half as many groups. Whether the step goes the plain way: V's scales are taken apart by one 2^e for all of its tokens
         auto take_scales = [&](int c) {
           const int in_tile = part * kPartTokens + c;
-          constexpr int kOfLane = kStepTokens / 32;
-          const uint16_t* src = tile_scales + ((2 * st + 1) * kTileTokens + in_tile + kOfLane * lane) * kGroups;
-          const uint2 raw = *reinterpret_cast<const uint2*>(src);
-          const uint32_t words[2] = {raw.x, raw.y};
-          uint32_t rest[2];
-          float2 of_token[kOfLane];
-          int e2s[kOfLane];
+          constexpr int kOfLane = kStepTokens / 32, kWords = 2 / kOfLane;  // words of a token
+          const uint16_t* src = tile_scales + (2 * st * kTileTokens + in_tile + kOfLane * lane) * kGroups;
+          const uint2 raw_k = *reinterpret_cast<const uint2*>(src), raw_v = *reinterpret_cast<const uint2*>(src + kTileTokens * kGroups);
+          uint32_t words[2] = {raw_v.x, raw_v.y}, top[kOfLane];  // top: a token's largest scale
+          bool bad[kOfLane];
+          int lowest = 1 << 16, highest = 0;                      // exponent fields of the lane's
 #pragma unroll
           for (int x = 0; x < kOfLane; ++x) {
-            uint32_t w[2 / kOfLane], top = 0u;
             const bool there = tile_tok + in_tile + kOfLane * lane + x < r.len;
+            uint32_t both = kOfLane == 1 ? __vmaxu2(raw_k.x & 0x7fff7fffu, raw_k.y & 0x7fff7fffu) : (x ? raw_k.y : raw_k.x) & 0x7fff7fffu;
+            top[x] = 0u;
 #pragma unroll
-            for (int e = 0; e < 2 / kOfLane; ++e) {
-              w[e] = there ? words[kOfLane == 1 ? e : x] : 0u;
-              top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+            for (int e = 0; e < kWords; ++e) {
+              uint32_t& w = words[kOfLane == 1 ? e : x];
+              if (!there) w = 0u;
+              top[x] = __vmaxu2(top[x], w & 0x7fff7fffu);
             }
-            top = max(top & 0xffffu, top >> 16);
-            const bool bad = top >= 0x7f80u;
-            const int e2 = bad || top == 0u ? 0 : min(max(static_cast<int>(top >> 7) - 126, kLeastExponent), 126);
-            e2s[x] = e2;
-            const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);  // 2^-e
-            of_token[x] = make_float2(bad ? __int_as_float(0x7fffffff) : static_cast<float>(e2), kSumUnit * down);
-#pragma unroll
-            for (int e = 0; e < 2 / kOfLane; ++e)
-              rest[kOfLane == 1 ? e : x] = bad ? 0u : pack_f16x2(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
+            if (!there) both = 0u;
+            both = __vmaxu2(both, top[x]);
+            bad[x] = max(both & 0xffffu, both >> 16) >= 0x7f80u;  // of K or of V: who sees the token is NaN
+            top[x] = max(top[x] & 0xffffu, top[x] >> 16);
+            const int of_token = static_cast<int>(top[x] >> 7);
+            if (!bad[x]) highest = max(highest, of_token);
+            if (top[x] != 0u || bad[x]) lowest = min(lowest, bad[x] ? -1 : of_token);
           }
-          float2* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
+          const int field = __reduce_max_sync(0xffffffffu, highest);
+          if (first_e == kNoExponent && field > 0) first_e = field - 126;
+          const bool plain = __all_sync(0xffffffffu, lowest >= max(field - kPlainExponents, 0)) && field > 126 + kLeastExponent && field <= 252 &&
+                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart;
+          float* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
           uint32_t* rests = v_rests + (2 * warp + turn) * (kStepTokens / 2) * kGroups;
+          uint32_t rest[2];
+          auto rest_of = [&](uint32_t w, float down) { return pack_f16x2(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down); };
+          if (plain) {
+            step_e = field - 126;
+            const float down = __uint_as_float(static_cast<uint32_t>(127 - step_e) << 23);  // 2^-e
+            rest[0] = rest_of(words[0], down);
+            rest[1] = rest_of(words[1], down);
+          } else {
+            bool is_far = false;
+#pragma unroll
+            for (int x = 0; x < kOfLane; ++x) {
+              const bool none = bad[x] || top[x] == 0u;
+              const int e2 = none ? 0 : min(max(static_cast<int>(top[x] >> 7) - 126, kLeastExponent), 126);
+              is_far = is_far || (!none && abs(e2 - first_e) > kFarExponents);
+              const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
+              tokens[x] = bad[x] ? __int_as_float(0x7fffffff) : static_cast<float>(e2);
+#pragma unroll
+              for (int e = 0; e < kWords; ++e) rest[kOfLane == 1 ? e : x] = bad[x] ? 0u : rest_of(words[kOfLane == 1 ? e : x], down);
+            }
+            far_apart = __any_sync(0xffffffffu, is_far) || far_apart;
+          }
           if constexpr (kOfLane == 1) {
-            tokens[0] = of_token[0];
             // lanes of a pair of tokens: the even one has groups 0 and 1 of both, the odd one 2 and 3
             const uint32_t other = __shfl_xor_sync(0xffffffffu, lane & 1 ? rest[0] : rest[1], 1);
-            const uint32_t near = lane & 1 ? other : rest[0], behind = lane & 1 ? rest[1] : other;
-            *reinterpret_cast<uint2*>(rests + 2 * lane) = make_uint2(__byte_perm(near, behind, 0x5410), __byte_perm(near, behind, 0x7632));
-          } else {
-            *reinterpret_cast<float4*>(tokens) = make_float4(of_token[0].x, of_token[0].y, of_token[kOfLane - 1].x, of_token[kOfLane - 1].y);
-            *reinterpret_cast<uint2*>(rests + 2 * lane) = make_uint2(__byte_perm(rest[0], rest[1], 0x5410), __byte_perm(rest[0], rest[1], 0x7632));
+            rest[0] = lane & 1 ? other : rest[0], rest[1] = lane & 1 ? rest[1] : other;
           }
-          if (first_e == 1000) first_e = __shfl_sync(0xffffffffu, e2s[0], 0);
-          bool is_far = false;
-#pragma unroll
-          for (int x = 0; x < kOfLane; ++x) is_far = is_far || abs(e2s[x] - first_e) > kFarExponents;
-          far_apart = __any_sync(0xffffffffu, is_far) || far_apart;
+          *reinterpret_cast<uint2*>(rests + 2 * lane) = make_uint2(__byte_perm(rest[0], rest[1], 0x5410), __byte_perm(rest[0], rest[1], 0x7632));
           __syncwarp();
+          return plain;
         };
-        auto work_on = [&](int c, auto far_tag) {
-          constexpr bool kFar = decltype(far_tag)::value;
+        auto work_on = [&](int c, auto plain_tag) {
+          constexpr bool kPlain = decltype(plain_tag)::value;
           const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
           // ---- S^T = K Q^T, 16 tokens and 32 dimensions at a time
           // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
@@ -446,8 +469,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
                   begin[e][nb] = qs[nb][ch + e];
                 } else {
                   q[e][nb] = my_q[(nb * kGroups + ch + e) * 32];
-                  const float2 sums = my_sums[(nb * kGroups + ch + e) * 4 + t];
-                  begin[e][nb] = make_float4(sums.x, sums.y, sums.x, sums.y);
+                  begin[e][nb] = my_sums[(nb * kGroups + ch + e) * 4 + t];
                 }
               }
 #pragma unroll
@@ -484,26 +506,23 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[nb][half][e] *= 0x1p24f;
           }
-          float2 near[kHalves], behind[kHalves];  // e and kSumUnit * 2^-e of tokens g, g + 8
-#pragma unroll
-          for (int half = 0; half < kHalves; ++half) {
-            near[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + g];
-            behind[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + 8 + g];
-          }
           uint32_t pb[kRowBlocks][kHalves][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
           bool moved = false;
           float2 a[kRowBlocks];
 #pragma unroll
           for (int nb = 0; nb < kRowBlocks; ++nb) {
-            // scores and e, masked where a row ends inside the step
+            // masked where a row ends inside the step; in the plain way scores as they are, else with the softmax scale and e
+            [[maybe_unused]] float near[kPlain ? 1 : kHalves], behind[kPlain ? 1 : kHalves];  // e of tokens g, g + 8
+            if constexpr (!kPlain) {
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) s[nb][half][e] = fmaf(s[nb][half][e], 0.f, s[nb][half][e]);  // an infinite scale: NaN
-              s[nb][half][0] = fmaf(s[nb][half][0], factor[nb].x, near[half].x);
-              s[nb][half][1] = fmaf(s[nb][half][1], factor[nb].y, near[half].x);
-              s[nb][half][2] = fmaf(s[nb][half][2], factor[nb].x, behind[half].x);
-              s[nb][half][3] = fmaf(s[nb][half][3], factor[nb].y, behind[half].x);
+              for (int half = 0; half < kHalves; ++half) {
+                near[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + g];
+                behind[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + 8 + g];
+                s[nb][half][0] = fmaf(s[nb][half][0], factor[nb].x, near[half]);
+                s[nb][half][1] = fmaf(s[nb][half][1], factor[nb].y, near[half]);
+                s[nb][half][2] = fmaf(s[nb][half][2], factor[nb].x, behind[half]);
+                s[nb][half][3] = fmaf(s[nb][half][3], factor[nb].y, behind[half]);
+              }
             }
             if (tok + kStepTokens > seen_by_all) {
 #pragma unroll
@@ -521,82 +540,113 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               mx = max3(mx, s[nb][half][0], s[nb][half][2]);
               my = max3(my, s[nb][half][1], s[nb][half][3]);
             }
-            mx = fmaxf(m[nb].x, column_max(mx));
-            my = fmaxf(m[nb].y, column_max(my));
-            // a row that has seen no key has o = l = 0: any finite factor will do
-            a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
-            if constexpr (kFar) {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
-              const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
-              const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
-              l[nb].x = l[nb].x * hx * hx;
-              l[nb].y = l[nb].y * hy * hy;
-              constexpr float kUp = 0x1p14f * kSumUnit;  // what the other sums are multiplied by
-#pragma unroll
-              for (int half = 0; half < kHalves; ++half) {
-                l[nb].x = fmaf(kUp, exp2f(s[nb][half][0] - near[half].x - vx) + exp2f(s[nb][half][2] - behind[half].x - vx), l[nb].x);
-                l[nb].y = fmaf(kUp, exp2f(s[nb][half][1] - near[half].x - vy) + exp2f(s[nb][half][3] - behind[half].x - vy), l[nb].y);
-              }
-            } else {
-              l[nb].x *= a[nb].x;
-              l[nb].y *= a[nb].y;
+            mx = column_max(mx);
+            my = column_max(my);
+            if constexpr (kPlain) {
+              mx = fmaf(mx, factor[nb].x, static_cast<float>(step_e));
+              my = fmaf(my, factor[nb].y, static_cast<float>(step_e));
             }
+            mx = fmaxf(m[nb].x, mx);
+            my = fmaxf(m[nb].y, my);
+            // a row that has seen no key has o = l = 0: any finite factor will do
+            const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
+            a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
             moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
-            m[nb] = make_float2(mx, my);
-            const float ux = mx == -INFINITY ? 0.f : mx - kBias, uy = my == -INFINITY ? 0.f : my - kBias;
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
-              const float x0 = ex2_approx(s[nb][half][0] - ux), y0 = ex2_approx(s[nb][half][1] - uy);
-              const float x1 = ex2_approx(s[nb][half][2] - ux), y1 = ex2_approx(s[nb][half][3] - uy);
-              if constexpr (!kFar) {
-                l[nb].x = fmaf(x1, behind[half].y, fmaf(x0, near[half].y, l[nb].x));
-                l[nb].y = fmaf(y1, behind[half].y, fmaf(y0, near[half].y, l[nb].y));
+              float2 w[2];
+              if constexpr (kPlain) {
+                const float2 up = make_float2(static_cast<float>(step_e) - vx + kBias, static_cast<float>(step_e) - vy + kBias);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) w[e] = fma2(make_float2(s[nb][half][2 * e], s[nb][half][2 * e + 1]), factor[nb], up);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const float of_token = e ? behind[half] : near[half], of_v = isnan(of_token) ? 0.f : of_token;  // NaN is in the scores of those who see the token
+                  w[e] = make_float2(s[nb][half][2 * e] - (vx - kBias), s[nb][half][2 * e + 1] - (vy - kBias));
+                  sum = add2(sum, make_float2(exp2f(s[nb][half][2 * e] - of_v - vx), exp2f(s[nb][half][2 * e + 1] - of_v - vy)));
+                }
               }
-              pb[nb][half][0] = transpose_8x8(pack_f16x2(x0, y0));
-              pb[nb][half][1] = transpose_8x8(pack_f16x2(x1, y1));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                w[e] = make_float2(ex2_approx(w[e].x), ex2_approx(w[e].y));
+                if constexpr (kPlain) sum = add2(sum, w[e]);
+                pb[nb][half][e] = transpose_8x8(pack_f16x2(w[e].x, w[e].y));
+              }
             }
+            if constexpr (kPlain) {
+              const float unit = kSumUnit * __uint_as_float(static_cast<uint32_t>(127 - step_e) << 23);
+              l[nb] = fma2(sum, make_float2(unit, unit), mul2(l[nb], a[nb]));
+            } else {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
+              const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
+              constexpr float kUp = 0x1p14f * kSumUnit;  // what the other sums are multiplied by
+              l[nb] = make_float2(fmaf(kUp, sum.x, l[nb].x * hx * hx), fmaf(kUp, sum.y, l[nb].y * hy * hy));
+            }
+            m[nb] = make_float2(mx, my);
           }
           if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int nb = 0; nb < kRowBlocks; ++nb)
 #pragma unroll
               for (int ch = 0; ch < kChunks; ++ch) {
-                o[nb][ch][0] *= a[nb].x;
-                o[nb][ch][1] *= a[nb].y;
-                o[nb][ch][2] *= a[nb].x;
-                o[nb][ch][3] *= a[nb].y;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                  const float2 x = mul2(make_float2(o[nb][ch][e], o[nb][ch][e + 1]), a[nb]);
+                  o[nb][ch][e] = x.x, o[nb][ch][e + 1] = x.y;
+                }
               }
           }
           // ---- O^T += V^T W^T, 16 tokens and 32 dimensions at a time
           const uint32_t v_smem = ring + st * kStageBytes + (kTileTokens + in_tile) * kRowBytes;
           const uint32_t* rests = v_rests + ((2 * warp + turn) * (kStepTokens / 2) + t) * kGroups;
 #pragma unroll
-          for (int half = 0; half < kHalves; ++half) {
+          for (int ch = 0; ch < kGroups; ch += 2) {
+            [[maybe_unused]] float less_of[2][4];  // -8 times the weights' sum (of even dimensions, rows 2t, 2t + 1; -128 times it of odd ones)
 #pragma unroll
-            for (int ch = 0; ch < kGroups; ch += 2) {
+            for (int half = 0; half < kHalves; ++half) {
               uint32_t vf[4];
               ldmatrix_x4_trans(v_smem + chunk_at(half * 16 + (mat & 1) * 8 + mrow, ch + (mat >> 1)), vf);
               const uint2 rest = *reinterpret_cast<const uint2*>(rests + half * 8 * kGroups + ch), rest8 = *reinterpret_cast<const uint2*>(rests + (half * 8 + 4) * kGroups + ch);
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t x[4], y[4];  // f16 pairs of two tokens: dimensions 4g to 4g + 3
-                codes_to_numbers(vf[2 * e], eights, x);
-                codes_to_numbers(vf[2 * e + 1], eights, y);
+                if constexpr (kOffsetOnTensorCores) {
+                  codes_to_subnormal(vf[2 * e], eights, x);
+                  codes_to_subnormal(vf[2 * e + 1], eights, y);
+                } else {
+                  codes_to_numbers(vf[2 * e], eights, parts, x);
+                  codes_to_numbers(vf[2 * e + 1], eights, parts, y);
+                }
 #pragma unroll
                 for (int nb = 0; nb < kRowBlocks; ++nb) {
                   const uint32_t w0 = mul_f16x2(pb[nb][half][0], e ? rest.y : rest.x), w1 = mul_f16x2(pb[nb][half][1], e ? rest8.y : rest8.x);
                   mma_16816<true>(o[nb][2 * (ch + e)], x[0], x[1], y[0], y[1], w0, w1);
                   mma_16816<true>(o[nb][2 * (ch + e) + 1], x[2], x[3], y[2], y[3], w0, w1);
+                  if constexpr (kOffsetOnTensorCores) {
+                    if (half == 0) mma_16816_from(less_of[e], make_float4(0.f, 0.f, 0.f, 0.f), less[0], less[1], less[0], less[1], w0, w1);
+                    else mma_16816<true>(less_of[e], less[0], less[1], less[0], less[1], w0, w1);
+                  }
                 }
               }
+            }
+            if constexpr (kOffsetOnTensorCores) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                  float (&to)[4] = o[0][2 * ch + e];
+                  const float2 x = add2(make_float2(to[j], to[j + 1]), make_float2(less_of[e / 2][j], less_of[e / 2][j + 1]));
+                  to[j] = x.x, to[j + 1] = x.y;
+                }
             }
           }
         };
         const int end = min(kPartTokens, seen_by_any - tile_tok - part * kPartTokens);
 #pragma unroll 1
         for (int c = 0; c < end; c += kStepTokens) {
-          take_scales(c);
-          if (!far_apart) work_on(c, std::false_type{});
-          else work_on(c, std::true_type{});
+          if (take_scales(c)) work_on(c, std::true_type{});
+          else work_on(c, std::false_type{});
           turn ^= 1;
         }
         // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
@@ -667,7 +717,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         for (int x = 0; x < 2; ++x) {
           const int row = my_row0 + 8 * nb + 2 * t + x;
           if (row >= row0 + n_rows) continue;
-          const float inv = sum[x] > 0.f ? 0x1p9f * kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN; codes were over 2^9
+          const float inv = sum[x] > 0.f ? kSumUnit / sum[x] : sum[x];  // 0 stays 0, NaN stays NaN
           const float lse2 = sum[x] == 0.f ? -INFINITY : mm[x] - kBias - log2f(kSumUnit) + log2f(sum[x]);
           auto dim_of = [&](int ch) { return 32 * ((part * kMine + ch) >> 1) + 4 * g + 2 * ((part * kMine + ch) & 1); };
           if (whole) {
@@ -675,7 +725,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             uint16_t* dst = p.out + (r.q0 + i) * p.o_row + hq * p.o_head;
 #pragma unroll
             for (int ch = 0; ch < kMine; ++ch) {
-              const float even = acc[ch][x] * inv, odd = acc[ch][2 + x] * inv;
+              const float even = acc[ch][x] * kEven * inv, odd = acc[ch][2 + x] * kOdd * inv;
               *reinterpret_cast<uint32_t*>(dst + dim_of(ch)) = p.f16 ? pack_f16x2(even, odd) : pack_bf16x2(even, odd);
             }
             if (g == 0 && part == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum[x] > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
@@ -683,7 +733,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const int64_t at = kCluster ? row - row0 : (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
             float* dst = (kCluster ? own_part : p.part_o) + at * kD;
 #pragma unroll
-            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + dim_of(ch)) = make_float2(acc[ch][x] * inv, acc[ch][2 + x] * inv);
+            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + dim_of(ch)) = make_float2(acc[ch][x] * kEven * inv, acc[ch][2 + x] * kOdd * inv);
             if (g == 0 && part == 0) (kCluster ? own_lse : p.part_lse)[at] = lse2;
           }
         }
