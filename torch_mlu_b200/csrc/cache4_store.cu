@@ -26,6 +26,8 @@ struct Store4Params {
   Store4Side side[2];  // keys, values
   const int32_t* slots;
   int tokens, heads, num_slots, shift;
+  uint32_t heads_inv;  // row / heads = (high half of row * heads_inv + row) >> heads_log, for rows below 2^31
+  int heads_log;
 };
 
 // kRows: rows (a head of a token) that a thread has a part of
@@ -42,7 +44,7 @@ __global__ void __launch_bounds__(kThreads) store4_kernel(const Store4Params p) 
   int slot[kRows], head[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    const int row = row0 + i * kRowsAtOnce, t = row / p.heads;
+    const int row = row0 + i * kRowsAtOnce, t = (__umulhi(row, p.heads_inv) + row) >> p.heads_log;
     head[i] = row - t * p.heads;
     held[i] = make_uint4(0u, 0u, 0u, 0u);
     slot[i] = -1;
@@ -60,10 +62,11 @@ __global__ void __launch_bounds__(kThreads) store4_kernel(const Store4Params p) 
     top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
     top = max(top & 0xffffu, top >> 16);
     const bool bad = top >= kInf;
-    const float most = unpack_16x2<kF16>(top).x;
-    float scale = __uint_as_float((__float_as_uint(__fdiv_rn(most, 7.f)) + 0x7ffffu) & 0xfff80000u);
-    scale = bad ? 1.f : fmaxf(scale, 0x1p-100f);
-    const float inv = __frcp_rn(scale);
+    // A little less than 1/7: what is 7 times a number of five bits does not get above it, and no other comes nearer than 2^-12 to one
+    const float seventh = unpack_16x2<kF16>(top).x * 0x1.249248p-3f;
+    const float scale = bad ? 1.f : fmaxf(__uint_as_float((__float_as_uint(seventh) + 0x7ffffu) & 0xfff80000u), 0x1p-100f);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
     const uint32_t words[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
     uint32_t code[8];
 #pragma unroll
@@ -99,6 +102,8 @@ int launch_store4(const sdpa_b200_cache_params& p, cudaStream_t stream) {
   s.heads = p.heads_kv;
   s.shift = block_shift(p.block_size);
   s.num_slots = p.num_blocks << s.shift;
+  for (s.heads_log = 0; (1 << s.heads_log) < p.heads_kv;) ++s.heads_log;
+  s.heads_inv = static_cast<uint32_t>(((1ull << 32) * ((1ull << s.heads_log) - p.heads_kv)) / p.heads_kv + 1);
   const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads_kv;
   const bool f16 = p.dtype == SDPA_B200_F16;
   cudaError_t err = cudaSuccess;

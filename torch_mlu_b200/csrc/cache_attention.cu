@@ -741,7 +741,8 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       // a block outside the cache: its scores are NaN, for those who see them
       w[i][x].scale = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
-      w[i][x].load(p.cache[x], p.scale[x], p.block[x], p.head[x], p.row[x], id[i], p.heads, h, place, p.shift, kD, at);
+      w[i][x].load(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + Eight<kCode>::code_at(at), p.scale[x],
+                   Eight<kCode>::scale_at(id[i], p.heads, h, place, p.shift, kD, at));
     }
   }
 #pragma unroll

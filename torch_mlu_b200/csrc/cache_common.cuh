@@ -32,10 +32,18 @@ __device__ __forceinline__ void codes_to_f16_by_two(uint32_t codes, uint32_t& ev
   }
 }
 
-// Four bits: eight codes, the even element in the low half of its byte, as their values
+// Four bits: eight codes, the even element in the low half of its byte, as their values. 0x6400 | u is the f16 number 1024 + u, with 16 u in its place 1024 + 16 u, u = code + 8
 __device__ __forceinline__ void codes4_to_floats(uint32_t codes, float (&x)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(static_cast<int>(codes << (28 - 4 * e)) >> 28);
+  for (int n = 0; n < 4; ++n) {  // elements n and n + 4
+    const uint32_t w = n < 2 ? codes : codes >> 8;
+    uint32_t h;
+    if (n & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(h) : "r"((w & 0x00f000f0u) ^ 0x64806480u), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
+    else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(h) : "r"((w & 0x000f000fu) ^ 0x64086408u), "r"(0x64086408u));                              // - 1032
+    const float2 f = unpack_16x2<true>(h);
+    x[n] = f.x;
+    x[n + 4] = f.y;
+  }
 }
 
 constexpr int kScaleGroup = 32;  // elements of a token and head that share a scale in a 4-bit cache
@@ -46,16 +54,21 @@ struct Eight {
   uint2 codes;
   float scale;
 
-  __device__ __forceinline__ void load(const uint8_t* cache, const void* scales, int64_t block_stride, int64_t head_stride, int64_t row_stride, int block, int heads, int head,
-                                       int place, int shift, int head_dim, int at) {
-    const uint8_t* row = cache + block * block_stride + head * head_stride + place * row_stride;
+  // Where elements from `at` on are: their codes, from those of the head's token on, and their scale
+  static __device__ __forceinline__ int code_at(int at) { return kCode == SDPA_B200_INT4 ? at / 2 : at; }
+  static __device__ __forceinline__ int64_t scale_at(int block, int heads, int head, int place, int shift, int head_dim, int at) {
     const int64_t of_head = static_cast<int64_t>(block) * heads + head;
+    return kCode == SDPA_B200_INT4 ? ((of_head << shift) + place) * (head_dim / kScaleGroup) + at / kScaleGroup : of_head;
+  }
+  // From one head's scale to the next one's
+  static __device__ __forceinline__ int scale_step(int shift, int head_dim) { return kCode == SDPA_B200_INT4 ? (head_dim / kScaleGroup) << shift : 1; }
+  __device__ __forceinline__ void load(const uint8_t* codes_at, const void* scales, int64_t scale_index) {
     if constexpr (kCode == SDPA_B200_INT4) {
-      codes = make_uint2(*reinterpret_cast<const uint32_t*>(row + at / 2), 0u);
-      scale = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[((of_head << shift) + place) * (head_dim / kScaleGroup) + at / kScaleGroup]) << 16);
+      codes = make_uint2(*reinterpret_cast<const uint32_t*>(codes_at), 0u);
+      scale = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[scale_index]) << 16);
     } else {
-      codes = *reinterpret_cast<const uint2*>(row + at);
-      scale = static_cast<const float*>(scales)[of_head];
+      codes = *reinterpret_cast<const uint2*>(codes_at);
+      scale = static_cast<const float*>(scales)[scale_index];
     }
   }
   __device__ __forceinline__ void values(float (&x)[8]) const {

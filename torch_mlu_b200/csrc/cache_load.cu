@@ -57,6 +57,14 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadParams p) {
     }
   }
   const int h0 = blockIdx.y * p.heads_each, h1 = min(h0 + p.heads_each, p.heads);
+  const uint8_t* codes[kTimes][2];
+  int64_t scale_at[kTimes];
+#pragma unroll
+  for (int i = 0; i < kTimes; ++i) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) codes[i][x] = p.cache[x] + id[i] * p.block[x] + h0 * p.head[x] + place[i] * p.row[x] + Eight<kCode>::code_at(at);
+    scale_at[i] = Eight<kCode>::scale_at(id[i], p.heads, h0, place[i], p.shift, kD, at);
+  }
 #pragma unroll 2
   for (int h = h0; h < h1; ++h) {
     Eight<kCode> w[kTimes][2];
@@ -66,7 +74,9 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadParams p) {
       for (int x = 0; x < 2; ++x) {
         w[i][x].codes = make_uint2(0u, 0u);
         w[i][x].scale = id[i] == -1 ? __int_as_float(0x7fffffff) : 0.f;
-        if (id[i] >= 0) w[i][x].load(p.cache[x], p.scale[x], p.block[x], p.head[x], p.row[x], id[i], p.heads, h, place[i], p.shift, kD, at);
+        if (id[i] >= 0) w[i][x].load(codes[i][x], p.scale[x], scale_at[i]);
+        codes[i][x] += p.head[x];
+        if (x == 1) scale_at[i] += Eight<kCode>::scale_step(p.shift, kD);
       }
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
