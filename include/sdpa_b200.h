@@ -391,7 +391,7 @@ typedef struct sdpa_b200_cache_params {
   float softmax_scale;
   uint32_t* device_status; /* as in sdpa_b200_params */
   /* load */
-  void* key_out; /* [num_tokens][heads_kv][head_dim], contiguous, 16-byte aligned */
+  void* key_out; /* [num_tokens][heads_kv][head_dim], contiguous, 32-byte aligned */
   void* value_out;
   const int32_t* first; /* [batch]: each request's first token; NULL: 0 */
   const int32_t* cu_seqlens_k; /* [batch + 1]: offsets of the requests' rows of key_out and value_out */

@@ -43,8 +43,8 @@ REFUSED = [
     ("cache_load", _set(block_table=0), _cabi.INVALID_ARG, "must be given"),
     ("cache_load", _set(cu_seqlens_k=0), _cabi.INVALID_ARG, "must be given"),
     ("cache_load", _set(first=4098), _cabi.INVALID_ARG, "4-byte aligned"),
-    ("cache_load", _set(value_out=4104), _cabi.INVALID_ARG, "value_out must be a 16-byte aligned"),
-    ("cache_load", _set(key_out=0), _cabi.INVALID_ARG, "key_out must be a 16-byte aligned"),
+    ("cache_load", _set(value_out=4112), _cabi.INVALID_ARG, "value_out must be a 32-byte aligned"),
+    ("cache_load", _set(key_out=0), _cabi.INVALID_ARG, "key_out must be a 32-byte aligned"),
 ]
 
 

@@ -685,13 +685,14 @@ struct GatherParams {
   int max_k, max_len;  // tokens that a request has here at most, that a table's row holds
 };
 
-constexpr int kGatherTokens = 32;  // of a block; with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
+// of a block, with 8 bytes of codes a thread. 8 bits: with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
+__host__ __device__ constexpr int gather_tokens(int code) { return code == SDPA_B200_INT4 ? 64 : 32; }
 constexpr int64_t kMostGatheredBytes = int64_t(4) << 30;  // of the 16-bit copies in the workspace
 constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, from a sequence's start
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
 
-// Block (i, h, b): tokens 32i to 32i + 31 of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
+// Block (i, h, b): gather_tokens tokens of request b, kv head h, keys and values. The prefill kernel's last tile of a sequence goes on into the rows behind it,
 // where a weight of 0 would meet another request's NaN, or whatever the workspace held. So every request's rows are filled up to a whole tile with zeros, and these
 // stand in the list of sequences as one of their own, without queries. A request that is longer than its table has the most tokens here that any may have, which
 // are no fewer than its rows, so that each of them sees the first; all are in a block that there is none of.
@@ -722,27 +723,28 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
       cu_k[2 * p.batch] = before + padded;
     }
   }
-  constexpr int kLanes = kD / 8, kTimes = kGatherTokens * kLanes / 256;  // eight codes of K and of V a thread and time: the stores of a warp leave no gaps
+  // eight bytes of codes of K and of V a thread and time: the stores of a warp leave no gaps
+  constexpr int kPer = kCode == SDPA_B200_INT4 ? 16 : 8, kLanes = kD / kPer, kTimes = gather_tokens(kCode) * kLanes / 256;
   static_assert(kTimes >= 1, "a block has threads to spare");
-  const int tok0 = blockIdx.x * kGatherTokens + tid / kLanes, at = tid % kLanes * 8;
+  const int tok0 = blockIdx.x * gather_tokens(kCode) + tid / kLanes, at = tid % kLanes * kPer;
   int id[kTimes];
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), page = tok >> p.shift;
     id[i] = tok < len && page < max_blocks ? p.block_table[b * p.table_stride + page] : -1;
   }
-  Eight<kCode> w[kTimes][2];
+  Span<kCode, kPer> w[kTimes][2];
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
     const int tok = tok0 + i * (256 / kLanes), place = tok & ((1 << p.shift) - 1);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      w[i][x].codes = make_uint2(0u, 0u);
+      w[i][x].clear();
       // a block outside the cache: its scores are NaN, for those who see them
       w[i][x].scale = tok < len && x == 0 ? __int_as_float(0x7fffffff) : 0.f;
       if (id[i] < 0 || id[i] >= p.num_blocks) continue;
-      w[i][x].load(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + Eight<kCode>::code_at(at), p.scale[x],
-                   Eight<kCode>::scale_at(id[i], p.heads, h, place, p.shift, kD, at));
+      w[i][x].load(p.cache[x] + id[i] * p.block[x] + h * p.head[x] + place * p.row[x] + Span<kCode, kPer>::code_at(at), p.scale[x],
+                   Span<kCode, kPer>::scale_at(id[i], p.heads, h, place, p.shift, kD, at));
     }
   }
 #pragma unroll
@@ -759,12 +761,9 @@ __global__ void __launch_bounds__(256) cache_gather_kernel(const GatherParams p)
     }
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      float v[8];
+      float v[kPer];
       w[i][x].values(v);
-      uint32_t f[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = pack_16x2_finite<kF16>(v[2 * e] * own[x], v[2 * e + 1] * own[x]);
-      *reinterpret_cast<uint4*>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
+      write_finite<kF16>(p.out[x] + ((static_cast<int64_t>(before) + tok) * p.heads + h) * kD + at, v, own[x]);
     }
   }
 }
@@ -1029,7 +1028,7 @@ int launch_gathered(const sdpa_b200_cache_params& c, int first, int count, char*
   g.shift = block_shift(c.block_size);
   g.max_k = most_gathered(c);
   g.max_len = table_tokens(c);
-  const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / kGatherTokens), c.heads_kv, count);
+  const dim3 grid(static_cast<unsigned>(padded_keys(g.max_k) / gather_tokens(c.code)), c.heads_kv, count);
   const bool f16 = c.dtype == SDPA_B200_F16;
   auto launch = [&](auto dim, auto code) {
     constexpr int kD = decltype(dim)::value, kCode = decltype(code)::value;

@@ -48,42 +48,57 @@ __device__ __forceinline__ void codes4_to_floats(uint32_t codes, float (&x)[8]) 
 
 constexpr int kScaleGroup = 32;  // elements of a token and head that share a scale in a 4-bit cache
 
-// Eight elements of a cache of any code, out of 64-bit or 32-bit words of codes and their scale
-template <int kCode>
-struct Eight {
-  uint2 codes;
+// kPer (8 or 16) elements of a cache of any code, whose scale is one
+template <int kCode, int kPer>
+struct Span {
+  static constexpr bool kFour = kCode == SDPA_B200_INT4;
+  static constexpr int kWords = kPer * (kFour ? 4 : 8) / 32;
+  uint32_t codes[kWords];
   float scale;
 
   // Where elements from `at` on are: their codes, from those of the head's token on, and their scale
-  static __device__ __forceinline__ int code_at(int at) { return kCode == SDPA_B200_INT4 ? at / 2 : at; }
+  static __device__ __forceinline__ int code_at(int at) { return kFour ? at / 2 : at; }
   static __device__ __forceinline__ int64_t scale_at(int block, int heads, int head, int place, int shift, int head_dim, int at) {
     const int64_t of_head = static_cast<int64_t>(block) * heads + head;
-    return kCode == SDPA_B200_INT4 ? ((of_head << shift) + place) * (head_dim / kScaleGroup) + at / kScaleGroup : of_head;
+    return kFour ? ((of_head << shift) + place) * (head_dim / kScaleGroup) + at / kScaleGroup : of_head;
   }
   // From one head's scale to the next one's
-  static __device__ __forceinline__ int scale_step(int shift, int head_dim) { return kCode == SDPA_B200_INT4 ? (head_dim / kScaleGroup) << shift : 1; }
-  __device__ __forceinline__ void load(const uint8_t* codes_at, const void* scales, int64_t scale_index) {
-    if constexpr (kCode == SDPA_B200_INT4) {
-      codes = make_uint2(*reinterpret_cast<const uint32_t*>(codes_at), 0u);
-      scale = __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[scale_index]) << 16);
-    } else {
-      codes = *reinterpret_cast<const uint2*>(codes_at);
-      scale = static_cast<const float*>(scales)[scale_index];
-    }
-  }
-  __device__ __forceinline__ void values(float (&x)[8]) const {
-    if constexpr (kCode == SDPA_B200_INT4) {
-      codes4_to_floats(codes.x, x);
-    } else {
-      uint32_t h[4];
-      codes_to_f16<kCode == SDPA_B200_INT8>(codes.x, h[0], h[1]);
-      codes_to_f16<kCode == SDPA_B200_INT8>(codes.y, h[2], h[3]);
+  static __device__ __forceinline__ int scale_step(int shift, int head_dim) { return kFour ? (head_dim / kScaleGroup) << shift : 1; }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 f = unpack_16x2<true>(h[e]);
-        x[2 * e] = f.x;
-        x[2 * e + 1] = f.y;
+    for (int i = 0; i < kWords; ++i) codes[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const uint8_t* codes_at, const void* scales, int64_t scale_index) {
+    if constexpr (kWords == 4) {
+      const uint4 w = *reinterpret_cast<const uint4*>(codes_at);
+      codes[0] = w.x, codes[1] = w.y, codes[2] = w.z, codes[3] = w.w;
+    } else if constexpr (kWords == 2) {
+      const uint2 w = *reinterpret_cast<const uint2*>(codes_at);
+      codes[0] = w.x, codes[1] = w.y;
+    } else {
+      codes[0] = *reinterpret_cast<const uint32_t*>(codes_at);
+    }
+    scale = kFour ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[scale_index]) << 16) : static_cast<const float*>(scales)[scale_index];
+  }
+  __device__ __forceinline__ void values(float (&x)[kPer]) const {
+#pragma unroll
+    for (int i = 0; i < kPer; i += 8) {
+      float v[8];
+      if constexpr (kFour) {
+        codes4_to_floats(codes[i / 8], v);
+      } else {
+        uint32_t h[4];
+        codes_to_f16<kCode == SDPA_B200_INT8>(codes[i / 4], h[0], h[1]);
+        codes_to_f16<kCode == SDPA_B200_INT8>(codes[i / 4 + 1], h[2], h[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack_16x2<true>(h[e]);
+          v[2 * e] = f.x;
+          v[2 * e + 1] = f.y;
+        }
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i + e] = v[e];
     }
   }
 };
@@ -96,6 +111,21 @@ __device__ __forceinline__ uint32_t pack_16x2_finite(float lo, float hi) {
   if constexpr (kF16) asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// kPer elements times their scale as 16-bit numbers, 16 bytes at a time or 32, to where as many bytes are aligned
+template <bool kF16, int kPer>
+__device__ __forceinline__ void write_finite(uint16_t* to, const float (&v)[kPer], float scale) {
+  uint32_t f[kPer / 2];
+#pragma unroll
+  for (int e = 0; e < kPer / 2; ++e) {
+    const float2 x = mul2(make_float2(v[2 * e], v[2 * e + 1]), make_float2(scale, scale));
+    f[e] = pack_16x2_finite<kF16>(x.x, x.y);
+  }
+  if constexpr (kPer == 16)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]), "r"(f[4]), "r"(f[5]), "r"(f[6]), "r"(f[7]) : "memory");
+  else
+    *reinterpret_cast<uint4*>(to) = make_uint4(f[0], f[1], f[2], f[3]);
 }
 
 // The smallest power of two 2^k, k >= -100, at which `largest` (finite, not negative) is a code: at most 448 = 1.75 * 2^8 of e4m3, 127 = 1.984375 * 2^6 of int8.

@@ -1,7 +1,7 @@
 // Tokens of requests out of the paged cache, as packed 16-bit keys and values. No counterpart in the reference, which has no paged cache.
 //
 // Row cu[b] + i is token first[b] + i of request b: code * scale, rounded once to 16 bits. Bound by HBM: 4.5 or 8 bits read and 16 written per element.
-// A CTA has 32 rows of some heads. It counts the requests that end in front of its first row with all threads at once; what stands behind is found from there.
+// A CTA has 64 rows of some heads. It counts the requests that end in front of its first row with all threads at once; what stands behind is found from there.
 #include <algorithm>
 #include <type_traits>
 
@@ -11,7 +11,8 @@ namespace sdpa_b200 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTokens = 32;  // of a CTA
+constexpr int kTokens = 64;  // of a CTA
+constexpr int kPer = 16;     // elements of a thread: 32 bytes of the result
 
 struct LoadParams {
   const uint8_t* cache[2];
@@ -27,8 +28,8 @@ struct LoadParams {
 
 template <int kD, int kCode, bool kF16>
 __global__ void __launch_bounds__(kThreads) load_kernel(const LoadParams p) {
-  constexpr int kLanes = kD / 8, kRowsAtOnce = kThreads / kLanes, kTimes = kTokens / kRowsAtOnce;
-  const int tid = threadIdx.x, at = tid % kLanes * 8, row0 = blockIdx.x * kTokens;
+  constexpr int kLanes = kD / kPer, kRowsAtOnce = kThreads / kLanes, kTimes = kTokens / kRowsAtOnce;
+  const int tid = threadIdx.x, at = tid % kLanes * kPer, row0 = blockIdx.x * kTokens;
   launch_dependents();
   wait_for_previous_grid();
   int ended = 0;  // requests that end at or in front of the CTA's first row
@@ -62,21 +63,21 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadParams p) {
 #pragma unroll
   for (int i = 0; i < kTimes; ++i) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) codes[i][x] = p.cache[x] + id[i] * p.block[x] + h0 * p.head[x] + place[i] * p.row[x] + Eight<kCode>::code_at(at);
-    scale_at[i] = Eight<kCode>::scale_at(id[i], p.heads, h0, place[i], p.shift, kD, at);
+    for (int x = 0; x < 2; ++x) codes[i][x] = p.cache[x] + id[i] * p.block[x] + h0 * p.head[x] + place[i] * p.row[x] + Span<kCode, kPer>::code_at(at);
+    scale_at[i] = Span<kCode, kPer>::scale_at(id[i], p.heads, h0, place[i], p.shift, kD, at);
   }
 #pragma unroll 2
   for (int h = h0; h < h1; ++h) {
-    Eight<kCode> w[kTimes][2];
+    Span<kCode, kPer> w[kTimes][2];
 #pragma unroll
     for (int i = 0; i < kTimes; ++i)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        w[i][x].codes = make_uint2(0u, 0u);
+        w[i][x].clear();
         w[i][x].scale = id[i] == -1 ? __int_as_float(0x7fffffff) : 0.f;
         if (id[i] >= 0) w[i][x].load(codes[i][x], p.scale[x], scale_at[i]);
         codes[i][x] += p.head[x];
-        if (x == 1) scale_at[i] += Eight<kCode>::scale_step(p.shift, kD);
+        if (x == 1) scale_at[i] += Span<kCode, kPer>::scale_step(p.shift, kD);
       }
 #pragma unroll
     for (int i = 0; i < kTimes; ++i) {
@@ -85,12 +86,9 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadParams p) {
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const float scale = fabsf(w[i][x].scale) == INFINITY ? __int_as_float(0x7fffffff) : w[i][x].scale;
-        float v[8];
+        float v[kPer];
         w[i][x].values(v);
-        uint32_t f[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = pack_16x2_finite<kF16>(v[2 * e] * scale, v[2 * e + 1] * scale);
-        *reinterpret_cast<uint4*>(p.out[x] + (static_cast<int64_t>(row) * p.heads + h) * kD + at) = make_uint4(f[0], f[1], f[2], f[3]);
+        write_finite<kF16>(p.out[x] + (static_cast<int64_t>(row) * p.heads + h) * kD + at, v, scale);
       }
     }
   }
@@ -117,8 +115,8 @@ extern "C" SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* 
   }
   const void* outs[2] = {p->key_out, p->value_out};
   for (int i = 0; i < 2; ++i) {
-    if (outs[i] == nullptr || (reinterpret_cast<uintptr_t>(outs[i]) & 15u) != 0) {
-      set_error("cache_load: %s must be a 16-byte aligned device pointer", i ? "value_out" : "key_out");
+    if (outs[i] == nullptr || (reinterpret_cast<uintptr_t>(outs[i]) & 31u) != 0) {
+      set_error("cache_load: %s must be a 32-byte aligned device pointer", i ? "value_out" : "key_out");
       return SDPA_B200_INVALID_ARG;
     }
   }

@@ -271,7 +271,14 @@ std::tuple<Tensor, Tensor> launch_load(const Tensor& key_cache, const Tensor& va
   TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative (got ", num_tokens, ")");
   p.num_tokens = to_int32(num_tokens, "num_tokens");
   c10::cuda::CUDAGuard guard(key_cache.device());
-  Tensor key = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache), value = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache);
+  const std::vector<int64_t> shape = {num_tokens, p.heads_kv, p.head_dim};
+  // both are cut out of one allocation, as the results of a plan are
+  const Tensor both = new_tensor({2, num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache);
+  Tensor key = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), both.dtype()), value = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(both.storage()), both.key_set(), both.dtype());
+  key.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  value.unsafeGetTensorImpl()->set_storage_offset(both.numel() / 2);
+  value.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
   if (num_tokens == 0) return {key, value};
   p.block_table = block_table.data_ptr<int32_t>();
   p.table_stride = table_stride(block_table);
