@@ -415,7 +415,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           const int field = __reduce_max_sync(0xffffffffu, highest);
           if (first_e == kNoExponent && field > 0) first_e = field - 126;
           const bool plain = __all_sync(0xffffffffu, lowest >= max(field - kPlainExponents, 0)) && field > 126 + kLeastExponent && field <= 252 &&
-                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart;
+                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart && !huge;
           float* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
           uint32_t* rests = v_rests + (2 * warp + turn) * (kStepTokens / 2) * kGroups;
           uint32_t rest[2];
@@ -448,8 +448,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           __syncwarp();
           return plain;
         };
-        auto work_on = [&](int c, auto plain_tag) {
-          constexpr bool kPlain = decltype(plain_tag)::value;
+        auto work_on = [&](int c) {
           const int in_tile = part * kPartTokens + c, tok = tile_tok + in_tile;
           // ---- S^T = K Q^T, 16 tokens and 32 dimensions at a time
           // s: tokens g, g, g + 8, g + 8 of each half, rows 2t, 2t + 1, 2t, 2t + 1
@@ -498,93 +497,98 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               }
             }
           }
-          if (huge) {
-#pragma unroll
-            for (int nb = 0; nb < kRowBlocks; ++nb)
-#pragma unroll
-              for (int half = 0; half < kHalves; ++half)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[nb][half][e] *= 0x1p24f;
-          }
+          const bool plain = take_scales(c);  // beside the products: neither waits for the other
           uint32_t pb[kRowBlocks][kHalves][2];  // weights as B fragments: tokens 2t, 2t + 1 (and 8 behind) of each half, row g
           bool moved = false;
           float2 a[kRowBlocks];
+          auto weigh = [&](auto plain_tag) {
+            constexpr bool kPlain = decltype(plain_tag)::value;
 #pragma unroll
-          for (int nb = 0; nb < kRowBlocks; ++nb) {
-            // masked where a row ends inside the step; in the plain way scores as they are, else with the softmax scale and e
-            [[maybe_unused]] float near[kPlain ? 1 : kHalves], behind[kPlain ? 1 : kHalves];  // e of tokens g, g + 8
-            if constexpr (!kPlain) {
+            for (int nb = 0; nb < kRowBlocks; ++nb) {
+              // masked where a row ends inside the step; in the plain way scores as they are, else with the softmax scale and e
+              [[maybe_unused]] float near[kPlain ? 1 : kHalves], behind[kPlain ? 1 : kHalves];  // e of tokens g, g + 8
+              if constexpr (!kPlain) {
+                const float2 by = huge ? make_float2(1.f, 1.f) : factor[nb];
+                if (huge) {
 #pragma unroll
-              for (int half = 0; half < kHalves; ++half) {
-                near[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + g];
-                behind[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + 8 + g];
-                s[nb][half][0] = fmaf(s[nb][half][0], factor[nb].x, near[half]);
-                s[nb][half][1] = fmaf(s[nb][half][1], factor[nb].y, near[half]);
-                s[nb][half][2] = fmaf(s[nb][half][2], factor[nb].x, behind[half]);
-                s[nb][half][3] = fmaf(s[nb][half][3], factor[nb].y, behind[half]);
-              }
-            }
-            if (tok + kStepTokens > seen_by_all) {
+                  for (int half = 0; half < kHalves; ++half)
 #pragma unroll
-              for (int half = 0; half < kHalves; ++half) {
-                const int j = tok + half * 16 + g;
-                if (j >= limit[nb].x) s[nb][half][0] = -INFINITY;
-                if (j >= limit[nb].y) s[nb][half][1] = -INFINITY;
-                if (j + 8 >= limit[nb].x) s[nb][half][2] = -INFINITY;
-                if (j + 8 >= limit[nb].y) s[nb][half][3] = -INFINITY;
-              }
-            }
-            float mx = s[nb][0][0], my = s[nb][0][1];
+                    for (int e = 0; e < 4; ++e) s[nb][half][e] = s[nb][half][e] * 0x1p24f * (e & 1 ? factor[nb].y : factor[nb].x);
+                }
 #pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
-              mx = max3(mx, s[nb][half][0], s[nb][half][2]);
-              my = max3(my, s[nb][half][1], s[nb][half][3]);
-            }
-            mx = column_max(mx);
-            my = column_max(my);
-            if constexpr (kPlain) {
-              mx = fmaf(mx, factor[nb].x, static_cast<float>(step_e));
-              my = fmaf(my, factor[nb].y, static_cast<float>(step_e));
-            }
-            mx = fmaxf(m[nb].x, mx);
-            my = fmaxf(m[nb].y, my);
-            // a row that has seen no key has o = l = 0: any finite factor will do
-            const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
-            a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
-            moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int half = 0; half < kHalves; ++half) {
-              float2 w[2];
-              if constexpr (kPlain) {
-                const float2 up = make_float2(static_cast<float>(step_e) - vx + kBias, static_cast<float>(step_e) - vy + kBias);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) w[e] = fma2(make_float2(s[nb][half][2 * e], s[nb][half][2 * e + 1]), factor[nb], up);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const float of_token = e ? behind[half] : near[half], of_v = isnan(of_token) ? 0.f : of_token;  // NaN is in the scores of those who see the token
-                  w[e] = make_float2(s[nb][half][2 * e] - (vx - kBias), s[nb][half][2 * e + 1] - (vy - kBias));
-                  sum = add2(sum, make_float2(exp2f(s[nb][half][2 * e] - of_v - vx), exp2f(s[nb][half][2 * e + 1] - of_v - vy)));
+                for (int half = 0; half < kHalves; ++half) {
+                  near[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + g];
+                  behind[half] = v_tokens[(2 * warp + turn) * kStepTokens + half * 16 + 8 + g];
+                  s[nb][half][0] = fmaf(s[nb][half][0], by.x, near[half]);
+                  s[nb][half][1] = fmaf(s[nb][half][1], by.y, near[half]);
+                  s[nb][half][2] = fmaf(s[nb][half][2], by.x, behind[half]);
+                  s[nb][half][3] = fmaf(s[nb][half][3], by.y, behind[half]);
                 }
               }
+              if (tok + kStepTokens > seen_by_all) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                w[e] = make_float2(ex2_approx(w[e].x), ex2_approx(w[e].y));
-                if constexpr (kPlain) sum = add2(sum, w[e]);
-                pb[nb][half][e] = transpose_8x8(pack_f16x2(w[e].x, w[e].y));
+                for (int half = 0; half < kHalves; ++half) {
+                  const int j = tok + half * 16 + g;
+                  if (j >= limit[nb].x) s[nb][half][0] = -INFINITY;
+                  if (j >= limit[nb].y) s[nb][half][1] = -INFINITY;
+                  if (j + 8 >= limit[nb].x) s[nb][half][2] = -INFINITY;
+                  if (j + 8 >= limit[nb].y) s[nb][half][3] = -INFINITY;
+                }
               }
+              float mx = s[nb][0][0], my = s[nb][0][1];
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                mx = max3(mx, s[nb][half][0], s[nb][half][2]);
+                my = max3(my, s[nb][half][1], s[nb][half][3]);
+              }
+              mx = column_max(mx);
+              my = column_max(my);
+              if constexpr (kPlain) {
+                mx = fmaf(mx, factor[nb].x, static_cast<float>(step_e));
+                my = fmaf(my, factor[nb].y, static_cast<float>(step_e));
+              }
+              mx = fmaxf(m[nb].x, mx);
+              my = fmaxf(m[nb].y, my);
+              // a row that has seen no key has o = l = 0: any finite factor will do
+              const float vx = mx == -INFINITY ? 0.f : mx, vy = my == -INFINITY ? 0.f : my;
+              a[nb] = make_float2(mx == -INFINITY ? 1.f : ex2_approx(m[nb].x - mx), my == -INFINITY ? 1.f : ex2_approx(m[nb].y - my));
+              moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int half = 0; half < kHalves; ++half) {
+                float2 w[2];
+                if constexpr (kPlain) {
+                  const float2 up = make_float2(static_cast<float>(step_e) - vx + kBias, static_cast<float>(step_e) - vy + kBias);
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) w[e] = fma2(make_float2(s[nb][half][2 * e], s[nb][half][2 * e + 1]), factor[nb], up);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const float of_token = e ? behind[half] : near[half], of_v = isnan(of_token) ? 0.f : of_token;  // NaN is in the scores of those who see the token
+                    w[e] = make_float2(s[nb][half][2 * e] - (vx - kBias), s[nb][half][2 * e + 1] - (vy - kBias));
+                    sum = add2(sum, make_float2(exp2f(s[nb][half][2 * e] - of_v - vx), exp2f(s[nb][half][2 * e + 1] - of_v - vy)));
+                  }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  w[e] = make_float2(ex2_approx(w[e].x), ex2_approx(w[e].y));
+                  if constexpr (kPlain) sum = add2(sum, w[e]);
+                  pb[nb][half][e] = transpose_8x8(pack_f16x2(w[e].x, w[e].y));
+                }
+              }
+              if constexpr (kPlain) {
+                const float unit = kSumUnit * __uint_as_float(static_cast<uint32_t>(127 - step_e) << 23);
+                l[nb] = fma2(sum, make_float2(unit, unit), mul2(l[nb], a[nb]));
+              } else {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
+                const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
+                constexpr float kUp = 0x1p14f * kSumUnit;  // what the other sums are multiplied by
+                l[nb] = make_float2(fmaf(kUp, sum.x, l[nb].x * hx * hx), fmaf(kUp, sum.y, l[nb].y * hy * hy));
+              }
+              m[nb] = make_float2(mx, my);
             }
-            if constexpr (kPlain) {
-              const float unit = kSumUnit * __uint_as_float(static_cast<uint32_t>(127 - step_e) << 23);
-              l[nb] = fma2(sum, make_float2(unit, unit), mul2(l[nb], a[nb]));
-            } else {  // sums take the factor in two steps, and weights without the scales; numbers below 2^-126 count
-              const float hx = exp2f(0.5f * (m[nb].x - vx)), hy = exp2f(0.5f * (m[nb].y - vy));
-              constexpr float kUp = 0x1p14f * kSumUnit;  // what the other sums are multiplied by
-              l[nb] = make_float2(fmaf(kUp, sum.x, l[nb].x * hx * hx), fmaf(kUp, sum.y, l[nb].y * hy * hy));
-            }
-            m[nb] = make_float2(mx, my);
-          }
+          };
+          if (plain) weigh(std::true_type{});
+          else weigh(std::false_type{});
           if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
             for (int nb = 0; nb < kRowBlocks; ++nb)
@@ -645,8 +649,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         const int end = min(kPartTokens, seen_by_any - tile_tok - part * kPartTokens);
 #pragma unroll 1
         for (int c = 0; c < end; c += kStepTokens) {
-          if (take_scales(c)) work_on(c, std::true_type{});
-          else work_on(c, std::false_type{});
+          work_on(c);
           turn ^= 1;
         }
         // every lane has read the tile: it may be filled again, but for the segment's last, whose place the warps hand their states over in
