@@ -184,58 +184,92 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     cur.group = ((tile * kTileTokens) >> p.shift) >> 5;
     nxt = far = cur;
     int id = block_at(cur), next_id = -1, far_id = -1;
+    // Scales are copied 16 bytes at a time, of one page: a lane's copies of a tile, and where they are in a page. The rest is kept in a form in which a tile costs few instructions: this
+    // warp's time for a tile bounds the call where the arithmetic does not.
+    constexpr int kTokensAtOnce = 8 / kGroups, kCopies = kTileTokens / kTokensAtOnce / 32;
+    const int64_t block_scales = (static_cast<int64_t>(p.heads_kv) << p.shift) * kGroups;
+    const bool has_k = warp == kWarps, has_v = warp == kWarps + kLoaders - 1;
+    const uint16_t *k_scales[kCopies], *v_scales[kCopies];  // those of block 0, for the unit's head
+    int unit_pages;
+    bool some_missing;  // among the group's blocks
+    auto enter = [&]() {
+      unit_pages = static_cast<int>((static_cast<int64_t>(cur.r.len) + (1 << p.shift) - 1) >> p.shift);
+      some_missing = __any_sync(0xffffffffu, id == p.num_blocks);
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int tok = (lane + 32 * i) * kTokensAtOnce;
+        const int64_t at = ((static_cast<int64_t>(cur.head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups;
+        k_scales[i] = static_cast<const uint16_t*>(p.k_scale) + at;
+        v_scales[i] = static_cast<const uint16_t*>(p.v_scale) + at;
+      }
+    };
     auto next_group = [&]() {
       cur = nxt, id = next_id;
       nxt = far, next_id = far_id;
       advance(far);
       far_id = block_at(far);
+      enter();
     };
     const int pages = kTileTokens >> p.shift;  // of a tile
-    bool ok = true, first = true;
-    int step = 0;
+    const uint32_t page_bytes = static_cast<uint32_t>(kRowBytes) << p.shift;
+    bool ok = true, first = true, filled = false;
+    uint32_t st = 0, phase = 1;  // the ring's next place; what is waited for there once it has been round
+    enter();
     for (int places = share.places; places > 0;) {
       const int page0 = (tile * kTileTokens) >> p.shift;
       if (page0 >> 5 != cur.group) next_group();  // the unit goes on in its next group
       if (tile * kTileTokens < cur.r.len) {
-        const uint32_t st = step % kSt, bar = full + 8 * st;
-        if (ok && step >= kSt) ok = mbar_wait(empty + 8 * st, (step / kSt + 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const int mine = __shfl_sync(0xffffffffu, id, ((page0 & 31) + lane) & 31);
-        const int n = __popc(__ballot_sync(0xffffffffu, lane < pages && mine >= 0));
-        const int sides = kLoaders == 1 ? 2 : 1;
-        if (elect_one()) mbar_expect_tx(bar, static_cast<uint32_t>(sides * n << p.shift) * kRowBytes);
-        const uint32_t dst = ring + st * kStageBytes;
-#pragma unroll 1
-        for (int i = 0; i < n; i += 4) {
-          int blocks[4];
+        const uint32_t bar = full + 8 * st, dst = ring + st * kStageBytes;
+        const int n = min(pages, unit_pages - page0);
+        int blocks[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, mine, (i + e) & 31);
+        for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, id, (page0 + e) & 31);
+        if (filled) {
+          if (ok) ok = mbar_wait(empty + 8 * st, phase, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        if (elect_one()) {
+          mbar_expect_tx(bar, (kLoaders == 1 ? 2 : 1) * n * page_bytes);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (e >= n) break;
+            if (has_k) tma_load_4d(dst + e * page_bytes, &tm_k, bar, 0, 0, cur.head, blocks[e]);
+            if (has_v) tma_load_4d(dst + kTileTokens * kRowBytes + e * page_bytes, &tm_v, bar, 0, 0, cur.head, blocks[e]);
+          }
+        }
+#pragma unroll 1
+        for (int i = 4; i < n; i += 4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) blocks[e] = __shfl_sync(0xffffffffu, id, (page0 + i + e) & 31);
           if (elect_one()) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              if (i + e >= n) continue;
-              const uint32_t page_dst = dst + ((i + e) << p.shift) * kRowBytes;
-              if (warp == kWarps) tma_load_4d(page_dst, &tm_k, bar, 0, 0, cur.head, blocks[e]);
-              if (warp == kWarps + kLoaders - 1) tma_load_4d(page_dst + kTileTokens * kRowBytes, &tm_v, bar, 0, 0, cur.head, blocks[e]);
+              if (i + e >= n) break;
+              if (has_k) tma_load_4d(dst + (i + e) * page_bytes, &tm_k, bar, 0, 0, cur.head, blocks[e]);
+              if (has_v) tma_load_4d(dst + kTileTokens * kRowBytes + (i + e) * page_bytes, &tm_v, bar, 0, 0, cur.head, blocks[e]);
             }
           }
         }
-        // 16 bytes of scales at a time, of one page; those of a block that is not there are NaN, those behind the last page stay what they are
-        constexpr int kTokensAtOnce = 8 / kGroups;
-        const uint32_t scale_dst = smem_u32(tile_scales + 2 * st * kTileTokens * kGroups);
+        // those of a block that is not there are NaN, those behind the last page stay what they are
+        const uint32_t scale_dst = smem_u32(tile_scales) + st * (2 * kTileTokens * kGroups * 2) + 16 * lane;
 #pragma unroll
-        for (int i = 0; i < kTileTokens / kTokensAtOnce / 32; ++i) {
-          const int tok = (lane + 32 * i) * kTokensAtOnce, block = __shfl_sync(0xffffffffu, mine, tok >> p.shift);
-          const int64_t at = (((static_cast<int64_t>(block) * p.heads_kv + cur.head) << p.shift) + (tok & ((1 << p.shift) - 1))) * kGroups;
-          const bool none = block == p.num_blocks;
-          if (block < 0) continue;
-          if (warp == kWarps) copy_16_async(scale_dst + (lane + 32 * i) * 16, none ? no_scales : static_cast<const void*>(static_cast<const uint16_t*>(p.k_scale) + at));
-          if (warp == kWarps + kLoaders - 1)
-            copy_16_async(scale_dst + kTileTokens * kGroups * 2 + (lane + 32 * i) * 16, none ? no_scales : static_cast<const void*>(static_cast<const uint16_t*>(p.v_scale) + at));
+        for (int i = 0; i < kCopies; ++i) {
+          const int page = ((lane + 32 * i) * kTokensAtOnce) >> p.shift, block = __shfl_sync(0xffffffffu, id, (page0 + page) & 31);
+          const int64_t at = block * block_scales;
+          const void *from_k = k_scales[i] + at, *from_v = v_scales[i] + at;
+          if (some_missing && block == p.num_blocks) from_k = from_v = no_scales;
+          if (page < n) {
+            if (has_k) copy_16_async(scale_dst + 32 * 16 * i, from_k);
+            if (has_v) copy_16_async(scale_dst + kTileTokens * kGroups * 2 + 32 * 16 * i, from_v);
+          }
         }
         arrive_behind_copies(bar);
-        ++step;
+        if (++st == kSt) {
+          st = 0;
+          phase ^= 1;
+          filled = true;
+        }
       }
       if (first) {  // the first copies are under way
         advance(nxt);
@@ -267,7 +301,10 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     };
     bool ok = true, far_apart = false;
     int first_e = kNoExponent, step_e = 0;  // of V's scales, the first that this warp has seen; that of a step that goes the plain way
-    int step = 0;  // tiles read
+    uint32_t st = 0, phase = 0;  // the ring's next place, its barrier's parity
+    auto next_place = [&]() {
+      if (++st == kSt) st = 0, phase ^= 1;
+    };
     int turn = 0;  // of the places for a step's scales
     const uint32_t none = *abort_flag & 0x40000000u;  // 0, which the compiler does not know: so that these stay in registers
     const uint32_t eights[2] = {0x00080008u | none, 0x00800080u | none};
@@ -380,8 +417,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       for (int i = 0; i < seg_tiles; ++i) {
         const int tile_tok = (tile + i) * kTileTokens;
         if (tile_tok >= r.len) break;  // a request without tokens
-        const uint32_t st = step % kSt;
-        if (ok) ok = mbar_wait(full + 8 * st, (step / kSt) & 1, abort_flag);
+        if (ok) ok = mbar_wait(full + 8 * st, phase, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         __syncwarp();
         // ---- the scales of a step: a lane has one token, or two with half as many groups. Whether the step goes the plain way: V's scales are taken apart by one 2^e for all of its tokens
@@ -656,11 +692,10 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         if (i + 1 < seg_tiles) {
           __syncwarp();
           if (lane == 0) mbar_arrive(empty + 8 * st);
-          ++step;
+          next_place();
         }
       }
       const bool tokens = r.len > 0;
-      const uint32_t st = step % kSt;
 #pragma unroll
       for (int nb = 0; nb < kRowBlocks; ++nb) l[nb] = make_float2(column_sum(l[nb].x), column_sum(l[nb].y));
       // ---- the parts of a tile's tokens come together, 8 rows at a time: every warp takes some of the dimensions, of all parts
@@ -745,7 +780,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         fence_proxy_async_smem();  // what was handed over goes before the copy into the same place
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + 8 * st);
-        ++step;
+        next_place();
       }
       // begun here, where the share ends; ended by the CTA whose share holds its last tile
       if (tile == 0 && !whole) left = {share.cta_behind(blockIdx.x, r.tiles - seg_tiles - 1), slot, head, row0, n_rows, r.q0};
