@@ -1,4 +1,5 @@
-// Attention over the 8-bit paged cache. No counterpart in the reference, which has no paged cache.
+// Attention over the paged cache: which way a call goes, the ways for 8-bit codes, and what brings codes of 8 and 4 bits to 16. The kernel that streams 4-bit codes is in cache4_attention.cu. No
+// counterpart in the reference, which has no paged cache.
 //
 //   s_ij = scale * ks[block(j), h] * <q_i, kc_j>,  out_i = sum_j softmax_j(s_i) * vs[block(j), h] * vc_j
 //
@@ -791,13 +792,16 @@ int gathered_at_once(const sdpa_b200_cache_params& p) {
 // token in the cache. So the length does not decide, and in units of 64 rows a token's gathering is 0.9 and a wave 95 (head_dim 64: 150). Measured, 4 requests of 5000
 // tokens, us, path 1 | 2: 32/8 heads of 128, 24 rows 58 | 86, 40 79 | 88, 56 99 | 88, 96 144 | 89; 16/16, 64 60 | 106, 128 101 | 107, 160 144 | 115; 64/8, 40 123 | 148,
 // 64 188 | 150; 16/4 of 64, 64 36 | 63, 128 61 | 64, 160 73 | 81. 16 requests of 1000, 32/8 of 128, 40 76 | 78, 64 95 | 79.
+// 4-bit codes cost a unit of 64 rows more, since four warps convert each: a wave is 40 there (head_dim 64: 85). 4 requests of 5000, 32/8 heads of 128, 24 rows 84 | 88, 40 113 | 90, 96 206 | 91;
+// 16/16, 96 145 | 108; 16/4 of 64, 64 45 | 65, 128 78 | 65. 16 requests of 1000, 32/8 of 128, 24 78 | 80, 40 111 | 81.
 bool streams(const sdpa_b200_cache_params& p) {
   const int64_t group = p.heads_q / p.heads_kv, batch = p.batch;
   if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64 || gathered_bytes(p) > kMostGatheredBytes) return true;
   // requests of equal rows, or of any: half a unit each is empty then
   const double units = p.total_q == batch * p.max_seqlen_q ? static_cast<double>(batch * ((p.max_seqlen_q * group + 63) / 64)) : p.total_q * group / 64.0 + 0.5 * batch;
   const int64_t blocks = p.heads_q * std::max<int64_t>(batch, (p.total_q + 255) / 256);
-  return (units - 0.9 * batch) * p.heads_kv <= (p.head_dim == 64 ? 150.0 : 95.0) * static_cast<double>((blocks + 147) / 148);
+  const double wave = p.code == SDPA_B200_INT4 ? (p.head_dim == 64 ? 85.0 : 40.0) : p.head_dim == 64 ? 150.0 : 95.0;
+  return (units - 0.9 * batch) * p.heads_kv <= wave * static_cast<double>((blocks + 147) / 148);
 }
 
 int check_attention(const sdpa_b200_cache_params* p) {
