@@ -9,12 +9,15 @@
 //   ones 16 times that, for which Q is divided by 16. The 8 comes off in the accumulators, which begin with -8 * 2^-24 * sum of the group's q instead of 0: u is small, so
 //   that the sums lose three of fp32's bits to it.
 // * The scale of K goes onto the group's fp32 sums: 4 multiply-adds for each 32 x 16 codes a warp converts, where scaling the codes would take 8.
-// * Codes of V become code * 2^-9 by one multiply-add each two more: sums over tens of thousands of tokens would lose too much to an offset.
-// * The scale of V is taken apart: 2^e, the power of two above the token's largest, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
-//   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of the token's largest has its products' full 11 bits only where the weight is that much above
-//   the smallest normal one.
+// * Codes of V are converted the same way. Their offset comes off in every step, by products of the weights with -8 (units of up to 8 rows) or by one multiply-add each two codes (more rows): sums
+//   over tens of thousands of tokens would lose too much to it.
+// * The scale of V is taken apart: a power of two 2^e, above the largest of a step's tokens, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
+//   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of 2^e has its products' full 11 bits only where the weight is that much above the smallest
+//   normal one; where tokens are further apart, each has an e of its own, and the sums of the softmax are formed without them, as the 8-bit kernel does for scales far apart.
 // * The loading warps only issue copies, codes by TMA and scales by cp.async, and wait for nothing but room. A warp of the arithmetic brings the scales of V of its own tokens into these
 //   forms, a token or two a lane, beside its products with K.
+// Measured, one token per request, 32/8 heads of 128: 64 requests of 2048 to 32768 tokens, 1.34 GB: 324 to 330 us, 4.1 TB/s, 62% of a copy's rate; 8 of 32768 78; one of 1000, in clusters, 7.0. Without
+// the arithmetic the first takes 228: it is the length of a step's chain in each warp that bounds it, with the logic pipe at 52% and the tensor pipe at 26%, no pipe alone.
 #include <type_traits>
 
 #include "cache_stream.cuh"
@@ -299,8 +302,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       if constexpr (kD == 128) return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
       return row * 32 + ((chunk ^ ((row >> 2) & 1)) << 4);
     };
-    bool ok = true, far_apart = false;
-    int first_e = kNoExponent, step_e = 0;  // of V's scales, the first that this warp has seen; that of a step that goes the plain way
+    bool ok = true;
     uint32_t st = 0, phase = 0;  // the ring's next place, its barrier's parity
     auto next_place = [&]() {
       if (++st == kSt) st = 0, phase ^= 1;
@@ -321,6 +323,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       const int row0 = unit / p.heads_kv * p.rows, head = unit - unit / p.heads_kv * p.heads_kv;
       const int n_rows = min(p.rows, r.rows_q * p.group - row0);
       const int my_row0 = row0 + kRowsOfWarp * row_group;
+      bool far_apart = false;
+      int first_e = kNoExponent, step_e = 0;  // of V's scales, the first that this warp sees of the unit; that of a step that goes the plain way
       // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 8t..8t+7 of every 32: pairs (n, n + 4), those of odd n over 16
       uint4 qb[kRowBlocks][kQInRegisters ? kGroups : 1];
       float4 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1, 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit

@@ -5,6 +5,9 @@
 // costs a step of 1/32 more on average. x has at most 11 bits, a scale 5: no quotient but a tie itself comes nearer than 2^-12 to the middle of two codes, so x * (1 / scale) with one
 // correction step, which gives quotients of few bits exactly, rounds as the exact quotient does.
 //
+// Measured: 8192 tokens of 4 prompts, 8 heads of 128, bf16 beside their queries: 15.6 us with 8 elements a thread, divisions and a conversion for each element (155 instructions for 8 elements, 71% of the
+// issue slots); 13.6 without the divisions; 10.6 with 16 elements a thread (4.0 TB/s). 64 tokens 3.7, which is a launch.
+//
 // A scale depends on its own 32 elements only: no runs to find, nothing read back, no order among tokens. A thread has 16 elements, two threads a scale.
 #include <type_traits>
 
