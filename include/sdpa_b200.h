@@ -421,7 +421,8 @@ SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* p, void* st
  * cache, or a scale of K that is infinite or NaN, and all rows of a request whose length passes the table's row. Nothing at or behind seq_lens
  * counts, whatever stands there. A NaN among the values, or a scale of V that is negative, infinite or NaN, may reach every row of its request
  * and kv head, as 0 * NaN. A scale of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few; there a value counts down to
- * 2^-39 of the largest product of a weight and a scale of V in its row. In a 4-bit cache scales of V may be negative, and a scale of K or V that is infinite or NaN reaches
+ * 2^-39 of the largest product of a weight and a scale of V in its row. In a 4-bit cache scales of V keep all their bits down to 2^-16 of the
+ * largest among 64 neighbouring tokens and count down to 2^-24 of it; they may be negative, and a scale of K or V that is infinite or NaN reaches
  * only the rows that see its token.
  * Where requests have many rows, codes * scales are brought to 16 bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB
  * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range. What is beyond its

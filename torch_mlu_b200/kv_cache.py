@@ -98,8 +98,8 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace and the prefill
     kernel runs: 4 * max_seqlen_k * heads_kv * head_dim bytes a request, for as many requests at a time as fit 4 GiB (where not even one does, the codes are streamed). That is exact with scales that are powers of two, as store gives
     them; with others every element is rounded once. Elements beyond the largest number of query's type are that number there (fp16: 65504, of which the code may be 65536),
-    and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24. A 4-bit cache takes the same two paths; where its codes are streamed, the scales of
-    a token's values count down to 2^-24 of the token's largest one, and to 2^-100.
+    and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24. A 4-bit cache takes the same two paths; where its codes are streamed, scales of
+    values keep all their bits down to 2^-16 of the largest among 64 neighbouring tokens, count down to 2^-24 of it, and to 2^-100.
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package), a length that passes the table's row all rows of its request.
