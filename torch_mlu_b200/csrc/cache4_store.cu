@@ -6,7 +6,8 @@
 // correction step, which gives quotients of few bits exactly, rounds as the exact quotient does.
 //
 // Measured: 8192 tokens of 4 prompts, 8 heads of 128, bf16 beside their queries: 15.6 us with 8 elements a thread, divisions and a conversion for each element (155 instructions for 8 elements, 71% of the
-// issue slots); 13.6 without the divisions; 10.6 with 16 elements a thread (4.0 TB/s). 64 tokens 3.7, which is a launch.
+// issue slots); 13.6 without the divisions; 10.6 with 16 elements a thread, two times; 10.0 with 16 once (4.3 TB/s), 12.5 four times. 64 tokens 3.7,
+// which is a launch.
 //
 // A scale depends on its own 32 elements only: no runs to find, nothing read back, no order among tokens. A thread has 16 elements, two threads a scale.
 #include <type_traits>
@@ -34,70 +35,59 @@ struct Store4Params {
   int heads_log;
 };
 
-// kRows: rows (a head of a token) that a thread has a part of
-template <int kD, bool kF16, int kRows>
+// A thread has a part of one row (a head of a token)
+template <int kD, bool kF16>
 __global__ void __launch_bounds__(kThreads) store4_kernel(const Store4Params p) {
   constexpr int kLanes = kD / kPer, kRowsAtOnce = kThreads / kLanes;
   constexpr uint32_t kInf = kF16 ? 0x7c00u : 0x7f80u;
   const Store4Side& x = p.side[blockIdx.x & 1];
   const int at = threadIdx.x % kLanes * kPer;
-  const int row0 = static_cast<int>(blockIdx.x >> 1) * (kRowsAtOnce * kRows) + threadIdx.x / kLanes;
+  const int row = static_cast<int>(blockIdx.x >> 1) * kRowsAtOnce + threadIdx.x / kLanes, t = (__umulhi(row, p.heads_inv) + row) >> p.heads_log, head = row - t * p.heads;
   launch_dependents();
   wait_for_previous_grid();
-  uint32_t held[kRows][kPer / 2];
-  int slot[kRows], head[kRows];
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const int row = row0 + i * kRowsAtOnce, t = (__umulhi(row, p.heads_inv) + row) >> p.heads_log;
-    head[i] = row - t * p.heads;
-    slot[i] = -1;
-    uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (t < p.tokens) {
-      slot[i] = p.slots[t];
-      if (t + 1 < p.tokens && p.slots[t + 1] == slot[i]) slot[i] = -1;  // the same slot again with the next token: the later stays
-      const uint4* src = reinterpret_cast<const uint4*>(x.in + t * x.in_row + head[i] * x.in_head + at);
-      w[0] = src[0], w[1] = src[1];
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) held[i][4 * e] = w[e].x, held[i][4 * e + 1] = w[e].y, held[i][4 * e + 2] = w[e].z, held[i][4 * e + 3] = w[e].w;
+  uint4 w[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+  int slot = -1;
+  if (t < p.tokens) {
+    slot = p.slots[t];
+    if (t + 1 < p.tokens && p.slots[t + 1] == slot) slot = -1;  // the same slot again with the next token: the later stays
+    const uint4* src = reinterpret_cast<const uint4*>(x.in + t * x.in_row + head * x.in_head + at);
+    w[0] = src[0], w[1] = src[1];
   }
+  const uint32_t held[kPer / 2] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+  // 16-bit floats without their signs are ordered as integers, infinity and NaN behind all numbers
+  uint32_t top = 0u;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    // 16-bit floats without their signs are ordered as integers, infinity and NaN behind all numbers
-    uint32_t top = 0u;
+  for (int e = 0; e < kPer / 2; ++e) top = __vmaxu2(top, held[e] & 0x7fff7fffu);
+  top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top & 0xffffu, top >> 16);
+  const bool bad = top >= kInf;
+  // A little less than 1/7: what is 7 times a number of five bits does not get above it, and no other comes nearer than 2^-12 to one
+  const float seventh = unpack_16x2<kF16>(top).x * 0x1.249248p-3f;
+  const float scale = bad ? 1.f : fmaxf(__uint_as_float((__float_as_uint(seventh) + 0x7ffffu) & 0xfff80000u), 0x1p-100f);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+  uint32_t packed[kPer / 8];
 #pragma unroll
-    for (int e = 0; e < kPer / 2; ++e) top = __vmaxu2(top, held[i][e] & 0x7fff7fffu);
-    top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top & 0xffffu, top >> 16);
-    const bool bad = top >= kInf;
-    // A little less than 1/7: what is 7 times a number of five bits does not get above it, and no other comes nearer than 2^-12 to one
-    const float seventh = unpack_16x2<kF16>(top).x * 0x1.249248p-3f;
-    const float scale = bad ? 1.f : fmaxf(__uint_as_float((__float_as_uint(seventh) + 0x7ffffu) & 0xfff80000u), 0x1p-100f);
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
-    uint32_t packed[kPer / 8];
+  for (int k = 0; k < kPer / 8; ++k) {
+    uint32_t code[8];
 #pragma unroll
-    for (int k = 0; k < kPer / 8; ++k) {
-      uint32_t code[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 v = unpack_16x2<kF16>(held[i][4 * k + e]);
-        const float2 q = mul2(v, make_float2(inv, inv));
-        const float2 off = fma2(q, make_float2(-scale, -scale), v);
-        const float2 n = add2(fma2(off, make_float2(inv, inv), q), make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23 + x has x, rounded, in its low bits
-        code[2 * e] = __float_as_uint(n.x);
-        code[2 * e + 1] = __float_as_uint(n.y);
-      }
-      auto bytes = [&](int e) { return __byte_perm(__byte_perm(code[e], code[e + 2], 0x0040), __byte_perm(code[e + 4], code[e + 6], 0x0040), 0x5410); };
-      packed[k] = (bytes(0) & 0x0f0f0f0fu) | (bytes(1) << 4 & 0xf0f0f0f0u);
-      if (bad) packed[k] = 0u;
+    for (int e = 0; e < 4; ++e) {
+      const float2 v = unpack_16x2<kF16>(held[4 * k + e]);
+      const float2 q = mul2(v, make_float2(inv, inv));
+      const float2 off = fma2(q, make_float2(-scale, -scale), v);
+      const float2 n = add2(fma2(off, make_float2(inv, inv), q), make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23 + x has x, rounded, in its low bits
+      code[2 * e] = __float_as_uint(n.x);
+      code[2 * e + 1] = __float_as_uint(n.y);
     }
-    if (slot[i] < 0 || slot[i] >= p.num_slots) continue;
-    const int block = slot[i] >> p.shift, place = slot[i] & ((1 << p.shift) - 1);
-    *reinterpret_cast<uint2*>(x.cache + block * x.block + head[i] * x.head + place * x.row + at / 2) = make_uint2(packed[0], packed[1]);
-    if (at % kScaleGroup == 0)
-      x.scale[((((static_cast<int64_t>(block) * p.heads + head[i]) << p.shift) + place) * kD + at) / kScaleGroup] = bad ? 0x7fc0u : static_cast<uint16_t>(__float_as_uint(scale) >> 16);
+    auto bytes = [&](int e) { return __byte_perm(__byte_perm(code[e], code[e + 2], 0x0040), __byte_perm(code[e + 4], code[e + 6], 0x0040), 0x5410); };
+    packed[k] = (bytes(0) & 0x0f0f0f0fu) | (bytes(1) << 4 & 0xf0f0f0f0u);
+    if (bad) packed[k] = 0u;
   }
+  if (slot < 0 || slot >= p.num_slots) return;
+  const int block = slot >> p.shift, place = slot & ((1 << p.shift) - 1);
+  *reinterpret_cast<uint2*>(x.cache + block * x.block + head * x.head + place * x.row + at / 2) = make_uint2(packed[0], packed[1]);
+  if (at % kScaleGroup == 0)
+    x.scale[((((static_cast<int64_t>(block) * p.heads + head) << p.shift) + place) * kD + at) / kScaleGroup] = bad ? 0x7fc0u : static_cast<uint16_t>(__float_as_uint(scale) >> 16);
 }
 
 }  // namespace
@@ -118,16 +108,12 @@ int launch_store4(const sdpa_b200_cache_params& p, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.num_tokens) * p.heads_kv;
   const bool f16 = p.dtype == SDPA_B200_F16;
   cudaError_t err = cudaSuccess;
-  auto launch = [&](auto dim, auto each) {
-    constexpr int kD = decltype(dim)::value, kRows = decltype(each)::value, kRowsOfCta = kThreads / (kD / kPer) * kRows;
+  auto launch = [&](auto dim) {
+    constexpr int kD = decltype(dim)::value, kRowsOfCta = kThreads / (kD / kPer);
     const unsigned grid = static_cast<unsigned>(2 * ((rows + kRowsOfCta - 1) / kRowsOfCta));
-    err = launch_behind(f16 ? store4_kernel<kD, true, kRows> : store4_kernel<kD, false, kRows>, dim3(grid), kThreads, 0, stream, true, 1, s);
+    err = launch_behind(f16 ? store4_kernel<kD, true> : store4_kernel<kD, false>, dim3(grid), kThreads, 0, stream, true, 1, s);
   };
-  auto launch_rows = [&](auto dim) {
-    // few rows: a thread has one, whose loads are all that there is to wait for
-    rows * p.head_dim <= 148 * 2048 * 8 ? launch(dim, std::integral_constant<int, 1>{}) : launch(dim, std::integral_constant<int, 2>{});
-  };
-  p.head_dim == 64 ? launch_rows(std::integral_constant<int, 64>{}) : launch_rows(std::integral_constant<int, 128>{});
+  p.head_dim == 64 ? launch(std::integral_constant<int, 64>{}) : launch(std::integral_constant<int, 128>{});
   if (err != cudaSuccess) {
     set_error("cache_store: launch failed: %s", cudaGetErrorString(err));
     return SDPA_B200_LAUNCH_FAILED;
