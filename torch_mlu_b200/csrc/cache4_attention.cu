@@ -9,8 +9,8 @@
 //   ones 16 times that, for which Q is divided by 16. The 8 comes off in the accumulators, which begin with -8 * 2^-24 * sum of the group's q instead of 0: u is small, so
 //   that the sums lose three of fp32's bits to it.
 // * The scale of K goes onto the group's fp32 sums: 4 multiply-adds for each 32 x 16 codes a warp converts, where scaling the codes would take 8.
-// * Codes of V are converted the same way. Their offset comes off in every step, by products of the weights with -8 (units of up to 8 rows) or by one multiply-add each two codes (more rows): sums
-//   over tens of thousands of tokens would lose too much to it.
+// * Codes of V become code * 2^-9 by one multiply-add each two more: sums over tens of thousands of tokens would lose too much to an offset. (Products of the weights with -8 in every step instead, off
+//   the step's products, were no faster: 8 requests of 32768 78.1 us, with the multiply-adds 77.3.)
 // * The scale of V is taken apart: a power of two 2^e, above the largest of a step's tokens, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
 //   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of 2^e has its products' full 11 bits only where the weight is that much above the smallest
 //   normal one; where tokens are further apart, each has an e of its own, and the sums of the softmax are formed without them, as the 8-bit kernel does for scales far apart.
@@ -114,10 +114,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
   constexpr int kTileTokens = tile_tokens<kD>(), kStepTokens = step_tokens<kD>(), kHalves = kStepTokens / 16;
   constexpr int kPartTokens = kTileTokens / kParts;
   constexpr int kRowsOfWarp = 8 * kRowBlocks;
-  // Codes of V less their offset: by a multiply-add each two (64 for 32 tokens), or, where rows are few, off the step's products, by products of the weights with the offset (8) and 16
-  // additions, which leaves 16 u of odd dimensions. Either in every step, so that no sum ever holds the offset of more than a step's tokens.
-  constexpr bool kOffsetOnTensorCores = kRowBlocks == 1;
-  constexpr float kEven = kOffsetOnTensorCores ? 0x1p24f : 0x1p9f, kOdd = kOffsetOnTensorCores ? 0x1p20f : 0x1p9f;  // what accumulators lack
+  constexpr float kUnit = 0x1p9f;                            // what accumulators lack
   constexpr int kState = kChunks * 4 * 32;                   // floats of a warp's accumulators, of 8 rows
   static_assert(kWarps * kState * 4 <= kStageBytes, "the warps' states do not fit a tile's place");
   static_assert(kSt >= 3, "too few tiles under way");
@@ -311,7 +308,6 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
     const uint32_t none = *abort_flag & 0x40000000u;  // 0, which the compiler does not know: so that these stay in registers
     const uint32_t eights[2] = {0x00080008u | none, 0x00800080u | none};
     const uint32_t parts[3] = {0x78007800u | none, 0x68006800u | none, 0xa400a400u | none};
-    const uint32_t less[2] = {0x80088008u | none, 0x80808080u | none};  // -8 and -128 in the subnormals' unit
     Request r = share.request;
     int unit = share.unit, tile = share.tile;
     Request next_r = r;
@@ -646,7 +642,6 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           const uint32_t* rests = v_rests + ((2 * warp + turn) * (kStepTokens / 2) + t) * kGroups;
 #pragma unroll
           for (int ch = 0; ch < kGroups; ch += 2) {
-            [[maybe_unused]] float less_of[2][4];  // -8 times the weights' sum (of even dimensions, rows 2t, 2t + 1; -128 times it of odd ones)
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
               uint32_t vf[4];
@@ -655,34 +650,15 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 uint32_t x[4], y[4];  // f16 pairs of two tokens: dimensions 4g to 4g + 3
-                if constexpr (kOffsetOnTensorCores) {
-                  codes_to_subnormal(vf[2 * e], eights, x);
-                  codes_to_subnormal(vf[2 * e + 1], eights, y);
-                } else {
-                  codes_to_numbers(vf[2 * e], eights, parts, x);
-                  codes_to_numbers(vf[2 * e + 1], eights, parts, y);
-                }
+                codes_to_numbers(vf[2 * e], eights, parts, x);
+                codes_to_numbers(vf[2 * e + 1], eights, parts, y);
 #pragma unroll
                 for (int nb = 0; nb < kRowBlocks; ++nb) {
                   const uint32_t w0 = mul_f16x2(pb[nb][half][0], e ? rest.y : rest.x), w1 = mul_f16x2(pb[nb][half][1], e ? rest8.y : rest8.x);
                   mma_16816<true>(o[nb][2 * (ch + e)], x[0], x[1], y[0], y[1], w0, w1);
                   mma_16816<true>(o[nb][2 * (ch + e) + 1], x[2], x[3], y[2], y[3], w0, w1);
-                  if constexpr (kOffsetOnTensorCores) {
-                    if (half == 0) mma_16816_from(less_of[e], make_float4(0.f, 0.f, 0.f, 0.f), less[0], less[1], less[0], less[1], w0, w1);
-                    else mma_16816<true>(less_of[e], less[0], less[1], less[0], less[1], w0, w1);
-                  }
                 }
               }
-            }
-            if constexpr (kOffsetOnTensorCores) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                  float (&to)[4] = o[0][2 * ch + e];
-                  const float2 x = add2(make_float2(to[j], to[j + 1]), make_float2(less_of[e / 2][j], less_of[e / 2][j + 1]));
-                  to[j] = x.x, to[j + 1] = x.y;
-                }
             }
           }
         };
@@ -767,7 +743,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             uint16_t* dst = p.out + (r.q0 + i) * p.o_row + hq * p.o_head;
 #pragma unroll
             for (int ch = 0; ch < kMine; ++ch) {
-              const float even = acc[ch][x] * kEven * inv, odd = acc[ch][2 + x] * kOdd * inv;
+              const float even = acc[ch][x] * kUnit * inv, odd = acc[ch][2 + x] * kUnit * inv;
               *reinterpret_cast<uint32_t*>(dst + dim_of(ch)) = p.f16 ? pack_f16x2(even, odd) : pack_bf16x2(even, odd);
             }
             if (g == 0 && part == 0) p.lse[static_cast<int64_t>(hq) * p.total_q + r.q0 + i] = sum[x] > 0.f ? lse2 * 0.6931471805599453f : INFINITY;
@@ -775,7 +751,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             const int64_t at = kCluster ? row - row0 : (2 * static_cast<int64_t>(blockIdx.x) + slot) * p.rows + row - row0;
             float* dst = (kCluster ? own_part : p.part_o) + at * kD;
 #pragma unroll
-            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + dim_of(ch)) = make_float2(acc[ch][x] * kEven * inv, acc[ch][2 + x] * kOdd * inv);
+            for (int ch = 0; ch < kMine; ++ch) *reinterpret_cast<float2*>(dst + dim_of(ch)) = make_float2(acc[ch][x] * kUnit * inv, acc[ch][2 + x] * kUnit * inv);
             if (g == 0 && part == 0) (kCluster ? own_lse : p.part_lse)[at] = lse2;
           }
         }
