@@ -16,8 +16,8 @@
 //   normal one; where tokens are further apart, each has an e of its own, and the sums of the softmax are formed without them, as the 8-bit kernel does for scales far apart.
 // * The loading warps only issue copies, codes by TMA and scales by cp.async, and wait for nothing but room. A warp of the arithmetic brings the scales of V of its own tokens into these
 //   forms, a token or two a lane, beside its products with K.
-// Measured, one token per request, 32/8 heads of 128: 64 requests of 2048 to 32768 tokens, 1.34 GB: 324 to 330 us, 4.1 TB/s, 62% of a copy's rate; 8 of 32768 78; one of 1000, in clusters, 7.0. Without
-// the arithmetic the first takes 228: it is the length of a step's chain in each warp that bounds it, with the logic pipe at 52% and the tensor pipe at 26%, no pipe alone.
+// Measured, one token per request, 32/8 heads of 128: 64 requests of 2048 to 32768 tokens, 1.34 GB: 323 us, 4.2 TB/s, 63% of a copy's rate; 8 of 32768 77; one of 1000, in clusters, 7.0. Without
+// the arithmetic the first takes 228: it is the length of a step's chain in each warp that bounds it, with the logic pipe at 53% and the tensor pipe at 22%, no pipe alone.
 #include <type_traits>
 
 #include "cache_stream.cuh"
