@@ -29,6 +29,9 @@ constexpr float kBias = 14.f;      // weights are kept times 2^14: times the res
 constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
 constexpr int kNoExponent = 1000;
 constexpr int kPlainExponents = 10;  // e of a step's tokens up to that far below the largest: the rests of V's scales stay normal f16 numbers, or the groups' own distance makes them less
+constexpr int kPlainScores = 20;     // the plain way is for scores below 2^20, of which a weight's exponent is told to 1/16: larger ones are rounded before their maximum is taken off, so that it becomes 0
+constexpr float kLeastFactor = 0x1p-126f;  // a row's factor, where it is a normal number: a masked score times 0 would be NaN
+constexpr float kMostFactor = 0x1p100f;
 constexpr int kFarExponents = 50;    // e that is further from the first one seen: of two tokens 2^100 apart the smaller one's weight may not fit 32 bits though it counts
 
 // Loading warps: one for K and one for V, or, where an SM has three CTAs and each of them more time for a tile, one for both
@@ -328,7 +331,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       float4* my_sums = q_sums + row_group * kRowBlocks * kGroups * 4;
       float2 factor[kRowBlocks];  // of rows 2t, 2t + 1, with the softmax scale and the 2^24 that the products lack
       int2 limit[kRowBlocks];     // how many tokens they see
-      bool huge = false;          // queries whose factor has no room for the 2^24: the scores take it
+      float least = INFINITY, most = 0.f;  // factor of the warp's rows
 #pragma unroll
       for (int nb = 0; nb < kRowBlocks; ++nb) {
         const int row = my_row0 + 8 * nb + g, i = row / p.group;
@@ -356,8 +359,9 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         largest = quad_max(largest);
         const int e2 = min(max(static_cast<int>(__float_as_uint(largest) >> 23) - 127, -100), 127);
         const float up = __uint_as_float(static_cast<uint32_t>(127 + 14 - e2) << 23);
-        const float down = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e2) << 23);
-        huge = huge || e2 > 90;
+        const float down = fminf(p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - 14 + e2) << 23), 0x1.fffffep127f);
+        least = fminf(least, down);
+        most = fmaxf(most, down);
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
           float x[8];
@@ -383,7 +387,14 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
         factor[nb] = make_float2(__shfl_sync(0xffffffffu, down, 8 * t), __shfl_sync(0xffffffffu, down, 8 * t + 4));
         limit[nb] = make_int2(__shfl_sync(0xffffffffu, sees, 8 * t), __shfl_sync(0xffffffffu, sees, 8 * t + 4));
       }
-      huge = __any_sync(0xffffffffu, huge);
+      // numbers that are not negative are ordered as integers
+      least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least)));
+      most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+      const bool huge = most > kMostFactor * 0x1p-24f;  // no room for the 2^24: the scores take it
+      // Scales of K (bf16 bits) from which on the plain way is left: |score| is at most kGroups * K's scale * 2^(exponent of the largest factor, 24 more, + 1) / 2. 0: always
+      const int most_field = static_cast<int>(__float_as_uint(most) >> 23) + 24;
+      uint32_t k_limit = static_cast<uint32_t>(min(127 + kPlainScores + 127 - (kGroups == 4 ? 2 : 1) - most_field, 255)) << 7;
+      if (huge || least * 0x1p24f < kLeastFactor) k_limit = 0u;
       if (!huge) {
 #pragma unroll
         for (int nb = 0; nb < kRowBlocks; ++nb) factor[nb] = make_float2(factor[nb].x * 0x1p24f, factor[nb].y * 0x1p24f);
@@ -428,11 +439,11 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
           const uint2 raw_k = *reinterpret_cast<const uint2*>(src), raw_v = *reinterpret_cast<const uint2*>(src + kTileTokens * kGroups);
           uint32_t words[2] = {raw_v.x, raw_v.y}, top[kOfLane];  // top: a token's largest scale
           bool bad[kOfLane];
-          int lowest = 1 << 16, highest = 0;                      // exponent fields of the lane's
+          int lowest = 1 << 16, highest = 0;                      // exponent fields of the lane's; lowest -1: not the plain way
 #pragma unroll
           for (int x = 0; x < kOfLane; ++x) {
             const bool there = tile_tok + in_tile + kOfLane * lane + x < r.len;
-            uint32_t both = kOfLane == 1 ? __vmaxu2(raw_k.x & 0x7fff7fffu, raw_k.y & 0x7fff7fffu) : (x ? raw_k.y : raw_k.x) & 0x7fff7fffu;
+            uint32_t of_k = kOfLane == 1 ? __vmaxu2(raw_k.x & 0x7fff7fffu, raw_k.y & 0x7fff7fffu) : (x ? raw_k.y : raw_k.x) & 0x7fff7fffu;
             top[x] = 0u;
 #pragma unroll
             for (int e = 0; e < kWords; ++e) {
@@ -440,18 +451,18 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
               if (!there) w = 0u;
               top[x] = __vmaxu2(top[x], w & 0x7fff7fffu);
             }
-            if (!there) both = 0u;
-            both = __vmaxu2(both, top[x]);
-            bad[x] = max(both & 0xffffu, both >> 16) >= 0x7f80u;  // of K or of V: who sees the token is NaN
+            of_k = there ? max(of_k & 0xffffu, of_k >> 16) : 0u;
             top[x] = max(top[x] & 0xffffu, top[x] >> 16);
+            bad[x] = max(of_k, top[x]) >= 0x7f80u;  // of K or of V: who sees the token is NaN
             const int of_token = static_cast<int>(top[x] >> 7);
             if (!bad[x]) highest = max(highest, of_token);
-            if (top[x] != 0u || bad[x]) lowest = min(lowest, bad[x] ? -1 : of_token);
+            if (top[x] != 0u) lowest = min(lowest, of_token);
+            if (bad[x] || of_k >= k_limit) lowest = -1;
           }
           const int field = __reduce_max_sync(0xffffffffu, highest);
           if (first_e == kNoExponent && field > 0) first_e = field - 126;
           const bool plain = __all_sync(0xffffffffu, lowest >= max(field - kPlainExponents, 0)) && field > 126 + kLeastExponent && field <= 252 &&
-                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart && !huge;
+                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart;
           float* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
           uint32_t* rests = v_rests + (2 * warp + turn) * (kStepTokens / 2) * kGroups;
           uint32_t rest[2];
@@ -601,8 +612,9 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
 #pragma unroll
                   for (int e = 0; e < 2; ++e) {
                     const float of_token = e ? behind[half] : near[half], of_v = isnan(of_token) ? 0.f : of_token;  // NaN is in the scores of those who see the token
-                    w[e] = make_float2(s[nb][half][2 * e] - (vx - kBias), s[nb][half][2 * e + 1] - (vy - kBias));
-                    sum = add2(sum, make_float2(exp2f(s[nb][half][2 * e] - of_v - vx), exp2f(s[nb][half][2 * e + 1] - of_v - vy)));
+                    const float2 below = make_float2(s[nb][half][2 * e] - vx, s[nb][half][2 * e + 1] - vy);  // 0 for the largest, however large that is
+                    w[e] = make_float2(below.x + kBias, below.y + kBias);
+                    sum = add2(sum, make_float2(exp2f(below.x - of_v), exp2f(below.y - of_v)));
                   }
                 }
 #pragma unroll

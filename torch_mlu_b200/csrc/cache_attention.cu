@@ -27,6 +27,7 @@
 //    in the workspace (exact with the powers of two that the store kernel chooses, within the type's range), and the prefill kernel does the rest. 512 tokens behind 7680,
 //    2 requests, 32 heads of 128: 134 to 139 us.
 #include <algorithm>
+#include <limits>
 #include <type_traits>
 
 #include "cache_stream.cuh"
@@ -931,7 +932,7 @@ int launch_stream(const sdpa_b200_cache_params& c, int first, int count, char* w
   p.shift = block_shift(c.block_size);
   p.causal = c.is_causal;
   p.f16 = c.dtype == SDPA_B200_F16;
-  p.scale_log2 = c.softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = std::min(c.softmax_scale * 1.4426950408889634f, std::numeric_limits<float>::max());
   // a CTA per tile, up to one wave
   const int64_t units = static_cast<int64_t>(count) * c.heads_kv * ((static_cast<int64_t>(c.max_seqlen_q) * p.group + p.rows - 1) / p.rows);
   const int64_t tiles = units * ((static_cast<int64_t>(c.max_seqlen_k) + (1 << p.tile_shift) - 1) >> p.tile_shift);
