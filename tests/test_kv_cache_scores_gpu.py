@@ -32,7 +32,7 @@ def _zero_some(b, rows):
     return b
 
 
-@pytest.mark.parametrize("code", [INT4])
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
 @pytest.mark.parametrize("rows", [1, 3, 30])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("scale", [1e-45, 1e-38, 1e-12])
@@ -42,7 +42,7 @@ def test_scales_at_which_all_scores_vanish(cuda_device, scale, dim, rows, code):
     assert ops.device_status() == 0
 
 
-@pytest.mark.parametrize("code", [INT4])
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
 @pytest.mark.parametrize("rows", [1, 3, 30])
 @pytest.mark.parametrize("scale", [2.0 ** 13, 2.0 ** 118, 1e36, 2.9e38])
 def test_rows_of_zeros_at_any_scale(cuda_device, scale, rows, code):
@@ -84,7 +84,7 @@ def _one_key(out, lse, b, scale):
     assert decided > 0.8 * out.shape[0] * hq
 
 
-@pytest.mark.parametrize("code", [INT4])
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
 @pytest.mark.parametrize("rows", [1, 3, 30])
 @pytest.mark.parametrize("scale", [2.0 ** 19, 2.0 ** 20, 2.0 ** 21, 2.0 ** 22, 2.0 ** 24, 1e18, 1e36])
 def test_scores_of_any_size(cuda_device, scale, rows, code):

@@ -407,8 +407,11 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
               for (int half = 0; half < kHalves; ++half) {
                 const float lv = sc[half].y;
-                l[nb].x += exp2f(s[nb][half][0] - lv - vx) + exp2f(s[nb][half][2] - lv - vx);
-                l[nb].y += exp2f(s[nb][half][1] - lv - vy) + exp2f(s[nb][half][3] - lv - vy);
+                // the maximum comes off first: 0 for the largest, however large that is
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nb][half][e] -= e & 1 ? vy : vx;
+                l[nb].x += exp2f(s[nb][half][0] - lv) + exp2f(s[nb][half][2] - lv);
+                l[nb].y += exp2f(s[nb][half][1] - lv) + exp2f(s[nb][half][3] - lv);
               }
             } else {
               l[nb].x *= a[nb].x;
@@ -416,7 +419,7 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
             moved = moved || a[nb].x != 1.f || a[nb].y != 1.f;
             m[nb] = make_float2(mx, my);
-            const float ux = mx == -INFINITY ? 0.f : mx - kBias, uy = my == -INFINITY ? 0.f : my - kBias;
+            const float ux = kFar ? -kBias : mx == -INFINITY ? 0.f : mx - kBias, uy = kFar ? -kBias : my == -INFINITY ? 0.f : my - kBias;
 #pragma unroll
             for (int half = 0; half < kHalves; ++half) {
               const float rv = sc[half].z;
@@ -426,8 +429,9 @@ cache_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 l[nb].x = fmaf(x0 + x1, rv, l[nb].x);
                 l[nb].y = fmaf(y0 + y1, rv, l[nb].y);
               }
-              pb[nb][half][0] = transpose_8x8(pack_f16x2(x0, y0));
-              pb[nb][half][1] = transpose_8x8(pack_f16x2(x1, y1));
+              // scores from 2^24 on are 2 and more apart, so that m - kBias may come out up to 16 below m: 2^16 is 65504 then, which is off by no more than a weight's rounding
+              pb[nb][half][0] = transpose_8x8(pack_16x2_finite<true>(x0, y0));
+              pb[nb][half][1] = transpose_8x8(pack_16x2_finite<true>(x1, y1));
             }
           }
           if (__any_sync(0xffffffffu, moved)) {
