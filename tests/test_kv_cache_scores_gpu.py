@@ -33,7 +33,7 @@ def _zero_some(b, rows):
 
 
 @pytest.mark.parametrize("code", [INT4, E4M3, INT8])
-@pytest.mark.parametrize("rows", [1, 3, 30])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("scale", [1e-45, 1e-38, 1e-12])
 def test_scales_at_which_all_scores_vanish(cuda_device, scale, dim, rows, code):
@@ -43,7 +43,7 @@ def test_scales_at_which_all_scores_vanish(cuda_device, scale, dim, rows, code):
 
 
 @pytest.mark.parametrize("code", [INT4, E4M3, INT8])
-@pytest.mark.parametrize("rows", [1, 3, 30])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
 @pytest.mark.parametrize("scale", [2.0 ** 13, 2.0 ** 118, 1e36, 2.9e38])
 def test_rows_of_zeros_at_any_scale(cuda_device, scale, rows, code):
     """Their scores are 0 whatever the scale."""
@@ -85,7 +85,7 @@ def _one_key(out, lse, b, scale):
 
 
 @pytest.mark.parametrize("code", [INT4, E4M3, INT8])
-@pytest.mark.parametrize("rows", [1, 3, 30])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
 @pytest.mark.parametrize("scale", [2.0 ** 19, 2.0 ** 20, 2.0 ** 21, 2.0 ** 22, 2.0 ** 24, 1e18, 1e36])
 def test_scores_of_any_size(cuda_device, scale, rows, code):
     """Queries of ones and of random numbers, whose scores are 2^20 and more: a weight is a power of two of their difference, in which a rounding of the score counts by whole steps."""

@@ -694,6 +694,9 @@ struct GatherParams {
 // of a block, with 8 bytes of codes a thread. 8 bits: with 64 the call of 512 rows took 137 us, with 32 135, with 64 and stores that left gaps to be filled by the next ones 140
 __host__ __device__ constexpr int gather_tokens(int code) { return code == SDPA_B200_INT4 ? 64 : 32; }
 constexpr int64_t kMostGatheredBytes = int64_t(4) << 30;  // of the 16-bit copies in the workspace
+// Softmax scales above it are for path 1, whose weights are right at scores of any size: the prefill kernel multiplies scores by the scale as it takes off their rounded maximum, which from
+// about 2^30 on is further off than a weight has room for (f16 2^27)
+constexpr float kMostGatheredScale = 0x1p16f;
 constexpr int kKeyTile = 128;  // keys that the prefill kernel reads at a time, from a sequence's start
 
 __host__ __device__ __forceinline__ int64_t padded_keys(int64_t n) { return (n + kKeyTile - 1) / kKeyTile * kKeyTile; }
@@ -802,6 +805,7 @@ int gathered_at_once(const sdpa_b200_cache_params& p) {
 bool streams(const sdpa_b200_cache_params& p) {
   const int64_t group = p.heads_q / p.heads_kv, batch = p.batch;
   if (p.cu_seqlens_q == nullptr || p.max_seqlen_q * group <= 64 || gathered_bytes(p) > kMostGatheredBytes) return true;
+  if (p.softmax_scale > kMostGatheredScale) return true;
   // requests of equal rows, or of any: half a unit each is empty then
   const double units = p.total_q == batch * p.max_seqlen_q ? static_cast<double>(batch * ((p.max_seqlen_q * group + 63) / 64)) : p.total_q * group / 64.0 + 0.5 * batch;
   const int64_t blocks = p.heads_q * std::max<int64_t>(batch, (p.total_q + 255) / 256);
