@@ -26,13 +26,15 @@ namespace sdpa_b200 {
 namespace {
 
 constexpr float kBias = 14.f;      // weights are kept times 2^14: times the rest of V's scale they fit f16
-constexpr int kLeastExponent = -99;  // of V's scales, where 2^-100 is the least that the store kernel chooses (and that of zeros)
-constexpr int kNoExponent = 1000;
+// Exponents e of V's scales. Between these two, weights, sums and what they are multiplied by when their maximum moves fit 32 bits for all keys that count, 2^-26 of the largest or more: they
+// are as far as 2^(20 + 80 + 26) apart. What is below the least (2^-100 is the smallest scale that the store kernel chooses) has smaller rests, down to 2^-24; a token without a scale has
+// that exponent, so that no other falls behind it. From the first scale above the most on, a unit's steps go the other way.
+constexpr int kLeastExponent = -80;
+constexpr int kMostExponent = 20;
 constexpr int kPlainExponents = 10;  // e of a step's tokens up to that far below the largest: the rests of V's scales stay normal f16 numbers, or the groups' own distance makes them less
 constexpr int kPlainScores = 20;     // the plain way is for scores below 2^20, of which a weight's exponent is told to 1/16: larger ones are rounded before their maximum is taken off, so that it becomes 0
 constexpr float kLeastFactor = 0x1p-126f;  // a row's factor, where it is a normal number: a masked score times 0 would be NaN
 constexpr float kMostFactor = 0x1p100f;
-constexpr int kFarExponents = 50;    // e that is further from the first one seen: of two tokens 2^100 apart the smaller one's weight may not fit 32 bits though it counts
 
 // Loading warps: one for K and one for V, or, where an SM has three CTAs and each of them more time for a tile, one for both
 template <int kRowBlocks>
@@ -323,7 +325,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
       const int n_rows = min(p.rows, r.rows_q * p.group - row0);
       const int my_row0 = row0 + kRowsOfWarp * row_group;
       bool far_apart = false;
-      int first_e = kNoExponent, step_e = 0;  // of V's scales, the first that this warp sees of the unit; that of a step that goes the plain way
+      int step_e = 0;  // of V's scales, of a step that goes the plain way
       // ---- this lane's row of Q as B fragments, row g of every 8: elements as f16. Thread t has dimensions 8t..8t+7 of every 32: pairs (n, n + 4), those of odd n over 16
       uint4 qb[kRowBlocks][kQInRegisters ? kGroups : 1];
       float4 qs[kRowBlocks][kQInRegisters ? kGroups : 1];  // of rows 2t, 2t + 1, 2t, 2t + 1: -8 times what the group's elements add up to, in the products' unit
@@ -460,9 +462,7 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             if (bad[x] || of_k >= k_limit) lowest = -1;
           }
           const int field = __reduce_max_sync(0xffffffffu, highest);
-          if (first_e == kNoExponent && field > 0) first_e = field - 126;
-          const bool plain = __all_sync(0xffffffffu, lowest >= max(field - kPlainExponents, 0)) && field > 126 + kLeastExponent && field <= 252 &&
-                             abs(field - 126 - first_e) <= kFarExponents - kPlainExponents && !far_apart;
+          const bool plain = __all_sync(0xffffffffu, lowest >= max(field - kPlainExponents, 0)) && field > 126 + kLeastExponent && field <= 126 + kMostExponent && !far_apart;
           float* tokens = v_tokens + (2 * warp + turn) * kStepTokens + kOfLane * lane;
           uint32_t* rests = v_rests + (2 * warp + turn) * (kStepTokens / 2) * kGroups;
           uint32_t rest[2];
@@ -476,9 +476,8 @@ cache4_stream_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_cons
             bool is_far = false;
 #pragma unroll
             for (int x = 0; x < kOfLane; ++x) {
-              const bool none = bad[x] || top[x] == 0u;
-              const int e2 = none ? 0 : min(max(static_cast<int>(top[x] >> 7) - 126, kLeastExponent), 126);
-              is_far = is_far || (!none && abs(e2 - first_e) > kFarExponents);
+              const int e2 = bad[x] ? 0 : min(max(static_cast<int>(top[x] >> 7) - 126, kLeastExponent), 126);
+              is_far = is_far || e2 > kMostExponent;
               const float down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23);
               tokens[x] = bad[x] ? __int_as_float(0x7fffffff) : static_cast<float>(e2);
 #pragma unroll
