@@ -1,11 +1,13 @@
 """The ends of the 4-bit cache's ranges, against the restatements in 64 bits: scales of V that are 0, all small or large, or different from group to group. Tolerances and helpers as in
 test_kv_cache4_gpu.py; each dimension is held to the mean of its own values' magnitudes, so that small ones decide where nothing else stands."""
+import io
+
 import pytest
 import torch
 
 from oracle import cache_oracle as orc
 from test_kv_cache4_gpu import INT4, _batch4, _cache4, _compare, _same
-from test_kv_cache_gpu import _ints, _run
+from test_kv_cache_gpu import E4M3, INT8, _cache, _ints, _run
 from torch_mlu_b200 import kv_cache, ops
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +119,21 @@ def test_stored_zeros(cuda_device, dim, dtype):
         out, lse = _run(b)
         _compare(out, lse, b)
         assert bool((out[:, 4:, 32:64] == 0).all())
+
+
+# ---------------------------------------------------------------------------------------------- load
+@pytest.mark.parametrize("code", [INT4, E4M3])
+def test_what_is_loaded_has_memory_of_its_own(cuda_device, code):
+    """Keys are kept, saved and changed without the values, and the other way round."""
+    heads, dim, block = 2, 64, 16
+    (kc, ks), (vc, vs) = (_cache4(cuda_device, 6, heads, block, dim, i) if code == INT4 else _cache(cuda_device, 6, heads, block, dim, code, i) for i in (1, 2))
+    args = kc, vc, ks, vs, _ints(cuda_device, [[3, 1, 2]]), _ints(cuda_device, [0, 45]), 45
+    key, value = kv_cache.load(*args)
+    again = kv_cache.load(*args)
+    for x in (key, value):
+        assert x.is_contiguous() and x.storage_offset() == 0 and x.untyped_storage().nbytes() == x.numel() * 2
+        with io.BytesIO() as f:
+            torch.save(x, f)
+            assert len(f.getvalue()) < x.numel() * 2 + 4096
+    key.zero_()
+    assert torch.equal(value, again[1])

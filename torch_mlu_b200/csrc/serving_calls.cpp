@@ -271,15 +271,9 @@ std::tuple<Tensor, Tensor> launch_load(const Tensor& key_cache, const Tensor& va
   TORCH_CHECK(num_tokens >= 0, "num_tokens must not be negative (got ", num_tokens, ")");
   p.num_tokens = to_int32(num_tokens, "num_tokens");
   c10::cuda::CUDAGuard guard(key_cache.device());
-  const std::vector<int64_t> shape = {num_tokens, p.heads_kv, p.head_dim};
-  // both are cut out of one allocation, as the results of a plan are
-  const Tensor both = new_tensor({2, num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache);
-  Tensor key = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), both.dtype()), value = at::detail::make_tensor<c10::TensorImpl>(
-      c10::Storage(both.storage()), both.key_set(), both.dtype());
-  key.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-  value.unsafeGetTensorImpl()->set_storage_offset(both.numel() / 2);
-  value.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
-  if (num_tokens == 0) return {key, value};
+  // memory of their own: either may be kept, saved or sent without the other
+  Tensor key = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache), value = new_tensor({num_tokens, p.heads_kv, p.head_dim}, dtype, key_cache);
+  if (num_tokens == 0) return {std::move(key), std::move(value)};
   p.block_table = block_table.data_ptr<int32_t>();
   p.table_stride = table_stride(block_table);
   p.max_blocks = to_int32(block_table.size(1), "max_blocks");
@@ -289,7 +283,7 @@ std::tuple<Tensor, Tensor> launch_load(const Tensor& key_cache, const Tensor& va
   p.key_out = key.data_ptr();
   p.value_out = value.data_ptr();
   check_status(sdpa_b200_cache_load(&p, stream_of(key_cache)), "sdpa_b200_cache_load");
-  return {key, value};
+  return {std::move(key), std::move(value)};
 }
 
 std::tuple<Tensor, Tensor> launch_attention(const Tensor& query, const Tensor& key_cache, const Tensor& value_cache, const Tensor& key_scale,
