@@ -410,8 +410,8 @@ typedef struct sdpa_b200_cache_params {
  * NaN or infinite one among them it is NaN and the codes are 0. */
 SDPA_B200_API int sdpa_b200_cache_store(const sdpa_b200_cache_params* p, void* stream);
 
-/* key_out, value_out <- tokens of the requests: row cu_seqlens_k[b] + i is token first[b] + i of request b, found through block_table, max_blocks blocks a row. code * scale
- * is rounded once to dtype; what is beyond its largest number is that number. NaN: a token in front of 0 or behind the table's row, a block number outside the cache, an
+/* key_out, value_out <- tokens of the requests: row cu_seqlens_k[b] + i is token first[b] + i of request b, found through block_table, max_blocks blocks a row. code * scale,
+ * a product in 32 bits, is rounded to dtype; what is beyond its largest number is that number. NaN: a token in front of 0 or behind the table's row, a block number outside the cache, an
  * infinite or NaN scale. Rows in front of cu_seqlens_k[0] and behind the last request are filled with zeros. Offsets that fall, or leave the outputs, write nothing outside
  * them; a row that several requests claim belongs to one of them. */
 SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* p, void* stream);
@@ -422,11 +422,11 @@ SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* p, void* st
  * counts, whatever stands there. A NaN among the values, or a scale of V that is negative, infinite or NaN, may reach every row of its request
  * and kv head, as 0 * NaN. A scale of V below 2^-100, as of a block of zeros, counts as 2^-100 where rows are few; there a value counts down to
  * 2^-39 of the largest product of a weight and a scale of V in its row. In a 4-bit cache scales of V keep all their bits down to 2^-16 of the
- * largest among 64 neighbouring tokens and count down to 2^-24 of it; they may be negative, and a scale of K or V that is infinite or NaN reaches
- * only the rows that see its token.
+ * largest among 64 neighbouring tokens, count down to 2^-24 of it and to 2^-100, and a weight times a scale counts down to 2^-38 of the largest product in its row of a weight and the largest
+ * scale among its 64 tokens (11 bits of it down to 2^-28); they may be negative, and a scale of K or V that is infinite or NaN reaches only the rows that see its token.
  * Scores may be of any size that 32 bits hold where rows are few or softmax_scale is above 2^16; else below 2^27, as in the prefill kernel.
  * Where requests have many rows, codes * scales are brought to 16 bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB
- * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded once, and within the type's range. What is beyond its
+ * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded as by load, and within the type's range. What is beyond its
  * largest number is that number (f16: 65504; the code of an element from 63488 on may be 65536), and f16 loses what is below 2^-24, as of a
  * cache that was filled from bf16. */
 SDPA_B200_API int sdpa_b200_cache_attention_workspace_bytes(const sdpa_b200_cache_params* p, size_t* bytes);

@@ -137,3 +137,25 @@ def test_what_is_loaded_has_memory_of_its_own(cuda_device, code):
             assert len(f.getvalue()) < x.numel() * 2 + 4096
     key.zero_()
     assert torch.equal(value, again[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
+def test_load_with_scales_of_all_their_bits(cuda_device, code, dtype):
+    """Scales that store does not write (8 significant bits of bf16, 24 of fp32), elements below fp16's normal numbers: a product in 32 bits, rounded to 16. With 4-bit codes that product is
+    exact."""
+    heads, dim, block, n = 3, 128, 16, 300
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    caches, scales, want = [], [], []
+    for i in (1, 2):
+        c, s = _cache4(cuda_device, 20, heads, block, dim, i) if code == INT4 else _cache(cuda_device, 20, heads, block, dim, code, i)
+        s = ((1 + torch.rand(s.shape, generator=g, device=cuda_device)) * torch.exp2(torch.randint(-30, 3, s.shape, generator=g, device=cuda_device).float())).to(s.dtype)
+        x = orc.numbers4(c).float() * s.float().repeat_interleave(32, -1) if code == INT4 else c.float() * s[:, :, None, None]
+        if code == INT4:
+            assert torch.equal(x.double(), orc.elements(c, s))
+        caches.append(c), scales.append(s)
+        largest = torch.finfo(dtype).max
+        want.append(x.clamp(-largest, largest).transpose(1, 2).flatten(0, 1)[:n].to(dtype))
+    got = kv_cache.load(*caches, *scales, torch.arange(20, dtype=torch.int32, device=cuda_device)[None], _ints(cuda_device, [0, n]), n, dtype=dtype)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)

@@ -81,8 +81,9 @@ def load(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens
     """(key, value), [num_tokens, heads_kv, head_dim] each: tokens of the requests out of the cache, packed as the varlen operators take them.
 
     Rows cu_seqlens[i] to cu_seqlens[i + 1] - 1 are request i's tokens from ``first[i]`` on ([requests] int32; from its first token without it), found through
-    ``block_table``. An element is code * scale, rounded once to ``dtype`` (bf16 or fp16; exact for 4-bit caches and for 8-bit ones that store filled), and the
-    type's largest number where it is beyond it. Rows of no request are zeros. A token behind the table's row, in a block outside the cache or with a
+    ``block_table``. An element is code * scale, a product in 32 bits that is rounded to ``dtype`` (bf16 or fp16), and the
+    type's largest number where it is beyond it. The product is exact for 4-bit caches, and for 8-bit ones whose scales have up to 16 significant bits; the result too where
+    ``store`` filled the cache, but for what is below fp16's normal numbers (2^-14). Rows of no request are zeros. A token behind the table's row, in a block outside the cache or with a
     scale that is infinite or NaN is NaN. Whether a request has the tokens is not known here: places that nothing was stored at hold anything. There is no gradient.
     """
     return _calls().cache_load(key_cache, value_cache, key_scale, value_scale, block_table, cu_seqlens, num_tokens, first, dtype)
@@ -98,9 +99,10 @@ def attention(query, key_cache, value_cache, key_scale, value_scale, block_table
     the table holds. Few rows per request stream the codes; with many (chunks of prompts) they are brought to 16 bits in the workspace and the prefill
     kernel runs: 4 * max_seqlen_k * heads_kv * head_dim bytes a request, for as many requests at a time as fit 4 GiB (where not even one does, or ``scale`` is above 2^16,
     the codes are streamed; scores of 2^27 and more need that). That is exact with scales that are powers of two, as store gives
-    them; with others every element is rounded once. Elements beyond the largest number of query's type are that number there (fp16: 65504, of which the code may be 65536),
+    them; with others every element is rounded, as in ``load``. Elements beyond the largest number of query's type are that number there (fp16: 65504, of which the code may be 65536),
     and fp16 queries over a cache that was filled from bf16 lose what fp16 cannot hold, below 2^-24. A 4-bit cache takes the same two paths; where its codes are streamed, scales of
-    values keep all their bits down to 2^-16 of the largest among 64 neighbouring tokens, count down to 2^-24 of it, and to 2^-100.
+    values keep all their bits down to 2^-16 of the largest among 64 neighbouring tokens, count down to 2^-24 of it, and to 2^-100; and a weight times a scale keeps its 11 bits down to 2^-28
+    of the largest such product in its row (of a weight with the largest scale among its 64 tokens), and counts down to 2^-38 of that.
 
     There is no gradient. A row without a visible key gets 0 and a logsumexp of +inf, rows outside every request are left unwritten, and a block number outside the
     cache makes the rows that see it NaN (their logsumexp +inf, as that of all NaN rows in this package), a length that passes the table's row all rows of its request.
