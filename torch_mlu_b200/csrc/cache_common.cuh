@@ -48,11 +48,12 @@ __device__ __forceinline__ void codes4_to_floats(uint32_t codes, float (&x)[8]) 
 
 constexpr int kScaleGroup = 32;  // elements of a token and head that share a scale in a 4-bit cache
 
-// kPer (8 or 16) elements of a cache of any code, whose scale is one
+// kPer elements of a cache of any code, whose scale is one: 16, or 8 of 8 bits
 template <int kCode, int kPer>
 struct Span {
   static constexpr bool kFour = kCode == SDPA_B200_INT4;
   static constexpr int kWords = kPer * (kFour ? 4 : 8) / 32;
+  static_assert(kWords == 2 || kWords == 4, "codes are read 8 or 16 bytes at a time");
   uint32_t codes[kWords];
   float scale;
 
@@ -72,11 +73,9 @@ struct Span {
     if constexpr (kWords == 4) {
       const uint4 w = *reinterpret_cast<const uint4*>(codes_at);
       codes[0] = w.x, codes[1] = w.y, codes[2] = w.z, codes[3] = w.w;
-    } else if constexpr (kWords == 2) {
+    } else {
       const uint2 w = *reinterpret_cast<const uint2*>(codes_at);
       codes[0] = w.x, codes[1] = w.y;
-    } else {
-      codes[0] = *reinterpret_cast<const uint32_t*>(codes_at);
     }
     scale = kFour ? __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(scales)[scale_index]) << 16) : static_cast<const float*>(scales)[scale_index];
   }
