@@ -424,7 +424,8 @@ SDPA_B200_API int sdpa_b200_cache_load(const sdpa_b200_cache_params* p, void* st
  * 2^-39 of the largest product of a weight and a scale of V in its row. In a 4-bit cache scales of V keep all their bits down to 2^-16 of the
  * largest among 64 neighbouring tokens, count down to 2^-24 of it and to 2^-100, and a weight times a scale counts down to 2^-38 of the largest product in its row of a weight and the largest
  * scale among its 64 tokens (11 bits of it down to 2^-28); they may be negative, and a scale of K or V that is infinite or NaN reaches only the rows that see its token.
- * Scores may be of any size that 32 bits hold where rows are few or softmax_scale is above 2^16; else below 2^27, as in the prefill kernel.
+ * Scores may be of any size that 32 bits hold where rows are few or softmax_scale is above 2^16; else below 2^27, and sums of values times weights of up to 2^8 must fit 32 bits, as in
+ * the prefill kernel.
  * Where requests have many rows, codes * scales are brought to 16 bits, q's type, in the workspace, of as many requests at a time as fit 4 GiB
  * at max_seqlen_k tokens each: exact with scales that are powers of two, else rounded as by load, and within the type's range. What is beyond its
  * largest number is that number (f16: 65504; the code of an element from 63488 on may be 65536), and f16 loses what is below 2^-24, as of a

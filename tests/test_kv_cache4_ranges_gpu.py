@@ -39,6 +39,15 @@ def test_scales_of_values_that_are_all_small_or_large(cuda_device, by, dim, bloc
     assert ops.device_status() == 0
 
 
+@pytest.mark.parametrize("rows", [1, 3, 9, 30])
+@pytest.mark.parametrize("dim,block", [(64, 16), (128, 64)])
+def test_largest_values(cuda_device, dim, block, rows):
+    """Values of up to 2^127, in units of which the streaming kernel's sums are held. (Where many rows are brought to 16 bits they are sums of 700 weights of up to 2^8 times values, in fp32: 2^127 *
+    700 * 2^8 does not fit it, and is no case there.)"""
+    b = _moved(cuda_device, rows, dim, block, 126, rows)
+    _compare(*_run(b), b)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 9, 30, 600])
 @pytest.mark.parametrize("dim,block", [(64, 16), (128, 64)])
 @pytest.mark.parametrize("by", [-80, -60, -40, -30, 0, 15, 18, 22, 60, 100])

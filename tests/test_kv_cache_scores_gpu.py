@@ -96,3 +96,42 @@ def test_scores_of_any_size(cuda_device, scale, rows, code):
         b[4][:] *= 2.0 ** 12
         _one_key(*_run(b, scale=scale), b, scale)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
+@pytest.mark.parametrize("dim,by", [(64, -100), (128, -60), (128, 60), (64, 100)])
+def test_small_queries_over_large_keys(cuda_device, dim, by, rows, code):
+    """Queries times a power of two over keys divided by it: the same scores, and the same tolerances."""
+    b = _any_batch(cuda_device, [700, 45, 130], [rows, min(rows, 40), 1], dim, code, rows + 2)
+    b = ((b[0].double() * 2.0 ** by).bfloat16(), *b[1:3], (b[3].double() * 2.0 ** -by).to(b[3].dtype), *b[4:])
+    (_compare4 if code == INT4 else _compare)(*_run(b), b, many=rows > 500)
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("code", [INT4, E4M3])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
+def test_the_same_call_gives_the_same_bits(cuda_device, rows, code):
+    b = _any_batch(cuda_device, [5000, 45, 1300] * 4, [rows, min(rows, 40), 1] * 4, 128, code, rows)
+    out, lse = _run(b)
+    for _ in range(5):
+        again = _run(b)
+        assert torch.equal(out.view(torch.int16), again[0].view(torch.int16)) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("code", [INT4, E4M3, INT8])
+@pytest.mark.parametrize("rows", [1, 3, 30, 600])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_queries_that_are_no_numbers(cuda_device, dim, rows, code):
+    """A NaN or an infinity in one head of a row makes that row and head NaN; those beside it in the same unit are as they would be."""
+    b = _any_batch(cuda_device, [700, 45, 130], [rows, min(rows, 40), 1], dim, code, rows + 3)
+    last = b[0].shape[0] - 1
+    b[0][0, 1, 5], b[0][last, 2, dim - 1], b[0][rows // 2, 6, 0] = math.nan, math.inf, -math.inf
+    out, lse = _run(b)
+    want = orc.attention(*b)[0]
+    assert torch.equal(out.isnan(), want.isnan()) and int(out.isnan().all(-1).sum()) == 3 and int(out.isnan().any(-1).sum()) == 3
+    at = out.isnan().any(-1)
+    b[0][at], out[at] = 0, 0
+    rest = orc.attention(*b)
+    out[at], lse.t()[at] = rest[0][at].to(out.dtype), rest[1].t()[at].float()
+    (_compare4 if code == INT4 else _compare)(out, lse, b, many=rows > 500)
