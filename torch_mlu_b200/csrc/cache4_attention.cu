@@ -13,11 +13,13 @@
 //   the step's products, were no faster: 8 requests of 32768 78.1 us, with the multiply-adds 77.3.)
 // * The scale of V is taken apart: a power of two 2^e, above the largest of a step's tokens, goes into the exponent of the softmax weight (as the 8-bit scale does), what is left, below 1 and exact
 //   in f16, onto the weights, 2 multiplications for 32 x 16 codes. A group whose scale is 2^-14 of 2^e has its products' full 11 bits only where the weight is that much above the smallest
-//   normal one; where tokens are further apart, each has an e of its own, and the sums of the softmax are formed without them, as the 8-bit kernel does for scales far apart: 64 requests of 8192 161 us instead of
+//   normal one; where tokens are further apart than 2^10, each has an e of its own, and the sums of the softmax are formed without them, as the 8-bit kernel does for scales far apart: 64 requests of 8192 161 us instead of
 //   147. Tokens of zeros, which the store gives 2^-100, have no part in that: with one, every 16th or all of them 147 to 149 (162 when any of them sent its unit that way).
+// * The plain way masks scores and takes their maximum in front of the row's factor. That needs a factor that is a normal number and scores below 2^20, which Q's largest elements and the
+//   step's scales of K bound; other steps multiply first and take the maximum off before anything else, so that scores of any size are right.
 // * The loading warps only issue copies, codes by TMA and scales by cp.async, and wait for nothing but room. A warp of the arithmetic brings the scales of V of its own tokens into these
 //   forms, a token or two a lane, beside its products with K.
-// Measured, one token per request, 32/8 heads of 128: 64 requests of 2048 to 32768 tokens, 1.34 GB: 323 us, 4.2 TB/s, 63% of a copy's rate; 8 of 32768 77; one of 1000, in clusters, 7.0. Without
+// Measured, one token per request, 32/8 heads of 128: 64 requests of 2048 to 32768 tokens, 1.34 GB: 327 us (312 to 330 by box and lengths), 4.1 TB/s, 62% of a copy's rate; 8 of 32768 78; one of 1000, in clusters, 7. Without
 // the arithmetic the first takes 228: it is the length of a step's chain in each warp that bounds it, with the logic pipe at 53% and the tensor pipe at 22%, no pipe alone.
 #include <type_traits>
 

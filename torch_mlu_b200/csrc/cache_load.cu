@@ -3,7 +3,7 @@
 // Row cu[b] + i is token first[b] + i of request b: code * scale, a product in 32 bits, rounded to 16. Bound by HBM: 4.5 or 8 bits read and 16 written per element.
 // A CTA has 64 rows of some heads. It counts the requests that end in front of its first row with all threads at once; what stands behind is found from there.
 // Measured, 8 heads of 128: 16 requests of 4096 to 8192 tokens out of 4 bits 113 us with each element converted by itself and each head's addresses anew, 88 now (5.2 TB/s); 8 of 8192 out of e4m3 62 (5.7 TB/s);
-// 301 tokens 5.2, four latencies behind the launch. Eight elements a thread instead of 16 89 and 66, five CTAs on an SM by fewer registers 94 and 69.
+// 301 tokens 5.2 to 6.0, four latencies behind the launch, and the host. Eight elements a thread instead of 16 89 and 66, five CTAs on an SM by fewer registers 94 and 69.
 #include <algorithm>
 #include <type_traits>
 
